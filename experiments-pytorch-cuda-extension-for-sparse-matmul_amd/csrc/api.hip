@@ -735,4 +735,229 @@ int bsa_attention_gradients(int dtype, const void *q, const void *k, const void 
                               batches, head_dim, scale, causal, stream);
 }
 
+
+// ---- packed sequences and paged caches ------------------------------------------------------------------
+static int check_alignment(const char *who, std::initializer_list<const void *> operands)
+{
+    for (const void *p : operands)
+        if ((uintptr_t)p & 15) return fail(BSA_ERR_UNSUPPORTED, "%s: operands must be aligned to 16 bytes", who);
+    return BSA_OK;
+}
+
+static int check_heads(const char *who, int heads, int key_heads, int head_dim)
+{
+    if (head_dim != 64 && head_dim != 128)
+        return fail(BSA_ERR_UNSUPPORTED, "%s: head_dim 64 and 128 are built, got %d", who, head_dim);
+    if (heads < 1 || key_heads < 1 || heads % key_heads != 0 || heads > 65535)
+        return fail(BSA_ERR_INVALID, "%s: %d query heads cannot share %d key heads", who, heads, key_heads);
+    return BSA_OK;
+}
+
+static int check_16_bit(const char *who, int dtype)
+{
+    if (dtype != BSA_F16 && dtype != BSA_BF16)
+        return fail(BSA_ERR_UNSUPPORTED, "%s: fp16 and bf16 are built, got dtype %d", who, dtype);
+    return BSA_OK;
+}
+
+// strides of 16-bit operands that are read 16 bytes at a time; a walk addresses 64 tokens by 32-bit offsets
+static int check_strides(const char *who, const int64_t *strides, int count)
+{
+    if (!strides) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    for (int i = 0; i < count; ++i) {
+        if (strides[i] < 0 || strides[i] % 8 != 0)
+            return fail(BSA_ERR_UNSUPPORTED, "%s: stride %lld is no multiple of 8 values", who, (long long)strides[i]);
+        if (strides[i] > (1LL << 40)) return fail(BSA_ERR_UNSUPPORTED, "%s: stride %lld is too large", who, (long long)strides[i]);
+    }
+    return BSA_OK;
+}
+
+static int packed(const char *who, int dtype, const void *q, const void *k, const void *v, const int32_t *offsets, int tokens,
+                  int sequences, int heads, int key_heads, int head_dim, const int64_t *strides, int operands, float scale,
+                  int causal, bsa::PackedArgs &p)
+{
+    int rc = check_16_bit(who, dtype);
+    if (!rc) rc = check_heads(who, heads, key_heads, head_dim);
+    if (!rc) rc = check_strides(who, strides, 2 * operands);
+    if (rc) return rc;
+    if (tokens < 1 || sequences < 1 || tokens > (1 << 30) || sequences > (1 << 24))
+        return fail(BSA_ERR_INVALID, "%s: %d tokens in %d sequences", who, tokens, sequences);
+    if (!q || !k || !v || !offsets) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    for (int i = 0; i < operands; ++i)
+        if (strides[2 * i] > (1LL << 24))
+            return fail(BSA_ERR_UNSUPPORTED, "%s: %lld values between tokens are too many", who, (long long)strides[2 * i]);
+    if ((long long)heads * (tokens / 32 + sequences) > (1LL << 30))
+        return fail(BSA_ERR_INVALID, "%s: grid of %d heads and %d tokens is too large", who, heads, tokens);
+    rc = check_alignment(who, {q, k, v});
+    if (rc) return rc;
+    p.q = q, p.k = k, p.v = v;
+    p.offsets = offsets;
+    p.tokens = tokens, p.sequences = sequences, p.heads = heads, p.key_heads = key_heads, p.head_dim = head_dim;
+    p.q_token = strides[0], p.q_head = strides[1], p.k_token = strides[2], p.k_head = strides[3];
+    p.v_token = strides[4], p.v_head = strides[5];
+    if (operands > 3) p.g_token = strides[6], p.g_head = strides[7];
+    p.scale = scale;
+    p.causal = causal != 0;
+    p.bf16 = dtype == BSA_BF16;
+    return BSA_OK;
+}
+
+int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, float *lse,
+                                 const int32_t *offsets, int tokens, int sequences, int heads, int key_heads, int head_dim,
+                                 const int64_t *strides, float scale, int causal, void *stream)
+{
+    const char *who = "bsa_packed_attention_forward";
+    bsa::PackedArgs p;
+    int rc = packed(who, dtype, q, k, v, offsets, tokens, sequences, heads, key_heads, head_dim, strides, 3, scale, causal, p);
+    if (rc) return rc;
+    if (!out) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    rc = check_alignment(who, {out});
+    if (rc) return rc;
+    p.out = out;
+    p.lse = lse;
+    return check_launch(bsa::launch_packed_forward(p, (hipStream_t)stream), who);
+}
+
+int bsa_packed_attention_backward(int dtype, const void *q, const void *k, const void *v, const void *dout, const void *out,
+                                  const float *lse, float *delta_ws, void *dq_out, void *dk_out, void *dv_out,
+                                  const int32_t *offsets, int tokens, int sequences, int heads, int key_heads, int head_dim,
+                                  const int64_t *strides, float scale, int causal, void *stream)
+{
+    const char *who = "bsa_packed_attention_backward";
+    bsa::PackedArgs p;
+    int rc = packed(who, dtype, q, k, v, offsets, tokens, sequences, heads, key_heads, head_dim, strides, 4, scale, causal, p);
+    if (rc) return rc;
+    if (!dout || !out || !lse || !delta_ws || !dq_out || (dk_out == nullptr) != (dv_out == nullptr))
+        return fail(BSA_ERR_INVALID, "%s: null pointer argument (dk_out and dv_out go together)", who);
+    rc = check_alignment(who, {dout, out, dq_out, dk_out, dv_out});
+    if (rc) return rc;
+    p.dout = dout, p.o = out;
+    p.lse = const_cast<float *>(lse);
+    p.delta = delta_ws;
+    p.out = dq_out, p.dk = dk_out, p.dv = dv_out;
+    return check_launch(bsa::launch_packed_backward(p, (hipStream_t)stream), who);
+}
+
+static int check_cache(const char *who, int cache_dtype, const void *keys, const void *values, const float *key_scales,
+                       const float *value_scales, int pages, int page, int &kind, int &shift)
+{
+    kind = cache_dtype == BSA_I8 ? 1 : cache_dtype == BSA_E4M3 ? 2 : 0;
+    if (kind == 0 && cache_dtype != BSA_F16 && cache_dtype != BSA_BF16)
+        return fail(BSA_ERR_UNSUPPORTED, "%s: a cache holds fp16, bf16, int8 or e4m3, got dtype %d", who, cache_dtype);
+    shift = page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : page == 256 ? 8 : 0;
+    if (shift == 0) return fail(BSA_ERR_UNSUPPORTED, "%s: pages of 32, 64, 128 and 256 tokens are built, got %d", who, page);
+    if (pages < 1 || (long long)pages << shift > 2147483647LL)
+        return fail(BSA_ERR_INVALID, "%s: %d pages of %d tokens", who, pages, page);
+    if (!keys || !values || (kind != 0 && (!key_scales || !value_scales)))
+        return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    return check_alignment(who, {keys, values, key_scales, value_scales});
+}
+
+static int cache_rows(const char *who, int cache_dtype, const void *k, const void *v, const int32_t *slots, const void *keys,
+                      const void *values, const float *key_scales, const float *value_scales, int tokens, int heads, int head_dim,
+                      int pages, int page, bsa::CacheRowsArgs &p)
+{
+    int rc = check_heads(who, heads, heads, head_dim);
+    if (!rc) rc = check_cache(who, cache_dtype, keys, values, key_scales, value_scales, pages, page, p.kind, p.page_shift);
+    if (rc) return rc;
+    if (tokens < 0 || (long long)tokens * heads > (1LL << 36))
+        return fail(BSA_ERR_INVALID, "%s: %d tokens of %d heads", who, tokens, heads);
+    if (tokens > 0 && (!k || !v || !slots)) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    rc = check_alignment(who, {k, v});
+    if (rc) return rc;
+    p.k = k, p.v = v;
+    p.slots = slots;
+    p.keys = const_cast<void *>(keys), p.values = const_cast<void *>(values);
+    p.key_scales = const_cast<float *>(key_scales), p.value_scales = const_cast<float *>(value_scales);
+    p.tokens = tokens, p.heads = heads, p.head_dim = head_dim, p.pages = pages;
+    p.held_bf16 = cache_dtype == BSA_BF16;
+    return BSA_OK;
+}
+
+int bsa_cache_write(int dtype, int cache_dtype, const void *k, const void *v, const int32_t *slots, void *keys, void *values,
+                    float *key_scales, float *value_scales, int tokens, int heads, int head_dim, int pages, int page,
+                    const int64_t *strides, void *stream)
+{
+    const char *who = "bsa_cache_write";
+    int rc = check_16_bit(who, dtype);
+    if (!rc) rc = check_strides(who, strides, 4);
+    if (rc) return rc;
+    bsa::CacheRowsArgs p;
+    rc = cache_rows(who, cache_dtype, k, v, slots, keys, values, key_scales, value_scales, tokens, heads, head_dim, pages, page, p);
+    if (rc || tokens == 0) return rc;
+    if (p.kind == 0 && dtype != cache_dtype)
+        return fail(BSA_ERR_UNSUPPORTED, "%s: a 16-bit cache takes rows of its own type", who);
+    p.k_token = strides[0], p.k_head = strides[1], p.v_token = strides[2], p.v_head = strides[3];
+    return check_launch(bsa::launch_cache_write(dtype, p, (hipStream_t)stream), who);
+}
+
+int bsa_cache_read(int dtype, int cache_dtype, const void *keys, const void *values, const float *key_scales,
+                   const float *value_scales, const int32_t *slots, void *k_out, void *v_out, int tokens, int heads, int head_dim,
+                   int pages, int page, void *stream)
+{
+    const char *who = "bsa_cache_read";
+    if (dtype != BSA_F32 && dtype != BSA_F16 && dtype != BSA_BF16)
+        return fail(BSA_ERR_UNSUPPORTED, "%s: rows are read as fp32, fp16 or bf16, got dtype %d", who, dtype);
+    bsa::CacheRowsArgs p;
+    const int rc = cache_rows(who, cache_dtype, k_out, v_out, slots, keys, values, key_scales, value_scales, tokens, heads,
+                              head_dim, pages, page, p);
+    if (rc || tokens == 0) return rc;
+    return check_launch(bsa::launch_cache_read(dtype, p, (hipStream_t)stream), who);
+}
+
+static int check_drafts(const char *who, int batch, int drafts, int heads, int key_heads, int head_dim, int width, int page)
+{
+    const int rc = check_heads(who, heads, key_heads, head_dim);
+    if (rc) return rc;
+    if (batch < 1 || batch > (1 << 20) || drafts < 1 || drafts > 1024 || width < 0 || (long long)width * page > 2147483647LL - 2048)
+        return fail(BSA_ERR_INVALID, "%s: %d sequences of %d new tokens and %d pages of %d", who, batch, drafts, width, page);
+    if ((long long)batch * heads * drafts > (1LL << 27))
+        return fail(BSA_ERR_INVALID, "%s: %d sequences of %d new tokens and %d heads are too many", who, batch, drafts, heads);
+    return BSA_OK;
+}
+
+size_t bsa_cached_attention_workspace_bytes(int batch, int drafts, int heads, int key_heads, int head_dim, int width, int page)
+{
+    if (check_drafts("bsa_cached_attention_workspace_bytes", batch, drafts, heads, key_heads, head_dim, width, page)) return 0;
+    bsa::CachedArgs p;
+    p.batch = batch, p.drafts = drafts, p.heads = heads, p.key_heads = key_heads, p.head_dim = head_dim, p.width = width;
+    p.page_shift = page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : 8;
+    return bsa::cached_attention_workspace_bytes(p);
+}
+
+int bsa_cached_attention(int dtype, int cache_dtype, const void *q, const void *k, const void *v, void *out, const void *keys,
+                         const void *values, const float *key_scales, const float *value_scales, const int32_t *table,
+                         const int32_t *lengths, const uint8_t *tree, int tree_shared, int batch, int drafts, int heads,
+                         int key_heads, int head_dim, int pages, int page, int width, const int64_t *strides, float scale,
+                         void *workspace, size_t workspace_bytes, void *stream)
+{
+    const char *who = "bsa_cached_attention";
+    bsa::CachedArgs p;
+    int rc = check_16_bit(who, dtype);
+    if (!rc) rc = check_cache(who, cache_dtype, keys, values, key_scales, value_scales, pages, page, p.kind, p.page_shift);
+    if (!rc) rc = check_drafts(who, batch, drafts, heads, key_heads, head_dim, width, page);
+    if (!rc) rc = check_strides(who, strides, 9);
+    if (rc) return rc;
+    if (p.kind == 0 && dtype != cache_dtype)
+        return fail(BSA_ERR_UNSUPPORTED, "%s: a 16-bit cache is attended to in its own type", who);
+    if (!q || !k || !v || !out || (!table && width > 0) || !lengths) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    rc = check_alignment(who, {q, k, v, out, workspace});
+    if (rc) return rc;
+    p.q = q, p.k = k, p.v = v, p.out = out;
+    p.keys = keys, p.values = values, p.key_scales = key_scales, p.value_scales = value_scales;
+    p.table = table, p.lengths = lengths, p.tree = tree;
+    p.batch = batch, p.drafts = drafts, p.heads = heads, p.key_heads = key_heads, p.head_dim = head_dim;
+    p.pages = pages, p.width = width;
+    p.bf16 = dtype == BSA_BF16, p.tree_shared = tree_shared != 0;
+    p.scale = scale;
+    p.q_batch = strides[0], p.q_token = strides[1], p.q_head = strides[2];
+    p.k_batch = strides[3], p.k_token = strides[4], p.k_head = strides[5];
+    p.v_batch = strides[6], p.v_token = strides[7], p.v_head = strides[8];
+    const size_t need = bsa::cached_attention_workspace_bytes(p);
+    if (need > 0 && (!workspace || workspace_bytes < need))
+        return fail(BSA_ERR_INVALID, "%s: workspace of %zu bytes needed, %zu given", who, need, workspace_bytes);
+    p.workspace = workspace;
+    return check_launch(bsa::launch_cached_attention(p, (hipStream_t)stream), who);
+}
+
 }  // extern "C"

@@ -152,4 +152,54 @@ hipError_t launch_attention_backward_scores(const AttentionArgs &p, hipStream_t 
 constexpr int AT_COLUMN_WAVES_128 = 4;    // waves per workgroup the column walk takes at head dim 128
 hipError_t launch_attention_backward_dkdv(const AttentionArgs &p, hipStream_t stream);   // groups = block columns
 
+// attention over packed sequences (packed_attention.hip); strides in values
+struct PackedArgs {
+    const void *q = nullptr, *k = nullptr, *v = nullptr;
+    const void *dout = nullptr, *o = nullptr;    // backward only; o: the forward result, dense
+    void *out = nullptr;                         // forward: the result; backward: dq
+    void *dk = nullptr, *dv = nullptr;           // both or neither
+    float *lse = nullptr;                        // [heads][tokens]; forward: written, may be null; backward: read
+    float *delta = nullptr;                      // backward: scratch of the same size
+    const int32_t *offsets = nullptr;
+    int tokens = 0, sequences = 0, heads = 0, key_heads = 0, head_dim = 64;
+    long long q_token = 0, q_head = 0, k_token = 0, k_head = 0, v_token = 0, v_head = 0, g_token = 0, g_head = 0;
+    float scale = 1.f;
+    bool causal = true, bf16 = false;
+};
+hipError_t launch_packed_forward(const PackedArgs &p, hipStream_t stream);
+hipError_t launch_packed_backward(const PackedArgs &p, hipStream_t stream);
+
+// rows into and out of a paged cache (cache_rows.hip); strides in values
+struct CacheRowsArgs {
+    const void *k = nullptr, *v = nullptr;       // write: read; read: the results
+    void *keys = nullptr, *values = nullptr;
+    float *key_scales = nullptr, *value_scales = nullptr;
+    const int32_t *slots = nullptr;
+    int tokens = 0, heads = 0, head_dim = 0, pages = 0, page_shift = 0, kind = 0;
+    bool held_bf16 = false;                      // what a 16-bit cache holds
+    long long k_token = 0, k_head = 0, v_token = 0, v_head = 0;
+};
+hipError_t launch_cache_write(int dtype, const CacheRowsArgs &p, hipStream_t stream);
+hipError_t launch_cache_read(int dtype, const CacheRowsArgs &p, hipStream_t stream);
+
+// new tokens over a paged cache and themselves (cached_attention.hip); strides in values
+struct CachedArgs {
+    const void *q = nullptr, *k = nullptr, *v = nullptr;
+    void *out = nullptr;                         // dense [batch][drafts][heads][head_dim]
+    const void *keys = nullptr, *values = nullptr;
+    const float *key_scales = nullptr, *value_scales = nullptr;
+    const int32_t *table = nullptr, *lengths = nullptr;
+    const unsigned char *tree = nullptr;
+    void *workspace = nullptr;
+    int batch = 0, drafts = 0, heads = 0, key_heads = 0, head_dim = 0, kind = 0, pages = 0, page_shift = 0, width = 0;
+    bool bf16 = false, tree_shared = false;
+    float scale = 1.f;
+    long long q_batch = 0, q_token = 0, q_head = 0, k_batch = 0, k_token = 0, k_head = 0, v_batch = 0, v_token = 0, v_head = 0;
+};
+bool cached_attention_splits(const CachedArgs &p);       // a sequence may have several chunks
+long long cached_attention_units(const CachedArgs &p);
+long long cached_attention_parts(const CachedArgs &p);   // rows that chunks can leave in the workspace
+size_t cached_attention_workspace_bytes(const CachedArgs &p);
+hipError_t launch_cached_attention(const CachedArgs &p, hipStream_t stream);
+
 }  // namespace bsa

@@ -9,8 +9,9 @@ import sys
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = ["api.hip", "layout_build.hip", "matmul.hip", "dsd_runs.hip", "softmax.hip", "attention.hip", "block_copy.hip",
-           "weight_panels.hip"]
-HEADERS = ["bench_yardstick.hip", "bsa_device.hpp", "lds_tiles.hpp", "lds_index_math.hpp", "bsa_internal.hpp", "group_walk.hpp", "attention_tiles.hpp", "panel_ring.hpp", os.path.join("..", "..", "include", "bsa.h")]
+           "weight_panels.hip", "packed_attention.hip", "cache_rows.hip", "cached_attention.hip"]
+HEADERS = ["bench_yardstick.hip", "bsa_device.hpp", "lds_tiles.hpp", "lds_index_math.hpp", "bsa_internal.hpp", "group_walk.hpp", "attention_tiles.hpp", "panel_ring.hpp",
+           "packed_tiles.hpp", "cache_values.hpp", os.path.join("..", "..", "include", "bsa.h")]
 LIB = os.path.join(HERE, "libbsa_hip.so")
 HOST_CALLS = os.path.join(HERE, "bsa_host_calls.so")
 

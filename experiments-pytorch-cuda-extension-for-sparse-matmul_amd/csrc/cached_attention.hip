@@ -1,0 +1,547 @@
+// Attention of N new tokens a sequence over what a paged cache holds of it and over themselves: q [B, N, Hq, D], new k and v
+// [B, N, Hk, D], cache positions 0 .. lengths[b] - 1 through pages[b], the new tokens under a mask tree[b][i][j] (a chain when
+// there is none).  One new token a sequence is a decode step, a tree of drafted ones the check of a draft.
+//
+//   S_ij = scale (q_i . y_j) s_j     y: the 8-bit values as 16-bit ones (exact), s: the scale of the token's row
+//   O_i  = sum_j softmax(S)_ij t_j z_j      the scales of the values ride on the probabilities, relative to their
+//                                           largest so far, so that fp16 holds them
+//
+// The query rows of a key head (N times the heads that share it) are the columns of 32 x 32 x 16 products; a tile is 32 tokens,
+// which lie in one page.  A workgroup has four waves: RG groups of 32 rows times 4 / RG groups of tiles.  RG = 1 (at most 32
+// rows): every wave walks tiles of its own through registers and its own LDS, with no barrier before the end.  Otherwise the waves
+// of a tile group share its tile, double buffered.
+// The work is cut where it lies: a unit is a chunk of the tiles of one sequence and key head, the chunk chosen on the device
+// from the lengths so that the units fill the machine, long sequences in many, short ones in one.  A sequence in several units
+// leaves (max, sum, O) of each in a workspace, which a second launch joins in the order of the chunks.
+#include "attention_tiles.hpp"
+#include "bsa_device.hpp"
+#include "bsa_internal.hpp"
+#include "cache_values.hpp"
+#include "packed_tiles.hpp"
+#include "../../include/bsa.h"
+
+namespace bsa {
+
+namespace {
+
+constexpr int CACHED_WAVES = 4;
+constexpr float CACHED_LAZY_SUM = 256.f;
+
+struct CachedOperands {
+    const half_t *q, *k, *v;
+    half_t *out;
+    const unsigned char *keys, *values;
+    const float *key_scales, *value_scales;
+    const int32_t *table, *lengths;
+    const unsigned char *tree;                   // [B or 1][N][N], may be null
+    float *parts;                                // [units][key heads][row blocks][rows of a block][HD], then (max, sum)
+    float2 *stats;
+    int batch, drafts, heads, key_heads, group;
+    int pages, page_shift, width;                // width: of the page table
+    int rows, row_blocks, least, target;         // rows: drafts * group; least: tiles of a chunk; target: units wanted
+    int tree_batch;                              // values between the masks of two sequences, 0: one mask for all
+    float scale2;
+    long long q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head;
+};
+
+__device__ __forceinline__ int cached_length(const CachedOperands &p, int b)
+{
+    const int n = p.lengths[b];
+    const long long room = (long long)p.width << p.page_shift;
+    return n < 0 ? 0 : n > room ? (int)room : n;
+}
+__device__ __forceinline__ int cached_tiles(const CachedOperands &p, int b)
+{
+    return (cached_length(p, b) + 31) / 32 + (p.drafts + 31) / 32;
+}
+// inclusive sums over the lanes of a wave
+__device__ __forceinline__ int wave_sums(int x)
+{
+    const int l = lane_id();
+#pragma unroll
+    for (int d = 1; d < WAVE; d *= 2) {
+        const int y = __shfl_up(x, d);
+        if (l >= d) x += y;
+    }
+    return x;
+}
+
+// tiles of a chunk: as many units as wanted, none shorter than `least` tiles
+__device__ __forceinline__ int cached_chunk(const CachedOperands &p)
+{
+    long long total = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += WAVE) {
+        const int b = b0 + lane_id();
+        total += __builtin_amdgcn_readlane(wave_sums(b < p.batch ? cached_tiles(p, b) : 0), WAVE - 1);
+    }
+    const long long per = (total * p.key_heads * p.row_blocks + p.target - 1) / p.target;
+    return (int)(per < p.least ? p.least : per);
+}
+
+struct CachedUnit {
+    int b, part, parts, first;                   // first: unit of part 0; b < 0: nothing to do
+};
+// sequence of a unit; or, with `unit` < 0, the units of sequence `of`
+__device__ __forceinline__ CachedUnit cached_unit(const CachedOperands &p, int chunk, int unit, int of)
+{
+    int before = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += WAVE) {
+        const int b = b0 + lane_id();
+        const int mine = b < p.batch ? (cached_tiles(p, b) + chunk - 1) / chunk : 0, upto = before + wave_sums(mine);
+        const bool hit = unit >= 0 ? upto - mine <= unit && unit < upto : b == of;
+        const unsigned long long found = __builtin_amdgcn_ballot_w64(hit);
+        if (found != 0ull) {
+            const int at = __builtin_ctzll(found);
+            const int parts = __builtin_amdgcn_readlane(mine, at), first = __builtin_amdgcn_readlane(upto, at) - parts;
+            return CachedUnit{b0 + at, unit - first, parts, first};
+        }
+        before = __builtin_amdgcn_readlane(upto, WAVE - 1);
+    }
+    return CachedUnit{-1, 0, 0, 0};
+}
+
+// 16 values of 8 bits as 16-bit ones
+template <bool BF, int KIND>
+__device__ __forceinline__ void widen_piece(uint4 raw, uint4 (&out)[2])
+{
+    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        float y[8];
+        widen_held<KIND>(w[2 * half], y);
+        widen_held<KIND>(w[2 * half + 1], y + 4);
+        h8 o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = narrow_16<BF>(y[j]);
+        out[half] = __builtin_bit_cast(uint4, o);
+    }
+}
+
+template <int HD, bool BF, int KIND, int RG>
+__global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(CachedOperands p)
+{
+    extern __shared__ __align__(16) unsigned char lds_raw[];
+    constexpr int KS = HD / 16, KG = CACHED_WAVES / RG, BUFFERS = RG > 1 ? 2 : 1, THREADS = 64 * RG;
+    constexpr int WIDTH = cache_value_bytes(KIND), PIECES = 32 * HD * WIDTH / 16, EACH = (PIECES + THREADS - 1) / THREADS;
+    constexpr int TILE = 64 * HD, SET = 2 * TILE + 256;                          // K, V, scales of a 32-token tile
+    constexpr bool SCALED = KIND != CACHE_16;
+    const float NEG_INF = -__builtin_inff();
+
+    const int xcd = (int)(blockIdx.x & 7u), turn = (int)(blockIdx.x >> 3);
+    const int rb = turn % p.row_blocks, pair = turn / p.row_blocks * 8 + xcd;    // row blocks of a chunk share an L2
+    const int key_head = pair % p.key_heads, unit = pair / p.key_heads;
+    const int chunk = cached_chunk(p);
+    const CachedUnit u = cached_unit(p, chunk, unit, 0);
+    if (u.b < 0) return;
+    const int b = u.b, len = __builtin_amdgcn_readfirstlane(cached_length(p, b));
+    const int held = (len + 31) / 32, tiles = held + (p.drafts + 31) / 32;
+    const int begin = u.part * chunk, end = min(tiles, begin + chunk);
+
+    const int w = wave_id(), l = lane_id(), qq = l & 31, h = l >> 5, rg = w % RG, kg = w / RG;
+    const int thread = l + 64 * rg;              // among those that share a tile
+    unsigned char *set0 = lds_raw + kg * BUFFERS * SET;
+    const TileReader rd(set0);
+
+    // query rows: row = draft * group + head of the group; those behind the last repeat it and are not stored
+    const int row = 32 * (rb * RG + rg) + qq, mine = min(row, p.rows - 1), draft = mine / p.group, sub = mine - draft * p.group;
+    h8 qop[KS];
+    const half_t *q_row = p.q + b * p.q_batch + draft * p.q_token + (long long)(key_head * p.group + sub) * p.q_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qop[s] = as_h8(ldg16(q_row + 16 * s + 8 * h));
+
+    // page numbers of 64 pages from `window` on, one a lane
+    int window = -1, page_of_lane = -1;
+    uint4 kraw[EACH], vraw[EACH];
+    float sraw = 0.f;
+    int there = 0;                               // tokens of the requested tile that the sequence has
+    auto request = [&](int t) {
+        there = 0;
+        if (t >= held) return;
+        const int page_index = t >> (p.page_shift - 5);
+        if (window < 0 || page_index - window >= WAVE) {
+            window = page_index;
+            page_of_lane = window + l < p.width ? p.table[(long long)b * p.width + window + l] : -1;
+        }
+        const int page = __builtin_amdgcn_readlane(page_of_lane, page_index - window);
+        if (page < 0 || page >= p.pages) return;
+        there = min(32, len - 32 * t);
+        const long long first = (((long long)page * p.key_heads + key_head) << p.page_shift) + ((32 * t) & ((1 << p.page_shift) - 1));
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int piece = thread + THREADS * i;
+            if (PIECES % THREADS == 0 || piece < PIECES) {
+                kraw[i] = ldg16_stream(p.keys + first * HD * WIDTH + 16 * piece);
+                vraw[i] = ldg16_stream(p.values + first * HD * WIDTH + 16 * piece);
+            }
+        }
+        if (SCALED && thread < 64) sraw = (thread < 32 ? p.key_scales : p.value_scales)[first + (thread & 31)];
+    };
+    // 8 values of token r of the tile into the panels that TileReader reads
+    auto put = [&](unsigned char *tile, int r, int piece, uint4 x) {
+        *reinterpret_cast<uint4 *>(tile + 4096 * (piece >> 3) + 128 * r + 16 * ((piece & 7) ^ panel_swizzle(r))) = x;
+    };
+    auto stage = [&](int t, unsigned char *set) {
+        const uint4 none = make_uint4(0, 0, 0, 0);
+        float *scales = reinterpret_cast<float *>(set + 2 * TILE);
+        if (t < held) {                          // tokens that the sequence does not have are zeros, whatever the page holds
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int piece = thread + THREADS * i;
+                if (PIECES % THREADS == 0 || piece < PIECES) {
+                    if (SCALED) {
+                        const int r = piece / (HD / 16), c = 2 * (piece % (HD / 16));
+                        uint4 a[2], z[2];
+                        widen_piece<BF, KIND>(r < there ? kraw[i] : none, a);
+                        widen_piece<BF, KIND>(r < there ? vraw[i] : none, z);
+                        put(set, r, c, a[0]), put(set, r, c + 1, a[1]);
+                        put(set + TILE, r, c, z[0]), put(set + TILE, r, c + 1, z[1]);
+                    } else {
+                        const int r = piece / (HD / 8), c = piece % (HD / 8);
+                        put(set, r, c, r < there ? kraw[i] : none);
+                        put(set + TILE, r, c, r < there ? vraw[i] : none);
+                    }
+                }
+            }
+            if (SCALED && thread < 64) scales[thread] = (thread & 31) < there ? (thread < 32 ? sraw * p.scale2 : sraw) : 0.f;
+            return;
+        }
+        const int j0 = 32 * (t - held);
+        constexpr int NEW = 32 * HD / 8;
+        for (int piece = thread; piece < NEW; piece += THREADS) {
+            const int r = piece / (HD / 8), c = piece % (HD / 8), j = j0 + r;
+            const bool is = j < p.drafts;
+            const half_t *kr = p.k + b * p.k_batch + j * p.k_token + key_head * p.k_head + 8 * c,
+                         *vr = p.v + b * p.v_batch + j * p.v_token + key_head * p.v_head + 8 * c;
+            put(set, r, c, is ? ldg16(kr) : none);
+            put(set + TILE, r, c, is ? ldg16(vr) : none);
+        }
+        if (SCALED && thread < 64) scales[thread] = thread < 32 ? p.scale2 : 1.f;
+    };
+
+    float m = NEG_INF, minus_m = 0.f, lsum = 0.f, top = 0.f;                     // top: what the value scales are relative to
+    bool fresh = true;
+    RowTile<HD> oacc;
+    clear<HD>(oacc);
+
+    request(begin + kg);
+    const int rounds = (end - begin + KG - 1) / KG;
+    for (int round = 0; round < rounds; ++round) {
+        const int t = begin + round * KG + kg;
+        const unsigned buffer = (RG > 1 ? round & 1 : 0) * SET;
+        unsigned char *set = set0 + buffer;
+        const bool work = t < end;
+        int have = 0;
+        if (work) {
+            have = t < held ? there : min(32, p.drafts - 32 * (t - held));
+            stage(t, set);
+            request(t + KG < end ? t + KG : held);
+        }
+        if (RG > 1) __syncthreads();
+        else wave_lds_fence();
+        if (!work || have <= 0) continue;
+        f16v sacc = {0};
+#pragma unroll
+        for (int s = 0; s < KS; ++s) sacc = mfma_16<BF>(rd.rows(buffer, s), qop[s], sacc);
+        const float *scales = reinterpret_cast<const float *>(set + 2 * TILE);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            if (SCALED) {
+                const f4v ks = *reinterpret_cast<const f4v *>(scales + 8 * g + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sacc[4 * g + j] *= ks[j];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) sacc[4 * g + j] *= p.scale2;
+            }
+        }
+        const bool drafted = t >= held;
+        unsigned sees = 0xFFFFu;                 // bit v: the key of accumulator value v is seen
+        if (drafted || have < 32) {
+            sees = 0;
+            const int j0 = 32 * (t - held);
+            const unsigned char *mask = p.tree + (long long)b * p.tree_batch + (long long)draft * p.drafts + j0;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int r = 8 * (v >> 2) + 4 * h + (v & 3);
+                bool seen = r < have;
+                if (drafted && seen) seen = p.tree != nullptr ? mask[r] != 0 : j0 + r <= draft;
+                sees |= seen ? 1u << v : 0u;
+            }
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                if (!((sees >> v) & 1u)) sacc[v] = NEG_INF;
+        }
+        float psum;
+        h8 pop[2];
+        float relative[16];                      // of the value scales
+        if (SCALED) {
+            float most = 0.f;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f4v vs = *reinterpret_cast<const f4v *>(scales + 32 + 8 * g + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) relative[4 * g + j] = vs[j], most = fmaxf(most, vs[j]);
+            }
+            most = fmaxf(most, at_lane_xor32(most));
+            if (most > top) {                    // the same in all lanes
+                const float keep = top / (2.f * most);
+                top = 2.f * most;                // twice: fewer of these
+                each<HD>(oacc, [&](float x, int) { return x * keep; });
+            }
+            const float inv = top > 0.f ? 1.f / top : 0.f;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) relative[v] *= inv;
+        }
+        auto exponentials = [&]() {
+            psum = 0.f;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const float pv = at_exp2(sacc[v] + minus_m);
+                psum += pv;
+                pop[v >> 3][v & 7] = narrow_16<BF>(SCALED ? pv * relative[v] : pv);
+            }
+        };
+        // A row moves its reference point by itself, so that its bits are its own: a row beside it, of NaN say, changes nothing.
+        bool move = m == NEG_INF;
+        if (fresh) psum = 0.f;
+        else exponentials();
+        move = move || psum > CACHED_LAZY_SUM;
+        if (__builtin_amdgcn_ballot_w64(move) != 0ull) {
+            const int other_moves = __builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)move);
+            move = move || other_moves != 0;
+            float bm = sacc[0];
+#pragma unroll
+            for (int v = 1; v < 16; ++v) bm = fmaxf(bm, sacc[v]);
+            bm = fmaxf(bm, at_lane_xor32(bm));
+            const float m_new = move ? fmaxf(m, bm) : m;
+            const float keep = m == NEG_INF ? 0.f : at_exp2(m - at_finite_or_zero(m_new));       // nothing accumulated so far: 0
+            m = m_new;
+            minus_m = -at_finite_or_zero(m_new);
+            lsum *= keep;
+            each<HD>(oacc, [&](float x, int) { return x * keep; });
+            fresh = __builtin_amdgcn_ballot_w64(m != NEG_INF) == 0ull;
+            exponentials();
+        }
+        lsum += psum;
+        if (drafted) {
+            const unsigned other = (unsigned)__builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)sees);
+            const unsigned lower = h == 0 ? sees : other, upper = h == 0 ? other : sees;
+            weigh_tile_masked<HD, BF, true>(rd, buffer + TILE, pop, oacc, [&](int r) {
+                return (((r & 4 ? upper : lower) >> (4 * (r >> 3) + (r & 3))) & 1u) != 0u;
+            });
+        } else {
+            weigh_tile<HD, BF>(rd, buffer + TILE, pop, oacc);
+        }
+        if (RG == 1) wave_lds_fence();
+    }
+    lsum += at_lane_xor32(lsum);
+    if (SCALED) each<HD>(oacc, [&](float x, int) { return x * top; });
+
+    // join the tile groups of the workgroup: all but the first park (max, sum) and O^T in LDS
+    __syncthreads();
+    if constexpr (KG > 1) {
+        constexpr int PARK = 2 * TILE + 256;     // O^T of a wave: 32 HD floats, and (max, sum) of 32 rows
+        static_assert(CACHED_WAVES * PARK <= KG * BUFFERS * SET, "the parked results take the tiles' place");
+        unsigned char *park = lds_raw + w * PARK;
+        if (kg > 0) {
+            each<HD>(oacc, [&](float x, int at) { return reinterpret_cast<float *>(park)[at] = x; });
+            if (h == 0) reinterpret_cast<float2 *>(park + 2 * TILE)[qq] = make_float2(m, lsum);
+        }
+        __syncthreads();
+        if (kg > 0) return;
+        float most = m;
+#pragma unroll
+        for (int o = 1; o < KG; ++o) most = fmaxf(most, reinterpret_cast<const float2 *>(park + o * RG * PARK + 2 * TILE)[qq].x);
+        const float to = at_finite_or_zero(most), own = at_exp2(m - to);
+        lsum *= own;
+        each<HD>(oacc, [&](float x, int) { return x * own; });
+#pragma unroll
+        for (int o = 1; o < KG; ++o) {
+            const unsigned char *from = park + o * RG * PARK;
+            const float2 st = reinterpret_cast<const float2 *>(from + 2 * TILE)[qq];
+            const float f = at_exp2(st.x - to);
+            lsum += st.y * f;
+            each<HD>(oacc, [&](float x, int at) { return x + reinterpret_cast<const float *>(from)[at] * f; });
+        }
+        m = most;
+    }
+    if (u.parts > 1) {
+        const long long block = ((long long)unit * p.key_heads + key_head) * p.row_blocks + rb;
+        const long long at = block * (32 * RG) + 32 * rg + qq;
+        if (row < p.rows) {
+            float *part = p.parts + at * HD;
+#pragma unroll
+            for (int t = 0; t < HD / 32; ++t)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f4v *>(part + 32 * t + 8 * g + 4 * h) =
+                        f4v{oacc[t][4 * g], oacc[t][4 * g + 1], oacc[t][4 * g + 2], oacc[t][4 * g + 3]};
+            if (h == 0) p.stats[at] = make_float2(m, lsum);
+        }
+        return;
+    }
+    if (row < p.rows) {
+        const float inv = lsum > 0.f || lsum != lsum ? 1.f / lsum : 0.f;
+        half_t *dst = p.out + (((long long)b * p.drafts + draft) * p.heads + key_head * p.group + sub) * HD;
+#pragma unroll
+        for (int t = 0; t < HD / 32; ++t)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                h4 o;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[j] = narrow_16<BF>(oacc[t][4 * g + j] * inv);
+                *reinterpret_cast<h4 *>(dst + 32 * t + 8 * g + 4 * h) = o;
+            }
+    }
+}
+
+// Joins the chunks of a row: HD / 4 lanes a row and chunk, ROWS rows a workgroup, the chunks of a row dealt to 1024 / ROWS of the
+// lanes in order and summed in order.
+template <int HD, bool BF, int ROWS>
+__global__ __launch_bounds__(32 * HD / 4) void cached_join_kernel(CachedOperands p, int block_rows)
+{
+    constexpr int LANES = HD / 4, LISTS = 32 / ROWS;                             // lists of chunks of a row
+    __shared__ float sums[32][HD];
+    __shared__ float2 stats[32];
+    const int chunk = cached_chunk(p);
+    const long long per = (p.rows + ROWS - 1) / ROWS;
+    const long long group = blockIdx.x;
+    const int b = (int)(group / (per * p.key_heads)), rest = (int)(group - b * per * p.key_heads);
+    const int key_head = rest / (int)per, list = (int)threadIdx.x / LANES, lane = (int)threadIdx.x % LANES;
+    const int row = (rest - key_head * (int)per) * ROWS + list / LISTS;
+    const CachedUnit u = cached_unit(p, chunk, -1, b);
+    if (u.parts <= 1) return;                    // the walk has stored the row
+    float m = -__builtin_inff(), lsum = 0.f;
+    f4v acc = {0.f, 0.f, 0.f, 0.f};
+    const bool is = row < p.rows;
+    auto at = [&](int part) {
+        const long long block = ((long long)(u.first + part) * p.key_heads + key_head) * p.row_blocks + row / block_rows;
+        return block * block_rows + row % block_rows;
+    };
+    if (is)
+        for (int part = list % LISTS; part < u.parts; part += LISTS) {
+            const float2 st = p.stats[at(part)];
+            const f4v x = *reinterpret_cast<const f4v *>(p.parts + at(part) * HD + 4 * lane);
+            const float top = fmaxf(m, st.x), to = at_finite_or_zero(top), keep = at_exp2(m - to), f = at_exp2(st.x - to);
+            m = top;
+            lsum = lsum * keep + st.y * f;
+            acc = acc * keep + x * f;
+        }
+    if (LISTS > 1) {
+        *reinterpret_cast<f4v *>(&sums[list][4 * lane]) = acc;
+        if (lane == 0) stats[list] = make_float2(m, lsum);
+        __syncthreads();
+        if (list % LISTS != 0) return;
+        for (int o = 1; o < LISTS; ++o) {
+            const float2 st = stats[list + o];
+            const f4v x = *reinterpret_cast<const f4v *>(&sums[list + o][4 * lane]);
+            const float top = fmaxf(m, st.x), to = at_finite_or_zero(top), keep = at_exp2(m - to), f = at_exp2(st.x - to);
+            m = top;
+            lsum = lsum * keep + st.y * f;
+            acc = acc * keep + x * f;
+        }
+    }
+    if (!is) return;
+    const float inv = lsum > 0.f || lsum != lsum ? 1.f / lsum : 0.f;
+    const int draft = row / p.group, sub = row - draft * p.group;
+    h4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = narrow_16<BF>(acc[j] * inv);
+    *reinterpret_cast<h4 *>(p.out + (((long long)b * p.drafts + draft) * p.heads + key_head * p.group + sub) * HD + 4 * lane) = o;
+}
+
+// ---- launchers ----------------------------------------------------------------------------------------
+constexpr int CACHED_UNITS = 768;                // wanted in a launch: three workgroups a compute unit
+constexpr int CACHED_LEAST = 8;                  // tiles of a chunk: two for each wave of RG = 1
+
+int row_groups(int rows) { return rows <= 32 ? 1 : 4; }
+
+CachedOperands operands(const CachedArgs &a)
+{
+    CachedOperands p;
+    p.q = (const half_t *)a.q, p.k = (const half_t *)a.k, p.v = (const half_t *)a.v, p.out = (half_t *)a.out;
+    p.keys = (const unsigned char *)a.keys, p.values = (const unsigned char *)a.values;
+    p.key_scales = a.key_scales, p.value_scales = a.value_scales;
+    p.table = a.table, p.lengths = a.lengths, p.tree = a.tree;
+    p.batch = a.batch, p.drafts = a.drafts, p.heads = a.heads, p.key_heads = a.key_heads, p.group = a.heads / a.key_heads;
+    p.pages = a.pages, p.page_shift = a.page_shift, p.width = a.width;
+    p.tree_batch = a.tree_shared ? 0 : a.drafts * a.drafts;
+    p.scale2 = a.scale * 1.4426950408889634f;
+    p.q_batch = a.q_batch, p.q_token = a.q_token, p.q_head = a.q_head;
+    p.k_batch = a.k_batch, p.k_token = a.k_token, p.k_head = a.k_head;
+    p.v_batch = a.v_batch, p.v_token = a.v_token, p.v_head = a.v_head;
+    p.rows = a.drafts * p.group;
+    const int rg = row_groups(p.rows);
+    p.row_blocks = (p.rows + 32 * rg - 1) / (32 * rg);
+    p.least = CACHED_LEAST;
+    p.target = CACHED_UNITS;
+    p.parts = (float *)a.workspace;
+    p.stats = (float2 *)(p.parts + cached_attention_parts(a) * a.head_dim);
+    return p;
+}
+
+template <int HD, bool BF, int KIND, int RG>
+hipError_t walk(const CachedArgs &a, hipStream_t st)
+{
+    const CachedOperands p = operands(a);
+    constexpr size_t lds = (CACHED_WAVES / RG) * (RG > 1 ? 2 : 1) * (128 * HD + 256);
+    auto kernel = cached_attention_kernel<HD, BF, KIND, RG>;
+    if (lds > 65536) {
+        const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (err != hipSuccess) return err;
+    }
+    const long long pairs = (cached_attention_units(a) * a.key_heads + 7) / 8 * 8;
+    kernel<<<(unsigned)(pairs * p.row_blocks), 64 * CACHED_WAVES, lds, st>>>(p);
+    hipError_t err = hipGetLastError();
+    if (err != hipSuccess || !cached_attention_splits(a)) return err;
+    const long long rows = (long long)a.batch * a.key_heads * p.rows;
+    if (rows >= 1024) cached_join_kernel<HD, BF, 32><<<(unsigned)((long long)a.batch * a.key_heads * ((p.rows + 31) / 32)), 32 * HD / 4, 0, st>>>(p, 32 * RG);
+    else cached_join_kernel<HD, BF, 1><<<(unsigned)rows, 32 * HD / 4, 0, st>>>(p, 32 * RG);
+    return hipGetLastError();
+}
+template <int HD, bool BF, int KIND>
+hipError_t walk_rows(const CachedArgs &a, hipStream_t st)
+{
+    return row_groups(a.drafts * (a.heads / a.key_heads)) == 1 ? walk<HD, BF, KIND, 1>(a, st) : walk<HD, BF, KIND, 4>(a, st);
+}
+template <int HD, bool BF>
+hipError_t walk_kind(const CachedArgs &a, hipStream_t st)
+{
+    if (a.kind == CACHE_INT8) return walk_rows<HD, BF, CACHE_INT8>(a, st);
+    if (a.kind == CACHE_E4M3) return walk_rows<HD, BF, CACHE_E4M3>(a, st);
+    return walk_rows<HD, BF, CACHE_16>(a, st);
+}
+
+}  // namespace
+
+// most tiles a sequence can have
+static long long most_tiles(const CachedArgs &a)
+{
+    return (((long long)a.width << a.page_shift) + 31) / 32 + (a.drafts + 31) / 32;
+}
+bool cached_attention_splits(const CachedArgs &a) { return most_tiles(a) > CACHED_LEAST; }
+// Most units (of all sequences) a launch can have: the chunk is at least total key_heads row_blocks / target, so that the whole
+// chunks are at most target / (key_heads row_blocks), and every sequence has one that is not.
+long long cached_attention_units(const CachedArgs &a)
+{
+    const int rows = a.drafts * (a.heads / a.key_heads), rg = row_groups(rows), blocks = (rows + 32 * rg - 1) / (32 * rg);
+    return a.batch + (cached_attention_splits(a) ? CACHED_UNITS / (a.key_heads * blocks) : 0);
+}
+long long cached_attention_parts(const CachedArgs &a)
+{
+    if (!cached_attention_splits(a)) return 0;
+    const int rows = a.drafts * (a.heads / a.key_heads), rg = row_groups(rows), blocks = (rows + 32 * rg - 1) / (32 * rg);
+    return cached_attention_units(a) * a.key_heads * blocks * 32 * rg;
+}
+size_t cached_attention_workspace_bytes(const CachedArgs &a)
+{
+    return (size_t)cached_attention_parts(a) * (a.head_dim + 2) * sizeof(float);
+}
+
+hipError_t launch_cached_attention(const CachedArgs &a, hipStream_t st)
+{
+    if (a.head_dim == 64) return a.bf16 ? walk_kind<64, true>(a, st) : walk_kind<64, false>(a, st);
+    return a.bf16 ? walk_kind<128, true>(a, st) : walk_kind<128, false>(a, st);
+}
+
+}  // namespace bsa

@@ -1,0 +1,372 @@
+// Causal (or full) attention over sequences of different lengths packed along the tokens, with grouped heads, and its gradients:
+// q [T, Hq, D], k and v [T, Hk, D], sequence b = rows offsets[b] .. offsets[b + 1] - 1, query head h over key head h / (Hq / Hk).
+//
+// One workgroup holds 32 W query rows of one head; its W waves share tiles of 64 keys and values in LDS (double buffered, loaded
+// straight to LDS, one barrier a tile), and each wave has 32 of the rows:
+//   S^T = K Q^T             a lane holds ONE query column and 32 of the 64 keys (the others sit in lane ^ 32)
+//   online softmax          per-lane reference point and sum; the point moves only when a tile's sum of exponentials passes 256
+//   O^T += V^T P^T          the probabilities go from accumulators to operands without leaving the registers
+// The lengths stay on the device: a launch has slots for the most tiles that T tokens in B sequences can make, and every workgroup
+// finds its sequence by a search over the offsets.  Slots that no sequence uses end at once.  Offsets are clamped to [0, T]
+// before anything is addressed with them.
+#include "attention_tiles.hpp"
+#include "bsa_device.hpp"
+#include "bsa_internal.hpp"
+#include "packed_tiles.hpp"
+#include "../../include/bsa.h"
+
+namespace bsa {
+
+namespace {
+
+constexpr float PACKED_LAZY_SUM = 256.f;         // fp16 holds what stays below it
+
+template <int HD, bool BF, int W>
+__global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperands p)
+{
+    extern __shared__ __align__(16) unsigned char lds_raw[];
+    constexpr int KS = HD / 16, ROWS = 32 * W;
+    const int cells = packed_grid(p.heads, p.head_sets, p.slots);
+    if ((int)blockIdx.x >= cells) return packed_clear(p, (int)blockIdx.x - cells, p.out, (long long)p.heads * HD);
+    const PackedItem item = packed_item<ROWS>(p, p.heads, true);
+    if (item.n == 0) return;
+    const int w = wave_id(), l = lane_id(), qq = l & 31, h = l >> 5, n = item.n, key_head = item.head / p.group;
+    const int row0 = item.tile * ROWS + 32 * w, row = row0 + qq;                 // rows and keys count from the sequence's start
+    const long long begin = item.begin;
+    const float NEG_INF = -__builtin_inff();
+
+    PairTiles<HD, W> tiles(p.k + begin * p.k_token + key_head * p.k_head, p.k_token,
+                           p.v + begin * p.v_token + key_head * p.v_head, p.v_token, lds_raw);
+    const int last_row = min(n, item.tile * ROWS + ROWS) - 1;
+    const int steps = p.causal ? last_row / 64 + 1 : (n + 63) / 64;
+    tiles.request(0, n, 0);
+
+    h8 qop[KS];
+    const half_t *q_row = p.q + (begin + min(row, n - 1)) * p.q_token + item.head * p.q_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) qop[s] = as_h8(ldg16(q_row + 16 * s + 8 * h));
+
+    // reference point of the query (both lane halves agree), minus it (0 while nothing was seen), this half's sum;
+    // fresh: no query of the wave has a reference point yet
+    float m = NEG_INF, minus_m = 0.f, lsum = 0.f;
+    bool fresh = true;
+    RowTile<HD> oacc;
+    clear<HD>(oacc);
+
+    for (int step = 0; step < steps; ++step) {
+        const int k0 = 64 * step;
+        tiles.arrived(step & 1);
+        if (step + 1 < steps) tiles.request(step + 1, n, (step + 1) & 1);
+        if (row0 >= n || (p.causal && k0 > row0 + 31)) continue;
+        f16v sacc[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            sacc[u] = f16v{0};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) sacc[u] = mfma_16<BF>(tiles.rows(0, u, s), qop[s], sacc[u]);
+        }
+        const bool masked = k0 + 64 > n || (p.causal && k0 + 63 > row0);
+        const int seen = (p.causal ? min(row, n - 1) : n - 1) - k0;              // last key of the tile that the query sees
+        float mul = p.scale2;                    // what is still to be applied to the scores in the exponent
+        if (masked) {                            // -inf only once scaled, whatever the scale's sign
+            mul = 1.f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    sacc[u][v] = 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? NEG_INF : sacc[u][v] * p.scale2;
+        }
+        float psum;
+        h8 pop[2][2];
+        auto exponentials = [&]() {
+            psum = 0.f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const float pv = at_exp2(__builtin_fmaf(sacc[u][v], mul, minus_m));
+                    psum += pv;
+                    pop[u][v >> 3][v & 7] = narrow_16<BF>(pv);
+                }
+        };
+        // A row moves its reference point by itself, so that its bits are its own: a row beside it, of NaN say, changes nothing.
+        bool move = m == NEG_INF;
+        if (fresh) psum = 0.f;
+        else exponentials();
+        move = move || psum > PACKED_LAZY_SUM;
+        if (__builtin_amdgcn_ballot_w64(move) != 0ull) {
+            const int other_moves = __builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)move);
+            move = move || other_moves != 0;
+            float bm = sacc[0][0] * mul;
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+                for (int v = 0; v < 16; ++v) bm = fmaxf(bm, sacc[u][v] * mul);
+            bm = fmaxf(bm, at_lane_xor32(bm));
+            const float m_new = move ? fmaxf(m, bm) : m;
+            const float keep = m == NEG_INF ? 0.f : at_exp2(m - at_finite_or_zero(m_new));       // nothing accumulated so far: 0
+            m = m_new;
+            minus_m = -at_finite_or_zero(m_new);
+            lsum *= keep;
+            each<HD>(oacc, [&](float x, int) { return x * keep; });
+            fresh = __builtin_amdgcn_ballot_w64(m != NEG_INF) == 0ull;
+            exponentials();
+        }
+        lsum += psum;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (masked) tiles.template weigh_masked<BF, true>(1, u, pop[u], oacc, [&](int r) { return 32 * u + r <= seen; });
+            else tiles.template weigh<BF>(1, u, pop[u], oacc);
+        }
+    }
+    lsum += at_lane_xor32(lsum);                 // both halves used the same reference point
+    const bool any = lsum > 0.f || lsum != lsum;
+    if (p.lse != nullptr && h == 0 && row < n)   // log2 of the row's sum, +inf for a row that sees nothing
+        p.lse[(size_t)item.head * p.tokens + begin + row] =
+            any ? at_finite_or_zero(m) + __builtin_amdgcn_logf(lsum) : __builtin_inff();
+    __syncthreads();                             // all are done with the tiles, whose place the results take
+    store_token_rows<HD, BF>(oacc, any ? 1.f / lsum : 0.f, lds_raw + 64 * HD * w,
+                             p.out + ((begin + row0) * p.heads + item.head) * HD, (long long)p.heads * HD, n - row0);
+}
+
+// ---------------------------------------------------------------------------
+// Gradients, as two walks that each rebuild the probabilities from the row statistics and write every result once (no atomics:
+// the same bits every time):
+//   rows      as the forward walk:  P = exp2(scale2 S - lse),  dS = P (dO V^T - delta),  dq^T += K^T dS^T;
+//             delta = rowsum(dO O) is made here and left for the other walk
+//   columns   a workgroup holds 32 W keys of one key head and walks the queries of all heads that share it:
+//             dv^T += dO^T P,  dk^T += Q^T dS
+// ---------------------------------------------------------------------------
+template <int HD, bool BF, int W>
+__global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p)
+{
+    extern __shared__ __align__(16) unsigned char lds_raw[];
+    constexpr int KS = HD / 16, ROWS = 32 * W;
+    const int cells = packed_grid(p.heads, p.head_sets, p.slots);
+    if ((int)blockIdx.x >= cells) return packed_clear(p, (int)blockIdx.x - cells, p.out, (long long)p.heads * HD);
+    const PackedItem item = packed_item<ROWS>(p, p.heads, true);
+    if (item.n == 0) return;
+    const int w = wave_id(), l = lane_id(), qq = l & 31, h = l >> 5, n = item.n, key_head = item.head / p.group;
+    const int row0 = item.tile * ROWS + 32 * w, row = row0 + qq;
+    const long long begin = item.begin;
+
+    PairTiles<HD, W> tiles(p.k + begin * p.k_token + key_head * p.k_head, p.k_token,
+                           p.v + begin * p.v_token + key_head * p.v_head, p.v_token, lds_raw);
+    const int last_row = min(n, item.tile * ROWS + ROWS) - 1;
+    const int steps = p.causal ? last_row / 64 + 1 : (n + 63) / 64;
+    tiles.request(0, n, 0);
+
+    h8 qop[KS], dop[KS];
+    float delta = 0.f;
+    const long long token = begin + min(row, n - 1);
+    const half_t *q_row = p.q + token * p.q_token + item.head * p.q_head, *g_row = p.dout + token * p.g_token + item.head * p.g_head,
+                 *o_row = p.o + (token * p.heads + item.head) * HD;
+    const float minus_lse = -p.lse[(size_t)item.head * p.tokens + token];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        qop[s] = as_h8(ldg16(q_row + 16 * s + 8 * h));
+        dop[s] = as_h8(ldg16(g_row + 16 * s + 8 * h));
+        const h8 o = as_h8(ldg16(o_row + 16 * s + 8 * h));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) delta += widen_16<BF>(dop[s][j]) * widen_16<BF>(o[j]);
+    }
+    delta += at_lane_xor32(delta);               // the other half of the head dim sits in lane ^ 32
+    if (h == 0 && row < n) p.delta[(size_t)item.head * p.tokens + token] = delta;
+
+    RowTile<HD> dq;
+    clear<HD>(dq);
+    for (int step = 0; step < steps; ++step) {
+        const int k0 = 64 * step;
+        tiles.arrived(step & 1);
+        if (step + 1 < steps) tiles.request(step + 1, n, (step + 1) & 1);
+        if (row0 >= n || (p.causal && k0 > row0 + 31)) continue;
+        const bool masked = k0 + 64 > n || (p.causal && k0 + 63 > row0);
+        const int seen = (p.causal ? min(row, n - 1) : n - 1) - k0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f16v sacc = {0}, dpacc = {0};
+#pragma unroll
+            for (int s = 0; s < KS; ++s) sacc = mfma_16<BF>(tiles.rows(0, u, s), qop[s], sacc);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) dpacc = mfma_16<BF>(tiles.rows(1, u, s), dop[s], dpacc);
+            h8 ds[2];
+            if (masked) {                        // a hidden score has no probability and no gradient, whatever it is
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const float grad = at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus_lse)) * (dpacc[v] - delta);
+                    ds[v >> 3][v & 7] = narrow_16<BF>(32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? 0.f : grad);
+                }
+                tiles.template weigh_masked<BF, false>(0, u, ds, dq, [&](int r) { return 32 * u + r <= seen; });
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v)
+                    ds[v >> 3][v & 7] = narrow_16<BF>(at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus_lse)) * (dpacc[v] - delta));
+                tiles.template weigh<BF>(0, u, ds, dq);
+            }
+        }
+    }
+    __syncthreads();
+    store_token_rows<HD, BF>(dq, p.scale, lds_raw + 64 * HD * w, p.out + ((begin + row0) * p.heads + item.head) * HD,
+                             (long long)p.heads * HD, n - row0);
+}
+
+// Behind the tiles of PairTiles: lse and delta of the 64 queries, per buffer.
+template <int HD, bool BF, int W>
+__global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperands p)
+{
+    extern __shared__ __align__(16) unsigned char lds_raw[];
+    constexpr int KS = HD / 16, ROWS = 32 * W;
+    const int key_heads = p.heads / p.group;
+    const int cells = packed_grid(key_heads, p.head_sets, p.slots);
+    if ((int)blockIdx.x >= cells) {
+        packed_clear(p, (int)blockIdx.x - cells, p.dk, (long long)key_heads * HD);
+        return packed_clear(p, (int)blockIdx.x - cells, p.dv, (long long)key_heads * HD);
+    }
+    const PackedItem item = packed_item<ROWS>(p, key_heads, false);
+    if (item.n == 0) return;
+    const int w = wave_id(), l = lane_id(), kk = l & 31, h = l >> 5, n = item.n;
+    const int key0 = item.tile * ROWS + 32 * w, key = key0 + kk;
+    const long long begin = item.begin, key_token = begin + min(key, n - 1);
+
+    h8 kop[KS], vop[KS];
+    const half_t *k_row = p.k + key_token * p.k_token + item.head * p.k_head, *v_row = p.v + key_token * p.v_token + item.head * p.v_head;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        kop[s] = as_h8(ldg16(k_row + 16 * s + 8 * h));
+        vop[s] = as_h8(ldg16(v_row + 16 * s + 8 * h));
+    }
+    RowTile<HD> dk, dv;
+    clear<HD>(dk);
+    clear<HD>(dv);
+
+    const int first = p.causal ? item.tile * ROWS / 64 : 0, last = (n + 63) / 64, steps = (last - first) * p.group;
+    float *stats = reinterpret_cast<float *>(lds_raw + PairTiles<HD, W>::lds_bytes());       // [2][lse 64, delta 64]
+    const unsigned stats_lds = __builtin_amdgcn_readfirstlane(lds_address(stats));
+    const int head0 = item.head * p.group;
+    PairTiles<HD, W> tiles(p.q + begin * p.q_token + head0 * p.q_head, p.q_token, p.dout + begin * p.g_token + head0 * p.g_head,
+                           p.g_token, lds_raw);
+    const float *stat = (w == 0 ? p.lse : p.delta) + (size_t)head0 * p.tokens + begin;
+    int next = first;                            // of the step requested next, whose head is in the pointers
+    auto request = [&](int buffer) {
+        tiles.request(next, n, buffer);
+        if (w < 2) dma4_gather(stat + min(64 * next + l, n - 1), stats_lds + 512 * buffer + 256 * w);
+        if (++next == last) {
+            next = first;
+            tiles.base[0] += 2 * p.q_head, tiles.base[1] += 2 * p.g_head, stat += p.tokens;
+        }
+    };
+    // fp16 probabilities of long sequences would be subnormal: they travel times 256
+    constexpr float UP = BF ? 1.f : 256.f, DOWN = 1.f / UP, LOG_UP = BF ? 0.f : 8.f;
+    const float ds_scale = p.scale * DOWN;
+    request(0);
+    int q0 = 64 * first;
+    for (int step = 0; step < steps; ++step) {
+        const int buffer = step & 1, at = q0;
+        tiles.arrived(buffer);
+        if (step + 1 < steps) request(buffer ^ 1);
+        q0 = q0 + 64 < 64 * last ? q0 + 64 : 64 * first;
+        if (key0 >= n || (p.causal && at + 63 < key0)) continue;
+        const bool masked = at + 64 > n || (p.causal && at < key0 + 31);
+        const int low = (p.causal ? key : 0) - at, high = n - at;                // queries of the tile that see the key
+        const float *stat_lds = stats + 128 * buffer;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            f16v prob = {0}, dpacc = {0};
+            h8 pop[2], ds[2];
+#pragma unroll
+            for (int s = 0; s < KS; ++s) prob = mfma_16<BF>(tiles.rows(0, u, s), kop[s], prob);
+#pragma unroll
+            for (int s = 0; s < KS; ++s) dpacc = mfma_16<BF>(tiles.rows(1, u, s), vop[s], dpacc);
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f4v ls = *reinterpret_cast<const f4v *>(stat_lds + 32 * u + 8 * g + 4 * h);
+                const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + 64 + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int v = 4 * g + j, r = 32 * u + 8 * g + 4 * h + j;
+                    float pr = at_exp2(__builtin_fmaf(prob[v], p.scale2, LOG_UP - ls[j])), grad = pr * ((dpacc[v] - dl[j]) * ds_scale);
+                    if (masked && (r < low || r >= high)) pr = grad = 0.f;
+                    pop[v >> 3][v & 7] = narrow_16<BF>(pr);
+                    ds[v >> 3][v & 7] = narrow_16<BF>(grad);
+                }
+            }
+            if (masked) {
+                auto sees = [&](int r) { return 32 * u + r >= low && 32 * u + r < high; };
+                tiles.template weigh_masked<BF, false>(0, u, ds, dk, sees);
+                tiles.template weigh_masked<BF, true>(1, u, pop, dv, sees);
+            } else {
+                tiles.template weigh<BF>(0, u, ds, dk);
+                tiles.template weigh<BF>(1, u, pop, dv);
+            }
+        }
+    }
+    __syncthreads();
+    const long long width = (long long)key_heads * HD, out = (begin + key0) * width + (long long)item.head * HD;
+    store_token_rows<HD, BF>(dv, DOWN, lds_raw + 64 * HD * w, p.dv + out, width, n - key0);
+    store_token_rows<HD, BF>(dk, 1.f, lds_raw + 64 * HD * w, p.dk + out, width, n - key0);
+}
+
+// ---- launchers ----------------------------------------------------------------------------------------
+constexpr int PACKED_WAVES = 4;
+
+PackedOperands operands(const PackedArgs &a)
+{
+    PackedOperands p;
+    p.q = (const half_t *)a.q, p.k = (const half_t *)a.k, p.v = (const half_t *)a.v;
+    p.dout = (const half_t *)a.dout, p.o = (const half_t *)a.o;
+    p.out = (half_t *)a.out, p.dk = (half_t *)a.dk, p.dv = (half_t *)a.dv;
+    p.lse = a.lse, p.delta = a.delta;
+    p.offsets = a.offsets;
+    p.tokens = a.tokens, p.sequences = a.sequences, p.heads = a.heads, p.group = a.heads / a.key_heads;
+    p.causal = a.causal;
+    p.scale = a.scale, p.scale2 = a.scale * 1.4426950408889634f;
+    p.q_token = a.q_token, p.q_head = a.q_head, p.k_token = a.k_token, p.k_head = a.k_head;
+    p.v_token = a.v_token, p.v_head = a.v_head, p.g_token = a.g_token, p.g_head = a.g_head;
+    return p;
+}
+
+// a launch gets 64 KB of LDS without asking
+template <class Kernel>
+hipError_t run_walk(Kernel kernel, PackedOperands p, int heads, int waves, size_t lds, hipStream_t st)
+{
+    if (lds > 65536) {
+        const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (err != hipSuccess) return err;
+    }
+    p.head_sets = packed_head_sets(heads);
+    p.slots = packed_slots(p.tokens, p.sequences, 32 * waves);
+    kernel<<<packed_grid(heads, p.head_sets, p.slots) + PACKED_CLEARING, 64 * waves, lds, st>>>(p);
+    return hipGetLastError();
+}
+
+template <int HD, bool BF>
+hipError_t forward(const PackedArgs &a, hipStream_t st)
+{
+    constexpr int W = PACKED_WAVES;
+    return run_walk(packed_forward_kernel<HD, BF, W>, operands(a), a.heads, W, PairTiles<HD, W>::lds_bytes(), st);
+}
+template <int HD, bool BF>
+hipError_t backward(const PackedArgs &a, hipStream_t st)
+{
+    constexpr int W = PACKED_WAVES;
+    const PackedOperands p = operands(a);
+    const hipError_t err = run_walk(packed_rows_kernel<HD, BF, W>, p, a.heads, W, PairTiles<HD, W>::lds_bytes(), st);
+    if (err != hipSuccess || a.dk == nullptr) return err;
+    return run_walk(packed_columns_kernel<HD, BF, W>, p, a.key_heads, W, PairTiles<HD, W>::lds_bytes() + 1024, st);
+}
+
+}  // namespace
+
+hipError_t launch_packed_forward(const PackedArgs &a, hipStream_t st)
+{
+    if (a.head_dim == 64) return a.bf16 ? forward<64, true>(a, st) : forward<64, false>(a, st);
+    return a.bf16 ? forward<128, true>(a, st) : forward<128, false>(a, st);
+}
+
+hipError_t launch_packed_backward(const PackedArgs &a, hipStream_t st)
+{
+    if (a.head_dim == 64) return a.bf16 ? backward<64, true>(a, st) : backward<64, false>(a, st);
+    return a.bf16 ? backward<128, true>(a, st) : backward<128, false>(a, st);
+}
+
+}  // namespace bsa

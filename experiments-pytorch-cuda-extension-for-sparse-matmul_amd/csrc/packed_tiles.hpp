@@ -1,0 +1,243 @@
+// What the walks over packed sequences share: finding the sequence of a workgroup, pairs of operand tiles of 64 tokens that all
+// waves of a workgroup read, products with hidden places, results of 32 tokens on their way out.
+#pragma once
+
+#include "attention_tiles.hpp"
+#include "bsa_device.hpp"
+
+namespace bsa {
+
+struct PackedOperands {
+    const half_t *q, *k, *v, *dout, *o;          // o: the forward result, [T][heads][HD], for the backward walks
+    half_t *out, *dk, *dv;                       // out: the result, or dq; all dense
+    float *lse, *delta;                          // [heads][T]
+    const int32_t *offsets;                      // [sequences + 1]
+    int tokens, sequences, heads, group;         // heads: query heads, group: of them to a key head
+    int head_sets, slots;                        // of a launch: sets of heads that XCDs share, workgroup slots of a head
+    int causal;
+    float scale, scale2;                         // scale2 = scale log2(e)
+    long long q_token, q_head, k_token, k_head, v_token, v_head, g_token, g_head;    // strides in values; g: dout
+};
+
+// Slots of a head: the most workgroups of `rows` tokens that `tokens` in `sequences` can need.
+__host__ __device__ __forceinline__ int packed_slots(int tokens, int sequences, int rows) { return tokens / rows + sequences; }
+// Workgroups that clear the results of tokens outside every sequence, behind those of the slots.
+constexpr int PACKED_CLEARING = 32;
+// Workgroup ids go round the 8 XCDs.  With `sets` = gcd(8, heads) the heads are cut into that many sets of neighbours, each set on
+// 8 / sets XCDs of its own, which take its slots in turn: a key head is read into as few L2s as the balance allows.
+__host__ __forceinline__ int packed_head_sets(int heads) { return heads % 8 == 0 ? 8 : heads % 4 == 0 ? 4 : heads % 2 == 0 ? 2 : 1; }
+__host__ __device__ __forceinline__ int packed_grid(int heads, int sets, int slots)
+{
+    const int share = 8 / sets;
+    return 8 * (heads / sets) * ((slots + share - 1) / share);
+}
+
+struct PackedItem {
+    int head, tile;              // tile: of the sequence, in workgroups' rows
+    int begin, n;                // first token, tokens; n == 0: nothing to do
+};
+
+__device__ __forceinline__ int packed_offset(const PackedOperands &p, int b)
+{
+    const int x = p.offsets[b];
+    return x < 0 ? 0 : x > p.tokens ? p.tokens : x;
+}
+
+// Slot floor(offset / ROWS) + b is the first of sequence b: strictly ascending in b, so 64 lanes search together.  `heads`: of
+// the launch; last_first: the slots are dealt from the highest on (the longest causal rows of a sequence first).
+template <int ROWS>
+__device__ __forceinline__ PackedItem packed_item(const PackedOperands &p, int heads, bool last_first)
+{
+    PackedItem item{0, 0, 0, 0};
+    const int x = (int)(blockIdx.x & 7u), t = (int)(blockIdx.x >> 3);
+    const int share = 8 / p.head_sets, in_set = heads / p.head_sets;
+    item.head = x / share * in_set + t % in_set;
+    int slot = t / in_set * share + x % share;
+    if (slot >= p.slots) return item;
+    if (last_first) slot = p.slots - 1 - slot;
+    const int l = lane_id();
+    int first = 0, count = p.sequences;
+    while (true) {
+        const int stride = (count + 63) / 64, b = first + l * stride;
+        const bool before = b < first + count && packed_offset(p, b) / ROWS + b <= slot;
+        const int seen = __popcll(__builtin_amdgcn_ballot_w64(before));
+        const int skip = (seen > 0 ? seen - 1 : 0) * stride;
+        first += skip;
+        count = count - skip < stride ? count - skip : stride;
+        if (stride == 1) break;
+    }
+    first = __builtin_amdgcn_readfirstlane(first);
+    const int begin = __builtin_amdgcn_readfirstlane(packed_offset(p, first));
+    const int end = __builtin_amdgcn_readfirstlane(packed_offset(p, first + 1));
+    item.tile = slot - (begin / ROWS + first);
+    if (item.tile < 0 || (long long)item.tile * ROWS >= end - begin) return item;
+    item.begin = begin;
+    item.n = end - begin;
+    return item;
+}
+
+// the tokens before the first and behind the last sequence
+__device__ __forceinline__ void packed_clear(const PackedOperands &p, int part, half_t *rows, long long width)
+{
+    const int head = packed_offset(p, 0), tail = packed_offset(p, p.sequences);
+    const long long pieces = width / 8, before = head < tail ? head : tail;
+    auto clear = [&](long long from, long long to) {
+        for (long long i = from * pieces + (long long)part * blockDim.x + threadIdx.x; i < to * pieces;
+             i += (long long)PACKED_CLEARING * blockDim.x)
+            stg16(rows + 8 * i, make_uint4(0, 0, 0, 0));
+    };
+    clear(0, before);
+    clear(tail, p.tokens);
+}
+
+// acc[t] += columns 32 t .. of a 32-row tile, its rows weighted by op
+template <int HD, bool BF>
+__device__ __forceinline__ void weigh_tile(const TileReader &rd, unsigned tile, const h8 (&op)[2], RowTile<HD> &acc)
+{
+#pragma unroll
+    for (int t = 0; t < HD / 32; ++t)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) acc[t] = mfma_16<BF>(rd.columns(tile, t, s), op[s], acc[t]);
+}
+
+// The same where some weights are zero because their place is hidden: an infinity or a NaN in a token must not reach the results
+// of those that do not see it, and zero times it would be NaN.  Such values are left out of the products and added to the
+// results of the lanes for which sees(row of the tile) holds, as themselves where the weights are probabilities, else as NaN.
+template <int HD, bool BF, bool PROBABILITIES, class Sees>
+__device__ __forceinline__ void weigh_tile_masked(const TileReader &rd, unsigned tile, const h8 (&op)[2], RowTile<HD> &acc, Sees sees)
+{
+    typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+    constexpr unsigned short INFINITE = BF ? 0x7F80 : 0x7C00;
+    us8 top = 0;
+#pragma unroll
+    for (int t = 0; t < HD / 32; ++t)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+            top = __builtin_elementwise_max(top, (us8)(__builtin_bit_cast(us8, rd.columns(tile, t, s)) & (unsigned short)0x7FFF));
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) finite = finite && top[j] < INFINITE;
+    if (__builtin_amdgcn_ballot_w64(!finite) == 0ull) {
+        weigh_tile<HD, BF>(rd, tile, op, acc);
+        return;
+    }
+#pragma unroll
+    for (int t = 0; t < HD / 32; ++t)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            us8 x = __builtin_bit_cast(us8, rd.columns(tile, t, s));
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = (x[j] & 0x7FFF) < INFINITE ? x[j] : (unsigned short)0;
+            acc[t] = mfma_16<BF>(__builtin_bit_cast(h8, x), op[s], acc[t]);
+        }
+    const int h = lane_id() >> 5;
+    typedef const half_t __attribute__((address_space(3))) *lds_half;
+    const unsigned first = (unsigned)__builtin_amdgcn_readfirstlane((int)(rd.row[0] - (unsigned)get_panel_addr(lane_id(), 0))) + tile;
+    for (int r = 0; r < 32; ++r) {
+        const bool seen = sees(r);
+#pragma unroll
+        for (int t = 0; t < HD / 32; ++t)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int d = 32 * t + 8 * (v >> 2) + 4 * h + (v & 3), x = d & 63;
+                const half_t raw = *(lds_half)(uintptr_t)(first + 4096 * (d >> 6) + 128 * r + 16 * ((x >> 3) ^ panel_swizzle(r)) + 2 * (x & 7));
+                const float value = widen_16<BF>(raw);
+                if (seen && (__builtin_bit_cast(unsigned short, raw) & 0x7FFF) >= INFINITE)
+                    acc[t][v] += PROBABILITIES ? value : value - value;
+            }
+    }
+}
+
+// Two operands (K and V, or Q and dO) in tiles of 64 tokens, double buffered, read by all W waves.  LDS of a buffer: the first
+// operand's two 32-row tiles (TileRequests' panels), then the second's.  A wave fetches HD / 8 / W kilobytes of each.
+template <int HD, int W>
+struct PairTiles {
+    static constexpr int TILE = 64 * HD, BUFFER = 4 * TILE, REQUESTS = HD / 8 / W;
+    TileReader rd;
+    const unsigned char *base[2];
+    long long stride[2];         // bytes between tokens
+    unsigned lds, row;           // row: of this lane inside a 32-row tile
+    unsigned piece;
+    int wave;
+    __device__ __forceinline__ PairTiles(const half_t *a, long long a_token, const half_t *b, long long b_token, unsigned char *lds_raw)
+        : rd(lds_raw + BUFFER)
+    {
+        wave = wave_id();
+        const int l = lane_id(), chunk = wave & 3;
+        base[0] = (const unsigned char *)a, base[1] = (const unsigned char *)b;
+        stride[0] = 2 * a_token, stride[1] = 2 * b_token;
+        lds = __builtin_amdgcn_readfirstlane(lds_address(lds_raw));
+        row = 8 * chunk + (l >> 3);
+        piece = 16 * panel_src_piece(l, chunk);
+    }
+    static constexpr size_t lds_bytes() { return 2 * (size_t)BUFFER; }
+    // tokens 64 step .. + 63 of n, those from n on as token n - 1 (what they give is hidden)
+    __device__ __forceinline__ void request(int step, int n, int buffer) const
+    {
+        const unsigned last = (unsigned)(n - 1 - 64 * step);
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            const unsigned char *from = base[o] + (long long)64 * step * stride[o];
+#pragma unroll
+            for (int i = 0; i < REQUESTS; ++i) {
+                const int rq = i * W + wave, sub = rq / (HD / 16), u = rq % (HD / 16) / 4, c = rq & 3;
+                unsigned r = 32 * sub + row;
+                r = r < last ? r : last;
+                dma16(from, r * (unsigned)stride[o] + 128 * u + piece,
+                      lds + (unsigned)(buffer * BUFFER + o * 2 * TILE + sub * TILE + 4096 * u + 1024 * c));
+            }
+        }
+    }
+    // every wave's part of the tile requested last has arrived, and all waves are done with the one before; buffers change
+    __device__ __forceinline__ void arrived(int buffer)
+    {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const unsigned d = buffer ? (unsigned)BUFFER : 0u - (unsigned)BUFFER;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) rd.row[s] += d;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) rd.tr[x][0] += d, rd.tr[x][1] += d;
+    }
+    __device__ __forceinline__ h8 rows(int operand, int u, int s) const { return rd.rows((unsigned)((2 * operand + u) * TILE), s); }
+    __device__ __forceinline__ h8 columns(int operand, int u, int t, int s) const
+    {
+        return rd.columns((unsigned)((2 * operand + u) * TILE), t, s);
+    }
+    template <bool BF>
+    __device__ __forceinline__ void weigh(int operand, int u, const h8 (&op)[2], RowTile<HD> &acc) const
+    {
+        weigh_tile<HD, BF>(rd, (unsigned)((2 * operand + u) * TILE), op, acc);
+    }
+    template <bool BF, bool PROBABILITIES, class Sees>
+    __device__ __forceinline__ void weigh_masked(int operand, int u, const h8 (&op)[2], RowTile<HD> &acc, Sees sees) const
+    {
+        weigh_tile_masked<HD, BF, PROBABILITIES>(rd, (unsigned)((2 * operand + u) * TILE), op, acc, sees);
+    }
+};
+
+// 32 result rows `stride` values apart, of which the first `valid` are stored; through 64 HD bytes of LDS, so that they leave
+// as whole lines
+template <int HD, bool BF>
+__device__ __forceinline__ void store_token_rows(const RowTile<HD> &acc, float mul, unsigned char *scratch, half_t *dst,
+                                                 long long stride, int valid)
+{
+    const int l = lane_id(), row = l & 31, h = l >> 5;
+    wave_lds_fence();
+#pragma unroll
+    for (int t = 0; t < HD / 32; ++t)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            h4 o;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = narrow_16<BF>(acc[t][4 * g + j] * mul);
+            *reinterpret_cast<h4 *>(scratch + out_row_addr(HD, row, 4 * t + g, h)) = o;
+        }
+    wave_lds_fence();
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j) {
+        const int slot = l + 64 * j, r = slot / (HD / 8), p = slot % (HD / 8);
+        if (r < valid) stg16(dst + r * stride + 8 * p, *reinterpret_cast<const uint4 *>(scratch + out_row_addr(HD, r, p, 0)));
+    }
+}
+
+}  // namespace bsa

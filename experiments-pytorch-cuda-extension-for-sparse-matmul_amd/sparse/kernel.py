@@ -18,7 +18,7 @@ import torch  # noqa: F401  (loads the HIP runtime the library binds to)
 _CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "csrc")
 LIBRARY_PATH = os.path.join(_CSRC, "libbsa_hip.so")
 
-BSA_F32, BSA_F16, BSA_BF16 = 0, 1, 2
+BSA_F32, BSA_F16, BSA_BF16, BSA_I8, BSA_E4M3 = 0, 1, 2, 3, 4
 BSA_SDD, BSA_DSD, BSA_DDS = 0, 1, 2
 BSA_OK, BSA_ERR_INVALID, BSA_ERR_LAUNCH, BSA_ERR_UNSUPPORTED = 0, -1, -2, -3
 MODES = {"sdd": BSA_SDD, "dsd": BSA_DSD, "dds": BSA_DDS}
@@ -61,6 +61,12 @@ SIGNATURES = {
                                                         _vp, ctypes.c_size_t, _i, _i, _i, _i, _i, _f, _i, _vp]),
     "bsa_attention_gradients": (_i, [_i] + [_vp] * 10 + [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i,
                                                         _vp, ctypes.c_size_t, _i, _i, _i, _i, _i, _f, _i, _vp]),
+    "bsa_packed_attention_forward": (_i, [_i] + [_vp] * 6 + [_i] * 5 + [_vp, _f, _i, _vp]),
+    "bsa_packed_attention_backward": (_i, [_i] + [_vp] * 11 + [_i] * 5 + [_vp, _f, _i, _vp]),
+    "bsa_cache_write": (_i, [_i, _i] + [_vp] * 7 + [_i] * 5 + [_vp, _vp]),
+    "bsa_cache_read": (_i, [_i, _i] + [_vp] * 7 + [_i] * 5 + [_vp]),
+    "bsa_cached_attention_workspace_bytes": (ctypes.c_size_t, [_i] * 7),
+    "bsa_cached_attention": (_i, [_i, _i] + [_vp] * 11 + [_i] * 9 + [_vp, _f, _vp, ctypes.c_size_t, _vp]),
 }
 
 

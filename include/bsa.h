@@ -58,7 +58,7 @@ enum bsa_status {
 };
 
 /* Library version, major * 10000 + minor * 100 + patch; the one these declarations are of. */
-#define BSA_VERSION 100
+#define BSA_VERSION 200
 int bsa_version(void);
 
 /* Message of the last failure on this thread ("" if none). Never NULL. */
@@ -400,6 +400,71 @@ int bsa_weight_grad_shares(int mask_rows, int mask_cols, int tokens);
 int bsa_weight_grad(int dtype, const void *a, const void *b, void *out, const int32_t *row_blocks,
                     const int32_t *row_offsets, int mask_rows, int mask_cols, int nnz, int tokens,
                     int shares, float *parts, size_t parts_bytes, void *stream);
+
+/* ---- sequences packed along the tokens ------------------------------------
+ * Attention inside every sequence of a packed batch, each query head over the key head it shares with
+ * heads / key_heads - 1 others (query head h reads key head h / (heads / key_heads)):
+ *   out[i] = softmax(scale q[i] k^T over the tokens of its sequence; with `causal` over those up to i) v
+ *   q, dout          [tokens, heads, head_dim],  k, v [tokens, key_heads, head_dim], with strides
+ *   out, dq          [tokens, heads, head_dim], dense;  dk, dv [tokens, key_heads, head_dim], dense
+ *   lse, delta_ws    float [heads, tokens]: log2 of each row's sum of exponentials (may be NULL in the forward call),
+ *                    scratch of the backward call
+ *   offsets          device int32[sequences + 1]: sequence b is tokens offsets[b] .. offsets[b + 1] - 1.  They stay on the
+ *                    device.  Ascending; sequences may be empty.  Tokens in front of the first and behind the last
+ *                    sequence get zeros in every result and are not read.  Values outside [0, tokens] are taken as the nearer end;
+ *                    of offsets that descend or overlap the results are unspecified.
+ *   strides          host int64: values between tokens and between heads of q, k, v (and dout); multiples of 8, the head
+ *                    dim itself is contiguous; at most 2^24 between tokens
+ * Results are the same bits in every call: each is summed in one order, by one workgroup.  An infinity or a NaN in a token
+ * reaches the results of the tokens that see it, not of others.
+ * fp16 and bf16, head_dim 64 or 128; operands start at multiples of 16 bytes.  dk_out and dv_out both NULL: dq alone.
+ */
+int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, float *lse,
+                                 const int32_t *offsets, int tokens, int sequences, int heads, int key_heads, int head_dim,
+                                 const int64_t *strides, float scale, int causal, void *stream);
+int bsa_packed_attention_backward(int dtype, const void *q, const void *k, const void *v, const void *dout, const void *out,
+                                  const float *lse, float *delta_ws, void *dq_out, void *dk_out, void *dv_out,
+                                  const int32_t *offsets, int tokens, int sequences, int heads, int key_heads, int head_dim,
+                                  const int64_t *strides, float scale, int causal, void *stream);
+
+/* ---- a paged cache of keys and values --------------------------------------
+ * keys, values   [pages, heads, page, head_dim] of fp16, bf16, BSA_I8 or BSA_E4M3
+ * *_scales       float [pages, heads, page], of the 8-bit types (NULL otherwise)
+ * slot           page * page size + place; page is 32, 64, 128 or 256 tokens; head_dim 64 or 128
+ *
+ * bsa_cache_write stores row t of k, v [tokens, heads, head_dim] (16-bit, strides as above) at slots[t] (device int32):
+ *   scale = max |x| / top,  value = x top / max |x| to the nearest, ties to even;  top = 127 (int8), 448 (e4m3)
+ * A row of zeros has scale 0; a row with an infinity or a NaN has scale NaN and values 0.  Rows whose slot is negative or
+ * behind the cache are left out.  No two rows of a call may have the same slot.
+ * bsa_cache_read gives value * scale of the slots, rounded once to fp32, fp16 or bf16, dense [tokens, heads, head_dim]; zeros for a slot
+ * that is negative or behind the cache.  A 16-bit cache takes rows of its own type and holds them as they are.
+ */
+#define BSA_I8 3
+#define BSA_E4M3 4
+int bsa_cache_write(int dtype, int cache_dtype, const void *k, const void *v, const int32_t *slots, void *keys, void *values,
+                    float *key_scales, float *value_scales, int tokens, int heads, int head_dim, int pages, int page,
+                    const int64_t *strides, void *stream);
+int bsa_cache_read(int dtype, int cache_dtype, const void *keys, const void *values, const float *key_scales,
+                   const float *value_scales, const int32_t *slots, void *k_out, void *v_out, int tokens, int heads, int head_dim,
+                   int pages, int page, void *stream);
+
+/* Attention of `drafts` new tokens of every sequence over what a cache holds of it and over one another:
+ *   q [batch, drafts, heads, head_dim], k, v [batch, drafts, key_heads, head_dim] with strides (batch, token, head of each);
+ *   out [batch, drafts, heads, head_dim], dense
+ *   table     device int32 [batch, width]: page numbers of a sequence;  lengths: device int32 [batch], tokens it has in the
+ *             cache (taken as 0 if negative, as width * page if larger).  Tokens on a page outside [0, pages) are not seen; what a
+ *             page holds behind the length is not looked at.
+ *   tree      device uint8 [batch, drafts, drafts], or [drafts, drafts] with tree_shared: nonzero where new token i sees new
+ *             token j; NULL: j <= i.  A token that sees nothing at all gets zeros.
+ * At most 1024 drafts.  `workspace` (bsa_cached_attention_workspace_bytes, any contents) takes the chunks of long sequences; the launches
+ * that use one at a time are to be ordered.  Results are the same bits in every call with the same lengths.
+ */
+size_t bsa_cached_attention_workspace_bytes(int batch, int drafts, int heads, int key_heads, int head_dim, int width, int page);
+int bsa_cached_attention(int dtype, int cache_dtype, const void *q, const void *k, const void *v, void *out, const void *keys,
+                         const void *values, const float *key_scales, const float *value_scales, const int32_t *table,
+                         const int32_t *lengths, const uint8_t *tree, int tree_shared, int batch, int drafts, int heads,
+                         int key_heads, int head_dim, int pages, int page, int width, const int64_t *strides, float scale,
+                         void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
