@@ -45,6 +45,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
     const half_t *q_row = p.q + (begin + min(row, n - 1)) * p.q_token + item.head * p.q_head;
 #pragma unroll
     for (int s = 0; s < KS; ++s) qop[s] = as_h8(ldg16(q_row + 16 * s + 8 * h));
+    loaded(qop);
 
     // reference point of the query (both lane halves agree), minus it (0 while nothing was seen), this half's sum;
     // fresh: no query of the wave has a reference point yet
@@ -59,11 +60,16 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
         if (step + 1 < steps) tiles.request(step + 1, n, (step + 1) & 1);
         if (row0 >= n || (p.causal && k0 > row0 + 31)) continue;
         f16v sacc[2];
+        {
+            h8 kop[2][KS];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            sacc[u] = f16v{0};
+            for (int u = 0; u < 2; ++u) read_rows<HD>(tiles.rd, tiles.at(0, u), kop[u]);
+            issue_order();
 #pragma unroll
-            for (int s = 0; s < KS; ++s) sacc[u] = mfma_16<BF>(tiles.rows(0, u, s), qop[s], sacc[u]);
+            for (int u = 0; u < 2; ++u) {
+                sacc[u] = f16v{0};
+                product<BF>(kop[u], qop, sacc[u]);
+            }
         }
         const bool masked = k0 + 64 > n || (p.causal && k0 + 63 > row0);
         const int seen = (p.causal ? min(row, n - 1) : n - 1) - k0;              // last key of the tile that the query sees
@@ -76,6 +82,10 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
                 for (int v = 0; v < 16; ++v)
                     sacc[u][v] = 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? NEG_INF : sacc[u][v] * p.scale2;
         }
+        h8 vop[2][HD / 32][2];                   // on their way while the exponentials are taken
+#pragma unroll
+        for (int u = 0; u < 2; ++u) read_columns<HD>(tiles.rd, tiles.at(1, u), vop[u]);
+        issue_order();
         float psum;
         h8 pop[2][2];
         auto exponentials = [&]() {
@@ -114,10 +124,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
         }
         lsum += psum;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            if (masked) tiles.template weigh_masked<BF, true>(1, u, pop[u], oacc, [&](int r) { return 32 * u + r <= seen; });
-            else tiles.template weigh<BF>(1, u, pop[u], oacc);
-        }
+        for (int u = 0; u < 2; ++u)
+            weigh<HD, BF, true>(tiles.rd, tiles.at(1, u), vop[u], pop[u], oacc, masked, [&](int r) { return 32 * u + r <= seen; });
     }
     lsum += at_lane_xor32(lsum);                 // both halves used the same reference point
     const bool any = lsum > 0.f || lsum != lsum;
@@ -172,6 +180,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
     }
     delta += at_lane_xor32(delta);               // the other half of the head dim sits in lane ^ 32
     if (h == 0 && row < n) p.delta[(size_t)item.head * p.tokens + token] = delta;
+    loaded(qop);
+    loaded(dop);
 
     RowTile<HD> dq;
     clear<HD>(dq);
@@ -185,24 +195,25 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             f16v sacc = {0}, dpacc = {0};
-#pragma unroll
-            for (int s = 0; s < KS; ++s) sacc = mfma_16<BF>(tiles.rows(0, u, s), qop[s], sacc);
-#pragma unroll
-            for (int s = 0; s < KS; ++s) dpacc = mfma_16<BF>(tiles.rows(1, u, s), dop[s], dpacc);
-            h8 ds[2];
-            if (masked) {                        // a hidden score has no probability and no gradient, whatever it is
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const float grad = at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus_lse)) * (dpacc[v] - delta);
-                    ds[v >> 3][v & 7] = narrow_16<BF>(32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? 0.f : grad);
-                }
-                tiles.template weigh_masked<BF, false>(0, u, ds, dq, [&](int r) { return 32 * u + r <= seen; });
-            } else {
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    ds[v >> 3][v & 7] = narrow_16<BF>(at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus_lse)) * (dpacc[v] - delta));
-                tiles.template weigh<BF>(0, u, ds, dq);
+            h8 ktr[HD / 32][2], ds[2];
+            {
+                h8 kop[KS], vop[KS];
+                read_rows<HD>(tiles.rd, tiles.at(0, u), kop);
+                read_rows<HD>(tiles.rd, tiles.at(1, u), vop);
+                issue_order();
+                product<BF>(kop, qop, sacc);
+                product<BF>(vop, dop, dpacc);
             }
+            read_columns<HD>(tiles.rd, tiles.at(0, u), ktr);
+            issue_order();
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {       // a hidden score has no probability and no gradient, whatever it is
+                float grad = at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus_lse)) * (dpacc[v] - delta);
+                if (masked && 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h) grad = 0.f;
+                ds[v >> 3][v & 7] = narrow_16<BF>(grad);
+            }
+            weigh<HD, BF, false>(tiles.rd, tiles.at(0, u), ktr, ds, dq, masked, [&](int r) { return 32 * u + r <= seen; });
+            issue_order();
         }
     }
     __syncthreads();
@@ -235,6 +246,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperand
         kop[s] = as_h8(ldg16(k_row + 16 * s + 8 * h));
         vop[s] = as_h8(ldg16(v_row + 16 * s + 8 * h));
     }
+    loaded(kop);
+    loaded(vop);
     RowTile<HD> dk, dv;
     clear<HD>(dk);
     clear<HD>(dv);
@@ -273,31 +286,49 @@ __global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperand
         for (int u = 0; u < 2; ++u) {
             f16v prob = {0}, dpacc = {0};
             h8 pop[2], ds[2];
+            // four operands of a tile in registers at a time
+            auto product_of_rows = [&](int operand, const h8 (&other)[KS], f16v &acc) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) prob = mfma_16<BF>(tiles.rows(0, u, s), kop[s], prob);
+                for (int s0 = 0; s0 < KS; s0 += 4) {
+                    h8 op[4];
 #pragma unroll
-            for (int s = 0; s < KS; ++s) dpacc = mfma_16<BF>(tiles.rows(1, u, s), vop[s], dpacc);
+                    for (int s = 0; s < 4; ++s) op[s] = tiles.rd.rows(tiles.at(operand, u), s0 + s);
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) acc = mfma_16<BF>(op[s], other[s0 + s], acc);
+                    if (KS > 4) issue_order();
+                }
+            };
+            product_of_rows(0, kop, prob);
+            issue_order();
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f4v ls = *reinterpret_cast<const f4v *>(stat_lds + 32 * u + 8 * g + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int v = 4 * g + j, r = 32 * u + 8 * g + 4 * h + j;
+                    prob[v] = at_exp2(__builtin_fmaf(prob[v], p.scale2, LOG_UP - ls[j]));
+                    if (masked && (r < low || r >= high)) prob[v] = 0.f;
+                    pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
+                }
+            }
+            issue_order();
+            product_of_rows(1, vop, dpacc);
+            issue_order();
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
                 const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + 64 + 32 * u + 8 * g + 4 * h);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int v = 4 * g + j, r = 32 * u + 8 * g + 4 * h + j;
-                    float pr = at_exp2(__builtin_fmaf(prob[v], p.scale2, LOG_UP - ls[j])), grad = pr * ((dpacc[v] - dl[j]) * ds_scale);
-                    if (masked && (r < low || r >= high)) pr = grad = 0.f;
-                    pop[v >> 3][v & 7] = narrow_16<BF>(pr);
-                    ds[v >> 3][v & 7] = narrow_16<BF>(grad);
+                    const float grad = prob[v] * ((dpacc[v] - dl[j]) * ds_scale);
+                    ds[v >> 3][v & 7] = narrow_16<BF>(masked && (r < low || r >= high) ? 0.f : grad);
                 }
             }
-            if (masked) {
-                auto sees = [&](int r) { return 32 * u + r >= low && 32 * u + r < high; };
-                tiles.template weigh_masked<BF, false>(0, u, ds, dk, sees);
-                tiles.template weigh_masked<BF, true>(1, u, pop, dv, sees);
-            } else {
-                tiles.template weigh<BF>(0, u, ds, dk);
-                tiles.template weigh<BF>(1, u, pop, dv);
-            }
+            issue_order();
+            auto sees = [&](int r) { return 32 * u + r >= low && 32 * u + r < high; };
+            weigh_tile<HD, BF, false>(tiles.rd, tiles.at(0, u), ds, dk, masked, sees);
+            weigh_tile<HD, BF, true>(tiles.rd, tiles.at(1, u), pop, dv, masked, sees);
+            issue_order();
         }
     }
     __syncthreads();

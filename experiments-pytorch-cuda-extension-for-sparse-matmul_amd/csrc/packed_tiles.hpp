@@ -90,62 +90,128 @@ __device__ __forceinline__ void packed_clear(const PackedOperands &p, int part, 
     clear(tail, p.tokens);
 }
 
-// acc[t] += columns 32 t .. of a 32-row tile, its rows weighted by op
-template <int HD, bool BF>
-__device__ __forceinline__ void weigh_tile(const TileReader &rd, unsigned tile, const h8 (&op)[2], RowTile<HD> &acc)
+// Keeps what is above in front of what is below: operands are requested from LDS before the work that hides their latency.
+__device__ __forceinline__ void issue_order() { __builtin_amdgcn_sched_barrier(0); }
+// Values loaded in front of a loop have arrived: otherwise the compiler waits for them inside it, and with them for the loads to
+// LDS that it does not know of.
+template <int N>
+__device__ __forceinline__ void loaded(h8 (&op)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(op[i]));
+}
+
+template <int HD>
+__device__ __forceinline__ void read_rows(const TileReader &rd, unsigned tile, h8 (&op)[HD / 16])
+{
+#pragma unroll
+    for (int s = 0; s < HD / 16; ++s) op[s] = rd.rows(tile, s);
+}
+template <int HD>
+__device__ __forceinline__ void read_columns(const TileReader &rd, unsigned tile, h8 (&op)[HD / 32][2])
 {
 #pragma unroll
     for (int t = 0; t < HD / 32; ++t)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) acc[t] = mfma_16<BF>(rd.columns(tile, t, s), op[s], acc[t]);
+        for (int s = 0; s < 2; ++s) op[t][s] = rd.columns(tile, t, s);
 }
-
-// The same where some weights are zero because their place is hidden: an infinity or a NaN in a token must not reach the results
-// of those that do not see it, and zero times it would be NaN.  Such values are left out of the products and added to the
-// results of the lanes for which sees(row of the tile) holds, as themselves where the weights are probabilities, else as NaN.
-template <int HD, bool BF, bool PROBABILITIES, class Sees>
-__device__ __forceinline__ void weigh_tile_masked(const TileReader &rd, unsigned tile, const h8 (&op)[2], RowTile<HD> &acc, Sees sees)
+template <bool BF, int N>
+__device__ __forceinline__ void product(const h8 (&a)[N], const h8 (&b)[N], f16v &acc)
+{
+#pragma unroll
+    for (int s = 0; s < N; ++s) acc = mfma_16<BF>(a[s], b[s], acc);
+}
+// Products with some weights zero because their place is hidden: an infinity or a NaN in a token must not reach the results of
+// those that do not see it, and zero times it would be NaN.  Where anything is hidden the operands are looked at; such values
+// are left out of the products, and add_not_finite adds them to the results of the lanes for which sees(row of the tile) holds, as
+// themselves where the weights are probabilities, else as NaN.
+template <bool BF, int T>
+__device__ __forceinline__ bool take_out_not_finite(h8 (&columns)[T][2])
 {
     typedef unsigned short us8 __attribute__((ext_vector_type(8)));
     constexpr unsigned short INFINITE = BF ? 0x7F80 : 0x7C00;
     us8 top = 0;
 #pragma unroll
-    for (int t = 0; t < HD / 32; ++t)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int s = 0; s < 2; ++s)
-            top = __builtin_elementwise_max(top, (us8)(__builtin_bit_cast(us8, rd.columns(tile, t, s)) & (unsigned short)0x7FFF));
+            top = __builtin_elementwise_max(top, (us8)(__builtin_bit_cast(us8, columns[t][s]) & (unsigned short)0x7FFF));
     bool finite = true;
 #pragma unroll
     for (int j = 0; j < 8; ++j) finite = finite && top[j] < INFINITE;
-    if (__builtin_amdgcn_ballot_w64(!finite) == 0ull) {
-        weigh_tile<HD, BF>(rd, tile, op, acc);
-        return;
-    }
+    if (__builtin_amdgcn_ballot_w64(!finite) == 0ull) return false;
 #pragma unroll
-    for (int t = 0; t < HD / 32; ++t)
+    for (int t = 0; t < T; ++t)
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-            us8 x = __builtin_bit_cast(us8, rd.columns(tile, t, s));
+            us8 x = __builtin_bit_cast(us8, columns[t][s]);
 #pragma unroll
             for (int j = 0; j < 8; ++j) x[j] = (x[j] & 0x7FFF) < INFINITE ? x[j] : (unsigned short)0;
-            acc[t] = mfma_16<BF>(__builtin_bit_cast(h8, x), op[s], acc[t]);
+            columns[t][s] = __builtin_bit_cast(h8, x);
         }
+    return true;
+}
+template <int HD, bool BF, bool PROBABILITIES, class Sees>
+__device__ __forceinline__ void add_not_finite(const TileReader &rd, unsigned tile, RowTile<HD> &acc, Sees sees)
+{
+    constexpr unsigned short INFINITE = BF ? 0x7F80 : 0x7C00;
     const int h = lane_id() >> 5;
-    typedef const half_t __attribute__((address_space(3))) *lds_half;
+    typedef const h4 __attribute__((address_space(3))) *lds_h4;
     const unsigned first = (unsigned)__builtin_amdgcn_readfirstlane((int)(rd.row[0] - (unsigned)get_panel_addr(lane_id(), 0))) + tile;
+#pragma unroll 1
     for (int r = 0; r < 32; ++r) {
         const bool seen = sees(r);
 #pragma unroll
-        for (int t = 0; t < HD / 32; ++t)
+        for (int t = 0; t < HD / 32; ++t) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int d = 32 * t + 8 * (v >> 2) + 4 * h + (v & 3), x = d & 63;
-                const half_t raw = *(lds_half)(uintptr_t)(first + 4096 * (d >> 6) + 128 * r + 16 * ((x >> 3) ^ panel_swizzle(r)) + 2 * (x & 7));
-                const float value = widen_16<BF>(raw);
-                if (seen && (__builtin_bit_cast(unsigned short, raw) & 0x7FFF) >= INFINITE)
-                    acc[t][v] += PROBABILITIES ? value : value - value;
+            for (int g = 0; g < 4; ++g) {
+                const int piece = 4 * (t & 1) + g;
+                const h4 raw = *(lds_h4)(uintptr_t)(first + 4096 * (t / 2) + 128 * r + 16 * (piece ^ panel_swizzle(r)) + 8 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const half_t one = raw[j];   // a bit cast of a vector's element itself takes the first one
+                    const float value = widen_16<BF>(one);
+                    if (seen && (__builtin_bit_cast(unsigned short, one) & 0x7FFF) >= INFINITE)
+                        acc[t][4 * g + j] += PROBABILITIES ? value : value - value;
+                }
             }
+            issue_order();
+        }
     }
+}
+
+// acc[t] += columns 32 t .. of a 32-row tile, its rows weighted by op; the columns have been read
+template <int HD, bool BF, bool PROBABILITIES, class Sees>
+__device__ __forceinline__ void weigh(const TileReader &rd, unsigned tile, h8 (&columns)[HD / 32][2], const h8 (&op)[2],
+                                      RowTile<HD> &acc, bool hidden, Sees sees)
+{
+    const bool out = hidden && take_out_not_finite<BF>(columns);
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int t = 0; t < HD / 32; ++t) acc[t] = mfma_16<BF>(columns[t][s], op[s], acc[t]);
+    if (out) add_not_finite<HD, BF, PROBABILITIES>(rd, tile, acc, sees);
+}
+// the same, 64 columns read at a time
+template <int HD, bool BF, bool PROBABILITIES, class Sees>
+__device__ __forceinline__ void weigh_tile(const TileReader &rd, unsigned tile, const h8 (&op)[2], RowTile<HD> &acc, bool hidden, Sees sees)
+{
+    bool out = false;
+#pragma unroll
+    for (int t0 = 0; t0 < HD / 32; t0 += 2) {
+        h8 tr[2][2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) tr[t][s] = rd.columns(tile, t0 + t, s);
+        if (hidden && take_out_not_finite<BF>(tr)) out = true;
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) acc[t0 + t] = mfma_16<BF>(tr[t][s], op[s], acc[t0 + t]);
+        if (HD > 64) issue_order();
+    }
+    if (out) add_not_finite<HD, BF, PROBABILITIES>(rd, tile, acc, sees);
 }
 
 // Two operands (K and V, or Q and dO) in tiles of 64 tokens, double buffered, read by all W waves.  LDS of a buffer: the first
@@ -198,21 +264,8 @@ struct PairTiles {
 #pragma unroll
         for (int x = 0; x < 2; ++x) rd.tr[x][0] += d, rd.tr[x][1] += d;
     }
-    __device__ __forceinline__ h8 rows(int operand, int u, int s) const { return rd.rows((unsigned)((2 * operand + u) * TILE), s); }
-    __device__ __forceinline__ h8 columns(int operand, int u, int t, int s) const
-    {
-        return rd.columns((unsigned)((2 * operand + u) * TILE), t, s);
-    }
-    template <bool BF>
-    __device__ __forceinline__ void weigh(int operand, int u, const h8 (&op)[2], RowTile<HD> &acc) const
-    {
-        weigh_tile<HD, BF>(rd, (unsigned)((2 * operand + u) * TILE), op, acc);
-    }
-    template <bool BF, bool PROBABILITIES, class Sees>
-    __device__ __forceinline__ void weigh_masked(int operand, int u, const h8 (&op)[2], RowTile<HD> &acc, Sees sees) const
-    {
-        weigh_tile_masked<HD, BF, PROBABILITIES>(rd, (unsigned)((2 * operand + u) * TILE), op, acc, sees);
-    }
+    // of subtile u of an operand, as TileReader's tile
+    static constexpr unsigned at(int operand, int u) { return (unsigned)((2 * operand + u) * TILE); }
 };
 
 // 32 result rows `stride` values apart, of which the first `valid` are stored; through 64 HD bytes of LDS, so that they leave
