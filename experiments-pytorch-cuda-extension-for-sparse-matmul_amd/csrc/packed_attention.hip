@@ -28,7 +28,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
     constexpr int KS = HD / 16, ROWS = 32 * W;
     const int cells = packed_grid(p.heads, p.head_sets, p.slots);
     if ((int)blockIdx.x >= cells) return packed_clear(p, (int)blockIdx.x - cells, p.out, (long long)p.heads * HD);
-    const PackedItem item = packed_item<ROWS>(p, p.heads, true);
+    const PackedItem item = packed_item<ROWS>(p, p.heads, false);
     if (item.n == 0) return;
     const int w = wave_id(), l = lane_id(), qq = l & 31, h = l >> 5, n = item.n, key_head = item.head / p.group;
     const int row0 = item.tile * ROWS + 32 * w, row = row0 + qq;                 // rows and keys count from the sequence's start
@@ -39,7 +39,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
                            p.v + begin * p.v_token + key_head * p.v_head, p.v_token, lds_raw);
     const int last_row = min(n, item.tile * ROWS + ROWS) - 1;
     const int steps = p.causal ? last_row / 64 + 1 : (n + 63) / 64;
-    tiles.request(0, n, 0);
+    tiles.request(0, 0, n, 0);
 
     h8 qop[KS];
     const half_t *q_row = p.q + (begin + min(row, n - 1)) * p.q_token + item.head * p.q_head;
@@ -47,63 +47,36 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
     for (int s = 0; s < KS; ++s) qop[s] = as_h8(ldg16(q_row + 16 * s + 8 * h));
     loaded(qop);
 
-    // reference point of the query (both lane halves agree), minus it (0 while nothing was seen), this half's sum;
-    // fresh: no query of the wave has a reference point yet
+    // reference point of the query (both lane halves agree), minus it (0 while nothing was seen), this half's sum
     float m = NEG_INF, minus_m = 0.f, lsum = 0.f;
-    bool fresh = true;
     RowTile<HD> oacc;
     clear<HD>(oacc);
 
-    for (int step = 0; step < steps; ++step) {
-        const int k0 = 64 * step;
-        tiles.arrived(step & 1);
-        if (step + 1 < steps) tiles.request(step + 1, n, (step + 1) & 1);
-        if (row0 >= n || (p.causal && k0 > row0 + 31)) continue;
-        f16v sacc[2];
-        {
-            h8 kop[2][KS];
+    auto scores = [&](int buffer, f16v (&sacc)[2]) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) read_rows<HD>(tiles.rd, tiles.at(0, u), kop[u]);
-            issue_order();
+        for (int u = 0; u < 2; ++u) {
+            h8 kop[KS];
+            read_rows<HD>(tiles.rd, tiles.at(buffer, 0, u), kop);
+            sacc[u] = f16v{0};
+            product<BF>(kop, qop, sacc[u]);
+        }
+    };
+    float psum;
+    h8 pop[2][2];
+    auto exponentials = [&](const f16v (&sacc)[2], float mul) {
+        psum = 0.f;
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                sacc[u] = f16v{0};
-                product<BF>(kop[u], qop, sacc[u]);
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const float pv = at_exp2(__builtin_fmaf(sacc[u][v], mul, minus_m));
+                psum += pv;
+                pop[u][v >> 3][v & 7] = narrow_16<BF>(pv);
             }
-        }
-        const bool masked = k0 + 64 > n || (p.causal && k0 + 63 > row0);
-        const int seen = (p.causal ? min(row, n - 1) : n - 1) - k0;              // last key of the tile that the query sees
-        float mul = p.scale2;                    // what is still to be applied to the scores in the exponent
-        if (masked) {                            // -inf only once scaled, whatever the scale's sign
-            mul = 1.f;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int v = 0; v < 16; ++v)
-                    sacc[u][v] = 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? NEG_INF : sacc[u][v] * p.scale2;
-        }
-        h8 vop[2][HD / 32][2];                   // on their way while the exponentials are taken
-#pragma unroll
-        for (int u = 0; u < 2; ++u) read_columns<HD>(tiles.rd, tiles.at(1, u), vop[u]);
-        issue_order();
-        float psum;
-        h8 pop[2][2];
-        auto exponentials = [&]() {
-            psum = 0.f;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const float pv = at_exp2(__builtin_fmaf(sacc[u][v], mul, minus_m));
-                    psum += pv;
-                    pop[u][v >> 3][v & 7] = narrow_16<BF>(pv);
-                }
-        };
-        // A row moves its reference point by itself, so that its bits are its own: a row beside it, of NaN say, changes nothing.
-        bool move = m == NEG_INF;
-        if (fresh) psum = 0.f;
-        else exponentials();
-        move = move || psum > PACKED_LAZY_SUM;
+    };
+    // A row moves its reference point by itself, so that its bits are its own: a row beside it, of NaN say, changes nothing.
+    auto settle = [&](const f16v (&sacc)[2], float mul) {
+        bool move = m == NEG_INF || psum > PACKED_LAZY_SUM;
         if (__builtin_amdgcn_ballot_w64(move) != 0ull) {
             const int other_moves = __builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)move);
             move = move || other_moves != 0;
@@ -119,14 +92,64 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
             minus_m = -at_finite_or_zero(m_new);
             lsum *= keep;
             each<HD>(oacc, [&](float x, int) { return x * keep; });
-            fresh = __builtin_amdgcn_ballot_w64(m != NEG_INF) == 0ull;
-            exponentials();
+            exponentials(sacc, mul);
         }
         lsum += psum;
+    };
+    // Round r has the keys of tile r and the values of tile r - 1, in buffer r % 2.
+    auto enter = [&](int r) {
+        tiles.arrived();
+        if (r >= steps) return;
+        if (r + 1 < steps) tiles.request(0, r + 1, n, (r & 1) ^ 1);
+        tiles.request(1, r, n, (r & 1) ^ 1);
+    };
+    // a tile that all queries of the wave see whole; the scores of the next one are made beside its exponentials
+    auto whole_tile = [&](int r, int buffer, const f16v (&sacc)[2], f16v (&next)[2]) {
+        enter(r);
+        scores(buffer, next);
+        exponentials(sacc, p.scale2);
+        settle(sacc, p.scale2);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            h8 vop[HD / 32][2];
+            read_columns<HD>(tiles.rd, tiles.at(buffer, 1, u), vop);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int t = 0; t < HD / 32; ++t) oacc[t] = mfma_16<BF>(vop[t][s], pop[u][s], oacc[t]);
+        }
+    };
+    const int mine = row0 >= n ? 0 : p.causal ? min(steps, (row0 + 31) / 64 + 1) : steps;        // tiles that this wave needs
+    const int whole = row0 >= n ? 0 : p.causal ? (row0 + 1) / 64 : n / 64;                       // that are whole to it
+    f16v sacc[2], next[2];
+    enter(0);
+    if (mine > 0) scores(0, sacc);
+    int r = 1;
+    for (; r + 1 <= whole; r += 2) {
+        whole_tile(r, 1, sacc, next);
+        whole_tile(r + 1, 0, next, sacc);
+    }
+    if (r <= whole) {
+        whole_tile(r, 1, sacc, next);
+        sacc[0] = next[0], sacc[1] = next[1];
+        ++r;
+    }
+    for (; r <= mine; ++r) {                     // the last ones, with places that are hidden
+        enter(r);
+        const int seen = (p.causal ? min(row, n - 1) : n - 1) - 64 * (r - 1);    // last key of the tile that the query sees
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-            weigh<HD, BF, true>(tiles.rd, tiles.at(1, u), vop[u], pop[u], oacc, masked, [&](int r) { return 32 * u + r <= seen; });
+#pragma unroll
+            for (int v = 0; v < 16; ++v)         // -inf only once scaled, whatever the scale's sign
+                sacc[u][v] = 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? NEG_INF : sacc[u][v] * p.scale2;
+        exponentials(sacc, 1.f);
+        settle(sacc, 1.f);
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+            weigh_tile<HD, BF, true>(tiles.rd, tiles.at(r & 1, 1, u), pop[u], oacc, true, [&](int at) { return 32 * u + at <= seen; });
+        if (r < mine) scores(r & 1, sacc);
     }
+    for (; r <= steps; ++r) enter(r);            // of the rows below
     lsum += at_lane_xor32(lsum);                 // both halves used the same reference point
     const bool any = lsum > 0.f || lsum != lsum;
     if (p.lse != nullptr && h == 0 && row < n)   // log2 of the row's sum, +inf for a row that sees nothing
@@ -152,7 +175,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
     constexpr int KS = HD / 16, ROWS = 32 * W;
     const int cells = packed_grid(p.heads, p.head_sets, p.slots);
     if ((int)blockIdx.x >= cells) return packed_clear(p, (int)blockIdx.x - cells, p.out, (long long)p.heads * HD);
-    const PackedItem item = packed_item<ROWS>(p, p.heads, true);
+    const PackedItem item = packed_item<ROWS>(p, p.heads, false);
     if (item.n == 0) return;
     const int w = wave_id(), l = lane_id(), qq = l & 31, h = l >> 5, n = item.n, key_head = item.head / p.group;
     const int row0 = item.tile * ROWS + 32 * w, row = row0 + qq;
@@ -187,8 +210,9 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
     clear<HD>(dq);
     for (int step = 0; step < steps; ++step) {
         const int k0 = 64 * step;
-        tiles.arrived(step & 1);
-        if (step + 1 < steps) tiles.request(step + 1, n, (step + 1) & 1);
+        const int buffer = step & 1;
+        tiles.arrived();
+        if (step + 1 < steps) tiles.request(step + 1, n, buffer ^ 1);
         if (row0 >= n || (p.causal && k0 > row0 + 31)) continue;
         const bool masked = k0 + 64 > n || (p.causal && k0 + 63 > row0);
         const int seen = (p.causal ? min(row, n - 1) : n - 1) - k0;
@@ -198,13 +222,13 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
             h8 ktr[HD / 32][2], ds[2];
             {
                 h8 kop[KS], vop[KS];
-                read_rows<HD>(tiles.rd, tiles.at(0, u), kop);
-                read_rows<HD>(tiles.rd, tiles.at(1, u), vop);
+                read_rows<HD>(tiles.rd, tiles.at(buffer, 0, u), kop);
+                read_rows<HD>(tiles.rd, tiles.at(buffer, 1, u), vop);
                 issue_order();
                 product<BF>(kop, qop, sacc);
                 product<BF>(vop, dop, dpacc);
             }
-            read_columns<HD>(tiles.rd, tiles.at(0, u), ktr);
+            read_columns<HD>(tiles.rd, tiles.at(buffer, 0, u), ktr);
             issue_order();
 #pragma unroll
             for (int v = 0; v < 16; ++v) {       // a hidden score has no probability and no gradient, whatever it is
@@ -212,7 +236,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
                 if (masked && 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h) grad = 0.f;
                 ds[v >> 3][v & 7] = narrow_16<BF>(grad);
             }
-            weigh<HD, BF, false>(tiles.rd, tiles.at(0, u), ktr, ds, dq, masked, [&](int r) { return 32 * u + r <= seen; });
+            weigh<HD, BF, false>(tiles.rd, tiles.at(buffer, 0, u), ktr, ds, dq, masked, [&](int r) { return 32 * u + r <= seen; });
             issue_order();
         }
     }
@@ -233,7 +257,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperand
         packed_clear(p, (int)blockIdx.x - cells, p.dk, (long long)key_heads * HD);
         return packed_clear(p, (int)blockIdx.x - cells, p.dv, (long long)key_heads * HD);
     }
-    const PackedItem item = packed_item<ROWS>(p, key_heads, false);
+    const PackedItem item = packed_item<ROWS>(p, key_heads, p.causal);
     if (item.n == 0) return;
     const int w = wave_id(), l = lane_id(), kk = l & 31, h = l >> 5, n = item.n;
     const int key0 = item.tile * ROWS + 32 * w, key = key0 + kk;
@@ -275,7 +299,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperand
     int q0 = 64 * first;
     for (int step = 0; step < steps; ++step) {
         const int buffer = step & 1, at = q0;
-        tiles.arrived(buffer);
+        tiles.arrived();
         if (step + 1 < steps) request(buffer ^ 1);
         q0 = q0 + 64 < 64 * last ? q0 + 64 : 64 * first;
         if (key0 >= n || (p.causal && at + 63 < key0)) continue;
@@ -292,7 +316,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperand
                 for (int s0 = 0; s0 < KS; s0 += 4) {
                     h8 op[4];
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) op[s] = tiles.rd.rows(tiles.at(operand, u), s0 + s);
+                    for (int s = 0; s < 4; ++s) op[s] = tiles.rd.rows(tiles.at(buffer, operand, u), s0 + s);
 #pragma unroll
                     for (int s = 0; s < 4; ++s) acc = mfma_16<BF>(op[s], other[s0 + s], acc);
                     if (KS > 4) issue_order();
@@ -326,8 +350,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperand
             }
             issue_order();
             auto sees = [&](int r) { return 32 * u + r >= low && 32 * u + r < high; };
-            weigh_tile<HD, BF, false>(tiles.rd, tiles.at(0, u), ds, dk, masked, sees);
-            weigh_tile<HD, BF, true>(tiles.rd, tiles.at(1, u), pop, dv, masked, sees);
+            weigh_tile<HD, BF, false>(tiles.rd, tiles.at(buffer, 0, u), ds, dk, masked, sees);
+            weigh_tile<HD, BF, true>(tiles.rd, tiles.at(buffer, 1, u), pop, dv, masked, sees);
             issue_order();
         }
     }

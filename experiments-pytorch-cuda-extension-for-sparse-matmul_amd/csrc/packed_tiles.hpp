@@ -43,19 +43,52 @@ __device__ __forceinline__ int packed_offset(const PackedOperands &p, int b)
     return x < 0 ? 0 : x > p.tokens ? p.tokens : x;
 }
 
-// Slot floor(offset / ROWS) + b is the first of sequence b: strictly ascending in b, so 64 lanes search together.  `heads`: of
-// the launch; last_first: the slots are dealt from the highest on (the longest causal rows of a sequence first).
+// The workgroup's head and tile.  The hardware starts workgroups in order, so the long ones come first: up to 64 sequences the
+// tiles of all of them are dealt by their index in the sequence, the highest first (from_end: the distance to the sequence's
+// end), each lane of a wave holding one sequence.  With more, slot floor(offset / ROWS) + b is the first of sequence b, strictly
+// ascending in b, so 64 lanes search together, and a sequence's own tiles come longest first.  `heads`: of the launch.
 template <int ROWS>
-__device__ __forceinline__ PackedItem packed_item(const PackedOperands &p, int heads, bool last_first)
+__device__ __forceinline__ PackedItem packed_item(const PackedOperands &p, int heads, bool from_end)
 {
     PackedItem item{0, 0, 0, 0};
     const int x = (int)(blockIdx.x & 7u), t = (int)(blockIdx.x >> 3);
     const int share = 8 / p.head_sets, in_set = heads / p.head_sets;
     item.head = x / share * in_set + t % in_set;
-    int slot = t / in_set * share + x % share;
+    const int slot = t / in_set * share + x % share;
     if (slot >= p.slots) return item;
-    if (last_first) slot = p.slots - 1 - slot;
     const int l = lane_id();
+    if (p.sequences <= WAVE) {
+        const int from = packed_offset(p, l < p.sequences ? l : p.sequences), to = packed_offset(p, l < p.sequences ? l + 1 : p.sequences);
+        const int tiles = to > from ? (to - from + ROWS - 1) / ROWS : 0;
+        // tiles with an index of at least `index`
+        auto beyond = [&](int index) {
+            int sum = 0;
+            for (int b = 0; b < p.sequences; ++b) {
+                const int more = __builtin_amdgcn_readlane(tiles, b) - index;
+                sum += more > 0 ? more : 0;
+            }
+            return sum;
+        };
+        // the highest index with more than `slot` tiles from it on, 64 candidates at a time, the first of which always has them
+        int index = 0, stride = p.slots, behind = 0;
+        do {
+            stride = (stride + WAVE - 1) / WAVE;
+            const int left = beyond(index + stride * l);
+            const int with = __popcll(__builtin_amdgcn_ballot_w64(left > slot));
+            if (with == 0) return item;          // the first time: there are fewer tiles
+            behind = with < WAVE ? __builtin_amdgcn_readlane(left, with) : beyond(index + stride * WAVE);
+            index += stride * (with - 1);
+        } while (stride > 1);
+        index = __builtin_amdgcn_readfirstlane(index);
+        const int place = slot - __builtin_amdgcn_readfirstlane(behind);         // among the sequences with such a tile
+        const unsigned long long with = __builtin_amdgcn_ballot_w64(tiles > index);
+        const int mine = __builtin_amdgcn_mbcnt_hi((unsigned)(with >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)with, 0u));
+        const int b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(tiles > index && mine == place));
+        item.begin = __builtin_amdgcn_readlane(from, b);
+        item.n = __builtin_amdgcn_readlane(to, b) - item.begin;
+        item.tile = from_end ? __builtin_amdgcn_readlane(tiles, b) - 1 - index : index;
+        return item;
+    }
     int first = 0, count = p.sequences;
     while (true) {
         const int stride = (count + 63) / 64, b = first + l * stride;
@@ -69,10 +102,11 @@ __device__ __forceinline__ PackedItem packed_item(const PackedOperands &p, int h
     first = __builtin_amdgcn_readfirstlane(first);
     const int begin = __builtin_amdgcn_readfirstlane(packed_offset(p, first));
     const int end = __builtin_amdgcn_readfirstlane(packed_offset(p, first + 1));
-    item.tile = slot - (begin / ROWS + first);
-    if (item.tile < 0 || (long long)item.tile * ROWS >= end - begin) return item;
+    const int tile = slot - (begin / ROWS + first), tiles = (end - begin + ROWS - 1) / ROWS;
+    if (end <= begin || tile < 0 || tile >= tiles) return item;
     item.begin = begin;
     item.n = end - begin;
+    item.tile = from_end ? tile : tiles - 1 - tile;
     return item;
 }
 
@@ -219,14 +253,14 @@ __device__ __forceinline__ void weigh_tile(const TileReader &rd, unsigned tile, 
 template <int HD, int W>
 struct PairTiles {
     static constexpr int TILE = 64 * HD, BUFFER = 4 * TILE, REQUESTS = HD / 8 / W;
-    TileReader rd;
+    const TileReader rd;         // of buffer 0
     const unsigned char *base[2];
     long long stride[2];         // bytes between tokens
-    unsigned lds, row;           // row: of this lane inside a 32-row tile
-    unsigned piece;
+    unsigned lds, row, piece;    // row: of this lane inside a 32-row tile
+    unsigned whole[2];           // what a lane fetches, from the first of its rows and pieces on
     int wave;
     __device__ __forceinline__ PairTiles(const half_t *a, long long a_token, const half_t *b, long long b_token, unsigned char *lds_raw)
-        : rd(lds_raw + BUFFER)
+        : rd(lds_raw)
     {
         wave = wave_id();
         const int l = lane_id(), chunk = wave & 3;
@@ -235,37 +269,43 @@ struct PairTiles {
         lds = __builtin_amdgcn_readfirstlane(lds_address(lds_raw));
         row = 8 * chunk + (l >> 3);
         piece = 16 * panel_src_piece(l, chunk);
+#pragma unroll
+        for (int o = 0; o < 2; ++o) whole[o] = row * (unsigned)stride[o] + piece;
     }
     static constexpr size_t lds_bytes() { return 2 * (size_t)BUFFER; }
-    // tokens 64 step .. + 63 of n, those from n on as token n - 1 (what they give is hidden)
-    __device__ __forceinline__ void request(int step, int n, int buffer) const
+    __device__ __forceinline__ int subtile(int i) const { return (i * W + wave) / (HD / 16); }
+    __device__ __forceinline__ int panel(int i) const { return (i * W + wave) % (HD / 16) / 4; }
+    // tokens 64 step .. + 63 of n of one operand, those from n on as token n - 1 (what they give is hidden)
+    __device__ __forceinline__ void request(int o, int step, int n, int buffer) const
     {
+        const unsigned char *from = base[o] + (long long)64 * step * stride[o];
+        const unsigned to = lds + (unsigned)(buffer * BUFFER + o * 2 * TILE + 1024 * (wave & 3));
+        if (64 * step + 64 <= n) {
+#pragma unroll
+            for (int i = 0; i < REQUESTS; ++i)
+                dma16(from + 32 * subtile(i) * stride[o] + 128 * panel(i), whole[o], to + TILE * subtile(i) + 4096 * panel(i));
+            return;
+        }
         const unsigned last = (unsigned)(n - 1 - 64 * step);
 #pragma unroll
-        for (int o = 0; o < 2; ++o) {
-            const unsigned char *from = base[o] + (long long)64 * step * stride[o];
-#pragma unroll
-            for (int i = 0; i < REQUESTS; ++i) {
-                const int rq = i * W + wave, sub = rq / (HD / 16), u = rq % (HD / 16) / 4, c = rq & 3;
-                unsigned r = 32 * sub + row;
-                r = r < last ? r : last;
-                dma16(from, r * (unsigned)stride[o] + 128 * u + piece,
-                      lds + (unsigned)(buffer * BUFFER + o * 2 * TILE + sub * TILE + 4096 * u + 1024 * c));
-            }
+        for (int i = 0; i < REQUESTS; ++i) {
+            unsigned r = 32 * subtile(i) + row;
+            r = r < last ? r : last;
+            dma16(from + 128 * panel(i), r * (unsigned)stride[o] + piece, to + TILE * subtile(i) + 4096 * panel(i));
         }
     }
-    // every wave's part of the tile requested last has arrived, and all waves are done with the one before; buffers change
-    __device__ __forceinline__ void arrived(int buffer)
+    __device__ __forceinline__ void request(int step, int n, int buffer) const
     {
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        const unsigned d = buffer ? (unsigned)BUFFER : 0u - (unsigned)BUFFER;
-#pragma unroll
-        for (int s = 0; s < 4; ++s) rd.row[s] += d;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) rd.tr[x][0] += d, rd.tr[x][1] += d;
+        request(0, step, n, buffer);
+        request(1, step, n, buffer);
     }
-    // of subtile u of an operand, as TileReader's tile
-    static constexpr unsigned at(int operand, int u) { return (unsigned)((2 * operand + u) * TILE); }
+    // this wave's part of what was requested has arrived, and everyone's; all waves are done with the buffer before
+    __device__ __forceinline__ void arrived() const { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+    // subtile u of an operand in a buffer, as TileReader's tile
+    static __device__ __forceinline__ constexpr unsigned at(int buffer, int operand, int u)
+    {
+        return (unsigned)(buffer * BUFFER + (2 * operand + u) * TILE);
+    }
 };
 
 // 32 result rows `stride` values apart, of which the first `valid` are stored; through 64 HD bytes of LDS, so that they leave
