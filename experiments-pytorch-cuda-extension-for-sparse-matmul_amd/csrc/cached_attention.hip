@@ -325,9 +325,10 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
         lsum += psum;
         const unsigned other = (unsigned)__builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)sees);
         const unsigned lower = h == 0 ? sees : other, upper = h == 0 ? other : sees;
-        weigh_tile<HD, BF, true>(rd, buffer + TILE, pop, oacc, drafted, [&](int r) {
-            return (((r & 4 ? upper : lower) >> (4 * (r >> 3) + (r & 3))) & 1u) != 0u;
-        });
+        if (weigh_tile<HD, BF>(rd, buffer + TILE, pop, oacc, drafted))
+            add_not_finite<HD, BF>(rd, buffer + TILE, oacc, [&](int r) {
+                return (((r & 4 ? upper : lower) >> (4 * (r >> 3) + (r & 3))) & 1u) != 0u;
+            });
         if (RG == 1) wave_lds_fence();
     }
     lsum += at_lane_xor32(lsum);

@@ -35,7 +35,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
     const long long begin = item.begin;
     const float NEG_INF = -__builtin_inff();
 
-    PairTiles<HD, W> tiles(p.k + begin * p.k_token + key_head * p.k_head, p.k_token,
+    PairTiles<HD, W, 2> tiles(p.k + begin * p.k_token + key_head * p.k_head, p.k_token,
                            p.v + begin * p.v_token + key_head * p.v_head, p.v_token, lds_raw);
     const int last_row = min(n, item.tile * ROWS + ROWS) - 1;
     const int steps = p.causal ? last_row / 64 + 1 : (n + 63) / 64;
@@ -68,10 +68,11 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const float pv = at_exp2(__builtin_fmaf(sacc[u][v], mul, minus_m));
-                psum += pv;
-                pop[u][v >> 3][v & 7] = narrow_16<BF>(pv);
+            for (int v = 0; v < 16; v += 2) {
+                const float p0 = at_exp2(__builtin_fmaf(sacc[u][v], mul, minus_m)), p1 = at_exp2(__builtin_fmaf(sacc[u][v + 1], mul, minus_m));
+                pop[u][v >> 3][v & 7] = narrow_16<BF>(p0);
+                pop[u][v >> 3][(v & 7) + 1] = narrow_16<BF>(p1);
+                psum = add_pair<BF>(pop[u][v >> 3][v & 7], pop[u][v >> 3][(v & 7) + 1], psum);
             }
     };
     // A row moves its reference point by itself, so that its bits are its own: a row beside it, of NaN say, changes nothing.
@@ -146,7 +147,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
         settle(sacc, 1.f);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-            weigh_tile<HD, BF, true>(tiles.rd, tiles.at(r & 1, 1, u), pop[u], oacc, true, [&](int at) { return 32 * u + at <= seen; });
+            if (weigh_tile<HD, BF>(tiles.rd, tiles.at(r & 1, 1, u), pop[u], oacc, true))
+                add_not_finite<HD, BF>(tiles.rd, tiles.at(r & 1, 1, u), oacc, [&](int at) { return 32 * u + at <= seen; });
         if (r < mine) scores(r & 1, sacc);
     }
     for (; r <= steps; ++r) enter(r);            // of the rows below
@@ -181,7 +183,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
     const int row0 = item.tile * ROWS + 32 * w, row = row0 + qq;
     const long long begin = item.begin;
 
-    PairTiles<HD, W> tiles(p.k + begin * p.k_token + key_head * p.k_head, p.k_token,
+    PairTiles<HD, W, 2> tiles(p.k + begin * p.k_token + key_head * p.k_head, p.k_token,
                            p.v + begin * p.v_token + key_head * p.v_head, p.v_token, lds_raw);
     const int last_row = min(n, item.tile * ROWS + ROWS) - 1;
     const int steps = p.causal ? last_row / 64 + 1 : (n + 63) / 64;
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
                 if (masked && 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h) grad = 0.f;
                 ds[v >> 3][v & 7] = narrow_16<BF>(grad);
             }
-            weigh<HD, BF, false>(tiles.rd, tiles.at(buffer, 0, u), ktr, ds, dq, masked, [&](int r) { return 32 * u + r <= seen; });
+            weigh<HD, BF>(ktr, ds, dq, masked);
             issue_order();
         }
     }
@@ -245,12 +247,14 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
                              (long long)p.heads * HD, n - row0);
 }
 
-// Behind the tiles of PairTiles: lse and delta of the 64 queries, per buffer.
-template <int HD, bool BF, int W>
-__global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperands p)
+// The waves are KT tiles of 32 keys times SUB subtiles of 32 queries, which add their parts in LDS at the end.  Behind the tiles of
+// PairTiles: lse and delta of a tile's queries, per buffer.
+template <int HD, bool BF, int KT, int SUB>
+__global__ __launch_bounds__(64 * KT * SUB, 2) void packed_columns_kernel(PackedOperands p)
 {
     extern __shared__ __align__(16) unsigned char lds_raw[];
-    constexpr int KS = HD / 16, ROWS = 32 * W;
+    constexpr int KS = HD / 16, W = KT * SUB, ROWS = 32 * KT, TOKENS = 32 * SUB;
+    using Tiles = PairTiles<HD, W, SUB>;
     const int key_heads = p.heads / p.group;
     const int cells = packed_grid(key_heads, p.head_sets, p.slots);
     if ((int)blockIdx.x >= cells) {
@@ -259,8 +263,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperand
     }
     const PackedItem item = packed_item<ROWS>(p, key_heads, p.causal);
     if (item.n == 0) return;
-    const int w = wave_id(), l = lane_id(), kk = l & 31, h = l >> 5, n = item.n;
-    const int key0 = item.tile * ROWS + 32 * w, key = key0 + kk;
+    const int w = wave_id(), l = lane_id(), kk = l & 31, h = l >> 5, n = item.n, kt = w / SUB, sub = w % SUB;
+    const int key0 = item.tile * ROWS + 32 * kt, key = key0 + kk;
     const long long begin = item.begin, key_token = begin + min(key, n - 1);
 
     h8 kop[KS], vop[KS];
@@ -276,17 +280,19 @@ __global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperand
     clear<HD>(dk);
     clear<HD>(dv);
 
-    const int first = p.causal ? item.tile * ROWS / 64 : 0, last = (n + 63) / 64, steps = (last - first) * p.group;
-    float *stats = reinterpret_cast<float *>(lds_raw + PairTiles<HD, W>::lds_bytes());       // [2][lse 64, delta 64]
+    const int first = p.causal ? item.tile * ROWS / TOKENS : 0, last = (n + TOKENS - 1) / TOKENS, steps = (last - first) * p.group;
+    float *stats = reinterpret_cast<float *>(lds_raw + Tiles::lds_bytes());      // [2][lse, delta][TOKENS]
     const unsigned stats_lds = __builtin_amdgcn_readfirstlane(lds_address(stats));
     const int head0 = item.head * p.group;
-    PairTiles<HD, W> tiles(p.q + begin * p.q_token + head0 * p.q_head, p.q_token, p.dout + begin * p.g_token + head0 * p.g_head,
-                           p.g_token, lds_raw);
-    const float *stat = (w == 0 ? p.lse : p.delta) + (size_t)head0 * p.tokens + begin;
+    Tiles tiles(p.q + begin * p.q_token + head0 * p.q_head, p.q_token, p.dout + begin * p.g_token + head0 * p.g_head, p.g_token, lds_raw);
+    // which 64 statistics of a tile this wave fetches, if any
+    constexpr int STATS = 2 * TOKENS / WAVE;
+    const int which = w * WAVE / TOKENS, place = w * WAVE % TOKENS + l;
+    const float *stat = (which == 0 ? p.lse : p.delta) + (size_t)head0 * p.tokens + begin;
     int next = first;                            // of the step requested next, whose head is in the pointers
     auto request = [&](int buffer) {
         tiles.request(next, n, buffer);
-        if (w < 2) dma4_gather(stat + min(64 * next + l, n - 1), stats_lds + 512 * buffer + 256 * w);
+        if (w < STATS) dma4_gather(stat + min(TOKENS * next + place, n - 1), stats_lds + 8 * TOKENS * buffer + 256 * w);
         if (++next == last) {
             next = first;
             tiles.base[0] += 2 * p.q_head, tiles.base[1] += 2 * p.g_head, stat += p.tokens;
@@ -296,69 +302,89 @@ __global__ __launch_bounds__(64 * W, 2) void packed_columns_kernel(PackedOperand
     constexpr float UP = BF ? 1.f : 256.f, DOWN = 1.f / UP, LOG_UP = BF ? 0.f : 8.f;
     const float ds_scale = p.scale * DOWN;
     request(0);
-    int q0 = 64 * first;
+    int q_tile = first;
     for (int step = 0; step < steps; ++step) {
-        const int buffer = step & 1, at = q0;
+        const int buffer = step & 1, at = TOKENS * q_tile + 32 * sub;            // first query of this wave
+        // some wave has hidden places in this tile: see the products with such places in packed_tiles.hpp
+        const bool masked = TOKENS * q_tile + TOKENS > n || (p.causal && TOKENS * q_tile < item.tile * ROWS + ROWS);
+        if (masked) tiles.template clean<BF>(buffer);
         tiles.arrived();
         if (step + 1 < steps) request(buffer ^ 1);
-        q0 = q0 + 64 < 64 * last ? q0 + 64 : 64 * first;
-        if (key0 >= n || (p.causal && at + 63 < key0)) continue;
-        const bool masked = at + 64 > n || (p.causal && at < key0 + 31);
-        const int low = (p.causal ? key : 0) - at, high = n - at;                // queries of the tile that see the key
-        const float *stat_lds = stats + 128 * buffer;
+        q_tile = q_tile + 1 < last ? q_tile + 1 : first;
+        if (key0 >= n || at >= n || (p.causal && at + 31 < key0)) continue;
+        const int low = (p.causal ? key : 0) - at, high = n - at;                // queries of the subtile that see the key
+        const float *stat_lds = stats + 2 * TOKENS * buffer + 32 * sub;
+        f16v prob = {0}, dpacc = {0};
+        h8 pop[2], ds[2];
+        // four operands of a tile in registers at a time
+        auto product_of_rows = [&](int operand, const h8 (&other)[KS], f16v &acc) {
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            f16v prob = {0}, dpacc = {0};
-            h8 pop[2], ds[2];
-            // four operands of a tile in registers at a time
-            auto product_of_rows = [&](int operand, const h8 (&other)[KS], f16v &acc) {
+            for (int s0 = 0; s0 < KS; s0 += 4) {
+                h8 op[4];
 #pragma unroll
-                for (int s0 = 0; s0 < KS; s0 += 4) {
-                    h8 op[4];
+                for (int s = 0; s < 4; ++s) op[s] = tiles.rd.rows(tiles.at(buffer, operand, sub), s0 + s);
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) op[s] = tiles.rd.rows(tiles.at(buffer, operand, u), s0 + s);
+                for (int s = 0; s < 4; ++s) acc = mfma_16<BF>(op[s], other[s0 + s], acc);
+                if (KS > 4) issue_order();
+            }
+        };
+        product_of_rows(0, kop, prob);
+        issue_order();
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) acc = mfma_16<BF>(op[s], other[s0 + s], acc);
-                    if (KS > 4) issue_order();
-                }
-            };
-            product_of_rows(0, kop, prob);
-            issue_order();
+        for (int g = 0; g < 4; ++g) {
+            const f4v ls = *reinterpret_cast<const f4v *>(stat_lds + 8 * g + 4 * h);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f4v ls = *reinterpret_cast<const f4v *>(stat_lds + 32 * u + 8 * g + 4 * h);
+            for (int j = 0; j < 4; ++j) {
+                const int v = 4 * g + j;
+                prob[v] = at_exp2(__builtin_fmaf(prob[v], p.scale2, LOG_UP - ls[j]));
+            }
+            if (masked) {                        // a dO that is no number, cleaned out of the tile, is in the weights by its delta
+                const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int v = 4 * g + j, r = 32 * u + 8 * g + 4 * h + j;
-                    prob[v] = at_exp2(__builtin_fmaf(prob[v], p.scale2, LOG_UP - ls[j]));
-                    if (masked && (r < low || r >= high)) prob[v] = 0.f;
-                    pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
+                    const int v = 4 * g + j, r = 8 * g + 4 * h + j;
+                    prob[v] = r < low || r >= high ? 0.f : prob[v] + (dl[j] - dl[j]);
                 }
             }
-            issue_order();
-            product_of_rows(1, vop, dpacc);
-            issue_order();
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + 64 + 32 * u + 8 * g + 4 * h);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int v = 4 * g + j, r = 32 * u + 8 * g + 4 * h + j;
-                    const float grad = prob[v] * ((dpacc[v] - dl[j]) * ds_scale);
-                    ds[v >> 3][v & 7] = narrow_16<BF>(masked && (r < low || r >= high) ? 0.f : grad);
-                }
-            }
-            issue_order();
-            auto sees = [&](int r) { return 32 * u + r >= low && 32 * u + r < high; };
-            weigh_tile<HD, BF, false>(tiles.rd, tiles.at(buffer, 0, u), ds, dk, masked, sees);
-            weigh_tile<HD, BF, true>(tiles.rd, tiles.at(buffer, 1, u), pop, dv, masked, sees);
-            issue_order();
+            for (int j = 0; j < 4; ++j) pop[(4 * g + j) >> 3][(4 * g + j) & 7] = narrow_16<BF>(prob[4 * g + j]);
         }
+        issue_order();
+        product_of_rows(1, vop, dpacc);
+        issue_order();
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int v = 4 * g + j, r = 8 * g + 4 * h + j;
+                const float grad = prob[v] * ((dpacc[v] - dl[j]) * ds_scale);
+                ds[v >> 3][v & 7] = narrow_16<BF>(masked && (r < low || r >= high) ? 0.f : grad);
+            }
+        }
+        issue_order();
+        weigh_tile<HD, BF>(tiles.rd, tiles.at(buffer, 0, sub), ds, dk);
+        weigh_tile<HD, BF>(tiles.rd, tiles.at(buffer, 1, sub), pop, dv);
     }
-    __syncthreads();
+    // the parts of a key tile add up in order of the subtiles, one accumulator set at a time in the tiles' place
     const long long width = (long long)key_heads * HD, out = (begin + key0) * width + (long long)item.head * HD;
-    store_token_rows<HD, BF>(dv, DOWN, lds_raw + 64 * HD * w, p.dv + out, width, n - key0);
-    store_token_rows<HD, BF>(dk, 1.f, lds_raw + 64 * HD * w, p.dk + out, width, n - key0);
+    static_assert((size_t)W * 2 * Tiles::TILE <= Tiles::lds_bytes(), "the parked parts take the tiles' place");
+    float *park = reinterpret_cast<float *>(lds_raw + (size_t)w * 2 * Tiles::TILE);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        RowTile<HD> &acc = which == 0 ? dv : dk;
+        __syncthreads();                         // all are done with the tiles, or with the set before
+        if (sub > 0) each<HD>(acc, [&](float x, int i) { return park[i] = x; });
+        __syncthreads();
+        if (sub > 0) continue;
+#pragma unroll 1
+        for (int o = 1; o < SUB; ++o) {
+            const float *from = park + o * 32 * HD;
+            each<HD>(acc, [&](float x, int i) { return x + from[i]; });
+        }
+        store_token_rows<HD, BF>(acc, which == 0 ? DOWN : 1.f, reinterpret_cast<unsigned char *>(park), (which == 0 ? p.dv : p.dk) + out,
+                                 width, n - key0);
+    }
 }
 
 // ---- launchers ----------------------------------------------------------------------------------------
@@ -382,14 +408,14 @@ PackedOperands operands(const PackedArgs &a)
 
 // a launch gets 64 KB of LDS without asking
 template <class Kernel>
-hipError_t run_walk(Kernel kernel, PackedOperands p, int heads, int waves, size_t lds, hipStream_t st)
+hipError_t run_walk(Kernel kernel, PackedOperands p, int heads, int rows, int waves, size_t lds, hipStream_t st)
 {
     if (lds > 65536) {
         const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (err != hipSuccess) return err;
     }
     p.head_sets = packed_head_sets(heads);
-    p.slots = packed_slots(p.tokens, p.sequences, 32 * waves);
+    p.slots = packed_slots(p.tokens, p.sequences, rows);
     kernel<<<packed_grid(heads, p.head_sets, p.slots) + PACKED_CLEARING, 64 * waves, lds, st>>>(p);
     return hipGetLastError();
 }
@@ -398,16 +424,18 @@ template <int HD, bool BF>
 hipError_t forward(const PackedArgs &a, hipStream_t st)
 {
     constexpr int W = PACKED_WAVES;
-    return run_walk(packed_forward_kernel<HD, BF, W>, operands(a), a.heads, W, PairTiles<HD, W>::lds_bytes(), st);
+    return run_walk(packed_forward_kernel<HD, BF, W>, operands(a), a.heads, 32 * W, W, PairTiles<HD, W, 2>::lds_bytes(), st);
 }
 template <int HD, bool BF>
 hipError_t backward(const PackedArgs &a, hipStream_t st)
 {
     constexpr int W = PACKED_WAVES;
     const PackedOperands p = operands(a);
-    const hipError_t err = run_walk(packed_rows_kernel<HD, BF, W>, p, a.heads, W, PairTiles<HD, W>::lds_bytes(), st);
+    const hipError_t err = run_walk(packed_rows_kernel<HD, BF, W>, p, a.heads, 32 * W, W, PairTiles<HD, W, 2>::lds_bytes(), st);
     if (err != hipSuccess || a.dk == nullptr) return err;
-    return run_walk(packed_columns_kernel<HD, BF, W>, p, a.key_heads, W, PairTiles<HD, W>::lds_bytes() + 1024, st);
+    constexpr int KT = 2, SUB = HD == 64 ? 2 : 4;
+    return run_walk(packed_columns_kernel<HD, BF, KT, SUB>, p, a.key_heads, 32 * KT, KT * SUB,
+                    PairTiles<HD, KT * SUB, SUB>::lds_bytes() + 16 * 32 * SUB, st);
 }
 
 }  // namespace

@@ -124,6 +124,20 @@ __device__ __forceinline__ void packed_clear(const PackedOperands &p, int part, 
     clear(tail, p.tokens);
 }
 
+// sum + a + b of two 16-bit values in one instruction (subnormal ones count).  Rows are normalised by the sum of the probabilities
+// as the products take them, so their rounding cancels where all of them share it.
+template <bool BF>
+__device__ __forceinline__ float add_pair(half_t a, half_t b, float sum)
+{
+    if (BF) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        const b2 x = {__builtin_bit_cast(__bf16, a), __builtin_bit_cast(__bf16, b)}, ones = {(__bf16)1.f, (__bf16)1.f};
+        return __builtin_amdgcn_fdot2_f32_bf16(x, ones, sum, false);
+    }
+    const h2 x = {a, b}, ones = {(half_t)1.f, (half_t)1.f};
+    return __builtin_amdgcn_fdot2(x, ones, sum, false);
+}
+
 // Keeps what is above in front of what is below: operands are requested from LDS before the work that hides their latency.
 __device__ __forceinline__ void issue_order() { __builtin_amdgcn_sched_barrier(0); }
 // Values loaded in front of a loop have arrived: otherwise the compiler waits for them inside it, and with them for the loads to
@@ -156,9 +170,10 @@ __device__ __forceinline__ void product(const h8 (&a)[N], const h8 (&b)[N], f16v
     for (int s = 0; s < N; ++s) acc = mfma_16<BF>(a[s], b[s], acc);
 }
 // Products with some weights zero because their place is hidden: an infinity or a NaN in a token must not reach the results of
-// those that do not see it, and zero times it would be NaN.  Where anything is hidden the operands are looked at; such values
-// are left out of the products, and add_not_finite adds them to the results of the lanes for which sees(row of the tile) holds, as
-// themselves where the weights are probabilities, else as NaN.
+// those that do not see it, and zero times it would be NaN.  Where anything is hidden the operands are looked at and such values left
+// out of the products.  In the forward pass add_not_finite then adds them to the results of the lanes for which
+// sees(row of the tile) holds.  In the backward pass nothing has to be added: such a token's statistics are no numbers either, and
+// with them the weights of all that see it.
 template <bool BF, int T>
 __device__ __forceinline__ bool take_out_not_finite(h8 (&columns)[T][2])
 {
@@ -185,7 +200,7 @@ __device__ __forceinline__ bool take_out_not_finite(h8 (&columns)[T][2])
         }
     return true;
 }
-template <int HD, bool BF, bool PROBABILITIES, class Sees>
+template <int HD, bool BF, class Sees>
 __device__ __forceinline__ void add_not_finite(const TileReader &rd, unsigned tile, RowTile<HD> &acc, Sees sees)
 {
     constexpr unsigned short INFINITE = BF ? 0x7F80 : 0x7C00;
@@ -206,7 +221,7 @@ __device__ __forceinline__ void add_not_finite(const TileReader &rd, unsigned ti
                     const half_t one = raw[j];   // a bit cast of a vector's element itself takes the first one
                     const float value = widen_16<BF>(one);
                     if (seen && (__builtin_bit_cast(unsigned short, one) & 0x7FFF) >= INFINITE)
-                        acc[t][4 * g + j] += PROBABILITIES ? value : value - value;
+                        acc[t][4 * g + j] += value;
                 }
             }
             issue_order();
@@ -215,20 +230,18 @@ __device__ __forceinline__ void add_not_finite(const TileReader &rd, unsigned ti
 }
 
 // acc[t] += columns 32 t .. of a 32-row tile, its rows weighted by op; the columns have been read
-template <int HD, bool BF, bool PROBABILITIES, class Sees>
-__device__ __forceinline__ void weigh(const TileReader &rd, unsigned tile, h8 (&columns)[HD / 32][2], const h8 (&op)[2],
-                                      RowTile<HD> &acc, bool hidden, Sees sees)
+template <int HD, bool BF>
+__device__ __forceinline__ void weigh(h8 (&columns)[HD / 32][2], const h8 (&op)[2], RowTile<HD> &acc, bool hidden)
 {
-    const bool out = hidden && take_out_not_finite<BF>(columns);
+    if (hidden) take_out_not_finite<BF>(columns);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int t = 0; t < HD / 32; ++t) acc[t] = mfma_16<BF>(columns[t][s], op[s], acc[t]);
-    if (out) add_not_finite<HD, BF, PROBABILITIES>(rd, tile, acc, sees);
 }
-// the same, 64 columns read at a time
-template <int HD, bool BF, bool PROBABILITIES, class Sees>
-__device__ __forceinline__ void weigh_tile(const TileReader &rd, unsigned tile, const h8 (&op)[2], RowTile<HD> &acc, bool hidden, Sees sees)
+// the same, 64 columns read at a time; whether values were left out
+template <int HD, bool BF>
+__device__ __forceinline__ bool weigh_tile(const TileReader &rd, unsigned tile, const h8 (&op)[2], RowTile<HD> &acc, bool hidden = false)
 {
     bool out = false;
 #pragma unroll
@@ -245,14 +258,14 @@ __device__ __forceinline__ void weigh_tile(const TileReader &rd, unsigned tile, 
             for (int t = 0; t < 2; ++t) acc[t0 + t] = mfma_16<BF>(tr[t][s], op[s], acc[t0 + t]);
         if (HD > 64) issue_order();
     }
-    if (out) add_not_finite<HD, BF, PROBABILITIES>(rd, tile, acc, sees);
+    return out;
 }
 
-// Two operands (K and V, or Q and dO) in tiles of 64 tokens, double buffered, read by all W waves.  LDS of a buffer: the first
-// operand's two 32-row tiles (TileRequests' panels), then the second's.  A wave fetches HD / 8 / W kilobytes of each.
-template <int HD, int W>
+// Two operands (K and V, or Q and dO) in tiles of 32 SUB tokens, double buffered, read by all W waves.  LDS of a buffer: the first
+// operand's 32-row tiles (TileRequests' panels), then the second's.  A wave fetches SUB HD / 16 / W kilobytes of each.
+template <int HD, int W, int SUB>
 struct PairTiles {
-    static constexpr int TILE = 64 * HD, BUFFER = 4 * TILE, REQUESTS = HD / 8 / W;
+    static constexpr int TOKENS = 32 * SUB, TILE = 64 * HD, BUFFER = 2 * SUB * TILE, REQUESTS = SUB * HD / 16 / W;
     const TileReader rd;         // of buffer 0
     const unsigned char *base[2];
     long long stride[2];         // bytes between tokens
@@ -275,18 +288,18 @@ struct PairTiles {
     static constexpr size_t lds_bytes() { return 2 * (size_t)BUFFER; }
     __device__ __forceinline__ int subtile(int i) const { return (i * W + wave) / (HD / 16); }
     __device__ __forceinline__ int panel(int i) const { return (i * W + wave) % (HD / 16) / 4; }
-    // tokens 64 step .. + 63 of n of one operand, those from n on as token n - 1 (what they give is hidden)
+    // tokens TOKENS step .. of n of one operand, those from n on as token n - 1 (what they give is hidden)
     __device__ __forceinline__ void request(int o, int step, int n, int buffer) const
     {
-        const unsigned char *from = base[o] + (long long)64 * step * stride[o];
-        const unsigned to = lds + (unsigned)(buffer * BUFFER + o * 2 * TILE + 1024 * (wave & 3));
-        if (64 * step + 64 <= n) {
+        const unsigned char *from = base[o] + (long long)TOKENS * step * stride[o];
+        const unsigned to = lds + (unsigned)(buffer * BUFFER + o * SUB * TILE + 1024 * (wave & 3));
+        if (TOKENS * step + TOKENS <= n) {
 #pragma unroll
             for (int i = 0; i < REQUESTS; ++i)
                 dma16(from + 32 * subtile(i) * stride[o] + 128 * panel(i), whole[o], to + TILE * subtile(i) + 4096 * panel(i));
             return;
         }
-        const unsigned last = (unsigned)(n - 1 - 64 * step);
+        const unsigned last = (unsigned)(n - 1 - TOKENS * step);
 #pragma unroll
         for (int i = 0; i < REQUESTS; ++i) {
             unsigned r = 32 * subtile(i) + row;
@@ -299,12 +312,38 @@ struct PairTiles {
         request(0, step, n, buffer);
         request(1, step, n, buffer);
     }
+    // Zeros in the place of infinities and NaN in what this wave has fetched of a buffer, once it has arrived and before the others
+    // read it.
+    template <bool BF>
+    __device__ __forceinline__ void clean(int buffer) const
+    {
+        typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+        typedef us8 __attribute__((address_space(3))) *lds_us8;
+        constexpr unsigned short INFINITE = BF ? 0x7F80 : 0x7C00;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int o = 0; o < 2; ++o)
+#pragma unroll
+            for (int i = 0; i < REQUESTS; ++i) {
+                const unsigned to = lds + (unsigned)(buffer * BUFFER + o * SUB * TILE + 1024 * (wave & 3)) + TILE * subtile(i) + 4096 * panel(i);
+                const lds_us8 at = (lds_us8)(uintptr_t)(to + 16u * (unsigned)lane_id());
+                us8 x = *at;
+                bool finite = true;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) finite = finite && (x[j] & 0x7FFF) < INFINITE;
+                if (!finite) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = (x[j] & 0x7FFF) < INFINITE ? x[j] : (unsigned short)0;
+                    *at = x;
+                }
+            }
+    }
     // this wave's part of what was requested has arrived, and everyone's; all waves are done with the buffer before
     __device__ __forceinline__ void arrived() const { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
     // subtile u of an operand in a buffer, as TileReader's tile
     static __device__ __forceinline__ constexpr unsigned at(int buffer, int operand, int u)
     {
-        return (unsigned)(buffer * BUFFER + (2 * operand + u) * TILE);
+        return (unsigned)(buffer * BUFFER + (SUB * operand + u) * TILE);
     }
 };
 
