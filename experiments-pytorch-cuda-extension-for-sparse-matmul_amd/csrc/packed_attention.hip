@@ -9,6 +9,8 @@
 // The lengths stay on the device: a launch has slots for the most tiles that T tokens in B sequences can make, and every workgroup
 // finds its sequence by a search over the offsets.  Slots that no sequence uses end at once.  Offsets are clamped to [0, T]
 // before anything is addressed with them.
+#include <type_traits>
+
 #include "attention_tiles.hpp"
 #include "bsa_device.hpp"
 #include "bsa_internal.hpp"
@@ -232,12 +234,16 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
             }
             read_columns<HD>(tiles.rd, tiles.at(buffer, 0, u), ktr);
             issue_order();
+            auto gradients = [&](auto some_hidden) {     // a hidden score has no probability and no gradient, whatever it is
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {       // a hidden score has no probability and no gradient, whatever it is
-                float grad = at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus_lse)) * (dpacc[v] - delta);
-                if (masked && 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h) grad = 0.f;
-                ds[v >> 3][v & 7] = narrow_16<BF>(grad);
-            }
+                for (int v = 0; v < 16; ++v) {
+                    float grad = at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus_lse)) * (dpacc[v] - delta);
+                    if (some_hidden) grad = 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? 0.f : grad;
+                    ds[v >> 3][v & 7] = narrow_16<BF>(grad);
+                }
+            };
+            if (masked) gradients(std::true_type());
+            else gradients(std::false_type());
             weigh<HD, BF>(ktr, ds, dq, masked);
             issue_order();
         }
@@ -267,15 +273,18 @@ __global__ __launch_bounds__(64 * KT * SUB, 2) void packed_columns_kernel(Packed
     const int key0 = item.tile * ROWS + 32 * kt, key = key0 + kk;
     const long long begin = item.begin, key_token = begin + min(key, n - 1);
 
-    h8 kop[KS], vop[KS];
-    const half_t *k_row = p.k + key_token * p.k_token + item.head * p.k_head, *v_row = p.v + key_token * p.v_token + item.head * p.v_head;
+    // K stays in registers, V in LDS behind the statistics: the accumulators, K and V together would leave no register for a tile
+    h8 kop[KS];
+    const half_t *k_row = p.k + key_token * p.k_token + item.head * p.k_head;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        kop[s] = as_h8(ldg16(k_row + 16 * s + 8 * h));
-        vop[s] = as_h8(ldg16(v_row + 16 * s + 8 * h));
+    for (int s = 0; s < KS; ++s) kop[s] = as_h8(ldg16(k_row + 16 * s + 8 * h));
+    constexpr unsigned V_TILE = (unsigned)Tiles::lds_bytes() + 16 * TOKENS;
+    const unsigned v_tile = V_TILE + kt * Tiles::TILE;
+    if (sub == 0) {
+        const half_t *v_rows = p.v + (begin + min(key0, n - 1)) * p.v_token + item.head * p.v_head;
+        request_rows<HD>(v_rows, p.v_token, n - key0, __builtin_amdgcn_readfirstlane(lds_address(lds_raw)) + v_tile);
     }
     loaded(kop);
-    loaded(vop);
     RowTile<HD> dk, dv;
     clear<HD>(dk);
     clear<HD>(dv);
@@ -312,56 +321,79 @@ __global__ __launch_bounds__(64 * KT * SUB, 2) void packed_columns_kernel(Packed
         if (step + 1 < steps) request(buffer ^ 1);
         q_tile = q_tile + 1 < last ? q_tile + 1 : first;
         if (key0 >= n || at >= n || (p.causal && at + 31 < key0)) continue;
-        const int low = (p.causal ? key : 0) - at, high = n - at;                // queries of the subtile that see the key
+        // bit v: the query of accumulator value v is hidden from the key.  As bits of one register; the compiler would keep 16 masks.
+        auto hidden_queries = [&]() {
+            const int low = (p.causal ? key : 0) - at, high = n - at;
+            unsigned bits = 0;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                const int r = 8 * (v >> 2) + 4 * h + (v & 3);
+                bits |= ((r < low) | (r >= high)) ? 1u << v : 0u;
+            }
+            asm volatile("" : "+v"(bits));
+            return bits;
+        };
+        const unsigned hidden = masked ? hidden_queries() : 0u;
         const float *stat_lds = stats + 2 * TOKENS * buffer + 32 * sub;
         f16v prob = {0}, dpacc = {0};
         h8 pop[2], ds[2];
-        // four operands of a tile in registers at a time
-        auto product_of_rows = [&](int operand, const h8 (&other)[KS], f16v &acc) {
+        {
+            h8 op[KS];
+            read_rows<HD>(tiles.rd, tiles.at(buffer, 0, sub), op);
+            issue_order();
+            product<BF>(op, kop, prob);
+        }
+        constexpr int HALF = HD == 64 ? 2 : 1;
+        h8 dop[HALF], vop[HALF];                 // the first operands of the next product, on their way beside the exponentials
+        auto read_values = [&](int s0) {
 #pragma unroll
-            for (int s0 = 0; s0 < KS; s0 += 4) {
-                h8 op[4];
-#pragma unroll
-                for (int s = 0; s < 4; ++s) op[s] = tiles.rd.rows(tiles.at(buffer, operand, sub), s0 + s);
-#pragma unroll
-                for (int s = 0; s < 4; ++s) acc = mfma_16<BF>(op[s], other[s0 + s], acc);
-                if (KS > 4) issue_order();
+            for (int s = 0; s < HALF; ++s) {
+                dop[s] = tiles.rd.rows(tiles.at(buffer, 1, sub), s0 + s);
+                vop[s] = tiles.rd.rows(v_tile, s0 + s);
             }
         };
-        product_of_rows(0, kop, prob);
+        read_values(0);
+        issue_order();
+        auto probabilities = [&](auto some_hidden) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f4v ls = *reinterpret_cast<const f4v *>(stat_lds + 8 * g + 4 * h);
+                f4v dl = {0.f, 0.f, 0.f, 0.f};
+                if (some_hidden) dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int v = 4 * g + j;
+                    prob[v] = at_exp2(__builtin_fmaf(prob[v], p.scale2, LOG_UP - ls[j]));
+                    // a dO that is no number, cleaned out of the tile, is in the weights by its delta
+                    if (some_hidden) prob[v] = (hidden >> v) & 1u ? 0.f : prob[v] + (dl[j] - dl[j]);
+                    pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
+                }
+            }
+        };
+        if (masked) probabilities(std::true_type());
+        else probabilities(std::false_type());
         issue_order();
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f4v ls = *reinterpret_cast<const f4v *>(stat_lds + 8 * g + 4 * h);
+        for (int s0 = 0; s0 < KS; s0 += HALF) {
+            product<BF>(dop, vop, dpacc);
+            if (s0 + HALF < KS) read_values(s0 + HALF);
+        }
+        issue_order();
+        auto gradients = [&](auto some_hidden) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int v = 4 * g + j;
-                prob[v] = at_exp2(__builtin_fmaf(prob[v], p.scale2, LOG_UP - ls[j]));
-            }
-            if (masked) {                        // a dO that is no number, cleaned out of the tile, is in the weights by its delta
+            for (int g = 0; g < 4; ++g) {
                 const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int v = 4 * g + j, r = 8 * g + 4 * h + j;
-                    prob[v] = r < low || r >= high ? 0.f : prob[v] + (dl[j] - dl[j]);
+                    const int v = 4 * g + j;
+                    float grad = prob[v] * ((dpacc[v] - dl[j]) * ds_scale);
+                    if (some_hidden) grad = (hidden >> v) & 1u ? 0.f : grad;
+                    ds[v >> 3][v & 7] = narrow_16<BF>(grad);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) pop[(4 * g + j) >> 3][(4 * g + j) & 7] = narrow_16<BF>(prob[4 * g + j]);
-        }
-        issue_order();
-        product_of_rows(1, vop, dpacc);
-        issue_order();
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int v = 4 * g + j, r = 8 * g + 4 * h + j;
-                const float grad = prob[v] * ((dpacc[v] - dl[j]) * ds_scale);
-                ds[v >> 3][v & 7] = narrow_16<BF>(masked && (r < low || r >= high) ? 0.f : grad);
-            }
-        }
+        };
+        if (masked) gradients(std::true_type());
+        else gradients(std::false_type());
         issue_order();
         weigh_tile<HD, BF>(tiles.rd, tiles.at(buffer, 0, sub), ds, dk);
         weigh_tile<HD, BF>(tiles.rd, tiles.at(buffer, 1, sub), pop, dv);
@@ -435,7 +467,7 @@ hipError_t backward(const PackedArgs &a, hipStream_t st)
     if (err != hipSuccess || a.dk == nullptr) return err;
     constexpr int KT = 2, SUB = HD == 64 ? 2 : 4;
     return run_walk(packed_columns_kernel<HD, BF, KT, SUB>, p, a.key_heads, 32 * KT, KT * SUB,
-                    PairTiles<HD, KT * SUB, SUB>::lds_bytes() + 16 * 32 * SUB, st);
+                    PairTiles<HD, KT * SUB, SUB>::lds_bytes() + 16 * 32 * SUB + KT * 64 * HD, st);
 }
 
 }  // namespace

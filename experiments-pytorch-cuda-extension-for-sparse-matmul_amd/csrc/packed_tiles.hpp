@@ -261,6 +261,20 @@ __device__ __forceinline__ bool weigh_tile(const TileReader &rd, unsigned tile, 
     return out;
 }
 
+// 32 rows `stride` values apart, of which `valid` are there (those behind as the last), to a tile at LDS address `to`, by one wave
+template <int HD>
+__device__ __forceinline__ void request_rows(const half_t *rows, long long stride, int valid, unsigned to)
+{
+    const int l = lane_id();
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+        const int r = 8 * c + (l >> 3), there = r < valid ? r : valid - 1;
+        const unsigned off = (unsigned)(there > 0 ? there : 0) * (unsigned)(2 * stride) + 16 * panel_src_piece(l, c);
+#pragma unroll
+        for (int u = 0; u < HD / 64; ++u) dma16((const unsigned char *)rows + 128 * u, off, to + 4096 * u + 1024 * c);
+    }
+}
+
 // Two operands (K and V, or Q and dO) in tiles of 32 SUB tokens, double buffered, read by all W waves.  LDS of a buffer: the first
 // operand's 32-row tiles (TileRequests' panels), then the second's.  A wave fetches SUB HD / 16 / W kilobytes of each.
 template <int HD, int W, int SUB>
