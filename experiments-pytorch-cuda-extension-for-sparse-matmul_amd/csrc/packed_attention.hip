@@ -253,13 +253,16 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
                              (long long)p.heads * HD, n - row0);
 }
 
-// The waves are KT tiles of 32 keys times SUB subtiles of 32 queries, which add their parts in LDS at the end.  Behind the tiles of
-// PairTiles: lse and delta of a tile's queries, per buffer.
-template <int HD, bool BF, int KT, int SUB>
-__global__ __launch_bounds__(64 * KT * SUB, 2) void packed_columns_kernel(PackedOperands p)
+// A workgroup has 64 keys; the waves are 2 / KPW groups, with KPW tiles of 32 keys each, times the SUB subtiles of 32 queries of a
+// tile.  They add their parts in LDS at the end.  At head dim 128 a wave has both key tiles (KPW = 2), so that what it reads of Q and dO
+// serves both: one wave a SIMD with 512 registers, half of them accumulators, a key tile's exponentials beside the other's
+// products.  At 64 one each, two waves a SIMD and more.
+// Behind the tiles of PairTiles: lse and delta of a tile's queries, per buffer, and the workgroup's V.
+template <int HD, bool BF, int KPW, int SUB>
+__global__ __launch_bounds__(64 * SUB * 2 / KPW, HD == 64 ? 2 : 1) void packed_columns_kernel(PackedOperands p)
 {
     extern __shared__ __align__(16) unsigned char lds_raw[];
-    constexpr int KS = HD / 16, W = KT * SUB, ROWS = 32 * KT, TOKENS = 32 * SUB;
+    constexpr int KS = HD / 16, ROWS = 64, TOKENS = 32 * SUB, W = SUB * 2 / KPW;
     using Tiles = PairTiles<HD, W, SUB>;
     const int key_heads = p.heads / p.group;
     const int cells = packed_grid(key_heads, p.head_sets, p.slots);
@@ -269,153 +272,176 @@ __global__ __launch_bounds__(64 * KT * SUB, 2) void packed_columns_kernel(Packed
     }
     const PackedItem item = packed_item<ROWS>(p, key_heads, p.causal);
     if (item.n == 0) return;
-    const int w = wave_id(), l = lane_id(), kk = l & 31, h = l >> 5, n = item.n, kt = w / SUB, sub = w % SUB;
-    const int key0 = item.tile * ROWS + 32 * kt, key = key0 + kk;
-    const long long begin = item.begin, key_token = begin + min(key, n - 1);
+    const int w = wave_id(), sub = w % SUB, l = lane_id(), kk = l & 31, h = l >> 5, n = item.n, tile0 = item.tile * ROWS;
+    const int first_tile = w / SUB * KPW, key0 = tile0 + 32 * first_tile;        // of this wave
+    const long long begin = item.begin;
 
-    // K stays in registers, V in LDS behind the statistics: the accumulators, K and V together would leave no register for a tile
-    h8 kop[KS];
-    const half_t *k_row = p.k + key_token * p.k_token + item.head * p.k_head;
+    constexpr unsigned V_TILES = (unsigned)Tiles::lds_bytes() + 16 * TOKENS;
+    h8 kop[KPW][KS];
 #pragma unroll
-    for (int s = 0; s < KS; ++s) kop[s] = as_h8(ldg16(k_row + 16 * s + 8 * h));
-    constexpr unsigned V_TILE = (unsigned)Tiles::lds_bytes() + 16 * TOKENS;
-    const unsigned v_tile = V_TILE + kt * Tiles::TILE;
-    if (sub == 0) {
-        const half_t *v_rows = p.v + (begin + min(key0, n - 1)) * p.v_token + item.head * p.v_head;
-        request_rows<HD>(v_rows, p.v_token, n - key0, __builtin_amdgcn_readfirstlane(lds_address(lds_raw)) + v_tile);
+    for (int kt = 0; kt < KPW; ++kt) {
+        const half_t *k_row = p.k + (begin + min(key0 + 32 * kt + kk, n - 1)) * p.k_token + item.head * p.k_head;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) kop[kt][s] = as_h8(ldg16(k_row + 16 * s + 8 * h));
     }
-    loaded(kop);
-    RowTile<HD> dk, dv;
-    clear<HD>(dk);
-    clear<HD>(dv);
+    const unsigned v_tiles = V_TILES + first_tile * Tiles::TILE;
+#pragma unroll
+    for (int kt = 0; kt < KPW; ++kt)
+        if (sub == kt) {
+            const int first_key = min(key0 + 32 * kt, n - 1);
+            request_rows<HD>(p.v + (begin + first_key) * p.v_token + item.head * p.v_head, p.v_token, n - first_key,
+                             __builtin_amdgcn_readfirstlane(lds_address(lds_raw)) + v_tiles + kt * Tiles::TILE);
+        }
+#pragma unroll
+    for (int kt = 0; kt < KPW; ++kt) loaded(kop[kt]);
+    RowTile<HD> dk[KPW], dv[KPW];
+#pragma unroll
+    for (int kt = 0; kt < KPW; ++kt) {
+        clear<HD>(dk[kt]);
+        clear<HD>(dv[kt]);
+    }
 
-    const int first = p.causal ? item.tile * ROWS / TOKENS : 0, last = (n + TOKENS - 1) / TOKENS, steps = (last - first) * p.group;
+    const int first = p.causal ? tile0 / TOKENS : 0, last = (n + TOKENS - 1) / TOKENS, steps = (last - first) * p.group;
     float *stats = reinterpret_cast<float *>(lds_raw + Tiles::lds_bytes());      // [2][lse, delta][TOKENS]
     const unsigned stats_lds = __builtin_amdgcn_readfirstlane(lds_address(stats));
     const int head0 = item.head * p.group;
     Tiles tiles(p.q + begin * p.q_token + head0 * p.q_head, p.q_token, p.dout + begin * p.g_token + head0 * p.g_head, p.g_token, lds_raw);
-    // which 64 statistics of a tile this wave fetches, if any
-    constexpr int STATS = 2 * TOKENS / WAVE;
-    const int which = w * WAVE / TOKENS, place = w * WAVE % TOKENS + l;
-    const float *stat = (which == 0 ? p.lse : p.delta) + (size_t)head0 * p.tokens + begin;
+    constexpr int STAT_WAVES = TOKENS / WAVE;    // waves that fetch lse and delta of 64 queries each
+    const float *lse = p.lse + (size_t)head0 * p.tokens + begin, *delta = p.delta + (size_t)head0 * p.tokens + begin;
     int next = first;                            // of the step requested next, whose head is in the pointers
     auto request = [&](int buffer) {
         tiles.request(next, n, buffer);
-        if (w < STATS) dma4_gather(stat + min(TOKENS * next + place, n - 1), stats_lds + 8 * TOKENS * buffer + 256 * w);
+        if (w < STAT_WAVES) {
+            const int query = min(TOKENS * next + WAVE * w + l, n - 1);
+            dma4_gather(lse + query, stats_lds + 8 * TOKENS * buffer + 256 * w);
+            dma4_gather(delta + query, stats_lds + 8 * TOKENS * buffer + 4 * TOKENS + 256 * w);
+        }
         if (++next == last) {
             next = first;
-            tiles.base[0] += 2 * p.q_head, tiles.base[1] += 2 * p.g_head, stat += p.tokens;
+            tiles.base[0] += 2 * p.q_head, tiles.base[1] += 2 * p.g_head, lse += p.tokens, delta += p.tokens;
         }
     };
     // fp16 probabilities of long sequences would be subnormal: they travel times 256
     constexpr float UP = BF ? 1.f : 256.f, DOWN = 1.f / UP, LOG_UP = BF ? 0.f : 8.f;
     const float ds_scale = p.scale * DOWN;
+
     request(0);
     int q_tile = first;
     for (int step = 0; step < steps; ++step) {
         const int buffer = step & 1, at = TOKENS * q_tile + 32 * sub;            // first query of this wave
-        // some wave has hidden places in this tile: see the products with such places in packed_tiles.hpp
-        const bool masked = TOKENS * q_tile + TOKENS > n || (p.causal && TOKENS * q_tile < item.tile * ROWS + ROWS);
-        if (masked) tiles.template clean<BF>(buffer);
+        // Some wave has hidden places in this tile: see the products with such places in packed_tiles.hpp.  A dO that is no number is
+        // cleaned out of the tile, and its delta, which is none either, moves into the lse.
+        const bool masked = TOKENS * q_tile + TOKENS > n || (p.causal && TOKENS * q_tile < tile0 + ROWS);
+        if (masked) {
+            tiles.template clean<BF>(buffer);
+            if (w < STAT_WAVES) {
+                float *mine = stats + 2 * TOKENS * buffer + WAVE * w + l;
+                const float d = mine[TOKENS];
+                if (!(__builtin_fabsf(d) < __builtin_inff())) {
+                    mine[0] = __builtin_nanf("");
+                    mine[TOKENS] = 0.f;
+                }
+            }
+        }
         tiles.arrived();
         if (step + 1 < steps) request(buffer ^ 1);
         q_tile = q_tile + 1 < last ? q_tile + 1 : first;
-        if (key0 >= n || at >= n || (p.causal && at + 31 < key0)) continue;
-        // bit v: the query of accumulator value v is hidden from the key.  As bits of one register; the compiler would keep 16 masks.
-        auto hidden_queries = [&]() {
-            const int low = (p.causal ? key : 0) - at, high = n - at;
-            unsigned bits = 0;
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int r = 8 * (v >> 2) + 4 * h + (v & 3);
-                bits |= ((r < low) | (r >= high)) ? 1u << v : 0u;
-            }
-            asm volatile("" : "+v"(bits));
-            return bits;
-        };
-        const unsigned hidden = masked ? hidden_queries() : 0u;
+
         const float *stat_lds = stats + 2 * TOKENS * buffer + 32 * sub;
-        f16v prob = {0}, dpacc = {0};
-        h8 pop[2], ds[2];
+        const unsigned q_at = tiles.at(buffer, 0, sub), do_at = tiles.at(buffer, 1, sub);
+        f16v prob[KPW], dpacc[KPW];
         {
             h8 op[KS];
-            read_rows<HD>(tiles.rd, tiles.at(buffer, 0, sub), op);
-            issue_order();
-            product<BF>(op, kop, prob);
-        }
-        constexpr int HALF = HD == 64 ? 2 : 1;
-        h8 dop[HALF], vop[HALF];                 // the first operands of the next product, on their way beside the exponentials
-        auto read_values = [&](int s0) {
+            read_rows<HD>(tiles.rd, q_at, op);
 #pragma unroll
-            for (int s = 0; s < HALF; ++s) {
-                dop[s] = tiles.rd.rows(tiles.at(buffer, 1, sub), s0 + s);
-                vop[s] = tiles.rd.rows(v_tile, s0 + s);
+            for (int kt = 0; kt < KPW; ++kt) {
+                prob[kt] = f16v{0};
+                product<BF>(op, kop[kt], prob[kt]);
             }
-        };
-        read_values(0);
+        }
         issue_order();
-        auto probabilities = [&](auto some_hidden) {
+        {
+            h8 op[KS];
+            read_rows<HD>(tiles.rd, do_at, op);
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f4v ls = *reinterpret_cast<const f4v *>(stat_lds + 8 * g + 4 * h);
-                f4v dl = {0.f, 0.f, 0.f, 0.f};
-                if (some_hidden) dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
+            for (int kt = 0; kt < KPW; ++kt) {
+                h8 vop[KS];
+                read_rows<HD>(tiles.rd, v_tiles + kt * Tiles::TILE, vop);
+                dpacc[kt] = f16v{0};
+                product<BF>(op, vop, dpacc[kt]);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f4v ls = *reinterpret_cast<const f4v *>(stat_lds + 8 * g + 4 * h);
+#pragma unroll
+            for (int kt = 0; kt < KPW; ++kt)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) prob[kt][4 * g + j] = at_exp2(__builtin_fmaf(prob[kt][4 * g + j], p.scale2, LOG_UP - ls[j]));
+        }
+        if (masked) {
+#pragma unroll
+            for (int kt = 0; kt < KPW; ++kt) {
+                int low = (p.causal ? key0 + 32 * kt + kk : 0) - at - 4 * h, high = n - at - 4 * h;
+                asm volatile("" : "+v"(low));
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int r = 8 * (v >> 2) + (v & 3);
+                    prob[kt][v] = ((r < low) | (r >= high)) ? 0.f : prob[kt][v];
+                }
+            }
+        }
+        issue_order();
+        h8 pop[KPW][2], ds[KPW][2];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
+#pragma unroll
+            for (int kt = 0; kt < KPW; ++kt)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int v = 4 * g + j;
-                    prob[v] = at_exp2(__builtin_fmaf(prob[v], p.scale2, LOG_UP - ls[j]));
-                    // a dO that is no number, cleaned out of the tile, is in the weights by its delta
-                    if (some_hidden) prob[v] = (hidden >> v) & 1u ? 0.f : prob[v] + (dl[j] - dl[j]);
-                    pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
+                    pop[kt][v >> 3][v & 7] = narrow_16<BF>(prob[kt][v]);
+                    ds[kt][v >> 3][v & 7] = narrow_16<BF>(prob[kt][v] * ((dpacc[kt][v] - dl[j]) * ds_scale));
                 }
-            }
-        };
-        if (masked) probabilities(std::true_type());
-        else probabilities(std::false_type());
-        issue_order();
-#pragma unroll
-        for (int s0 = 0; s0 < KS; s0 += HALF) {
-            product<BF>(dop, vop, dpacc);
-            if (s0 + HALF < KS) read_values(s0 + HALF);
         }
         issue_order();
-        auto gradients = [&](auto some_hidden) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
+        for (int t = 0; t < HD / 32; ++t) {
+            h8 qc[2], dc[2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int v = 4 * g + j;
-                    float grad = prob[v] * ((dpacc[v] - dl[j]) * ds_scale);
-                    if (some_hidden) grad = (hidden >> v) & 1u ? 0.f : grad;
-                    ds[v >> 3][v & 7] = narrow_16<BF>(grad);
-                }
+            for (int s = 0; s < 2; ++s) {
+                qc[s] = tiles.rd.columns(q_at, t, s);
+                dc[s] = tiles.rd.columns(do_at, t, s);
             }
-        };
-        if (masked) gradients(std::true_type());
-        else gradients(std::false_type());
-        issue_order();
-        weigh_tile<HD, BF>(tiles.rd, tiles.at(buffer, 0, sub), ds, dk);
-        weigh_tile<HD, BF>(tiles.rd, tiles.at(buffer, 1, sub), pop, dv);
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int kt = 0; kt < KPW; ++kt) {
+                    dk[kt][t] = mfma_16<BF>(qc[s], ds[kt][s], dk[kt][t]);
+                    dv[kt][t] = mfma_16<BF>(dc[s], pop[kt][s], dv[kt][t]);
+                }
+        }
     }
     // the parts of a key tile add up in order of the subtiles, one accumulator set at a time in the tiles' place
     const long long width = (long long)key_heads * HD, out = (begin + key0) * width + (long long)item.head * HD;
     static_assert((size_t)W * 2 * Tiles::TILE <= Tiles::lds_bytes(), "the parked parts take the tiles' place");
     float *park = reinterpret_cast<float *>(lds_raw + (size_t)w * 2 * Tiles::TILE);
+    const float *parts = reinterpret_cast<const float *>(lds_raw + (size_t)(w - sub) * 2 * Tiles::TILE);
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        RowTile<HD> &acc = which == 0 ? dv : dk;
+    for (int set = 0; set < 2 * KPW; ++set) {    // subtile `set` of each group sums and stores it
+        const int kt = set % KPW;
+        const bool values = set < KPW;
+        RowTile<HD> &acc = values ? dv[kt] : dk[kt];
         __syncthreads();                         // all are done with the tiles, or with the set before
-        if (sub > 0) each<HD>(acc, [&](float x, int i) { return park[i] = x; });
+        each<HD>(acc, [&](float x, int i) { return park[i] = x; });
         __syncthreads();
-        if (sub > 0) continue;
+        if (sub != set % SUB) continue;
+        clear<HD>(acc);
 #pragma unroll 1
-        for (int o = 1; o < SUB; ++o) {
-            const float *from = park + o * 32 * HD;
-            each<HD>(acc, [&](float x, int i) { return x + from[i]; });
-        }
-        store_token_rows<HD, BF>(acc, which == 0 ? DOWN : 1.f, reinterpret_cast<unsigned char *>(park), (which == 0 ? p.dv : p.dk) + out,
-                                 width, n - key0);
+        for (int o = 0; o < SUB; ++o) each<HD>(acc, [&](float x, int i) { return x + parts[o * 32 * HD + i]; });
+        store_token_rows<HD, BF>(acc, values ? DOWN : 1.f, reinterpret_cast<unsigned char *>(park), (values ? p.dv : p.dk) + out + 32 * kt * width,
+                                 width, n - key0 - 32 * kt);
     }
 }
 
@@ -465,9 +491,9 @@ hipError_t backward(const PackedArgs &a, hipStream_t st)
     const PackedOperands p = operands(a);
     const hipError_t err = run_walk(packed_rows_kernel<HD, BF, W>, p, a.heads, 32 * W, W, PairTiles<HD, W, 2>::lds_bytes(), st);
     if (err != hipSuccess || a.dk == nullptr) return err;
-    constexpr int KT = 2, SUB = HD == 64 ? 2 : 4;
-    return run_walk(packed_columns_kernel<HD, BF, KT, SUB>, p, a.key_heads, 32 * KT, KT * SUB,
-                    PairTiles<HD, KT * SUB, SUB>::lds_bytes() + 16 * 32 * SUB + KT * 64 * HD, st);
+    constexpr int KPW = HD == 64 ? 1 : 2, SUB = HD == 64 ? 2 : 4, CW = SUB * 2 / KPW;
+    return run_walk(packed_columns_kernel<HD, BF, KPW, SUB>, p, a.key_heads, 64, CW,
+                    PairTiles<HD, CW, SUB>::lds_bytes() + 16 * 32 * SUB + 2 * 64 * HD, st);
 }
 
 }  // namespace
