@@ -253,16 +253,17 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
                              (long long)p.heads * HD, n - row0);
 }
 
-// A workgroup has 64 keys; the waves are 2 / KPW groups, with KPW tiles of 32 keys each, times the SUB subtiles of 32 queries of a
-// tile.  They add their parts in LDS at the end.  At head dim 128 a wave has both key tiles (KPW = 2), so that what it reads of Q and dO
-// serves both: one wave a SIMD with 512 registers, half of them accumulators, a key tile's exponentials beside the other's
-// products.  At 64 one each, two waves a SIMD and more.
+// A workgroup has two tiles of 32 keys, each wave one of them for one of the SUB subtiles of 32 queries of a tile; the subtiles'
+// parts add up in LDS at the end.  128 queries a tile at head dim 128, 64 at 64.  K stays in registers, V in LDS: with the
+// accumulators they would leave too few for two waves a SIMD at head dim 128 (256 registers each, none spilled: what is spilled
+// is waited for behind the tiles on their way).  One wave a SIMD with 512 registers and both key tiles, which reads Q and dO half
+// as often, took 430 us where this takes 345 (8191 tokens, 16 heads over 4): nothing runs beside what a wave waits for.
 // Behind the tiles of PairTiles: lse and delta of a tile's queries, per buffer, and the workgroup's V.
-template <int HD, bool BF, int KPW, int SUB>
-__global__ __launch_bounds__(64 * SUB * 2 / KPW, HD == 64 ? 2 : 1) void packed_columns_kernel(PackedOperands p)
+template <int HD, bool BF, int SUB>
+__global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOperands p)
 {
     extern __shared__ __align__(16) unsigned char lds_raw[];
-    constexpr int KS = HD / 16, ROWS = 64, TOKENS = 32 * SUB, W = SUB * 2 / KPW;
+    constexpr int KS = HD / 16, ROWS = 64, TOKENS = 32 * SUB, W = 2 * SUB;
     using Tiles = PairTiles<HD, W, SUB>;
     const int key_heads = p.heads / p.group;
     const int cells = packed_grid(key_heads, p.head_sets, p.slots);
@@ -273,33 +274,23 @@ __global__ __launch_bounds__(64 * SUB * 2 / KPW, HD == 64 ? 2 : 1) void packed_c
     const PackedItem item = packed_item<ROWS>(p, key_heads, p.causal);
     if (item.n == 0) return;
     const int w = wave_id(), sub = w % SUB, l = lane_id(), kk = l & 31, h = l >> 5, n = item.n, tile0 = item.tile * ROWS;
-    const int first_tile = w / SUB * KPW, key0 = tile0 + 32 * first_tile;        // of this wave
+    const int key0 = tile0 + 32 * (w / SUB), key = key0 + kk;                     // of this wave, of this lane
     const long long begin = item.begin;
 
     constexpr unsigned V_TILES = (unsigned)Tiles::lds_bytes() + 16 * TOKENS;
-    h8 kop[KPW][KS];
+    const unsigned v_tile = V_TILES + w / SUB * Tiles::TILE;
+    const int there = min(key0, n - 1);
+    if (sub == 0)
+        request_rows<HD>(p.v + (begin + there) * p.v_token + item.head * p.v_head, p.v_token, n - there,
+                         __builtin_amdgcn_readfirstlane(lds_address(lds_raw)) + v_tile);
+    h8 kop[KS];
+    const half_t *k_row = p.k + (begin + min(key, n - 1)) * p.k_token + item.head * p.k_head;
 #pragma unroll
-    for (int kt = 0; kt < KPW; ++kt) {
-        const half_t *k_row = p.k + (begin + min(key0 + 32 * kt + kk, n - 1)) * p.k_token + item.head * p.k_head;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) kop[kt][s] = as_h8(ldg16(k_row + 16 * s + 8 * h));
-    }
-    const unsigned v_tiles = V_TILES + first_tile * Tiles::TILE;
-#pragma unroll
-    for (int kt = 0; kt < KPW; ++kt)
-        if (sub == kt) {
-            const int first_key = min(key0 + 32 * kt, n - 1);
-            request_rows<HD>(p.v + (begin + first_key) * p.v_token + item.head * p.v_head, p.v_token, n - first_key,
-                             __builtin_amdgcn_readfirstlane(lds_address(lds_raw)) + v_tiles + kt * Tiles::TILE);
-        }
-#pragma unroll
-    for (int kt = 0; kt < KPW; ++kt) loaded(kop[kt]);
-    RowTile<HD> dk[KPW], dv[KPW];
-#pragma unroll
-    for (int kt = 0; kt < KPW; ++kt) {
-        clear<HD>(dk[kt]);
-        clear<HD>(dv[kt]);
-    }
+    for (int s = 0; s < KS; ++s) kop[s] = as_h8(ldg16(k_row + 16 * s + 8 * h));
+    loaded(kop);
+    RowTile<HD> dk, dv;
+    clear<HD>(dk);
+    clear<HD>(dv);
 
     const int first = p.causal ? tile0 / TOKENS : 0, last = (n + TOKENS - 1) / TOKENS, steps = (last - first) * p.group;
     float *stats = reinterpret_cast<float *>(lds_raw + Tiles::lds_bytes());      // [2][lse, delta][TOKENS]
@@ -349,61 +340,45 @@ __global__ __launch_bounds__(64 * SUB * 2 / KPW, HD == 64 ? 2 : 1) void packed_c
 
         const float *stat_lds = stats + 2 * TOKENS * buffer + 32 * sub;
         const unsigned q_at = tiles.at(buffer, 0, sub), do_at = tiles.at(buffer, 1, sub);
-        f16v prob[KPW], dpacc[KPW];
+        f16v prob = {0}, dpacc = {0};
         {
             h8 op[KS];
             read_rows<HD>(tiles.rd, q_at, op);
-#pragma unroll
-            for (int kt = 0; kt < KPW; ++kt) {
-                prob[kt] = f16v{0};
-                product<BF>(op, kop[kt], prob[kt]);
-            }
+            product<BF>(op, kop, prob);
         }
         issue_order();
         {
             h8 op[KS];
             read_rows<HD>(tiles.rd, do_at, op);
 #pragma unroll
-            for (int kt = 0; kt < KPW; ++kt) {
-                h8 vop[KS];
-                read_rows<HD>(tiles.rd, v_tiles + kt * Tiles::TILE, vop);
-                dpacc[kt] = f16v{0};
-                product<BF>(op, vop, dpacc[kt]);
-            }
+            for (int s = 0; s < KS; ++s) dpacc = mfma_16<BF>(op[s], tiles.rd.rows(v_tile, s), dpacc);
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f4v ls = *reinterpret_cast<const f4v *>(stat_lds + 8 * g + 4 * h);
 #pragma unroll
-            for (int kt = 0; kt < KPW; ++kt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) prob[kt][4 * g + j] = at_exp2(__builtin_fmaf(prob[kt][4 * g + j], p.scale2, LOG_UP - ls[j]));
+            for (int j = 0; j < 4; ++j) prob[4 * g + j] = at_exp2(__builtin_fmaf(prob[4 * g + j], p.scale2, LOG_UP - ls[j]));
         }
         if (masked) {
+            int low = (p.causal ? key : 0) - at - 4 * h, high = n - at - 4 * h;  // queries of the subtile that see the key
+            asm volatile("" : "+v"(low));        // the comparisons stay here: the compiler would keep 16 masks through the walk
 #pragma unroll
-            for (int kt = 0; kt < KPW; ++kt) {
-                int low = (p.causal ? key0 + 32 * kt + kk : 0) - at - 4 * h, high = n - at - 4 * h;
-                asm volatile("" : "+v"(low));
-#pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    const int r = 8 * (v >> 2) + (v & 3);
-                    prob[kt][v] = ((r < low) | (r >= high)) ? 0.f : prob[kt][v];
-                }
+            for (int v = 0; v < 16; ++v) {
+                const int r = 8 * (v >> 2) + (v & 3);
+                prob[v] = ((r < low) | (r >= high)) ? 0.f : prob[v];
             }
         }
         issue_order();
-        h8 pop[KPW][2], ds[KPW][2];
+        h8 pop[2], ds[2];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
 #pragma unroll
-            for (int kt = 0; kt < KPW; ++kt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int v = 4 * g + j;
-                    pop[kt][v >> 3][v & 7] = narrow_16<BF>(prob[kt][v]);
-                    ds[kt][v >> 3][v & 7] = narrow_16<BF>(prob[kt][v] * ((dpacc[kt][v] - dl[j]) * ds_scale));
-                }
+            for (int j = 0; j < 4; ++j) {
+                const int v = 4 * g + j;
+                pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
+                ds[v >> 3][v & 7] = narrow_16<BF>(prob[v] * ((dpacc[v] - dl[j]) * ds_scale));
+            }
         }
         issue_order();
 #pragma unroll
@@ -415,12 +390,10 @@ __global__ __launch_bounds__(64 * SUB * 2 / KPW, HD == 64 ? 2 : 1) void packed_c
                 dc[s] = tiles.rd.columns(do_at, t, s);
             }
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int kt = 0; kt < KPW; ++kt) {
-                    dk[kt][t] = mfma_16<BF>(qc[s], ds[kt][s], dk[kt][t]);
-                    dv[kt][t] = mfma_16<BF>(dc[s], pop[kt][s], dv[kt][t]);
-                }
+            for (int s = 0; s < 2; ++s) {
+                dk[t] = mfma_16<BF>(qc[s], ds[s], dk[t]);
+                dv[t] = mfma_16<BF>(dc[s], pop[s], dv[t]);
+            }
         }
     }
     // the parts of a key tile add up in order of the subtiles, one accumulator set at a time in the tiles' place
@@ -429,19 +402,17 @@ __global__ __launch_bounds__(64 * SUB * 2 / KPW, HD == 64 ? 2 : 1) void packed_c
     float *park = reinterpret_cast<float *>(lds_raw + (size_t)w * 2 * Tiles::TILE);
     const float *parts = reinterpret_cast<const float *>(lds_raw + (size_t)(w - sub) * 2 * Tiles::TILE);
 #pragma unroll
-    for (int set = 0; set < 2 * KPW; ++set) {    // subtile `set` of each group sums and stores it
-        const int kt = set % KPW;
-        const bool values = set < KPW;
-        RowTile<HD> &acc = values ? dv[kt] : dk[kt];
+    for (int set = 0; set < 2; ++set) {          // subtile `set` of each key tile sums and stores it
+        RowTile<HD> &acc = set == 0 ? dv : dk;
         __syncthreads();                         // all are done with the tiles, or with the set before
         each<HD>(acc, [&](float x, int i) { return park[i] = x; });
         __syncthreads();
-        if (sub != set % SUB) continue;
+        if (sub != set) continue;
         clear<HD>(acc);
 #pragma unroll 1
         for (int o = 0; o < SUB; ++o) each<HD>(acc, [&](float x, int i) { return x + parts[o * 32 * HD + i]; });
-        store_token_rows<HD, BF>(acc, values ? DOWN : 1.f, reinterpret_cast<unsigned char *>(park), (values ? p.dv : p.dk) + out + 32 * kt * width,
-                                 width, n - key0 - 32 * kt);
+        store_token_rows<HD, BF>(acc, set == 0 ? DOWN : 1.f, reinterpret_cast<unsigned char *>(park), (set == 0 ? p.dv : p.dk) + out, width,
+                                 n - key0);
     }
 }
 
@@ -491,9 +462,9 @@ hipError_t backward(const PackedArgs &a, hipStream_t st)
     const PackedOperands p = operands(a);
     const hipError_t err = run_walk(packed_rows_kernel<HD, BF, W>, p, a.heads, 32 * W, W, PairTiles<HD, W, 2>::lds_bytes(), st);
     if (err != hipSuccess || a.dk == nullptr) return err;
-    constexpr int KPW = HD == 64 ? 1 : 2, SUB = HD == 64 ? 2 : 4, CW = SUB * 2 / KPW;
-    return run_walk(packed_columns_kernel<HD, BF, KPW, SUB>, p, a.key_heads, 64, CW,
-                    PairTiles<HD, CW, SUB>::lds_bytes() + 16 * 32 * SUB + 2 * 64 * HD, st);
+    constexpr int SUB = HD == 64 ? 2 : 4;
+    return run_walk(packed_columns_kernel<HD, BF, SUB>, p, a.key_heads, 64, 2 * SUB,
+                    PairTiles<HD, 2 * SUB, SUB>::lds_bytes() + 16 * 32 * SUB + 2 * 64 * HD, st);
 }
 
 }  // namespace
