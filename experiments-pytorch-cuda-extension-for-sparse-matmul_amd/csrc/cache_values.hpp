@@ -46,4 +46,36 @@ __device__ __forceinline__ void widen_held(unsigned w, float *y)
     for (int j = 0; j < 4; ++j) y[j] = (float)((int)(w << (24 - 8 * j)) >> 24);
 }
 
+// 8 values as 16-bit ones, all of them exactly
+template <bool BF, int KIND>
+__device__ __forceinline__ h8 widen_held_16(unsigned lo, unsigned hi)
+{
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const unsigned w[2] = {lo, hi};
+    unsigned o[4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        if (KIND == CACHE_E4M3) {                // the conversion's own scale is 1
+            if (BF) {
+                o[2 * j] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j], 1.f, false));
+                o[2 * j + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[j], 1.f, true));
+            } else {
+                o[2 * j] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[j], 1.f, false));
+                o[2 * j + 1] = __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[j], 1.f, true));
+            }
+        } else if (BF) {
+            float y[4];
+            widen_held<KIND>(w[j], y);
+            o[2 * j] = __builtin_bit_cast(unsigned, b2{(__bf16)y[0], (__bf16)y[1]});
+            o[2 * j + 1] = __builtin_bit_cast(unsigned, b2{(__bf16)y[2], (__bf16)y[3]});
+        } else {                                 // x + 128 in the low bits of 1024, less 1152
+            const unsigned u = w[j] ^ 0x80808080u;
+            const h2 off = {(half_t)-1152.f, (half_t)-1152.f};
+            o[2 * j] = __builtin_bit_cast(unsigned, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) + off);
+            o[2 * j + 1] = __builtin_bit_cast(unsigned, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) + off);
+        }
+    }
+    return __builtin_bit_cast(h8, make_uint4(o[0], o[1], o[2], o[3]));
+}
+
 }  // namespace bsa

@@ -25,6 +25,11 @@ namespace bsa {
 namespace {
 
 constexpr int CACHED_WAVES = 4;
+constexpr int cached_row_groups(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
+// tiles of 32 tokens that the waves of a tile group take at a time
+constexpr int cached_subtiles(int rg) { return rg == 1 ? 1 : 2; }
+// K, V and the scales of them
+constexpr int cached_set_bytes(int hd, int rg) { return cached_subtiles(rg) * (128 * hd + 256); }
 constexpr float CACHED_LAZY_SUM = 256.f;
 
 struct CachedOperands {
@@ -38,7 +43,8 @@ struct CachedOperands {
     float2 *stats;
     int batch, drafts, heads, key_heads, group;
     int pages, page_shift, width;                // width: of the page table
-    int rows, row_blocks, least, target;         // rows: drafts * group; least: tiles of a chunk; target: units wanted
+    int rows, row_blocks, least, together, target;   // rows: drafts * group; a chunk has `least` tiles or more, a
+                                                 // multiple of `together`; target: units wanted
     int tree_batch;                              // values between the masks of two sequences, 0: one mask for all
     float scale2;
     long long q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head;
@@ -54,15 +60,15 @@ __device__ __forceinline__ int cached_tiles(const CachedOperands &p, int b)
 {
     return (cached_length(p, b) + 31) / 32 + (p.drafts + 31) / 32;
 }
-// inclusive sums over the lanes of a wave
+// inclusive sums over the lanes of a wave, by additions across lanes without LDS (they stand in front of everything else)
 __device__ __forceinline__ int wave_sums(int x)
 {
-    const int l = lane_id();
-#pragma unroll
-    for (int d = 1; d < WAVE; d *= 2) {
-        const int y = __shfl_up(x, d);
-        if (l >= d) x += y;
-    }
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);              // from 1, 2, 4 and 8 lanes below in a row of 16,
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);              // from the last lane of the row below to rows 1 and 3,
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);              // from the last lane of the lower half to the upper
     return x;
 }
 
@@ -75,7 +81,7 @@ __device__ __forceinline__ int cached_chunk(const CachedOperands &p)
         total += __builtin_amdgcn_readlane(wave_sums(b < p.batch ? cached_tiles(p, b) : 0), WAVE - 1);
     }
     const long long per = (total * p.key_heads * p.row_blocks + p.target - 1) / p.target;
-    return (int)(per < p.least ? p.least : per);
+    return ((int)(per < p.least ? p.least : per) + p.together - 1) / p.together * p.together;
 }
 
 struct CachedUnit {
@@ -100,31 +106,15 @@ __device__ __forceinline__ CachedUnit cached_unit(const CachedOperands &p, int c
     return CachedUnit{-1, 0, 0, 0};
 }
 
-// 16 values of 8 bits as 16-bit ones
-template <bool BF, int KIND>
-__device__ __forceinline__ void widen_piece(uint4 raw, uint4 (&out)[2])
-{
-    const unsigned w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        float y[8];
-        widen_held<KIND>(w[2 * half], y);
-        widen_held<KIND>(w[2 * half + 1], y + 4);
-        h8 o;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = narrow_16<BF>(y[j]);
-        out[half] = __builtin_bit_cast(uint4, o);
-    }
-}
-
 template <int HD, bool BF, int KIND, int RG>
 __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(CachedOperands p)
 {
     extern __shared__ __align__(16) unsigned char lds_raw[];
-    constexpr int KS = HD / 16, KG = CACHED_WAVES / RG, BUFFERS = RG > 1 ? 2 : 1, THREADS = 64 * RG;
-    constexpr int WIDTH = cache_value_bytes(KIND), PIECES = 32 * HD * WIDTH / 16, EACH = (PIECES + THREADS - 1) / THREADS;
-    constexpr int TILE = 64 * HD, SET = 2 * TILE + 256;                          // K, V, scales of a 32-token tile
+    constexpr int KS = HD / 16, KG = CACHED_WAVES / RG, BUFFERS = RG > 1 ? 2 : 1, THREADS = 64 * RG, SUBT = cached_subtiles(RG);
+    constexpr int WIDTH = cache_value_bytes(KIND), PIECES = 32 * HD * WIDTH / 16, EACH = SUBT * PIECES / THREADS;
+    constexpr int TILE = 64 * HD, SET = cached_set_bytes(HD, RG), SCALES = 2 * SUBT * TILE;
     constexpr bool SCALED = KIND != CACHE_16;
+    static_assert(EACH * THREADS == SUBT * PIECES && PIECES % 64 == 0, "a wave's pieces lie in one subtile");
     const float NEG_INF = -__builtin_inff();
 
     const int xcd = (int)(blockIdx.x & 7u), turn = (int)(blockIdx.x >> 3);
@@ -142,6 +132,93 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
     unsigned char *set0 = lds_raw + kg * BUFFERS * SET;
     const TileReader rd(set0);
 
+    // page numbers of 64 pages from `window` on, one a lane
+    int window = -1, page_of_lane = -1;
+    uint4 kraw[EACH], vraw[EACH];
+    float sraw[SUBT];
+    int there[SUBT];                             // tokens of the requested tiles that the sequence has in the cache
+    auto subtile_of = [&](int i) { return SUBT == 1 ? 0 : (THREADS * i + 64 * rg) / PIECES; };
+    auto request = [&](int t0) {
+        long long first[SUBT];
+#pragma unroll
+        for (int s = 0; s < SUBT; ++s) {
+            const int t = t0 + s;
+            there[s] = 0;
+            first[s] = 0;
+            if (t >= held || t >= end) continue;
+            const int page_index = t >> (p.page_shift - 5);
+            if (window < 0 || page_index - window >= WAVE) {
+                window = page_index;
+                page_of_lane = window + l < p.width ? p.table[(long long)b * p.width + window + l] : -1;
+            }
+            const int page = __builtin_amdgcn_readlane(page_of_lane, page_index - window);
+            if (page < 0 || page >= p.pages) continue;
+            there[s] = min(32, len - 32 * t);
+            first[s] = (((long long)page * p.key_heads + key_head) << p.page_shift) + ((32 * t) & ((1 << p.page_shift) - 1));
+        }
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int s = subtile_of(i), piece = thread + THREADS * i - PIECES * s;
+            const long long row0 = SUBT == 1 || s == 0 ? first[0] : first[SUBT - 1];
+            if ((SUBT == 1 || s == 0 ? there[0] : there[SUBT - 1]) > 0) {
+                kraw[i] = ldg16_stream(p.keys + row0 * HD * WIDTH + 16 * piece);
+                vraw[i] = ldg16_stream(p.values + row0 * HD * WIDTH + 16 * piece);
+            }
+        }
+        if (SCALED && rg == 0)
+#pragma unroll
+            for (int s = 0; s < SUBT; ++s)
+                if (there[s] > 0) sraw[s] = (l < 32 ? p.key_scales : p.value_scales)[first[s] + (l & 31)];
+    };
+    // 8 values of token r of a tile into the panels that TileReader reads
+    auto put = [&](unsigned char *tile, int r, int piece, uint4 x) {
+        *reinterpret_cast<uint4 *>(tile + 4096 * (piece >> 3) + 128 * r + 16 * ((piece & 7) ^ panel_swizzle(r))) = x;
+    };
+    auto stage = [&](int t0, unsigned char *set) {
+        const uint4 none = make_uint4(0, 0, 0, 0);
+        float *scales = reinterpret_cast<float *>(set + SCALES);
+        // tokens that the sequence does not have are zeros, whatever the page holds
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+            const int s = subtile_of(i), piece = thread + THREADS * i - PIECES * s;
+            const int has = SUBT == 1 || s == 0 ? there[0] : there[SUBT - 1];
+            unsigned char *k_tile = set + s * TILE, *v_tile = set + (SUBT + s) * TILE;
+            if (t0 + s >= held) continue;
+            if (SCALED) {
+                const int r = piece / (HD / 16), c = 2 * (piece % (HD / 16)), swap = (c >> 3) & 1;       // the panels' halves in turn: banks
+                const uint4 kp = r < has ? kraw[i] : none, vp = r < has ? vraw[i] : none;
+                const h8 k0 = widen_held_16<BF, KIND>(kp.x, kp.y), k1 = widen_held_16<BF, KIND>(kp.z, kp.w);
+                const h8 v0 = widen_held_16<BF, KIND>(vp.x, vp.y), v1 = widen_held_16<BF, KIND>(vp.z, vp.w);
+                put(k_tile, r, c + swap, __builtin_bit_cast(uint4, swap ? k1 : k0)), put(k_tile, r, c + 1 - swap, __builtin_bit_cast(uint4, swap ? k0 : k1));
+                put(v_tile, r, c + swap, __builtin_bit_cast(uint4, swap ? v1 : v0)), put(v_tile, r, c + 1 - swap, __builtin_bit_cast(uint4, swap ? v0 : v1));
+            } else {
+                const int r = piece / (HD / 8), c = piece % (HD / 8);
+                put(k_tile, r, c, r < has ? kraw[i] : none);
+                put(v_tile, r, c, r < has ? vraw[i] : none);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < SUBT; ++s) {
+            if (t0 + s < held) {
+                if (SCALED && rg == 0) scales[64 * s + l] = (l & 31) < there[s] ? (l < 32 ? sraw[s] * p.scale2 : sraw[s]) : 0.f;
+                continue;
+            }
+            const int j0 = 32 * (t0 + s - held);
+            constexpr int NEW = 32 * HD / 8;
+#pragma unroll 1
+            for (int piece = thread; piece < NEW; piece += THREADS) {
+                const int r = piece / (HD / 8), c = piece % (HD / 8), j = j0 + r;
+                const bool is = j < p.drafts;
+                const half_t *kr = p.k + b * p.k_batch + j * p.k_token + key_head * p.k_head + 8 * c,
+                             *vr = p.v + b * p.v_batch + j * p.v_token + key_head * p.v_head + 8 * c;
+                put(set + s * TILE, r, c, is ? ldg16(kr) : none);
+                put(set + (SUBT + s) * TILE, r, c, is ? ldg16(vr) : none);
+            }
+            if (SCALED && rg == 0) scales[64 * s + l] = l < 32 ? p.scale2 : 1.f;
+        }
+    };
+    request(begin + kg * SUBT);
+
     // query rows: row = draft * group + head of the group; those behind the last repeat it and are not stored
     const int row = 32 * (rb * RG + rg) + qq, mine = min(row, p.rows - 1), draft = mine / p.group, sub = mine - draft * p.group;
     h8 qop[KS];
@@ -149,190 +226,165 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
 #pragma unroll
     for (int s = 0; s < KS; ++s) qop[s] = as_h8(ldg16(q_row + 16 * s + 8 * h));
 
-    // page numbers of 64 pages from `window` on, one a lane
-    int window = -1, page_of_lane = -1;
-    uint4 kraw[EACH], vraw[EACH];
-    float sraw = 0.f;
-    int there = 0;                               // tokens of the requested tile that the sequence has
-    auto request = [&](int t) {
-        there = 0;
-        if (t >= held) return;
-        const int page_index = t >> (p.page_shift - 5);
-        if (window < 0 || page_index - window >= WAVE) {
-            window = page_index;
-            page_of_lane = window + l < p.width ? p.table[(long long)b * p.width + window + l] : -1;
-        }
-        const int page = __builtin_amdgcn_readlane(page_of_lane, page_index - window);
-        if (page < 0 || page >= p.pages) return;
-        there = min(32, len - 32 * t);
-        const long long first = (((long long)page * p.key_heads + key_head) << p.page_shift) + ((32 * t) & ((1 << p.page_shift) - 1));
-#pragma unroll
-        for (int i = 0; i < EACH; ++i) {
-            const int piece = thread + THREADS * i;
-            if (PIECES % THREADS == 0 || piece < PIECES) {
-                kraw[i] = ldg16_stream(p.keys + first * HD * WIDTH + 16 * piece);
-                vraw[i] = ldg16_stream(p.values + first * HD * WIDTH + 16 * piece);
-            }
-        }
-        if (SCALED && thread < 64) sraw = (thread < 32 ? p.key_scales : p.value_scales)[first + (thread & 31)];
-    };
-    // 8 values of token r of the tile into the panels that TileReader reads
-    auto put = [&](unsigned char *tile, int r, int piece, uint4 x) {
-        *reinterpret_cast<uint4 *>(tile + 4096 * (piece >> 3) + 128 * r + 16 * ((piece & 7) ^ panel_swizzle(r))) = x;
-    };
-    auto stage = [&](int t, unsigned char *set) {
-        const uint4 none = make_uint4(0, 0, 0, 0);
-        float *scales = reinterpret_cast<float *>(set + 2 * TILE);
-        if (t < held) {                          // tokens that the sequence does not have are zeros, whatever the page holds
-#pragma unroll
-            for (int i = 0; i < EACH; ++i) {
-                const int piece = thread + THREADS * i;
-                if (PIECES % THREADS == 0 || piece < PIECES) {
-                    if (SCALED) {
-                        const int r = piece / (HD / 16), c = 2 * (piece % (HD / 16));
-                        uint4 a[2], z[2];
-                        widen_piece<BF, KIND>(r < there ? kraw[i] : none, a);
-                        widen_piece<BF, KIND>(r < there ? vraw[i] : none, z);
-                        put(set, r, c, a[0]), put(set, r, c + 1, a[1]);
-                        put(set + TILE, r, c, z[0]), put(set + TILE, r, c + 1, z[1]);
-                    } else {
-                        const int r = piece / (HD / 8), c = piece % (HD / 8);
-                        put(set, r, c, r < there ? kraw[i] : none);
-                        put(set + TILE, r, c, r < there ? vraw[i] : none);
-                    }
-                }
-            }
-            if (SCALED && thread < 64) scales[thread] = (thread & 31) < there ? (thread < 32 ? sraw * p.scale2 : sraw) : 0.f;
-            return;
-        }
-        const int j0 = 32 * (t - held);
-        constexpr int NEW = 32 * HD / 8;
-        for (int piece = thread; piece < NEW; piece += THREADS) {
-            const int r = piece / (HD / 8), c = piece % (HD / 8), j = j0 + r;
-            const bool is = j < p.drafts;
-            const half_t *kr = p.k + b * p.k_batch + j * p.k_token + key_head * p.k_head + 8 * c,
-                         *vr = p.v + b * p.v_batch + j * p.v_token + key_head * p.v_head + 8 * c;
-            put(set, r, c, is ? ldg16(kr) : none);
-            put(set + TILE, r, c, is ? ldg16(vr) : none);
-        }
-        if (SCALED && thread < 64) scales[thread] = thread < 32 ? p.scale2 : 1.f;
-    };
-
-    float m = NEG_INF, minus_m = 0.f, lsum = 0.f, top = 0.f;                     // top: what the value scales are relative to
+    // Reference point of the exponentials: the row's own m, and `shift`, log2 of a power of two above every value scale so far.  A
+    // weight p t, t the scale of its value row, is then at most 256, whatever the scales are; sum and results are relative
+    // to both alike.
+    float m = NEG_INF, lsum = 0.f, shift = 0.f, most_scale = 0.f, minus_ref = 0.f, most_sum = CACHED_LAZY_SUM;
     bool fresh = true;
     RowTile<HD> oacc;
     clear<HD>(oacc);
-
-    request(begin + kg);
-    const int rounds = (end - begin + KG - 1) / KG;
+    constexpr int ALL = KG * SUBT;
+    const int rounds = (end - begin + ALL - 1) / ALL;
     for (int round = 0; round < rounds; ++round) {
-        const int t = begin + round * KG + kg;
+        const int t0 = begin + round * ALL + kg * SUBT;
         const unsigned buffer = (RG > 1 ? round & 1 : 0) * SET;
         unsigned char *set = set0 + buffer;
-        const bool work = t < end;
-        int have = 0;
-        if (work) {
-            have = t < held ? there : min(32, p.drafts - 32 * (t - held));
-            stage(t, set);
-            request(t + KG < end ? t + KG : held);
+        int have[SUBT];
+        bool any = false, partial = false;
+#pragma unroll
+        for (int s = 0; s < SUBT; ++s) {
+            const int t = t0 + s;
+            have[s] = t >= end ? 0 : t < held ? there[s] : min(32, p.drafts - 32 * (t - held));
+            any = any || have[s] > 0;
+            partial = partial || t >= held || have[s] < 32;
+        }
+        if (t0 < end) {
+            stage(t0, set);
+            request(t0 + ALL);
         }
         if (RG > 1) __syncthreads();
         else wave_lds_fence();
-        if (!work || have <= 0) continue;
-        f16v sacc = {0};
+        if (!any) continue;
+        f16v sacc[SUBT];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) sacc = mfma_16<BF>(rd.rows(buffer, s), qop[s], sacc);
-        const float *scales = reinterpret_cast<const float *>(set + 2 * TILE);
+        for (int s = 0; s < SUBT; ++s) {
+            sacc[s] = f16v{0};
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            if (SCALED) {
-                const f4v ks = *reinterpret_cast<const f4v *>(scales + 8 * g + 4 * h);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sacc[4 * g + j] *= ks[j];
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) sacc[4 * g + j] *= p.scale2;
-            }
+            for (int k = 0; k < KS; ++k) sacc[s] = mfma_16<BF>(rd.rows(buffer + s * TILE, k), qop[k], sacc[s]);
         }
-        const bool drafted = t >= held;
-        unsigned sees = 0xFFFFu;                 // bit v: the key of accumulator value v is seen
-        if (drafted || have < 32) {
-            sees = 0;
-            const int j0 = 32 * (t - held);
-            const unsigned char *mask = p.tree + (long long)b * p.tree_batch + (long long)draft * p.drafts + j0;
-#pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const int r = 8 * (v >> 2) + 4 * h + (v & 3);
-                bool seen = r < have;
-                if (drafted && seen) seen = p.tree != nullptr ? mask[r] != 0 : j0 + r <= draft;
-                sees |= seen ? 1u << v : 0u;
-            }
-#pragma unroll
-            for (int v = 0; v < 16; ++v)
-                if (!((sees >> v) & 1u)) sacc[v] = NEG_INF;
-        }
-        float psum;
-        h8 pop[2];
-        float relative[16];                      // of the value scales
+        const float *scales = reinterpret_cast<const float *>(set + SCALES);
         if (SCALED) {
             float most = 0.f;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f4v vs = *reinterpret_cast<const f4v *>(scales + 32 + 8 * g + 4 * h);
+            for (int s = 0; s < SUBT; ++s)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) relative[4 * g + j] = vs[j], most = fmaxf(most, vs[j]);
-            }
+                for (int g = 0; g < 4; ++g) {
+                    const f4v vs = *reinterpret_cast<const f4v *>(scales + 64 * s + 32 + 8 * g + 4 * h);
+                    most = fmaxf(fmaxf(most, fmaxf(vs[0], vs[1])), fmaxf(vs[2], vs[3]));
+                }
             most = fmaxf(most, at_lane_xor32(most));
-            if (most > top) {                    // the same in all lanes
-                const float keep = top / (2.f * most);
-                top = 2.f * most;                // twice: fewer of these
+            if (most > most_scale) {             // the same in all lanes
+                const float to = (float)__builtin_amdgcn_frexp_expf(most) + 1.f, keep = at_exp2(shift - to);       // twice: fewer of these
+                most_scale = at_exp2(to);
+                shift = to;
+                minus_ref = -(at_finite_or_zero(m) + shift);
+                most_sum = CACHED_LAZY_SUM / most_scale;
+                lsum *= keep;
                 each<HD>(oacc, [&](float x, int) { return x * keep; });
             }
-            const float inv = top > 0.f ? 1.f / top : 0.f;
-#pragma unroll
-            for (int v = 0; v < 16; ++v) relative[v] *= inv;
         }
+        unsigned sees[SUBT];                     // bit v: the key of accumulator value v is seen
+        if (partial) {
+#pragma unroll
+            for (int s = 0; s < SUBT; ++s) {
+                sees[s] = 0;
+                const bool drafted = t0 + s >= held;
+                const int j0 = 32 * (t0 + s - held);
+                const unsigned char *mask = p.tree + (long long)b * p.tree_batch + (long long)draft * p.drafts + j0;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const int r = 8 * (v >> 2) + 4 * h + (v & 3);
+                    bool seen = r < have[s];
+                    if (drafted && seen) seen = p.tree != nullptr ? mask[r] != 0 : j0 + r <= draft;
+                    sees[s] |= seen ? 1u << v : 0u;
+                }
+                asm volatile("" : "+v"(sees[s]));        // as bits of one register: the compiler would keep 16 masks
+            }
+        }
+        // scores, in the exponent's units where `scaled`; a hidden one is -inf only once scaled, whatever the scale's sign
+        auto scale_of = [&](int s, int g) {
+            if (SCALED) return *reinterpret_cast<const f4v *>(scales + 64 * s + 8 * g + 4 * h);
+            return f4v{p.scale2, p.scale2, p.scale2, p.scale2};
+        };
+        if (partial) {
+#pragma unroll
+            for (int s = 0; s < SUBT; ++s)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const f4v ks = scale_of(s, g);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int v = 4 * g + j;
+                        sacc[s][v] = (sees[s] >> v) & 1u ? sacc[s][v] * ks[j] : NEG_INF;
+                    }
+                }
+        }
+        float psum;
+        h8 pop[SUBT][2];
         auto exponentials = [&]() {
             psum = 0.f;
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                const float pv = at_exp2(sacc[v] + minus_m);
-                psum += pv;
-                pop[v >> 3][v & 7] = narrow_16<BF>(SCALED ? pv * relative[v] : pv);
-            }
+            for (int s = 0; s < SUBT; ++s)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f4v ks = scale_of(s, g), vs = {1.f, 1.f, 1.f, 1.f};
+                    if (partial) ks = f4v{1.f, 1.f, 1.f, 1.f};
+                    if (SCALED) vs = *reinterpret_cast<const f4v *>(scales + 64 * s + 32 + 8 * g + 4 * h);
+                    half_t pair[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float pv = at_exp2(__builtin_fmaf(sacc[s][4 * g + j], ks[j], minus_ref));
+                        if (SCALED) psum += pv;
+                        pair[j] = narrow_16<BF>(SCALED ? pv * vs[j] : pv);
+                        pop[s][g >> 1][4 * (g & 1) + j] = pair[j];
+                    }
+                    if (!SCALED) psum = add_pair<BF>(pair[2], pair[3], add_pair<BF>(pair[0], pair[1], psum));
+                }
         };
         // A row moves its reference point by itself, so that its bits are its own: a row beside it, of NaN say, changes nothing.
         bool move = m == NEG_INF;
         if (fresh) psum = 0.f;
         else exponentials();
-        move = move || psum > CACHED_LAZY_SUM;
+        move = move || psum > most_sum;
         if (__builtin_amdgcn_ballot_w64(move) != 0ull) {
             const int other_moves = __builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)move);
             move = move || other_moves != 0;
-            float bm = sacc[0];
+            float bm = NEG_INF;
 #pragma unroll
-            for (int v = 1; v < 16; ++v) bm = fmaxf(bm, sacc[v]);
+            for (int s = 0; s < SUBT; ++s)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    f4v ks = scale_of(s, g);
+                    if (partial) ks = f4v{1.f, 1.f, 1.f, 1.f};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) bm = fmaxf(bm, sacc[s][4 * g + j] * ks[j]);
+                }
             bm = fmaxf(bm, at_lane_xor32(bm));
             const float m_new = move ? fmaxf(m, bm) : m;
             const float keep = m == NEG_INF ? 0.f : at_exp2(m - at_finite_or_zero(m_new));       // nothing accumulated so far: 0
             m = m_new;
-            minus_m = -at_finite_or_zero(m_new);
+            minus_ref = -(at_finite_or_zero(m_new) + shift);
             lsum *= keep;
             each<HD>(oacc, [&](float x, int) { return x * keep; });
             fresh = __builtin_amdgcn_ballot_w64(m != NEG_INF) == 0ull;
             exponentials();
         }
         lsum += psum;
-        const unsigned other = (unsigned)__builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)sees);
-        const unsigned lower = h == 0 ? sees : other, upper = h == 0 ? other : sees;
-        if (weigh_tile<HD, BF>(rd, buffer + TILE, pop, oacc, drafted))
-            add_not_finite<HD, BF>(rd, buffer + TILE, oacc, [&](int r) {
-                return (((r & 4 ? upper : lower) >> (4 * (r >> 3) + (r & 3))) & 1u) != 0u;
-            });
+#pragma unroll
+        for (int s = 0; s < SUBT; ++s) {
+            const unsigned v_tile = buffer + (SUBT + s) * TILE;
+            if (weigh_tile<HD, BF>(rd, v_tile, pop[s], oacc, t0 + s >= held)) {
+                const unsigned other = (unsigned)__builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)sees[s]);
+                const unsigned lower = h == 0 ? sees[s] : other, upper = h == 0 ? other : sees[s];
+                add_not_finite<HD, BF>(rd, v_tile, oacc, [&](int r) {
+                    return (((r & 4 ? upper : lower) >> (4 * (r >> 3) + (r & 3))) & 1u) != 0u;
+                });
+            }
+        }
         if (RG == 1) wave_lds_fence();
     }
     lsum += at_lane_xor32(lsum);
-    if (SCALED) each<HD>(oacc, [&](float x, int) { return x * top; });
+    m += shift;                                  // what sum and results are relative to
 
     // join the tile groups of the workgroup: all but the first park (max, sum) and O^T in LDS
     __syncthreads();
@@ -392,66 +444,73 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
     }
 }
 
-// Joins the chunks of a row: HD / 4 lanes a row and chunk, ROWS rows a workgroup, the chunks of a row dealt to 1024 / ROWS of the
-// lanes in order and summed in order.
-template <int HD, bool BF, int ROWS>
-__global__ __launch_bounds__(32 * HD / 4) void cached_join_kernel(CachedOperands p, int block_rows)
+// Joins the chunks of the rows of a sequence and key head: HD / 4 lanes a row and list, the chunks of a row dealt to `lists` lists,
+// which are then joined pair by pair.  JOIN_BATCH chunks are loaded at a time: with one at a time each waited for the one before (384
+// chunks: 9.8 us).  The order of the sums is given by the number of chunks and of lists.
+constexpr int JOIN_BATCH = 8;
+struct JoinPart {
+    float m, sum;
+    f4v acc;
+    __device__ __forceinline__ void add(float om, float osum, f4v oacc)
+    {
+        const float top = fmaxf(m, om), to = at_finite_or_zero(top), keep = at_exp2(m - to), f = at_exp2(om - to);
+        m = top;
+        sum = sum * keep + osum * f;
+        acc = acc * keep + oacc * f;
+    }
+};
+template <int HD, bool BF>
+__global__ __launch_bounds__(1024) void cached_join_kernel(CachedOperands p, int block_rows, int lists)
 {
-    constexpr int LANES = HD / 4, LISTS = 32 / ROWS;                             // lists of chunks of a row
-    __shared__ float sums[32][HD];
-    __shared__ float2 stats[32];
-    const int chunk = cached_chunk(p);
-    const long long per = (p.rows + ROWS - 1) / ROWS;
-    const long long group = blockIdx.x;
-    const int b = (int)(group / (per * p.key_heads)), rest = (int)(group - b * per * p.key_heads);
-    const int key_head = rest / (int)per, list = (int)threadIdx.x / LANES, lane = (int)threadIdx.x % LANES;
-    const int row = (rest - key_head * (int)per) * ROWS + list / LISTS;
+    constexpr int LANES = HD / 4, GROUPS = 1024 / LANES;
+    __shared__ f4v sums[GROUPS][LANES];
+    __shared__ float2 stats[GROUPS];
+    const int chunk = cached_chunk(p), rows = GROUPS / lists;                    // rows of this workgroup
+    const int per = (p.rows + rows - 1) / rows, group = (int)blockIdx.x;
+    const int key_head = group / per % p.key_heads, b = group / per / p.key_heads;
+    const int place = (int)threadIdx.x / LANES, lane = (int)threadIdx.x % LANES, list = place % lists;
+    const int row = group % per * rows + place / lists;
     const CachedUnit u = cached_unit(p, chunk, -1, b);
-    if (u.parts <= 1) return;                    // the walk has stored the row
-    float m = -__builtin_inff(), lsum = 0.f;
-    f4v acc = {0.f, 0.f, 0.f, 0.f};
-    const bool is = row < p.rows;
-    auto at = [&](int part) {
-        const long long block = ((long long)(u.first + part) * p.key_heads + key_head) * p.row_blocks + row / block_rows;
-        return block * block_rows + row % block_rows;
-    };
-    if (is)
-        for (int part = list % LISTS; part < u.parts; part += LISTS) {
-            const float2 st = p.stats[at(part)];
-            const f4v x = *reinterpret_cast<const f4v *>(p.parts + at(part) * HD + 4 * lane);
-            const float top = fmaxf(m, st.x), to = at_finite_or_zero(top), keep = at_exp2(m - to), f = at_exp2(st.x - to);
-            m = top;
-            lsum = lsum * keep + st.y * f;
-            acc = acc * keep + x * f;
-        }
-    if (LISTS > 1) {
-        *reinterpret_cast<f4v *>(&sums[list][4 * lane]) = acc;
-        if (lane == 0) stats[list] = make_float2(m, lsum);
-        __syncthreads();
-        if (list % LISTS != 0) return;
-        for (int o = 1; o < LISTS; ++o) {
-            const float2 st = stats[list + o];
-            const f4v x = *reinterpret_cast<const f4v *>(&sums[list + o][4 * lane]);
-            const float top = fmaxf(m, st.x), to = at_finite_or_zero(top), keep = at_exp2(m - to), f = at_exp2(st.x - to);
-            m = top;
-            lsum = lsum * keep + st.y * f;
-            acc = acc * keep + x * f;
+    if (u.parts <= 1) return;                    // the walk has stored the rows
+    JoinPart mine = {-__builtin_inff(), 0.f, {0.f, 0.f, 0.f, 0.f}};
+    if (row < p.rows) {
+        const long long stride = (long long)p.key_heads * p.row_blocks * block_rows;
+        const long long first = (((long long)u.first * p.key_heads + key_head) * p.row_blocks + row / block_rows) * block_rows + row % block_rows;
+        for (int part0 = list; part0 < u.parts; part0 += JOIN_BATCH * lists) {
+            float2 st[JOIN_BATCH];
+            f4v x[JOIN_BATCH];
+#pragma unroll
+            for (int i = 0; i < JOIN_BATCH; ++i) {
+                const int part = part0 + i * lists;
+                const long long at = first + stride * (part < u.parts ? part : part0);
+                st[i] = p.stats[at];
+                x[i] = *reinterpret_cast<const f4v *>(p.parts + at * HD + 4 * lane);
+            }
+#pragma unroll
+            for (int i = 0; i < JOIN_BATCH; ++i)
+                if (part0 + i * lists < u.parts) mine.add(st[i].x, st[i].y, x[i]);
         }
     }
-    if (!is) return;
-    const float inv = lsum > 0.f || lsum != lsum ? 1.f / lsum : 0.f;
+    for (int apart = 1; apart < lists; apart *= 2) {
+        if (list % (2 * apart) == apart) {
+            sums[place][lane] = mine.acc;
+            if (lane == 0) stats[place] = make_float2(mine.m, mine.sum);
+        }
+        __syncthreads();
+        if (list % (2 * apart) == 0) mine.add(stats[place + apart].x, stats[place + apart].y, sums[place + apart][lane]);
+    }
+    if (list != 0 || row >= p.rows) return;
+    const float inv = mine.sum > 0.f || mine.sum != mine.sum ? 1.f / mine.sum : 0.f;
     const int draft = row / p.group, sub = row - draft * p.group;
     h4 o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = narrow_16<BF>(acc[j] * inv);
+    for (int j = 0; j < 4; ++j) o[j] = narrow_16<BF>(mine.acc[j] * inv);
     *reinterpret_cast<h4 *>(p.out + (((long long)b * p.drafts + draft) * p.heads + key_head * p.group + sub) * HD + 4 * lane) = o;
 }
 
 // ---- launchers ----------------------------------------------------------------------------------------
-constexpr int CACHED_UNITS = 768;                // wanted in a launch: three workgroups a compute unit
+constexpr int CACHED_UNITS = 512;                // wanted in a launch: two workgroups a compute unit
 constexpr int CACHED_LEAST = 8;                  // tiles of a chunk: two for each wave of RG = 1
-
-int row_groups(int rows) { return rows <= 32 ? 1 : 4; }
 
 CachedOperands operands(const CachedArgs &a)
 {
@@ -468,9 +527,10 @@ CachedOperands operands(const CachedArgs &a)
     p.k_batch = a.k_batch, p.k_token = a.k_token, p.k_head = a.k_head;
     p.v_batch = a.v_batch, p.v_token = a.v_token, p.v_head = a.v_head;
     p.rows = a.drafts * p.group;
-    const int rg = row_groups(p.rows);
+    const int rg = cached_row_groups(p.rows);
     p.row_blocks = (p.rows + 32 * rg - 1) / (32 * rg);
     p.least = CACHED_LEAST;
+    p.together = CACHED_WAVES / rg * cached_subtiles(rg);
     p.target = CACHED_UNITS;
     p.parts = (float *)a.workspace;
     p.stats = (float2 *)(p.parts + cached_attention_parts(a) * a.head_dim);
@@ -481,7 +541,7 @@ template <int HD, bool BF, int KIND, int RG>
 hipError_t walk(const CachedArgs &a, hipStream_t st)
 {
     const CachedOperands p = operands(a);
-    constexpr size_t lds = (CACHED_WAVES / RG) * (RG > 1 ? 2 : 1) * (128 * HD + 256);
+    constexpr size_t lds = (CACHED_WAVES / RG) * (RG > 1 ? 2 : 1) * cached_set_bytes(HD, RG);
     auto kernel = cached_attention_kernel<HD, BF, KIND, RG>;
     if (lds > 65536) {
         const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -491,15 +551,19 @@ hipError_t walk(const CachedArgs &a, hipStream_t st)
     kernel<<<(unsigned)(pairs * p.row_blocks), 64 * CACHED_WAVES, lds, st>>>(p);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess || !cached_attention_splits(a)) return err;
-    const long long rows = (long long)a.batch * a.key_heads * p.rows;
-    if (rows >= 1024) cached_join_kernel<HD, BF, 32><<<(unsigned)((long long)a.batch * a.key_heads * ((p.rows + 31) / 32)), 32 * HD / 4, 0, st>>>(p, 32 * RG);
-    else cached_join_kernel<HD, BF, 1><<<(unsigned)rows, 32 * HD / 4, 0, st>>>(p, 32 * RG);
+    // as many lists as give the machine a workgroup a compute unit
+    constexpr int GROUPS = 1024 / (HD / 4);
+    int lists = 1;
+    auto workgroups = [&]() { return (long long)a.batch * a.key_heads * ((p.rows + GROUPS / lists - 1) / (GROUPS / lists)); };
+    while (lists < GROUPS && workgroups() < 256) lists *= 2;
+    cached_join_kernel<HD, BF><<<(unsigned)workgroups(), 1024, 0, st>>>(p, 32 * RG, lists);
     return hipGetLastError();
 }
 template <int HD, bool BF, int KIND>
 hipError_t walk_rows(const CachedArgs &a, hipStream_t st)
 {
-    return row_groups(a.drafts * (a.heads / a.key_heads)) == 1 ? walk<HD, BF, KIND, 1>(a, st) : walk<HD, BF, KIND, 4>(a, st);
+    const int rg = cached_row_groups(a.drafts * (a.heads / a.key_heads));
+    return rg == 1 ? walk<HD, BF, KIND, 1>(a, st) : rg == 2 ? walk<HD, BF, KIND, 2>(a, st) : walk<HD, BF, KIND, 4>(a, st);
 }
 template <int HD, bool BF>
 hipError_t walk_kind(const CachedArgs &a, hipStream_t st)
@@ -521,13 +585,13 @@ bool cached_attention_splits(const CachedArgs &a) { return most_tiles(a) > CACHE
 // chunks are at most target / (key_heads row_blocks), and every sequence has one that is not.
 long long cached_attention_units(const CachedArgs &a)
 {
-    const int rows = a.drafts * (a.heads / a.key_heads), rg = row_groups(rows), blocks = (rows + 32 * rg - 1) / (32 * rg);
+    const int rows = a.drafts * (a.heads / a.key_heads), rg = cached_row_groups(rows), blocks = (rows + 32 * rg - 1) / (32 * rg);
     return a.batch + (cached_attention_splits(a) ? CACHED_UNITS / (a.key_heads * blocks) : 0);
 }
 long long cached_attention_parts(const CachedArgs &a)
 {
     if (!cached_attention_splits(a)) return 0;
-    const int rows = a.drafts * (a.heads / a.key_heads), rg = row_groups(rows), blocks = (rows + 32 * rg - 1) / (32 * rg);
+    const int rows = a.drafts * (a.heads / a.key_heads), rg = cached_row_groups(rows), blocks = (rows + 32 * rg - 1) / (32 * rg);
     return cached_attention_units(a) * a.key_heads * blocks * 32 * rg;
 }
 size_t cached_attention_workspace_bytes(const CachedArgs &a)

@@ -15,8 +15,10 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/grad_mode.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -51,11 +53,18 @@ struct Entry {
     decltype(&bsa_softmax_backward) softmax_backward;
     decltype(&bsa_attention_forward) attention_forward;
     decltype(&bsa_attention_gradients) attention_gradients;
+    decltype(&bsa_packed_attention_forward) packed_forward;
+    decltype(&bsa_packed_attention_backward) packed_backward;
+    decltype(&bsa_cache_write) cache_write;
+    decltype(&bsa_cache_read) cache_read;
+    decltype(&bsa_cached_attention_workspace_bytes) cached_workspace;
+    decltype(&bsa_cached_attention) cached_attention;
 } lib;
 struct PythonSide {
     PyObject *matmul, *softmax, *attention;                                     // autograd Functions' apply
     PyObject *plan_matmul, *plan_weight, *plan_softmax, *plan_softmax_backward, *plan_attention, *plan_attention_backward;
     PyObject *run_matmul, *run_weight, *run_softmax_backward, *run_attention_backward;      // without a plan
+    PyObject *packed, *run_packed_backward;
     PyObject *failed;
     PyDictObject *settings[2];               // of the modules whose globals decide routes
     PyObject *name_plans, *name_row, *name_col, *modes[3];
@@ -785,6 +794,281 @@ PyObject *attention(PyObject *, PyObject *const *args, Py_ssize_t nargs)    // q
     END_HANDLE_TH_ERRORS
 }
 
+// ---- packed sequences and paged caches -------------------------------------------------------------------
+// A dense CUDA tensor of the current device, contiguous or not
+bool plain_strided(const Tensor &t)
+{
+    static const uint64_t allowed = c10::DispatchKeySet({c10::DispatchKey::CUDA, c10::DispatchKey::AutogradCUDA,
+                                                         c10::DispatchKey::AutocastCUDA, c10::DispatchKey::ADInplaceOrView}).raw_repr();
+    return t.defined() && (t.key_set().raw_repr() & ~allowed) == 0 && on_current_device(t);
+}
+bool half_type(at::ScalarType t) { return t == at::kHalf || t == at::kBFloat16; }
+int code_of(at::ScalarType t)
+{
+    return t == at::kFloat ? BSA_F32 : t == at::kHalf ? BSA_F16 : t == at::kBFloat16 ? BSA_BF16 : t == at::kChar ? BSA_I8
+         : t == at::kFloat8_e4m3fn ? BSA_E4M3 : -1;
+}
+// packed.rows_of: the kernels read it in place
+bool readable_rows(const Tensor &t)
+{
+    if (t.dim() < 2 || t.stride(-1) != 1 || !at_16_bytes(t)) return false;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+        if (t.size(i) > 1 && ((t.stride(i) & 7) != 0 || t.stride(i) > (1 << 24))) return false;
+    return true;
+}
+int64_t stride_of(const Tensor &t, int64_t i) { return t.size(i) > 1 ? t.stride(i) : 0; }
+bool index_tensor(const Tensor &t, int64_t dims) { return t.scalar_type() == at::kInt && t.dim() == dims && plain(t) && on_current_device(t); }
+// packed.check_heads
+bool heads_fit(const Tensor &q, const Tensor &k, const Tensor &v, int64_t dims)
+{
+    for (const Tensor *t : {&q, &k, &v})
+        if (!plain_strided(*t) || t->dim() != dims || t->scalar_type() != q.scalar_type() || !readable_rows(*t) || forward_mode(*t)) return false;
+    const int64_t dim = q.size(-1);
+    if (!half_type(q.scalar_type()) || (dim != 64 && dim != 128) || k.sizes() != v.sizes() || k.size(-1) != dim) return false;
+    if (q.sizes().slice(0, dims - 2) != k.sizes().slice(0, dims - 2)) return false;
+    return k.size(-2) >= 1 && q.size(-2) >= 1 && q.size(-2) % k.size(-2) == 0;
+}
+bool number(PyObject *x) { return PyFloat_CheckExact(x) || PyLong_CheckExact(x); }
+bool tensors(PyObject *const *args, int n)
+{
+    for (int i = 0; i < n; ++i)
+        if (!THPVariable_CheckExact(args[i])) return false;
+    return true;
+}
+void launched(int status)
+{
+    if (status == 0) return;
+    py::gil_scoped_acquire gil;
+    PyObject *none = PyObject_CallFunction(python.failed, "iOO", status, Py_None, Py_None);
+    if (none != nullptr) {                   // it raises
+        Py_DECREF(none);
+        TORCH_CHECK(false, "bsa status ", status);
+    }
+    raise_pending();
+}
+
+// sparse/packed.py, PackedAttention.backward
+struct PackedNode : public Node {
+    SavedVariable q_, k_, v_, out_, lse_, offsets_;
+    double scale;
+    bool causal;
+    std::string name() const override { return "PackedAttentionBackward"; }
+    void release_variables() override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *s : {&q_, &k_, &v_, &out_, &lse_, &offsets_}) s->reset_data();
+    }
+    variable_list apply(variable_list &&grads) override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        const Tensor q = q_.unpack(), k = k_.unpack(), v = v_.unpack(), out = out_.unpack(getptr()), lse = lse_.unpack(), offsets = offsets_.unpack();
+        Tensor dout = grads[0].defined() ? grads[0] : node_zeros();
+        const bool dkdv = task_should_compute_output(1) || task_should_compute_output(2);
+        variable_list result;
+        {
+            at::AutoGradMode off(false);
+            if (plain_strided(dout) && !readable_rows(dout)) dout = dout.clone(at::MemoryFormat::Contiguous);
+            bool direct = heads_fit(q, k, v, 3) && plain_strided(dout) && readable_rows(dout) && plain(out) && on_current_device(out) &&
+                          plain(lse) && on_current_device(lse) && index_tensor(offsets, 1) && offsets.numel() >= 2 && q.size(0) > 0;
+            direct = direct && dout.sizes() == q.sizes() && out.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() &&
+                     out.scalar_type() == q.scalar_type() && lse.scalar_type() == at::kFloat && lse.dim() == 2 &&
+                     lse.size(0) == q.size(1) && lse.size(1) == q.size(0);
+            if (!direct) {
+                py::gil_scoped_acquire gil;
+                Borrow pq(q), pk(k), pv(v), pd(dout), po(out), pl(lse), pf(offsets);
+                py::object s = py::float_(scale);
+                PyObject *got = PyObject_CallFunctionObjArgs(python.run_packed_backward, pq.get(), pk.get(), pv.get(), pd.get(), po.get(), pl.get(),
+                                                             pf.get(), s.ptr(), py_bool(causal), py_bool(dkdv), nullptr);
+                if (got == nullptr) raise_pending();
+                py::tuple t = py::reinterpret_steal<py::tuple>(got);
+                for (auto x : t) result.push_back(x.is_none() ? Tensor() : THPVariable_Unpack(x.ptr()));
+            } else {
+                Tensor dq = at::empty(q.sizes(), q.options()), delta = at::empty(lse.sizes(), lse.options()), dk, dv;
+                if (dkdv) {
+                    dk = at::empty(k.sizes(), k.options());
+                    dv = at::empty(v.sizes(), v.options());
+                }
+                const int64_t strides[8] = {stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0), stride_of(v, 1),
+                                            stride_of(dout, 0), stride_of(dout, 1)};
+                launched(lib.packed_backward(code_of(q.scalar_type()), q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(),
+                                             lse.data_ptr<float>(), delta.data_ptr<float>(), dq.data_ptr(), dkdv ? dk.data_ptr() : nullptr,
+                                             dkdv ? dv.data_ptr() : nullptr, offsets.data_ptr<int32_t>(), (int)q.size(0),
+                                             (int)(offsets.numel() - 1), (int)q.size(1), (int)k.size(1), (int)q.size(2), strides, (float)scale,
+                                             causal, current_stream()));
+                result = {dq, dk, dv};
+            }
+        }
+        if (at::GradMode::is_enabled()) {    // asked for a graph of the gradients: there is none, and who differentiates them is told
+            for (Tensor &t : result)
+                if (t.defined()) t.set_requires_grad(true);
+            result = torch::autograd::DelayedError("trying to differentiate twice a function that was marked with @once_differentiable",
+                                                   (int64_t)result.size()).apply(std::move(result));
+        }
+        return result;
+    }
+    Tensor node_zeros() const { return input_metadata(0).zeros_like(); }
+};
+
+PyObject *packed_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs)     // q, k, v, offsets, scale, causal
+{
+    HANDLE_TH_ERRORS
+    const int causal = nargs == 6 ? truth(args[5]) : -1;
+    if (causal < 0 || !number(args[4]) || !tensors(args, 4) || !plain_thread()) return general(python.packed, args, nargs);
+    const Tensor &q = THPVariable_Unpack(args[0]), &k = THPVariable_Unpack(args[1]), &v = THPVariable_Unpack(args[2]),
+                 &offsets = THPVariable_Unpack(args[3]);
+    if (!heads_fit(q, k, v, 3) || !index_tensor(offsets, 1) || offsets.numel() < 2 || q.size(0) < 1) return general(python.packed, args, nargs);
+    const double scale = PyFloat_AsDouble(args[4]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    std::shared_ptr<PackedNode> node;
+    if (needs_grad({&q, &k, &v})) {
+        node = std::shared_ptr<PackedNode>(new PackedNode(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(q, k, v));
+        node->q_ = SavedVariable(q, false);
+        node->k_ = SavedVariable(k, false);
+        node->v_ = SavedVariable(v, false);
+        node->offsets_ = SavedVariable(offsets, false);
+        node->scale = scale;
+        node->causal = causal;
+    }
+    Tensor out, lse;
+    {
+        py::gil_scoped_release unlocked;
+        out = at::empty(q.sizes(), q.options());
+        if (node) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+        const int64_t strides[6] = {stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0), stride_of(v, 1)};
+        launched(lib.packed_forward(code_of(q.scalar_type()), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+                                    node ? lse.data_ptr<float>() : nullptr, offsets.data_ptr<int32_t>(), (int)q.size(0),
+                                    (int)(offsets.numel() - 1), (int)q.size(1), (int)k.size(1), (int)q.size(2), strides, (float)scale, causal,
+                                    current_stream()));
+    }
+    if (node) {
+        torch::autograd::set_history(out, node);
+        node->out_ = SavedVariable(out, true);
+        node->lse_ = SavedVariable(lse, false);
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// What a KeyValueCache holds, as its calls need it
+struct HeldCache {
+    Tensor keys, values, key_scales, value_scales;
+    int pages, heads, head_dim, page, code;
+    const float *scales(const Tensor &t) const { return t.defined() ? t.data_ptr<float>() : nullptr; }
+};
+constexpr const char *CACHE_CAPSULE = "bsa_cache";
+HeldCache *cache_of(PyObject *capsule)
+{
+    return PyCapsule_IsValid(capsule, CACHE_CAPSULE) ? static_cast<HeldCache *>(PyCapsule_GetPointer(capsule, CACHE_CAPSULE)) : nullptr;
+}
+PyObject *new_cache(PyObject *, PyObject *args)      // keys, values, key_scales, value_scales (tensors or None)
+{
+    HANDLE_TH_ERRORS
+    PyObject *t[4];
+    if (!PyArg_ParseTuple(args, "OOOO", &t[0], &t[1], &t[2], &t[3])) return nullptr;
+    auto held = std::make_unique<HeldCache>();
+    Tensor *into[4] = {&held->keys, &held->values, &held->key_scales, &held->value_scales};
+    for (int i = 0; i < 4; ++i)
+        if (t[i] != Py_None) *into[i] = THPVariable_Unpack(t[i]);
+    held->pages = (int)held->keys.size(0), held->heads = (int)held->keys.size(1), held->page = (int)held->keys.size(2);
+    held->head_dim = (int)held->keys.size(3), held->code = code_of(held->keys.scalar_type());
+    return PyCapsule_New(held.release(), CACHE_CAPSULE, [](PyObject *capsule) {
+        delete static_cast<HeldCache *>(PyCapsule_GetPointer(capsule, CACHE_CAPSULE));
+    });
+    END_HANDLE_TH_ERRORS
+}
+
+// The next three answer None where the Python side has to look at the call.
+PyObject *cache_write(PyObject *, PyObject *const *args, Py_ssize_t nargs)  // capsule, k, v, slots
+{
+    HANDLE_TH_ERRORS
+    HeldCache *c = nargs == 4 ? cache_of(args[0]) : nullptr;
+    if (c == nullptr || !tensors(args + 1, 3) || !plain_thread()) Py_RETURN_NONE;
+    const Tensor &k = THPVariable_Unpack(args[1]), &v = THPVariable_Unpack(args[2]), &slots = THPVariable_Unpack(args[3]);
+    for (const Tensor *t : {&k, &v})
+        if (!plain_strided(*t) || !half_type(t->scalar_type()) || t->scalar_type() != k.scalar_type() || t->dim() != 3 || t->size(1) != c->heads ||
+            t->size(2) != c->head_dim || t->size(0) != k.size(0) || !readable_rows(*t))
+            Py_RETURN_NONE;
+    if (!on_current_device(c->keys) || !index_tensor(slots, 1) || slots.numel() != k.size(0) || k.size(0) > (1 << 30)) Py_RETURN_NONE;
+    const int code = code_of(k.scalar_type());
+    if (c->code != BSA_I8 && c->code != BSA_E4M3 && c->code != code) Py_RETURN_NONE;
+    {
+        py::gil_scoped_release unlocked;
+        const int64_t strides[4] = {stride_of(k, 0), stride_of(k, 1), stride_of(v, 0), stride_of(v, 1)};
+        launched(lib.cache_write(code, c->code, k.data_ptr(), v.data_ptr(), slots.data_ptr<int32_t>(), c->keys.data_ptr(), c->values.data_ptr(),
+                                 const_cast<float *>(c->scales(c->key_scales)), const_cast<float *>(c->scales(c->value_scales)), (int)k.size(0),
+                                 c->heads, c->head_dim, c->pages, c->page, strides, current_stream()));
+    }
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *cache_read(PyObject *, PyObject *const *args, Py_ssize_t nargs)   // capsule, slots, dtype
+{
+    HANDLE_TH_ERRORS
+    HeldCache *c = nargs == 3 ? cache_of(args[0]) : nullptr;
+    if (c == nullptr || !tensors(args + 1, 1) || !THPDtype_Check(args[2]) || !plain_thread()) Py_RETURN_NONE;
+    const Tensor &slots = THPVariable_Unpack(args[1]);
+    const at::ScalarType type = reinterpret_cast<THPDtype *>(args[2])->scalar_type;
+    if (!(half_type(type) || type == at::kFloat) || !on_current_device(c->keys) || !index_tensor(slots, 1) || slots.numel() > (1 << 30)) Py_RETURN_NONE;
+    Tensor k, v;
+    {
+        py::gil_scoped_release unlocked;
+        k = at::empty({slots.numel(), c->heads, c->head_dim}, c->keys.options().dtype(type));
+        v = at::empty(k.sizes(), k.options());
+        launched(lib.cache_read(code_of(type), c->code, c->keys.data_ptr(), c->values.data_ptr(), c->scales(c->key_scales), c->scales(c->value_scales),
+                                slots.data_ptr<int32_t>(), k.data_ptr(), v.data_ptr(), (int)slots.numel(), c->heads, c->head_dim, c->pages, c->page,
+                                current_stream()));
+    }
+    return PyTuple_Pack(2, py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(k))).ptr(),
+                        py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(v))).ptr());
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *cached_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs)     // q, k, v, capsule, pages, lengths, tree, scale
+{
+    HANDLE_TH_ERRORS
+    HeldCache *c = nargs == 8 ? cache_of(args[3]) : nullptr;
+    if (c == nullptr || !tensors(args, 3) || !tensors(args + 4, 2) || !number(args[7]) || !plain_thread()) Py_RETURN_NONE;
+    if (args[6] != Py_None && !THPVariable_CheckExact(args[6])) Py_RETURN_NONE;
+    const Tensor &q = THPVariable_Unpack(args[0]), &k = THPVariable_Unpack(args[1]), &v = THPVariable_Unpack(args[2]),
+                 &pages = THPVariable_Unpack(args[4]), &lengths = THPVariable_Unpack(args[5]);
+    const Tensor tree = args[6] == Py_None ? Tensor() : THPVariable_Unpack(args[6]);
+    const double scale = PyFloat_AsDouble(args[7]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    if (!heads_fit(q, k, v, 4) || !on_current_device(c->keys) || k.size(2) != c->heads || q.size(3) != c->head_dim) Py_RETURN_NONE;
+    const int code = code_of(q.scalar_type());
+    if (c->code != BSA_I8 && c->code != BSA_E4M3 && c->code != code) Py_RETURN_NONE;
+    const int64_t batch = q.size(0), drafts = q.size(1);
+    if (batch < 1 || drafts < 1 || drafts > 1024 || batch > (1 << 20) || pages.size(-1) > (1 << 24)) Py_RETURN_NONE;
+    if (!index_tensor(pages, 2) || !index_tensor(lengths, 1) || pages.size(0) != batch || lengths.numel() != batch) Py_RETURN_NONE;
+    bool shared = false;
+    if (tree.defined()) {
+        if (!plain(tree) || !on_current_device(tree) || tree.scalar_type() != at::kBool) Py_RETURN_NONE;
+        shared = tree.dim() == 2;
+        if (!(shared ? tree.size(0) == drafts && tree.size(1) == drafts
+                     : tree.dim() == 3 && tree.size(0) == batch && tree.size(1) == drafts && tree.size(2) == drafts))
+            Py_RETURN_NONE;
+    }
+    Tensor out;
+    {
+        py::gil_scoped_release unlocked;
+        out = at::empty(q.sizes(), q.options());
+        const int heads = (int)q.size(2), width = (int)pages.size(1);
+        const size_t need = lib.cached_workspace((int)batch, (int)drafts, heads, c->heads, c->head_dim, width, c->page);
+        const Tensor workspace = at::empty({(int64_t)need}, q.options().dtype(at::kByte));
+        const int64_t strides[9] = {stride_of(q, 0), stride_of(q, 1), stride_of(q, 2), stride_of(k, 0), stride_of(k, 1), stride_of(k, 2),
+                                    stride_of(v, 0), stride_of(v, 1), stride_of(v, 2)};
+        launched(lib.cached_attention(code, c->code, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), c->keys.data_ptr(),
+                                      c->values.data_ptr(), c->scales(c->key_scales), c->scales(c->value_scales), pages.data_ptr<int32_t>(),
+                                      lengths.data_ptr<int32_t>(), tree.defined() ? static_cast<const uint8_t *>(tree.data_ptr()) : nullptr, shared,
+                                      (int)batch, (int)drafts, heads, c->heads, c->head_dim, c->pages, c->page, width, strides, (float)scale,
+                                      need ? workspace.data_ptr() : nullptr, need, current_stream()));
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 // entry points (addresses by name), Python functions (by name), the two modules' dicts
 PyObject *setup(PyObject *, PyObject *args)
 {
@@ -809,6 +1093,12 @@ PyObject *setup(PyObject *, PyObject *args)
     address("bsa_softmax_backward", lib.softmax_backward);
     address("bsa_attention_forward", lib.attention_forward);
     address("bsa_attention_gradients", lib.attention_gradients);
+    address("bsa_packed_attention_forward", lib.packed_forward);
+    address("bsa_packed_attention_backward", lib.packed_backward);
+    address("bsa_cache_write", lib.cache_write);
+    address("bsa_cache_read", lib.cache_read);
+    address("bsa_cached_attention_workspace_bytes", lib.cached_workspace);
+    address("bsa_cached_attention", lib.cached_attention);
     auto function = [&](const char *name, PyObject *&f) {
         PyObject *x = PyDict_GetItemString(functions, name);
         if (x == nullptr) PyErr_Format(PyExc_KeyError, "%s", name);
@@ -828,6 +1118,8 @@ PyObject *setup(PyObject *, PyObject *args)
     function("run_weight", python.run_weight);
     function("run_softmax_backward", python.run_softmax_backward);
     function("run_attention_backward", python.run_attention_backward);
+    function("packed", python.packed);
+    function("run_packed_backward", python.run_packed_backward);
     function("failed", python.failed);
     Py_INCREF(first);
     Py_INCREF(second);
@@ -852,6 +1144,12 @@ PyMethodDef methods[] = {
     {"matmul", (PyCFunction)(void (*)(void))matmul, METH_FASTCALL, "matmul(a, b, mode, layout, trans_a=False, trans_b=False)"},
     {"softmax", (PyCFunction)(void (*)(void))softmax, METH_FASTCALL, "softmax(x, layout, scale, causal)"},
     {"attention", (PyCFunction)(void (*)(void))attention, METH_FASTCALL, "attention(q, k, v, layout, scale, causal)"},
+    {"packed_attention", (PyCFunction)(void (*)(void))packed_attention, METH_FASTCALL, "packed_attention(q, k, v, offsets, scale, causal)"},
+    {"new_cache", new_cache, METH_VARARGS, nullptr},
+    {"cache_write", (PyCFunction)(void (*)(void))cache_write, METH_FASTCALL, "cache_write(cache, k, v, slots)"},
+    {"cache_read", (PyCFunction)(void (*)(void))cache_read, METH_FASTCALL, "cache_read(cache, slots, dtype)"},
+    {"cached_attention", (PyCFunction)(void (*)(void))cached_attention, METH_FASTCALL,
+     "cached_attention(q, k, v, cache, pages, lengths, tree, scale)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "bsa_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -23,7 +23,8 @@ _HELD = {torch.float16: _k.BSA_F16, torch.bfloat16: _k.BSA_BF16, **_QUANTISED}
 class KeyValueCache:
     """``pages`` pages of ``page`` tokens for ``heads`` key heads: ``keys``, ``values`` ``[pages, heads, page, head_dim]`` of
     ``dtype`` (int8, float8_e4m3fn, float16 or bfloat16) and, for the 8-bit types, ``key_scales``, ``value_scales``
-    ``[pages, heads, page]`` in float32 (else ``None``).  A token's place is its slot, ``page number * page + place``."""
+    ``[pages, heads, page]`` in float32 (else ``None``).  A token's place is its slot, ``page number * page + place``.  The
+    tensors may be written to, not replaced."""
 
     def __init__(self, pages: int, heads: int, head_dim: int, dtype: torch.dtype = torch.float8_e4m3fn, page: int = 64, device=None):
         if dtype not in _HELD:
@@ -41,10 +42,22 @@ class KeyValueCache:
             device = torch.device("cuda", torch.cuda.current_device())
         self.pages, self.heads, self.head_dim, self.dtype, self.page, self.device = pages, heads, head_dim, dtype, page, device
         shape = (pages, heads, page)
-        self.keys, self.values = (torch.empty(shape + (head_dim,), dtype=dtype, device=device) for _ in range(2))
-        self.key_scales = self.value_scales = None
-        if dtype in _QUANTISED:
-            self.key_scales, self.value_scales = (torch.empty(shape, dtype=torch.float32, device=device) for _ in range(2))
+        held = [torch.empty(shape + (head_dim,), dtype=dtype, device=device) for _ in range(2)]
+        held += [torch.empty(shape, dtype=torch.float32, device=device) if dtype in _QUANTISED else None for _ in range(2)]
+        self._held, self._native = tuple(held), _k.host_calls.new_cache(*held)
+
+    keys = property(lambda self: self._held[0])
+    values = property(lambda self: self._held[1])
+    key_scales = property(lambda self: self._held[2])
+    value_scales = property(lambda self: self._held[3])
+
+    def __getstate__(self):
+        return {name: value for name, value in self.__dict__.items() if name != "_native"}
+
+    def __setstate__(self, state):
+        self.__dict__.update(state)
+        self.device = self.keys.device
+        self._native = _k.host_calls.new_cache(*self._held)
 
     def _tensors(self):
         scales = (self.key_scales, self.value_scales)
@@ -58,6 +71,8 @@ class KeyValueCache:
         the scale is the row's largest magnitude over 127 or 448, values are rounded to the nearest, ties to even.  Rows
         with a negative slot (refused drafts, padding) or one behind the cache are left out; no two rows of a call may have the same
         slot.  A row with an infinity or a NaN is kept as NaN.  Not differentiable."""
+        if _k.host_calls.cache_write(self._native, k, v, slots):
+            return
         for t, name in ((k, "k"), (v, "v")):
             if t.dtype not in (torch.float16, torch.bfloat16) or t.dtype != k.dtype:
                 raise TypeError(f"k and v must both be float16 or both bfloat16, got {name}: {t.dtype}")
@@ -78,6 +93,9 @@ class KeyValueCache:
     def read(self, slots: torch.Tensor, dtype: torch.dtype) -> Tuple[torch.Tensor, torch.Tensor]:
         """Keys and values at ``slots``, ``[tokens, heads, head_dim]`` each, in float32, float16 or bfloat16; zeros for a slot that is
         negative or behind the cache."""
+        rows = _k.host_calls.cache_read(self._native, slots, dtype)
+        if rows is not None:
+            return rows
         if dtype not in _ROWS:
             raise TypeError(f"rows are read as float32, float16 or bfloat16, got {dtype}")
         check_index(slots, "slots", self.device, 1)
@@ -98,9 +116,12 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: K
     many tokens it has in them, both int32 on the GPU.  ``tree``, bool ``[n, n]`` or ``[batch, n, n]``: whether new token ``i`` sees new
     token ``j`` (itself too, where it should); without it they are a chain, ``j <= i``.  ``n = 1`` is a decode step.  Every new token sees
     the whole cached part of its sequence; one that sees nothing gets zeros.  At most 1024 new tokens a sequence.  Not differentiable."""
-    check_heads(q, k, v, 4)
     if not isinstance(cache, KeyValueCache):
         raise TypeError(f"cache must be a KeyValueCache, got {type(cache).__name__}")
+    out = _k.host_calls.cached_attention(q, k, v, cache._native, pages, lengths, tree, scale)
+    if out is not None:
+        return out
+    check_heads(q, k, v, 4)
     batch, drafts, heads, dim = q.shape
     if (cache.heads, cache.head_dim) != (k.size(2), dim) or cache.device != q.device:
         raise ValueError(f"k {tuple(k.shape)} on {k.device} does not fit a cache of {cache.heads} heads of {cache.head_dim} on {cache.device}")

@@ -73,7 +73,7 @@ def _forward(q, k, v, offsets, scale, causal, with_lse):
     return out, lse
 
 
-def _backward(q, k, v, dout, out, lse, offsets, scale, causal, with_dkdv):
+def run_backward(q, k, v, dout, out, lse, offsets, scale, causal, with_dkdv):
     tokens, heads, dim = q.shape
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2)) if with_dkdv else (None, None)
@@ -103,8 +103,15 @@ class PackedAttention(torch.autograd.Function):
     @once_differentiable
     def backward(ctx: Any, dout: torch.Tensor) -> Tuple[Optional[torch.Tensor], ...]:
         q, k, v, out, lse, offsets = ctx.saved_tensors
-        grads = _backward(q, k, v, dout, out, lse, offsets, ctx.scale, ctx.causal, any(ctx.needs_input_grad[1:3]))
+        grads = run_backward(q, k, v, dout, out, lse, offsets, ctx.scale, ctx.causal, any(ctx.needs_input_grad[1:3]))
         return grads + (None, None, None)
+
+
+def general(q, k, v, offsets, scale, causal):
+    """The call without the native side, which hands over whatever it does not take."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
+        return PackedAttention.apply(q, k, v, offsets, scale, causal)
+    return _forward(q, k, v, offsets, scale, causal, False)[0]
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, scale: float = 1.0,
@@ -117,6 +124,4 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     Tokens outside every sequence (the padding of a batch) are not read; their results and gradients are zero.  Operands may be
     slices of a larger tensor (a fused projection); they are copied only where a row does not start at a multiple of 16 bytes.
     Differentiable once in ``q``, ``k`` and ``v``, with the same bits in every call."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
-        return PackedAttention.apply(q, k, v, offsets, scale, causal)
-    return _forward(q, k, v, offsets, scale, causal, False)[0]
+    return _k.host_calls.packed_attention(q, k, v, offsets, scale, causal)
