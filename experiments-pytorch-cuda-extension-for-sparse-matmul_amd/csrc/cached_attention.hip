@@ -29,7 +29,7 @@ constexpr int cached_row_groups(int rows) { return rows <= 32 ? 1 : rows <= 64 ?
 // tiles of 32 tokens that the waves of a tile group take at a time
 constexpr int cached_subtiles(int rg) { return rg == 1 ? 1 : 2; }
 // K, V and the scales of them
-constexpr int cached_set_bytes(int hd, int rg) { return cached_subtiles(rg) * (128 * hd + 256); }
+constexpr int cached_set_bytes(int hd, int rg) { return cached_subtiles(rg) * (128 * hd + 256) + 256; }
 constexpr float CACHED_LAZY_SUM = 256.f;
 
 struct CachedOperands {
@@ -56,10 +56,6 @@ __device__ __forceinline__ int cached_length(const CachedOperands &p, int b)
     const long long room = (long long)p.width << p.page_shift;
     return n < 0 ? 0 : n > room ? (int)room : n;
 }
-__device__ __forceinline__ int cached_tiles(const CachedOperands &p, int b)
-{
-    return (cached_length(p, b) + 31) / 32 + (p.drafts + 31) / 32;
-}
 // inclusive sums over the lanes of a wave, by additions across lanes without LDS (they stand in front of everything else)
 __device__ __forceinline__ int wave_sums(int x)
 {
@@ -72,38 +68,47 @@ __device__ __forceinline__ int wave_sums(int x)
     return x;
 }
 
-// tiles of a chunk: as many units as wanted, none shorter than `least` tiles
-__device__ __forceinline__ int cached_chunk(const CachedOperands &p)
+// the largest of lanes 32 .. 63, in lane 63
+__device__ __forceinline__ float upper_half_most(float x)
 {
-    long long total = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += WAVE) {
-        const int b = b0 + lane_id();
-        total += __builtin_amdgcn_readlane(wave_sums(b < p.batch ? cached_tiles(p, b) : 0), WAVE - 1);
-    }
-    const long long per = (total * p.key_heads * p.row_blocks + p.target - 1) / p.target;
-    return ((int)(per < p.least ? p.least : per) + p.together - 1) / p.together * p.together;
+    auto with = [&](int y) { x = fmaxf(x, __int_as_float(y)); };
+    with(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x111, 0xF, 0xF, false));
+    with(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x112, 0xF, 0xF, false));
+    with(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x114, 0xF, 0xF, false));
+    with(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x118, 0xF, 0xF, false));
+    with(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), 0x142, 0xA, 0xF, false));
+    return x;
 }
 
+// How the lengths cut the work: the tiles of a chunk, as many units as wanted and none shorter than `least` tiles, and the
+// sequence of a unit, or, with `unit` < 0, the units of sequence `of`.  Up to 64 sequences the lengths are loaded once.
 struct CachedUnit {
-    int b, part, parts, first;                   // first: unit of part 0; b < 0: nothing to do
+    int b, len, part, parts, first, chunk;       // first: unit of part 0; b < 0: nothing to do
 };
-// sequence of a unit; or, with `unit` < 0, the units of sequence `of`
-__device__ __forceinline__ CachedUnit cached_unit(const CachedOperands &p, int chunk, int unit, int of)
+__device__ __forceinline__ CachedUnit cached_unit(const CachedOperands &p, int unit, int of)
 {
+    const int l = lane_id(), drafted = (p.drafts + 31) / 32;
+    auto length = [&](int b0) { return b0 + l < p.batch ? cached_length(p, b0 + l) : 0; };
+    auto tiles = [&](int b0, int len) { return b0 + l < p.batch ? (len + 31) / 32 + drafted : 0; };
+    int len = length(0);
+    long long total = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += WAVE)
+        total += __builtin_amdgcn_readlane(wave_sums(tiles(b0, b0 == 0 ? len : length(b0))), WAVE - 1);
+    const long long wanted = (total * p.key_heads * p.row_blocks + p.target - 1) / p.target;
+    const int chunk = ((int)(wanted < p.least ? p.least : wanted) + p.together - 1) / p.together * p.together;
     int before = 0;
     for (int b0 = 0; b0 < p.batch; b0 += WAVE) {
-        const int b = b0 + lane_id();
-        const int mine = b < p.batch ? (cached_tiles(p, b) + chunk - 1) / chunk : 0, upto = before + wave_sums(mine);
-        const bool hit = unit >= 0 ? upto - mine <= unit && unit < upto : b == of;
-        const unsigned long long found = __builtin_amdgcn_ballot_w64(hit);
+        if (b0 > 0) len = length(b0);
+        const int mine = (tiles(b0, len) + chunk - 1) / chunk, upto = before + wave_sums(mine);
+        const unsigned long long found = __builtin_amdgcn_ballot_w64(unit >= 0 ? upto - mine <= unit && unit < upto : b0 + l == of);
         if (found != 0ull) {
             const int at = __builtin_ctzll(found);
             const int parts = __builtin_amdgcn_readlane(mine, at), first = __builtin_amdgcn_readlane(upto, at) - parts;
-            return CachedUnit{b0 + at, unit - first, parts, first};
+            return CachedUnit{b0 + at, __builtin_amdgcn_readlane(len, at), unit - first, parts, first, chunk};
         }
         before = __builtin_amdgcn_readlane(upto, WAVE - 1);
     }
-    return CachedUnit{-1, 0, 0, 0};
+    return CachedUnit{-1, 0, 0, 0, 0, chunk};
 }
 
 template <int HD, bool BF, int KIND, int RG>
@@ -120,10 +125,9 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
     const int xcd = (int)(blockIdx.x & 7u), turn = (int)(blockIdx.x >> 3);
     const int rb = turn % p.row_blocks, pair = turn / p.row_blocks * 8 + xcd;    // row blocks of a chunk share an L2
     const int key_head = pair % p.key_heads, unit = pair / p.key_heads;
-    const int chunk = cached_chunk(p);
-    const CachedUnit u = cached_unit(p, chunk, unit, 0);
+    const CachedUnit u = cached_unit(p, unit, 0);
     if (u.b < 0) return;
-    const int b = u.b, len = __builtin_amdgcn_readfirstlane(cached_length(p, b));
+    const int b = u.b, len = u.len, chunk = u.chunk;
     const int held = (len + 31) / 32, tiles = held + (p.drafts + 31) / 32;
     const int begin = u.part * chunk, end = min(tiles, begin + chunk);
 
@@ -177,6 +181,12 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
     auto stage = [&](int t0, unsigned char *set) {
         const uint4 none = make_uint4(0, 0, 0, 0);
         float *scales = reinterpret_cast<float *>(set + SCALES);
+        // of the keys, times the call's scale, of the values, and behind them the largest of the values'
+        auto put_scales = [&](int s, float x) {
+            scales[64 * s + l] = x;
+            const float most = upper_half_most(x);
+            if (l == 63) scales[64 * SUBT + s] = most;
+        };
         // tokens that the sequence does not have are zeros, whatever the page holds
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
@@ -200,7 +210,7 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
 #pragma unroll
         for (int s = 0; s < SUBT; ++s) {
             if (t0 + s < held) {
-                if (SCALED && rg == 0) scales[64 * s + l] = (l & 31) < there[s] ? (l < 32 ? sraw[s] * p.scale2 : sraw[s]) : 0.f;
+                if (SCALED && rg == 0) put_scales(s, (l & 31) < there[s] ? (l < 32 ? sraw[s] * p.scale2 : sraw[s]) : l < 32 ? p.scale2 : 0.f);
                 continue;
             }
             const int j0 = 32 * (t0 + s - held);
@@ -214,7 +224,7 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
                 put(set + s * TILE, r, c, is ? ldg16(kr) : none);
                 put(set + (SUBT + s) * TILE, r, c, is ? ldg16(vr) : none);
             }
-            if (SCALED && rg == 0) scales[64 * s + l] = l < 32 ? p.scale2 : 1.f;
+            if (SCALED && rg == 0) put_scales(s, l < 32 ? p.scale2 : 1.f);
         }
     };
     request(begin + kg * SUBT);
@@ -264,15 +274,8 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
         }
         const float *scales = reinterpret_cast<const float *>(set + SCALES);
         if (SCALED) {
-            float most = 0.f;
-#pragma unroll
-            for (int s = 0; s < SUBT; ++s)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f4v vs = *reinterpret_cast<const f4v *>(scales + 64 * s + 32 + 8 * g + 4 * h);
-                    most = fmaxf(fmaxf(most, fmaxf(vs[0], vs[1])), fmaxf(vs[2], vs[3]));
-                }
-            most = fmaxf(most, at_lane_xor32(most));
+            float most = scales[64 * SUBT];
+            if (SUBT > 1) most = fmaxf(most, scales[64 * SUBT + 1]);
             if (most > most_scale) {             // the same in all lanes
                 const float to = (float)__builtin_amdgcn_frexp_expf(most) + 1.f, keep = at_exp2(shift - to);       // twice: fewer of these
                 most_scale = at_exp2(to);
@@ -301,23 +304,16 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
                 asm volatile("" : "+v"(sees[s]));        // as bits of one register: the compiler would keep 16 masks
             }
         }
-        // scores, in the exponent's units where `scaled`; a hidden one is -inf only once scaled, whatever the scale's sign
         auto scale_of = [&](int s, int g) {
             if (SCALED) return *reinterpret_cast<const f4v *>(scales + 64 * s + 8 * g + 4 * h);
             return f4v{p.scale2, p.scale2, p.scale2, p.scale2};
         };
-        if (partial) {
+        if (partial) {                           // the scales of what is hidden are the call's, which is not zero
+            const float hidden = p.scale2 < 0.f ? __builtin_inff() : NEG_INF;
 #pragma unroll
             for (int s = 0; s < SUBT; ++s)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const f4v ks = scale_of(s, g);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int v = 4 * g + j;
-                        sacc[s][v] = (sees[s] >> v) & 1u ? sacc[s][v] * ks[j] : NEG_INF;
-                    }
-                }
+                for (int v = 0; v < 16; ++v) sacc[s][v] = (sees[s] >> v) & 1u ? sacc[s][v] : hidden;
         }
         float psum;
         h8 pop[SUBT][2];
@@ -327,8 +323,8 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
             for (int s = 0; s < SUBT; ++s)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    f4v ks = scale_of(s, g), vs = {1.f, 1.f, 1.f, 1.f};
-                    if (partial) ks = f4v{1.f, 1.f, 1.f, 1.f};
+                    const f4v ks = scale_of(s, g);
+                    f4v vs = {1.f, 1.f, 1.f, 1.f};
                     if (SCALED) vs = *reinterpret_cast<const f4v *>(scales + 64 * s + 32 + 8 * g + 4 * h);
                     half_t pair[4];
 #pragma unroll
@@ -354,8 +350,7 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
             for (int s = 0; s < SUBT; ++s)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    f4v ks = scale_of(s, g);
-                    if (partial) ks = f4v{1.f, 1.f, 1.f, 1.f};
+                    const f4v ks = scale_of(s, g);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) bm = fmaxf(bm, sacc[s][4 * g + j] * ks[j]);
                 }
@@ -465,12 +460,12 @@ __global__ __launch_bounds__(1024) void cached_join_kernel(CachedOperands p, int
     constexpr int LANES = HD / 4, GROUPS = 1024 / LANES;
     __shared__ f4v sums[GROUPS][LANES];
     __shared__ float2 stats[GROUPS];
-    const int chunk = cached_chunk(p), rows = GROUPS / lists;                    // rows of this workgroup
+    const int rows = GROUPS / lists;                    // rows of this workgroup
     const int per = (p.rows + rows - 1) / rows, group = (int)blockIdx.x;
     const int key_head = group / per % p.key_heads, b = group / per / p.key_heads;
     const int place = (int)threadIdx.x / LANES, lane = (int)threadIdx.x % LANES, list = place % lists;
     const int row = group % per * rows + place / lists;
-    const CachedUnit u = cached_unit(p, chunk, -1, b);
+    const CachedUnit u = cached_unit(p, -1, b);
     if (u.parts <= 1) return;                    // the walk has stored the rows
     JoinPart mine = {-__builtin_inff(), 0.f, {0.f, 0.f, 0.f, 0.f}};
     if (row < p.rows) {
@@ -509,7 +504,8 @@ __global__ __launch_bounds__(1024) void cached_join_kernel(CachedOperands p, int
 }
 
 // ---- launchers ----------------------------------------------------------------------------------------
-constexpr int CACHED_UNITS = 512;                // wanted in a launch: two workgroups a compute unit
+// units wanted in a launch: two or three workgroups a compute unit
+constexpr int cached_units(int rg) { return rg == 1 ? 512 : 768; }
 constexpr int CACHED_LEAST = 8;                  // tiles of a chunk: two for each wave of RG = 1
 
 CachedOperands operands(const CachedArgs &a)
@@ -522,7 +518,8 @@ CachedOperands operands(const CachedArgs &a)
     p.batch = a.batch, p.drafts = a.drafts, p.heads = a.heads, p.key_heads = a.key_heads, p.group = a.heads / a.key_heads;
     p.pages = a.pages, p.page_shift = a.page_shift, p.width = a.width;
     p.tree_batch = a.tree_shared ? 0 : a.drafts * a.drafts;
-    p.scale2 = a.scale * 1.4426950408889634f;
+    // a hidden score is an infinity whose product with this is -inf: never zero (1e-30 leaves every exponent of a zero scale at 0)
+    p.scale2 = a.scale == 0.f ? 1e-30f : a.scale * 1.4426950408889634f;
     p.q_batch = a.q_batch, p.q_token = a.q_token, p.q_head = a.q_head;
     p.k_batch = a.k_batch, p.k_token = a.k_token, p.k_head = a.k_head;
     p.v_batch = a.v_batch, p.v_token = a.v_token, p.v_head = a.v_head;
@@ -531,7 +528,7 @@ CachedOperands operands(const CachedArgs &a)
     p.row_blocks = (p.rows + 32 * rg - 1) / (32 * rg);
     p.least = CACHED_LEAST;
     p.together = CACHED_WAVES / rg * cached_subtiles(rg);
-    p.target = CACHED_UNITS;
+    p.target = cached_units(rg);
     p.parts = (float *)a.workspace;
     p.stats = (float2 *)(p.parts + cached_attention_parts(a) * a.head_dim);
     return p;
@@ -586,7 +583,7 @@ bool cached_attention_splits(const CachedArgs &a) { return most_tiles(a) > CACHE
 long long cached_attention_units(const CachedArgs &a)
 {
     const int rows = a.drafts * (a.heads / a.key_heads), rg = cached_row_groups(rows), blocks = (rows + 32 * rg - 1) / (32 * rg);
-    return a.batch + (cached_attention_splits(a) ? CACHED_UNITS / (a.key_heads * blocks) : 0);
+    return a.batch + (cached_attention_splits(a) ? cached_units(rg) / (a.key_heads * blocks) : 0);
 }
 long long cached_attention_parts(const CachedArgs &a)
 {
