@@ -7,9 +7,9 @@
 //                                           largest so far, so that fp16 holds them
 //
 // The query rows of a key head (N times the heads that share it) are the columns of 32 x 32 x 16 products; a tile is 32 tokens,
-// which lie in one page.  A workgroup has four waves: RG groups of 32 rows times 4 / RG groups of tiles.  RG = 1 (at most 32
-// rows): every wave walks tiles of its own through registers and its own LDS, with no barrier before the end.  Otherwise the waves
-// of a tile group share its tile, double buffered.
+// which lie in one page.  A workgroup has four waves: RG groups of 32 rows times 4 / RG groups of tiles.  RG = 1: every wave walks
+// tiles of its own through registers and its own LDS, with no barrier before the end.  RG = 4: 128 rows, whose waves share the
+// tile, double buffered.
 // The work is cut where it lies: a unit is a chunk of the tiles of one sequence and key head, the chunk chosen on the device
 // from the lengths so that the units fill the machine, long sequences in many, short ones in one.  A sequence in several units
 // leaves (max, sum, O) of each in a workspace, which a second launch joins in the order of the chunks.
@@ -25,11 +25,15 @@ namespace bsa {
 namespace {
 
 constexpr int CACHED_WAVES = 4;
-constexpr int cached_row_groups(int rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : 4; }
-// tiles of 32 tokens that the waves of a tile group take at a time
-constexpr int cached_subtiles(int rg) { return rg == 1 ? 1 : 2; }
+// Rows are taken by 32 as long as a cached tile is then widened at most twice.  Measured (us, RG = 1 against 4): 64 rows of 64
+// sequences of 2000 tokens 36 / 68, of one of 8000 15 / 20; 112 rows of 64 sequences 78 / 69, at head dim 128 144 / 93; 108
+// rows of 4 sequences 40 / 34, 244 rows of 48 long ones 335 / 258.  (RG = 2 lost to RG = 1 up to 64 rows, 48 us for those 36.)
+constexpr int cached_row_groups(int rows) { return rows <= 64 ? 1 : 4; }
+// Tiles of 32 tokens that the waves of a tile group take at a time: two where registers allow (244 rows, head dim 64: 258 us, one
+// 298), one at head dim 128 (the same time, where two spilled 25 registers).
+constexpr int cached_subtiles(int hd, int rg) { return rg == 1 || hd == 128 ? 1 : 2; }
 // K, V and the scales of them
-constexpr int cached_set_bytes(int hd, int rg) { return cached_subtiles(rg) * (128 * hd + 256) + 256; }
+constexpr int cached_set_bytes(int hd, int rg) { return cached_subtiles(hd, rg) * (128 * hd + 256) + 256; }
 constexpr float CACHED_LAZY_SUM = 256.f;
 
 struct CachedOperands {
@@ -115,7 +119,7 @@ template <int HD, bool BF, int KIND, int RG>
 __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(CachedOperands p)
 {
     extern __shared__ __align__(16) unsigned char lds_raw[];
-    constexpr int KS = HD / 16, KG = CACHED_WAVES / RG, BUFFERS = RG > 1 ? 2 : 1, THREADS = 64 * RG, SUBT = cached_subtiles(RG);
+    constexpr int KS = HD / 16, KG = CACHED_WAVES / RG, BUFFERS = RG > 1 ? 2 : 1, THREADS = 64 * RG, SUBT = cached_subtiles(HD, RG);
     constexpr int WIDTH = cache_value_bytes(KIND), PIECES = 32 * HD * WIDTH / 16, EACH = SUBT * PIECES / THREADS;
     constexpr int TILE = 64 * HD, SET = cached_set_bytes(HD, RG), SCALES = 2 * SUBT * TILE;
     constexpr bool SCALED = KIND != CACHE_16;
@@ -527,7 +531,9 @@ __global__ __launch_bounds__(1024) void cached_join_kernel(CachedOperands p, int
 }
 
 // ---- launchers ----------------------------------------------------------------------------------------
-// units wanted in a launch: two or three workgroups a compute unit
+// Units wanted in a launch.  RG = 1: the 512 workgroups that the machine holds at once (1024: 36 us where 512 take 30, one long
+// sequence a key head).  RG = 4 is better balanced with more (48 uneven sequences: 512 292 us, 768 258, 1536 250), but
+// 1536 took 171 us where 768 take 157 (64 sequences of 500 to 4000 tokens, 120 rows).
 constexpr int cached_units(int rg) { return rg == 1 ? 512 : 768; }
 constexpr int CACHED_LEAST = 8;                  // tiles of a chunk: two for each wave of RG = 1
 
@@ -550,8 +556,11 @@ CachedOperands operands(const CachedArgs &a)
     const int rg = cached_row_groups(p.rows);
     p.row_blocks = (p.rows + 32 * rg - 1) / (32 * rg);
     p.least = CACHED_LEAST;
-    p.together = CACHED_WAVES / rg * cached_subtiles(rg);
+    p.together = CACHED_WAVES / rg * cached_subtiles(a.head_dim, rg);
     p.target = cached_units(rg);
+    // Every sequence ends in a unit that is shorter, which comes on top.  With few of them the wanted ones make room, so that all run at
+    // once: 33 sequences of 300 to 16000 tokens 64 us, without 78; 64 sequences 51 and 50.
+    if (rg == 1 && 2ll * a.batch * a.key_heads * p.row_blocks <= p.target) p.target -= a.batch * a.key_heads * p.row_blocks;
     p.parts = (float *)a.workspace;
     p.stats = (float2 *)(p.parts + cached_attention_parts(a) * a.head_dim);
     return p;
@@ -583,7 +592,7 @@ template <int HD, bool BF, int KIND>
 hipError_t walk_rows(const CachedArgs &a, hipStream_t st)
 {
     const int rg = cached_row_groups(a.drafts * (a.heads / a.key_heads));
-    return rg == 1 ? walk<HD, BF, KIND, 1>(a, st) : rg == 2 ? walk<HD, BF, KIND, 2>(a, st) : walk<HD, BF, KIND, 4>(a, st);
+    return rg == 1 ? walk<HD, BF, KIND, 1>(a, st) : walk<HD, BF, KIND, 4>(a, st);
 }
 template <int HD, bool BF>
 hipError_t walk_kind(const CachedArgs &a, hipStream_t st)
