@@ -802,7 +802,7 @@ static int packed(const char *who, int dtype, const void *q, const void *k, cons
     return BSA_OK;
 }
 
-int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, float *lse,
+int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, void *rest, float *lse,
                                  const int32_t *offsets, int tokens, int sequences, int heads, int key_heads, int head_dim,
                                  const int64_t *strides, float scale, int causal, void *stream)
 {
@@ -811,15 +811,16 @@ int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const 
     int rc = packed(who, dtype, q, k, v, offsets, tokens, sequences, heads, key_heads, head_dim, strides, 3, scale, causal, p);
     if (rc) return rc;
     if (!out) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
-    rc = check_alignment(who, {out});
+    rc = check_alignment(who, {out, rest});
     if (rc) return rc;
     p.out = out;
+    p.rest = rest;
     p.lse = lse;
     return check_launch(bsa::launch_packed_forward(p, (hipStream_t)stream), who);
 }
 
 int bsa_packed_attention_backward(int dtype, const void *q, const void *k, const void *v, const void *dout, const void *out,
-                                  const float *lse, float *delta_ws, void *dq_out, void *dk_out, void *dv_out,
+                                  const void *rest, const float *lse, float *delta_ws, void *dq_out, void *dk_out, void *dv_out,
                                   const int32_t *offsets, int tokens, int sequences, int heads, int key_heads, int head_dim,
                                   const int64_t *strides, float scale, int causal, void *stream)
 {
@@ -827,11 +828,11 @@ int bsa_packed_attention_backward(int dtype, const void *q, const void *k, const
     bsa::PackedArgs p;
     int rc = packed(who, dtype, q, k, v, offsets, tokens, sequences, heads, key_heads, head_dim, strides, 4, scale, causal, p);
     if (rc) return rc;
-    if (!dout || !out || !lse || !delta_ws || !dq_out || (dk_out == nullptr) != (dv_out == nullptr))
+    if (!dout || !out || !rest || !lse || !delta_ws || !dq_out || (dk_out == nullptr) != (dv_out == nullptr))
         return fail(BSA_ERR_INVALID, "%s: null pointer argument (dk_out and dv_out go together)", who);
-    rc = check_alignment(who, {dout, out, dq_out, dk_out, dv_out});
+    rc = check_alignment(who, {dout, out, rest, dq_out, dk_out, dv_out});
     if (rc) return rc;
-    p.dout = dout, p.o = out;
+    p.dout = dout, p.o = out, p.o_rest = rest;
     p.lse = const_cast<float *>(lse);
     p.delta = delta_ws;
     p.out = dq_out, p.dk = dk_out, p.dv = dv_out;

@@ -155,8 +155,9 @@ hipError_t launch_attention_backward_dkdv(const AttentionArgs &p, hipStream_t st
 // attention over packed sequences (packed_attention.hip); strides in values
 struct PackedArgs {
     const void *q = nullptr, *k = nullptr, *v = nullptr;
-    const void *dout = nullptr, *o = nullptr;    // backward only; o: the forward result, dense
+    const void *dout = nullptr, *o = nullptr, *o_rest = nullptr;     // backward only; o: the forward result, o_rest: its rest; dense
     void *out = nullptr;                         // forward: the result; backward: dq
+    void *rest = nullptr;                        // forward: what the result's rounding took, may be null
     void *dk = nullptr, *dv = nullptr;           // both or neither
     float *lse = nullptr;                        // [heads][tokens]; forward: written, may be null; backward: read
     float *delta = nullptr;                      // backward: scratch of the same size

@@ -849,19 +849,20 @@ void launched(int status)
 
 // sparse/packed.py, PackedAttention.backward
 struct PackedNode : public Node {
-    SavedVariable q_, k_, v_, out_, lse_, offsets_;
+    SavedVariable q_, k_, v_, out_, rest_, lse_, offsets_;
     double scale;
     bool causal;
     std::string name() const override { return "PackedAttentionBackward"; }
     void release_variables() override
     {
         std::lock_guard<std::mutex> lock(mutex_);
-        for (SavedVariable *s : {&q_, &k_, &v_, &out_, &lse_, &offsets_}) s->reset_data();
+        for (SavedVariable *s : {&q_, &k_, &v_, &out_, &rest_, &lse_, &offsets_}) s->reset_data();
     }
     variable_list apply(variable_list &&grads) override
     {
         std::lock_guard<std::mutex> lock(mutex_);
-        const Tensor q = q_.unpack(), k = k_.unpack(), v = v_.unpack(), out = out_.unpack(getptr()), lse = lse_.unpack(), offsets = offsets_.unpack();
+        const Tensor q = q_.unpack(), k = k_.unpack(), v = v_.unpack(), out = out_.unpack(getptr()), rest = rest_.unpack(), lse = lse_.unpack(),
+                     offsets = offsets_.unpack();
         Tensor dout = grads[0].defined() ? grads[0] : node_zeros();
         const bool dkdv = task_should_compute_output(1) || task_should_compute_output(2);
         variable_list result;
@@ -869,16 +870,17 @@ struct PackedNode : public Node {
             at::AutoGradMode off(false);
             if (plain_strided(dout) && !readable_rows(dout)) dout = dout.clone(at::MemoryFormat::Contiguous);
             bool direct = heads_fit(q, k, v, 3) && plain_strided(dout) && readable_rows(dout) && plain(out) && on_current_device(out) &&
+                          plain(rest) && on_current_device(rest) && rest.sizes() == q.sizes() && rest.scalar_type() == q.scalar_type() &&
                           plain(lse) && on_current_device(lse) && index_tensor(offsets, 1) && offsets.numel() >= 2 && q.size(0) > 0;
             direct = direct && dout.sizes() == q.sizes() && out.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() &&
                      out.scalar_type() == q.scalar_type() && lse.scalar_type() == at::kFloat && lse.dim() == 2 &&
                      lse.size(0) == q.size(1) && lse.size(1) == q.size(0);
             if (!direct) {
                 py::gil_scoped_acquire gil;
-                Borrow pq(q), pk(k), pv(v), pd(dout), po(out), pl(lse), pf(offsets);
+                Borrow pq(q), pk(k), pv(v), pd(dout), po(out), pr(rest), pl(lse), pf(offsets);
                 py::object s = py::float_(scale);
-                PyObject *got = PyObject_CallFunctionObjArgs(python.run_packed_backward, pq.get(), pk.get(), pv.get(), pd.get(), po.get(), pl.get(),
-                                                             pf.get(), s.ptr(), py_bool(causal), py_bool(dkdv), nullptr);
+                PyObject *got = PyObject_CallFunctionObjArgs(python.run_packed_backward, pq.get(), pk.get(), pv.get(), pd.get(), po.get(), pr.get(),
+                                                             pl.get(), pf.get(), s.ptr(), py_bool(causal), py_bool(dkdv), nullptr);
                 if (got == nullptr) raise_pending();
                 py::tuple t = py::reinterpret_steal<py::tuple>(got);
                 for (auto x : t) result.push_back(x.is_none() ? Tensor() : THPVariable_Unpack(x.ptr()));
@@ -891,7 +893,7 @@ struct PackedNode : public Node {
                 const int64_t strides[8] = {stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0), stride_of(v, 1),
                                             stride_of(dout, 0), stride_of(dout, 1)};
                 launched(lib.packed_backward(code_of(q.scalar_type()), q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(),
-                                             lse.data_ptr<float>(), delta.data_ptr<float>(), dq.data_ptr(), dkdv ? dk.data_ptr() : nullptr,
+                                             rest.data_ptr(), lse.data_ptr<float>(), delta.data_ptr<float>(), dq.data_ptr(), dkdv ? dk.data_ptr() : nullptr,
                                              dkdv ? dv.data_ptr() : nullptr, offsets.data_ptr<int32_t>(), (int)q.size(0),
                                              (int)(offsets.numel() - 1), (int)q.size(1), (int)k.size(1), (int)q.size(2), strides, (float)scale,
                                              causal, current_stream()));
@@ -930,20 +932,24 @@ PyObject *packed_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
         node->scale = scale;
         node->causal = causal;
     }
-    Tensor out, lse;
+    Tensor out, rest, lse;
     {
         py::gil_scoped_release unlocked;
         out = at::empty(q.sizes(), q.options());
-        if (node) lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+        if (node) {
+            rest = at::empty(q.sizes(), q.options());
+            lse = at::empty({q.size(1), q.size(0)}, q.options().dtype(at::kFloat));
+        }
         const int64_t strides[6] = {stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0), stride_of(v, 1)};
         launched(lib.packed_forward(code_of(q.scalar_type()), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                                    node ? lse.data_ptr<float>() : nullptr, offsets.data_ptr<int32_t>(), (int)q.size(0),
+                                    node ? rest.data_ptr() : nullptr, node ? lse.data_ptr<float>() : nullptr, offsets.data_ptr<int32_t>(), (int)q.size(0),
                                     (int)(offsets.numel() - 1), (int)q.size(1), (int)k.size(1), (int)q.size(2), strides, (float)scale, causal,
                                     current_stream()));
     }
     if (node) {
         torch::autograd::set_history(out, node);
         node->out_ = SavedVariable(out, true);
+        node->rest_ = SavedVariable(rest, false);
         node->lse_ = SavedVariable(lse, false);
     }
     return THPVariable_Wrap(std::move(out));

@@ -162,13 +162,18 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
     __syncthreads();                             // all are done with the tiles, whose place the results take
     store_token_rows<HD, BF>(oacc, any ? 1.f / lsum : 0.f, lds_raw + 64 * HD * w,
                              p.out + ((begin + row0) * p.heads + item.head) * HD, (long long)p.heads * HD, n - row0);
+    if (p.rest != nullptr)
+        store_token_rows<HD, BF, true>(oacc, any ? 1.f / lsum : 0.f, lds_raw + 64 * HD * w,
+                                       p.rest + ((begin + row0) * p.heads + item.head) * HD, (long long)p.heads * HD, n - row0);
 }
 
 // ---------------------------------------------------------------------------
 // Gradients, as two walks that each rebuild the probabilities from the row statistics and write every result once (no atomics:
 // the same bits every time):
 //   rows      as the forward walk:  P = exp2(scale2 S - lse),  dS = P (dO V^T - delta),  dq^T += K^T dS^T;
-//             delta = rowsum(dO O) is made here and left for the other walk
+//             delta = rowsum(dO O) is made here, O with what its rounding took, and left for the other walk.  From the rounded O
+//             alone its error moves a whole row of dS the same way: dq and dk were 1.6 times as far from float64 as their own
+//             rounding leaves them, with it 1.45 (dS in 16 bits), for 2 % of a training step
 //   columns   a workgroup holds 32 W keys of one key head and walks the queries of all heads that share it:
 //             dv^T += dO^T P,  dk^T += Q^T dS
 // ---------------------------------------------------------------------------
@@ -195,15 +200,15 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
     float delta = 0.f;
     const long long token = begin + min(row, n - 1);
     const half_t *q_row = p.q + token * p.q_token + item.head * p.q_head, *g_row = p.dout + token * p.g_token + item.head * p.g_head,
-                 *o_row = p.o + (token * p.heads + item.head) * HD;
+                 *o_row = p.o + (token * p.heads + item.head) * HD, *rest_row = p.o_rest + (token * p.heads + item.head) * HD;
     const float minus_lse = -p.lse[(size_t)item.head * p.tokens + token];
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
         qop[s] = as_h8(ldg16(q_row + 16 * s + 8 * h));
         dop[s] = as_h8(ldg16(g_row + 16 * s + 8 * h));
-        const h8 o = as_h8(ldg16(o_row + 16 * s + 8 * h));
+        const h8 o = as_h8(ldg16(o_row + 16 * s + 8 * h)), rest = as_h8(ldg16(rest_row + 16 * s + 8 * h));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) delta += widen_16<BF>(dop[s][j]) * widen_16<BF>(o[j]);
+        for (int j = 0; j < 8; ++j) delta += widen_16<BF>(dop[s][j]) * (widen_16<BF>(o[j]) + widen_16<BF>(rest[j]));
     }
     delta += at_lane_xor32(delta);               // the other half of the head dim sits in lane ^ 32
     if (h == 0 && row < n) p.delta[(size_t)item.head * p.tokens + token] = delta;
@@ -423,8 +428,8 @@ PackedOperands operands(const PackedArgs &a)
 {
     PackedOperands p;
     p.q = (const half_t *)a.q, p.k = (const half_t *)a.k, p.v = (const half_t *)a.v;
-    p.dout = (const half_t *)a.dout, p.o = (const half_t *)a.o;
-    p.out = (half_t *)a.out, p.dk = (half_t *)a.dk, p.dv = (half_t *)a.dv;
+    p.dout = (const half_t *)a.dout, p.o = (const half_t *)a.o, p.o_rest = (const half_t *)a.o_rest;
+    p.out = (half_t *)a.out, p.rest = (half_t *)a.rest, p.dk = (half_t *)a.dk, p.dv = (half_t *)a.dv;
     p.lse = a.lse, p.delta = a.delta;
     p.offsets = a.offsets;
     p.tokens = a.tokens, p.sequences = a.sequences, p.heads = a.heads, p.group = a.heads / a.key_heads;

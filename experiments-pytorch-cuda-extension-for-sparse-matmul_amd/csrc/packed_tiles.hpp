@@ -8,8 +8,8 @@
 namespace bsa {
 
 struct PackedOperands {
-    const half_t *q, *k, *v, *dout, *o;          // o: the forward result, [T][heads][HD], for the backward walks
-    half_t *out, *dk, *dv;                       // out: the result, or dq; all dense
+    const half_t *q, *k, *v, *dout, *o, *o_rest; // o: the forward result, [T][heads][HD], for the backward walks
+    half_t *out, *rest, *dk, *dv;                // out: the result, or dq; rest, o_rest: what its rounding took; all dense
     float *lse, *delta;                          // [heads][T]
     const int32_t *offsets;                      // [sequences + 1]
     int tokens, sequences, heads, group;         // heads: query heads, group: of them to a key head
@@ -362,8 +362,8 @@ struct PairTiles {
 };
 
 // 32 result rows `stride` values apart, of which the first `valid` are stored; through 64 HD bytes of LDS, so that they leave
-// as whole lines
-template <int HD, bool BF>
+// as whole lines.  REST: what the rounding takes from them instead.
+template <int HD, bool BF, bool REST = false>
 __device__ __forceinline__ void store_token_rows(const RowTile<HD> &acc, float mul, unsigned char *scratch, half_t *dst,
                                                  long long stride, int valid)
 {
@@ -375,7 +375,10 @@ __device__ __forceinline__ void store_token_rows(const RowTile<HD> &acc, float m
         for (int g = 0; g < 4; ++g) {
             h4 o;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = narrow_16<BF>(acc[t][4 * g + j] * mul);
+            for (int j = 0; j < 4; ++j) {
+                const float x = acc[t][4 * g + j] * mul;
+                o[j] = narrow_16<BF>(REST ? x - widen_16<BF>(narrow_16<BF>(x)) : x);
+            }
             *reinterpret_cast<h4 *>(scratch + out_row_addr(HD, row, 4 * t + g, h)) = o;
         }
     wave_lds_fence();

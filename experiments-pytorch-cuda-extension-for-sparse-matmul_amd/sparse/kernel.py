@@ -61,8 +61,8 @@ SIGNATURES = {
                                                         _vp, ctypes.c_size_t, _i, _i, _i, _i, _i, _f, _i, _vp]),
     "bsa_attention_gradients": (_i, [_i] + [_vp] * 10 + [_vp, _vp, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i, _i, _i,
                                                         _vp, ctypes.c_size_t, _i, _i, _i, _i, _i, _f, _i, _vp]),
-    "bsa_packed_attention_forward": (_i, [_i] + [_vp] * 6 + [_i] * 5 + [_vp, _f, _i, _vp]),
-    "bsa_packed_attention_backward": (_i, [_i] + [_vp] * 11 + [_i] * 5 + [_vp, _f, _i, _vp]),
+    "bsa_packed_attention_forward": (_i, [_i] + [_vp] * 7 + [_i] * 5 + [_vp, _f, _i, _vp]),
+    "bsa_packed_attention_backward": (_i, [_i] + [_vp] * 12 + [_i] * 5 + [_vp, _f, _i, _vp]),
     "bsa_cache_write": (_i, [_i, _i] + [_vp] * 7 + [_i] * 5 + [_vp, _vp]),
     "bsa_cache_read": (_i, [_i, _i] + [_vp] * 7 + [_i] * 5 + [_vp]),
     "bsa_cached_attention_workspace_bytes": (ctypes.c_size_t, [_i] * 7),

@@ -52,28 +52,28 @@ def check_index(t: Any, name: str, device: torch.device, dims: int) -> None:
         raise ValueError(f"{name} must live on the GPU of the operands")
 
 
-def _forward(q, k, v, offsets, scale, causal, with_lse):
+def _forward(q, k, v, offsets, scale, causal, for_backward):
     check_heads(q, k, v, 3)
     check_index(offsets, "offsets", q.device, 1)
     if offsets.numel() < 1:
         raise ValueError("offsets needs one entry more than there are sequences")
     tokens, heads, dim = q.shape
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    lse = torch.empty((heads, tokens), dtype=torch.float32, device=q.device) if with_lse else None
+    rest, lse = (torch.empty_like(out), torch.empty((heads, tokens), dtype=torch.float32, device=q.device)) if for_backward else (None, None)
     if tokens == 0:
-        return out, lse
+        return out, rest, lse
     if offsets.numel() == 1:                    # no sequence: no token is in one
-        return out.zero_(), lse
+        return out.zero_(), rest, lse
     q, k, v = rows_of(q), rows_of(k), rows_of(v)
     with _k.on_device(q.device):
         _k.check(_k.lib.bsa_packed_attention_forward(
-            _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr() if with_lse else None,
-            offsets.data_ptr(), tokens, offsets.numel() - 1, heads, k.size(1), dim, strides_of(q, k, v), float(scale),
+            _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
+            rest.data_ptr() if for_backward else None, lse.data_ptr() if for_backward else None, offsets.data_ptr(), tokens, offsets.numel() - 1, heads, k.size(1), dim, strides_of(q, k, v), float(scale),
             int(bool(causal)), _k.current_stream()))
-    return out, lse
+    return out, rest, lse
 
 
-def run_backward(q, k, v, dout, out, lse, offsets, scale, causal, with_dkdv):
+def run_backward(q, k, v, dout, out, rest, lse, offsets, scale, causal, with_dkdv):
     tokens, heads, dim = q.shape
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2)) if with_dkdv else (None, None)
@@ -83,7 +83,7 @@ def run_backward(q, k, v, dout, out, lse, offsets, scale, causal, with_dkdv):
     delta = torch.empty_like(lse)
     with _k.on_device(q.device):
         _k.check(_k.lib.bsa_packed_attention_backward(
-            _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), out.data_ptr(), rest.data_ptr(), lse.data_ptr(),
             delta.data_ptr(), dq.data_ptr(), dk.data_ptr() if with_dkdv else None, dv.data_ptr() if with_dkdv else None,
             offsets.data_ptr(), tokens, offsets.numel() - 1, heads, k.size(1), dim, strides_of(q, k, v, dout), float(scale),
             int(bool(causal)), _k.current_stream()))
@@ -94,16 +94,16 @@ class PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx: Any, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, scale: float,
                 causal: bool) -> torch.Tensor:
-        out, lse = _forward(q, k, v, offsets, scale, causal, True)
-        ctx.save_for_backward(q, k, v, out, lse, offsets)
+        out, rest, lse = _forward(q, k, v, offsets, scale, causal, True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, offsets)
         ctx.scale, ctx.causal = scale, causal
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx: Any, dout: torch.Tensor) -> Tuple[Optional[torch.Tensor], ...]:
-        q, k, v, out, lse, offsets = ctx.saved_tensors
-        grads = run_backward(q, k, v, dout, out, lse, offsets, ctx.scale, ctx.causal, any(ctx.needs_input_grad[1:3]))
+        q, k, v, out, rest, lse, offsets = ctx.saved_tensors
+        grads = run_backward(q, k, v, dout, out, rest, lse, offsets, ctx.scale, ctx.causal, any(ctx.needs_input_grad[1:3]))
         return grads + (None, None, None)
 
 

@@ -407,8 +407,9 @@ int bsa_weight_grad(int dtype, const void *a, const void *b, void *out, const in
  *   out[i] = softmax(scale q[i] k^T over the tokens of its sequence; with `causal` over those up to i) v
  *   q, dout          [tokens, heads, head_dim],  k, v [tokens, key_heads, head_dim], with strides
  *   out, dq          [tokens, heads, head_dim], dense;  dk, dv [tokens, key_heads, head_dim], dense
- *   lse, delta_ws    float [heads, tokens]: log2 of each row's sum of exponentials (may be NULL in the forward call),
- *                    scratch of the backward call
+ *   rest             as out: what the rounding to 16 bits took from it.  The backward call needs it and lse; both may be
+ *                    NULL in the forward call.
+ *   lse, delta_ws    float [heads, tokens]: log2 of each row's sum of exponentials; scratch of the backward call
  *   offsets          device int32[sequences + 1]: sequence b is tokens offsets[b] .. offsets[b + 1] - 1.  They stay on the
  *                    device.  Ascending; sequences may be empty.  Tokens in front of the first and behind the last
  *                    sequence get zeros in every result and are not read.  Values outside [0, tokens] are taken as the nearer end;
@@ -419,11 +420,11 @@ int bsa_weight_grad(int dtype, const void *a, const void *b, void *out, const in
  * reaches the results of the tokens that see it, not of others.
  * fp16 and bf16, head_dim 64 or 128; operands start at multiples of 16 bytes.  dk_out and dv_out both NULL: dq alone.
  */
-int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, float *lse,
+int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, void *rest, float *lse,
                                  const int32_t *offsets, int tokens, int sequences, int heads, int key_heads, int head_dim,
                                  const int64_t *strides, float scale, int causal, void *stream);
 int bsa_packed_attention_backward(int dtype, const void *q, const void *k, const void *v, const void *dout, const void *out,
-                                  const float *lse, float *delta_ws, void *dq_out, void *dk_out, void *dv_out,
+                                  const void *rest, const float *lse, float *delta_ws, void *dq_out, void *dk_out, void *dv_out,
                                   const int32_t *offsets, int tokens, int sequences, int heads, int key_heads, int head_dim,
                                   const int64_t *strides, float scale, int causal, void *stream);
 
