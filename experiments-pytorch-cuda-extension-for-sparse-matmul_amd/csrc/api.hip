@@ -786,8 +786,8 @@ static int packed(const char *who, int dtype, const void *q, const void *k, cons
     for (int i = 0; i < operands; ++i)
         if (strides[2 * i] > (1LL << 24))
             return fail(BSA_ERR_UNSUPPORTED, "%s: %lld values between tokens are too many", who, (long long)strides[2 * i]);
-    if ((long long)heads * (tokens / 32 + sequences) > (1LL << 30))
-        return fail(BSA_ERR_INVALID, "%s: grid of %d heads and %d tokens is too large", who, heads, tokens);
+    if (heads * (tokens / 128 + sequences + 8LL) > (1LL << 24) - 64)     // workgroups of 256 threads: fewer than 2^32 threads
+        return fail(BSA_ERR_INVALID, "%s: %d tokens in %d sequences of %d heads are too many", who, tokens, sequences, heads);
     rc = check_alignment(who, {q, k, v});
     if (rc) return rc;
     p.q = q, p.k = k, p.v = v;
@@ -861,7 +861,7 @@ static int cache_rows(const char *who, int cache_dtype, const void *k, const voi
     int rc = check_heads(who, heads, heads, head_dim);
     if (!rc) rc = check_cache(who, cache_dtype, keys, values, key_scales, value_scales, pages, page, p.kind, p.page_shift);
     if (rc) return rc;
-    if (tokens < 0 || (long long)tokens * heads > (1LL << 36))
+    if (tokens < 0 || (long long)tokens * heads * (head_dim / 8) >= (1LL << 32) - 256)      // a thread for 8 values
         return fail(BSA_ERR_INVALID, "%s: %d tokens of %d heads", who, tokens, heads);
     if (tokens > 0 && (!k || !v || !slots)) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
     rc = check_alignment(who, {k, v});
@@ -910,10 +910,14 @@ static int check_drafts(const char *who, int batch, int drafts, int heads, int k
 {
     const int rc = check_heads(who, heads, key_heads, head_dim);
     if (rc) return rc;
-    if (batch < 1 || batch > (1 << 20) || drafts < 1 || drafts > 1024 || width < 0 || (long long)width * page > 2147483647LL - 2048)
+    // the tiles of 64 sequences are added up in 32 bits
+    if (batch < 1 || batch > (1 << 20) || drafts < 1 || drafts > 1024 || width < 0 || (long long)width * page > (1LL << 30) - 2048)
         return fail(BSA_ERR_INVALID, "%s: %d sequences of %d new tokens and %d pages of %d", who, batch, drafts, width, page);
-    if ((long long)batch * heads * drafts > (1LL << 27))
-        return fail(BSA_ERR_INVALID, "%s: %d sequences of %d new tokens and %d heads are too many", who, batch, drafts, heads);
+    // blocks of rows: workgroups of 1024 threads, fewer than 2^32 threads; and the tiles a unit may get, in 32 bits
+    const long long blocks = (long long)batch * key_heads * ((drafts * (heads / key_heads) + 31) / 32);
+    if (blocks >= (1LL << 22) || blocks * (((long long)width * page + drafts) / 32 + 2) > (1LL << 38))
+        return fail(BSA_ERR_INVALID, "%s: %d sequences of %d new tokens and %d heads over %d pages of %d are too many", who, batch, drafts,
+                    heads, width, page);
     return BSA_OK;
 }
 

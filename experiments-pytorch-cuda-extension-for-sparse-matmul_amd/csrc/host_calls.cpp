@@ -918,7 +918,9 @@ PyObject *packed_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
     if (causal < 0 || !number(args[4]) || !tensors(args, 4) || !plain_thread()) return general(python.packed, args, nargs);
     const Tensor &q = THPVariable_Unpack(args[0]), &k = THPVariable_Unpack(args[1]), &v = THPVariable_Unpack(args[2]),
                  &offsets = THPVariable_Unpack(args[3]);
-    if (!heads_fit(q, k, v, 3) || !index_tensor(offsets, 1) || offsets.numel() < 2 || q.size(0) < 1) return general(python.packed, args, nargs);
+    if (!heads_fit(q, k, v, 3) || !index_tensor(offsets, 1) || offsets.numel() < 2 || offsets.numel() > (1 << 24) || q.size(0) < 1 ||
+        q.size(0) > (1 << 30))
+        return general(python.packed, args, nargs);
     const double scale = PyFloat_AsDouble(args[4]);
     if (scale == -1.0 && PyErr_Occurred()) return nullptr;
     std::shared_ptr<PackedNode> node;
@@ -1046,8 +1048,8 @@ PyObject *cached_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
     const int code = code_of(q.scalar_type());
     if (c->code != BSA_I8 && c->code != BSA_E4M3 && c->code != code) Py_RETURN_NONE;
     const int64_t batch = q.size(0), drafts = q.size(1);
-    if (batch < 1 || drafts < 1 || drafts > 1024 || batch > (1 << 20) || pages.size(-1) > (1 << 24)) Py_RETURN_NONE;
-    if (!index_tensor(pages, 2) || !index_tensor(lengths, 1) || pages.size(0) != batch || lengths.numel() != batch) Py_RETURN_NONE;
+    if (batch < 1 || drafts < 1 || drafts > 1024 || batch > (1 << 20)) Py_RETURN_NONE;
+    if (!index_tensor(pages, 2) || pages.size(1) > (1 << 24) || !index_tensor(lengths, 1) || pages.size(0) != batch || lengths.numel() != batch) Py_RETURN_NONE;
     bool shared = false;
     if (tree.defined()) {
         if (!plain(tree) || !on_current_device(tree) || tree.scalar_type() != at::kBool) Py_RETURN_NONE;

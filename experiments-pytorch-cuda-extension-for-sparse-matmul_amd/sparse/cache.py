@@ -11,7 +11,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import kernel as _k
-from .packed import HEAD_DIMS, check_heads, check_index, rows_of, strides_of
+from .packed import HEAD_DIMS, MOST_ROWS, check_heads, check_index, rows_of, strides_of
 
 PAGES = (32, 64, 128, 256)
 MOST_DRAFTS = 1024
@@ -52,10 +52,14 @@ class KeyValueCache:
     value_scales = property(lambda self: self._held[3])
 
     def __getstate__(self):
-        return {name: value for name, value in self.__dict__.items() if name != "_native"}
+        state = {name: value for name, value in self.__dict__.items() if name != "_native"}
+        # as bytes: pickle has no float8 storage
+        state["_held"] = tuple(t.view(torch.uint8) for t in self._held[:2]) + self._held[2:]
+        return state
 
     def __setstate__(self, state):
         self.__dict__.update(state)
+        self._held = tuple(t.view(self.dtype) for t in self._held[:2]) + self._held[2:]
         self.device = self.keys.device
         self._native = _k.host_calls.new_cache(*self._held)
 
@@ -83,7 +87,7 @@ class KeyValueCache:
         if self.dtype not in _QUANTISED and k.dtype != self.dtype:
             raise TypeError(f"a cache of {self.dtype} takes rows of that type, got {k.dtype}")
         check_index(slots, "slots", self.device, 1)
-        if slots.numel() != k.size(0):
+        if slots.numel() != k.size(0) or k.size(0) > MOST_ROWS:
             raise ValueError(f"{k.size(0)} rows and {slots.numel()} slots")
         k, v = rows_of(k.detach()), rows_of(v.detach())
         with _k.on_device(self.device):
@@ -99,6 +103,8 @@ class KeyValueCache:
         if dtype not in _ROWS:
             raise TypeError(f"rows are read as float32, float16 or bfloat16, got {dtype}")
         check_index(slots, "slots", self.device, 1)
+        if slots.numel() > MOST_ROWS:
+            raise ValueError(f"{slots.numel()} slots are too many")
         shape = (slots.numel(), self.heads, self.head_dim)
         k, v = (torch.empty(shape, dtype=dtype, device=self.device) for _ in range(2))
         with _k.on_device(self.device):
@@ -129,12 +135,12 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: K
         raise TypeError(f"a cache of {cache.dtype} is attended to in that type, got {q.dtype}")
     check_index(pages, "pages", q.device, 2)
     check_index(lengths, "lengths", q.device, 1)
-    if pages.size(0) != batch or lengths.numel() != batch:
+    if pages.size(0) != batch or lengths.numel() != batch or pages.numel() > MOST_ROWS:
         raise ValueError(f"{batch} sequences, pages {tuple(pages.shape)} and lengths {tuple(lengths.shape)}")
     if drafts > MOST_DRAFTS:
         raise ValueError(f"at most {MOST_DRAFTS} new tokens a sequence, got {drafts}")
     if tree is not None:
-        if tree.dtype != torch.bool or tree.device != q.device or tuple(tree.shape) not in ((drafts, drafts), (batch, drafts, drafts)):
+        if not isinstance(tree, torch.Tensor) or tree.dtype != torch.bool or tree.device != q.device or tuple(tree.shape) not in ((drafts, drafts), (batch, drafts, drafts)):
             raise ValueError(f"tree must be bool [{drafts}, {drafts}] or [{batch}, {drafts}, {drafts}] on the GPU of the operands")
         tree = tree.contiguous()
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)

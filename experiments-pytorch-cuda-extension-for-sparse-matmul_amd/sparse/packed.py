@@ -14,6 +14,7 @@ from . import kernel as _k
 
 _DTYPES = {torch.float16: _k.BSA_F16, torch.bfloat16: _k.BSA_BF16}
 HEAD_DIMS = (64, 128)
+MOST_ROWS = 1 << 30                             # of a call
 
 
 def rows_of(t: torch.Tensor, copy: bool = False) -> torch.Tensor:
@@ -33,6 +34,7 @@ def check_heads(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, dims: int) ->
     for t, name in ((q, "q"), (k, "k"), (v, "v")):
         if t.dtype not in _DTYPES or t.dtype != q.dtype:
             raise TypeError(f"q, k, v must all be float16 or all bfloat16, got {name}: {t.dtype}")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
         if not t.is_cuda or t.device != q.device:
             raise ValueError("q, k, v must live on the same GPU")
         if t.dim() != dims:
@@ -58,8 +60,11 @@ def _forward(q, k, v, offsets, scale, causal, for_backward):
     if offsets.numel() < 1:
         raise ValueError("offsets needs one entry more than there are sequences")
     tokens, heads, dim = q.shape
+    if tokens > MOST_ROWS or offsets.numel() > 1 << 24:
+        raise ValueError(f"{tokens} tokens in {offsets.numel() - 1} sequences are too many")
     out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    rest, lse = (torch.empty_like(out), torch.empty((heads, tokens), dtype=torch.float32, device=q.device)) if for_backward else (None, None)
+    rest = torch.empty_like(out) if for_backward else None
+    lse = torch.empty((heads, tokens), dtype=torch.float32, device=q.device) if for_backward else None
     if tokens == 0:
         return out, rest, lse
     if offsets.numel() == 1:                    # no sequence: no token is in one
@@ -68,8 +73,8 @@ def _forward(q, k, v, offsets, scale, causal, for_backward):
     with _k.on_device(q.device):
         _k.check(_k.lib.bsa_packed_attention_forward(
             _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-            rest.data_ptr() if for_backward else None, lse.data_ptr() if for_backward else None, offsets.data_ptr(), tokens, offsets.numel() - 1, heads, k.size(1), dim, strides_of(q, k, v), float(scale),
-            int(bool(causal)), _k.current_stream()))
+            rest.data_ptr() if for_backward else None, lse.data_ptr() if for_backward else None, offsets.data_ptr(), tokens,
+            offsets.numel() - 1, heads, k.size(1), dim, strides_of(q, k, v), float(scale), int(bool(causal)), _k.current_stream()))
     return out, rest, lse
 
 
@@ -107,9 +112,14 @@ class PackedAttention(torch.autograd.Function):
         return grads + (None, None, None)
 
 
+def _forward_mode(t):
+    return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
+
+
 def general(q, k, v, offsets, scale, causal):
     """The call without the native side, which hands over whatever it does not take."""
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v)):
+    tracked = torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v))
+    if tracked or any(isinstance(t, torch.Tensor) and _forward_mode(t) for t in (q, k, v)):
         return PackedAttention.apply(q, k, v, offsets, scale, causal)
     return _forward(q, k, v, offsets, scale, causal, False)[0]
 

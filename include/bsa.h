@@ -457,8 +457,9 @@ int bsa_cache_read(int dtype, int cache_dtype, const void *keys, const void *val
  *             page holds behind the length is not looked at.
  *   tree      device uint8 [batch, drafts, drafts], or [drafts, drafts] with tree_shared: nonzero where new token i sees new
  *             token j; NULL: j <= i.  A token that sees nothing at all gets zeros.
- * At most 1024 drafts.  `workspace` (bsa_cached_attention_workspace_bytes, any contents) takes the chunks of long sequences; the launches
- * that use one at a time are to be ordered.  Results are the same bits in every call with the same lengths.
+ * At most 1024 drafts, width * page at most 2^30 - 2048.  `workspace` (bsa_cached_attention_workspace_bytes, any contents)
+ * takes the chunks of long sequences; the launches that use one at a time are to be ordered.  Results are the same bits in
+ * every call with the same lengths.
  */
 size_t bsa_cached_attention_workspace_bytes(int batch, int drafts, int heads, int key_heads, int head_dim, int width, int page);
 int bsa_cached_attention(int dtype, int cache_dtype, const void *q, const void *k, const void *v, void *out, const void *keys,

@@ -9,6 +9,7 @@ Modules
 layout_oracle   block-index tables (bit-exact contract), to_sparse / to_dense
 matmul_oracle   SDD / DSD / DDS dense semantics in float64 + backward algebra
 softmax_oracle  block-sparse softmax forward / backward in float64
+packed_oracle   packed attention, quantised rows, attention over a cache, with bounds
 configs         seeded synthetic inputs of the five benchmark configurations
 cpu_baseline    masked-dense torch-CPU timing used as the reported CPU baseline
 bsa_oracle.c    plain-C block-walk restatement (second, independent checker)
