@@ -913,7 +913,7 @@ static int check_drafts(const char *who, int batch, int drafts, int heads, int k
     // the tiles of 64 sequences are added up in 32 bits
     if (batch < 1 || batch > (1 << 20) || drafts < 1 || drafts > 1024 || width < 0 || (long long)width * page > (1LL << 30) - 2048)
         return fail(BSA_ERR_INVALID, "%s: %d sequences of %d new tokens and %d pages of %d", who, batch, drafts, width, page);
-    // blocks of rows: workgroups of 1024 threads, fewer than 2^32 threads; and the tiles a unit may get, in 32 bits
+    // blocks of 32 rows: up to four workgroups of 256 threads, fewer than 2^32 threads; and the tiles a unit may get, in 32 bits
     const long long blocks = (long long)batch * key_heads * ((drafts * (heads / key_heads) + 31) / 32);
     if (blocks >= (1LL << 22) || blocks * (((long long)width * page + drafts) / 32 + 2) > (1LL << 38))
         return fail(BSA_ERR_INVALID, "%s: %d sequences of %d new tokens and %d heads over %d pages of %d are too many", who, batch, drafts,

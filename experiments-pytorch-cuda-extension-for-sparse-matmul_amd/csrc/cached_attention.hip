@@ -87,7 +87,7 @@ __device__ __forceinline__ float upper_half_most(float x)
 // How the lengths cut the work: the tiles of a chunk, as many units as wanted and none shorter than `least` tiles, and the
 // sequence of a unit, or, with `unit` < 0, the units of sequence `of`.  Up to 64 sequences the lengths are loaded once.
 struct CachedUnit {
-    int b, len, part, parts, first, chunk;       // first: unit of part 0; b < 0: nothing to do
+    int b, len, part, parts, first, chunk;       // first: unit of part 0; chunk: its tiles; b < 0: nothing to do
 };
 __device__ __forceinline__ CachedUnit cached_unit(const CachedOperands &p, int unit, int of)
 {
@@ -108,11 +108,13 @@ __device__ __forceinline__ CachedUnit cached_unit(const CachedOperands &p, int u
         if (found != 0ull) {
             const int at = __builtin_ctzll(found);
             const int parts = __builtin_amdgcn_readlane(mine, at), first = __builtin_amdgcn_readlane(upto, at) - parts;
-            return CachedUnit{b0 + at, __builtin_amdgcn_readlane(len, at), unit - first, parts, first, chunk};
+            // as many units as such chunks make, but of even lengths: 48 trees over uneven sequences 239 us, 260 with a short last one
+            const int length = __builtin_amdgcn_readlane(len, at), even = ((length + 31) / 32 + drafted + parts - 1) / parts;
+            return CachedUnit{b0 + at, length, unit - first, parts, first, (even + p.together - 1) / p.together * p.together};
         }
         before = __builtin_amdgcn_readlane(upto, WAVE - 1);
     }
-    return CachedUnit{-1, 0, 0, 0, 0, chunk};
+    return CachedUnit{-1, 0, 0, 0, 0, 0};
 }
 
 template <int HD, bool BF, int KIND, int RG>
@@ -468,8 +470,9 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
 
 // Joins the chunks of the rows of a sequence and key head: HD / 4 lanes a row and list, the chunks of a row dealt to `lists` lists,
 // which are then joined pair by pair.  JOIN_BATCH chunks are loaded at a time: with one at a time each waited for the one before (384
-// chunks: 9.8 us).  The order of the sums is given by the number of chunks and of lists.
-constexpr int JOIN_BATCH = 8;
+// chunks: 9.8 us).  The order of the sums is given by the number of chunks and of lists.  Bound by latency: lengths, chunks, LDS.
+// 256 threads a workgroup: 108 rows of 4 sequences, walk and join 28.7 us, with 512 threads 32.8, with 1024 34.3.
+constexpr int JOIN_BATCH = 8, JOIN_THREADS = 256;
 struct JoinPart {
     float m, sum;
     f4v acc;
@@ -482,9 +485,9 @@ struct JoinPart {
     }
 };
 template <int HD, bool BF>
-__global__ __launch_bounds__(1024) void cached_join_kernel(CachedOperands p, int block_rows, int lists)
+__global__ __launch_bounds__(JOIN_THREADS) void cached_join_kernel(CachedOperands p, int block_rows, int lists)
 {
-    constexpr int LANES = HD / 4, GROUPS = 1024 / LANES;
+    constexpr int LANES = HD / 4, GROUPS = JOIN_THREADS / LANES;
     __shared__ f4v sums[GROUPS][LANES];
     __shared__ float2 stats[GROUPS];
     const int rows = GROUPS / lists;                    // rows of this workgroup
@@ -558,8 +561,8 @@ CachedOperands operands(const CachedArgs &a)
     p.least = CACHED_LEAST;
     p.together = CACHED_WAVES / rg * cached_subtiles(a.head_dim, rg);
     p.target = cached_units(rg);
-    // Every sequence ends in a unit that is shorter, which comes on top.  With few of them the wanted ones make room, so that all run at
-    // once: 33 sequences of 300 to 16000 tokens 64 us, without 78; 64 sequences 51 and 50.
+    // A sequence may have one unit more than its share of the wanted ones.  With few of them the wanted ones make room, so that all
+    // run at once: 33 sequences of 300 to 16000 tokens 64 us, without 78; 64 sequences 51 and 50.
     if (rg == 1 && 2ll * a.batch * a.key_heads * p.row_blocks <= p.target) p.target -= a.batch * a.key_heads * p.row_blocks;
     p.parts = (float *)a.workspace;
     p.stats = (float2 *)(p.parts + cached_attention_parts(a) * a.head_dim);
@@ -581,11 +584,11 @@ hipError_t walk(const CachedArgs &a, hipStream_t st)
     hipError_t err = hipGetLastError();
     if (err != hipSuccess || !cached_attention_splits(a)) return err;
     // as many lists as give the machine a workgroup a compute unit
-    constexpr int GROUPS = 1024 / (HD / 4);
+    constexpr int GROUPS = JOIN_THREADS / (HD / 4);
     int lists = 1;
     auto workgroups = [&]() { return (long long)a.batch * a.key_heads * ((p.rows + GROUPS / lists - 1) / (GROUPS / lists)); };
     while (lists < GROUPS && workgroups() < 256) lists *= 2;
-    cached_join_kernel<HD, BF><<<(unsigned)workgroups(), 1024, 0, st>>>(p, 32 * RG, lists);
+    cached_join_kernel<HD, BF><<<(unsigned)workgroups(), JOIN_THREADS, 0, st>>>(p, 32 * RG, lists);
     return hipGetLastError();
 }
 template <int HD, bool BF, int KIND>
