@@ -262,7 +262,11 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
 // parts add up in LDS at the end.  128 queries a tile at head dim 128, 64 at 64.  K stays in registers, V in LDS: with the
 // accumulators they would leave too few for two waves a SIMD at head dim 128 (256 registers each, none spilled: what is spilled
 // is waited for behind the tiles on their way).  One wave a SIMD with 512 registers and both key tiles, which reads Q and dO half
-// as often, took 430 us where this takes 345 (8191 tokens, 16 heads over 4): nothing runs beside what a wave waits for.
+// as often, took 430 us where this takes 338 (sequences of 4096, 2976 and 1119 tokens, 16 heads over 4, 650 TFLOP/s of the four
+// products): nothing runs beside what a wave waits for.  What bounds it: a step of the workgroup takes 6.3k clocks, of which the
+// products fill 2.0k, LDS 2.6k (Q and dO are read both ways) and the exponentials 1.0k, and the two waves of a SIMD, which the barrier
+// keeps in step, overlap little of it; and the first keys of the longest sequence have 128 steps where a compute unit has 106 on
+// average.  A static priority for one of the two waves changed nothing (622 us a training step for 619).
 // Behind the tiles of PairTiles: lse and delta of a tile's queries, per buffer, and the workgroup's V.
 template <int HD, bool BF, int SUB>
 __global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOperands p)
@@ -351,7 +355,6 @@ __global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOper
             read_rows<HD>(tiles.rd, q_at, op);
             product<BF>(op, kop, prob);
         }
-        issue_order();
         {
             h8 op[KS];
             read_rows<HD>(tiles.rd, do_at, op);
@@ -373,7 +376,6 @@ __global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOper
                 prob[v] = ((r < low) | (r >= high)) ? 0.f : prob[v];
             }
         }
-        issue_order();
         h8 pop[2], ds[2];
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
@@ -385,7 +387,6 @@ __global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOper
                 ds[v >> 3][v & 7] = narrow_16<BF>(prob[v] * ((dpacc[v] - dl[j]) * ds_scale));
             }
         }
-        issue_order();
 #pragma unroll
         for (int t = 0; t < HD / 32; ++t) {
             h8 qc[2], dc[2];
