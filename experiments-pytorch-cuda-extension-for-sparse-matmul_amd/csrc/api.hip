@@ -813,6 +813,7 @@ int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const 
     if (!out) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
     rc = check_alignment(who, {out, rest});
     if (rc) return rc;
+    if ((rest == nullptr) != (lse == nullptr)) return fail(BSA_ERR_INVALID, "%s: null pointer argument (rest and lse go together)", who);
     p.out = out;
     p.rest = rest;
     p.lse = lse;

@@ -157,7 +157,7 @@ struct PackedArgs {
     const void *q = nullptr, *k = nullptr, *v = nullptr;
     const void *dout = nullptr, *o = nullptr, *o_rest = nullptr;     // backward only; o: the forward result, o_rest: its rest; dense
     void *out = nullptr;                         // forward: the result; backward: dq
-    void *rest = nullptr;                        // forward: what the result's rounding took, may be null
+    void *rest = nullptr;                        // forward: what the result's rounding took; null with lse
     void *dk = nullptr, *dv = nullptr;           // both or neither
     float *lse = nullptr;                        // [heads][tokens]; forward: written, may be null; backward: read
     float *delta = nullptr;                      // backward: scratch of the same size

@@ -23,7 +23,9 @@ namespace {
 
 constexpr float PACKED_LAZY_SUM = 256.f;         // fp16 holds what stays below it
 
-template <int HD, bool BF, int W>
+// TRAIN: the row statistics and the result's rest are wanted.  The result is normalised by the sum of the rounded probabilities, so that
+// their common error cancels; the statistics are of the exponentials before that, which is what the backward walks make again.
+template <int HD, bool BF, int W, bool TRAIN>
 __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperands p)
 {
     extern __shared__ __align__(16) unsigned char lds_raw[];
@@ -50,7 +52,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
     loaded(qop);
 
     // reference point of the query (both lane halves agree), minus it (0 while nothing was seen), this half's sum
-    float m = NEG_INF, minus_m = 0.f, lsum = 0.f;
+    float m = NEG_INF, minus_m = 0.f, lsum = 0.f, exact_sum = 0.f;
     RowTile<HD> oacc;
     clear<HD>(oacc);
 
@@ -63,10 +65,10 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
             product<BF>(kop, qop, sacc[u]);
         }
     };
-    float psum;
+    float psum, pexact;
     h8 pop[2][2];
     auto exponentials = [&](const f16v (&sacc)[2], float mul) {
-        psum = 0.f;
+        psum = 0.f, pexact = 0.f;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -75,6 +77,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
                 pop[u][v >> 3][v & 7] = narrow_16<BF>(p0);
                 pop[u][v >> 3][(v & 7) + 1] = narrow_16<BF>(p1);
                 psum = add_pair<BF>(pop[u][v >> 3][v & 7], pop[u][v >> 3][(v & 7) + 1], psum);
+                if (TRAIN) pexact += p0 + p1;
             }
     };
     // A row moves its reference point by itself, so that its bits are its own: a row beside it, of NaN say, changes nothing.
@@ -93,11 +96,11 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
             const float keep = m == NEG_INF ? 0.f : at_exp2(m - at_finite_or_zero(m_new));       // nothing accumulated so far: 0
             m = m_new;
             minus_m = -at_finite_or_zero(m_new);
-            lsum *= keep;
+            lsum *= keep, exact_sum *= keep;
             each<HD>(oacc, [&](float x, int) { return x * keep; });
             exponentials(sacc, mul);
         }
-        lsum += psum;
+        lsum += psum, exact_sum += pexact;
     };
     // Round r has the keys of tile r and the values of tile r - 1, in buffer r % 2.
     auto enter = [&](int r) {
@@ -156,13 +159,14 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
     for (; r <= steps; ++r) enter(r);            // of the rows below
     lsum += at_lane_xor32(lsum);                 // both halves used the same reference point
     const bool any = lsum > 0.f || lsum != lsum;
-    if (p.lse != nullptr && h == 0 && row < n)   // log2 of the row's sum, +inf for a row that sees nothing
+    if (TRAIN) exact_sum += at_lane_xor32(exact_sum);
+    if (TRAIN && h == 0 && row < n)              // log2 of the row's sum, +inf for a row that sees nothing
         p.lse[(size_t)item.head * p.tokens + begin + row] =
-            any ? at_finite_or_zero(m) + __builtin_amdgcn_logf(lsum) : __builtin_inff();
+            any ? at_finite_or_zero(m) + __builtin_amdgcn_logf(exact_sum) : __builtin_inff();
     __syncthreads();                             // all are done with the tiles, whose place the results take
     store_token_rows<HD, BF>(oacc, any ? 1.f / lsum : 0.f, lds_raw + 64 * HD * w,
                              p.out + ((begin + row0) * p.heads + item.head) * HD, (long long)p.heads * HD, n - row0);
-    if (p.rest != nullptr)
+    if (TRAIN)
         store_token_rows<HD, BF, true>(oacc, any ? 1.f / lsum : 0.f, lds_raw + 64 * HD * w,
                                        p.rest + ((begin + row0) * p.heads + item.head) * HD, (long long)p.heads * HD, n - row0);
 }
@@ -173,7 +177,9 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
 //   rows      as the forward walk:  P = exp2(scale2 S - lse),  dS = P (dO V^T - delta),  dq^T += K^T dS^T;
 //             delta = rowsum(dO O) is made here, O with what its rounding took, and left for the other walk.  From the rounded O
 //             alone its error moves a whole row of dS the same way: dq and dk were 1.6 times as far from float64 as their own
-//             rounding leaves them, with it 1.45 (dS in 16 bits), at no time that could be measured
+//             rounding leaves them, with it 1.46, at no time that could be measured, and 1.44 with the statistics of the exponentials
+//             before they are rounded (1 % of a training step).  dS itself in 16 bits gives 1.42 of that; its low parts as a
+//             second operand would leave 1.05 but take 8 % (bf16, head dim 64)
 //   columns   a workgroup holds 32 W keys of one key head and walks the queries of all heads that share it:
 //             dv^T += dO^T P,  dk^T += Q^T dS
 // ---------------------------------------------------------------------------
@@ -459,7 +465,8 @@ template <int HD, bool BF>
 hipError_t forward(const PackedArgs &a, hipStream_t st)
 {
     constexpr int W = PACKED_WAVES;
-    return run_walk(packed_forward_kernel<HD, BF, W>, operands(a), a.heads, 32 * W, W, PairTiles<HD, W, 2>::lds_bytes(), st);
+    return run_walk(a.lse != nullptr ? packed_forward_kernel<HD, BF, W, true> : packed_forward_kernel<HD, BF, W, false>, operands(a), a.heads,
+                    32 * W, W, PairTiles<HD, W, 2>::lds_bytes(), st);
 }
 template <int HD, bool BF>
 hipError_t backward(const PackedArgs &a, hipStream_t st)

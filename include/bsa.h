@@ -407,8 +407,8 @@ int bsa_weight_grad(int dtype, const void *a, const void *b, void *out, const in
  *   out[i] = softmax(scale q[i] k^T over the tokens of its sequence; with `causal` over those up to i) v
  *   q, dout          [tokens, heads, head_dim],  k, v [tokens, key_heads, head_dim], with strides
  *   out, dq          [tokens, heads, head_dim], dense;  dk, dv [tokens, key_heads, head_dim], dense
- *   rest             as out: what the rounding to 16 bits took from it.  The backward call needs it and lse; both may be
- *                    NULL in the forward call.
+ *   rest             as out: what the rounding to 16 bits took from it.  The backward call needs it and lse; the
+ *                    forward call makes both or, where both are NULL, neither.
  *   lse, delta_ws    float [heads, tokens]: log2 of each row's sum of exponentials; scratch of the backward call
  *   offsets          device int32[sequences + 1]: sequence b is tokens offsets[b] .. offsets[b + 1] - 1.  They stay on the
  *                    device.  Ascending; sequences may be empty.  Tokens in front of the first and behind the last

@@ -42,7 +42,7 @@ def backward(k, dtype=F16, q=P, dout=P, out=P, rest=P, lse=P, delta=P, dq=P, dk=
     (dict(tokens=1 << 30, heads=64, key_heads=8), "too many"), (dict(sequences=1 << 23), "too many"),
     (dict(q=None), "null"), (dict(kk=None), "null"), (dict(v=None), "null"), (dict(out=None), "null"), (dict(offsets=None), "null"),
     (dict(q=P + 8), "aligned to 16"), (dict(v=P + 2), "aligned to 16"), (dict(out=P + 8), "aligned to 16"), (dict(rest=P + 8), "aligned to 16"),
-    (dict(s=()), "null"),
+    (dict(s=()), "null"), (dict(rest=P), "go together"),
 ])
 def test_packed_forward(k, kw, needle):
     refused(k, forward(k, **kw), "bsa_packed_attention_forward", needle)
