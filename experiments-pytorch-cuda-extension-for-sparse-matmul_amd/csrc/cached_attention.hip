@@ -10,6 +10,10 @@
 // which lie in one page.  A workgroup has four waves: RG groups of 32 rows times 4 / RG groups of tiles.  RG = 1: every wave walks
 // tiles of its own through registers and its own LDS, with no barrier before the end.  RG = 4: 128 rows, whose waves share the
 // tile, double buffered.
+// What bounds it: with few rows the cache's bytes and the way of a chunk's first ones through page table, memory and LDS (one sequence of
+// 131071 int8 tokens, 2 key heads: 24 us, 2.9 TB/s; 16 of 0 to 8192 e4m3 tokens, 4 key heads: 11.5); with many the widening of a tile, its exponentials and the
+// barrier of a step (244 rows a sequence over 48 long ones: 235 us with the join, 283 TFLOP/s; the vector pipe is busy in 35 % of
+// the clocks, the matrix pipe in 11 %, and waves wait in 46 %).
 // The work is cut where it lies: a unit is a chunk of the tiles of one sequence and key head, the chunk chosen on the device
 // from the lengths so that the units fill the machine, long sequences in many, short ones in one.  A sequence in several units
 // leaves (max, sum, O) of each in a workspace, which a second launch joins in the order of the chunks.
