@@ -6,9 +6,9 @@
 //   S^T = K Q^T             a lane holds ONE query column and 32 of the 64 keys (the others sit in lane ^ 32)
 //   online softmax          per-lane reference point and sum; the point moves only when a tile's sum of exponentials passes 256
 //   O^T += V^T P^T          the probabilities go from accumulators to operands without leaving the registers
-// What bounds it: 32 exponentials a lane and tile (8 clocks each, 2 x 64 keys of a wave take 1.0k) beside 16 products of 32 clocks at
-// head dim 64 and 32 at 128, so the scores of the next tile are made beside the exponentials of this one, and two waves a SIMD fill
-// what is left.  Causal, 16384 tokens, 16 heads at head dim 64: 614 to 632 us, 870 to 895 TFLOP/s; sequences of 4096 to 97 tokens at head
+// What bounds it: a tile has 32 exponentials a lane (8 clocks each, as much again for scaling, rounding and sums) beside 16 products of 32
+// clocks at head dim 64 and 32 at 128, so the scores of the next tile are made beside the exponentials of this one, and two waves a
+// SIMD fill what is left.  Causal, 16384 tokens, 16 heads at head dim 64: 614 to 632 us, 870 to 895 TFLOP/s; sequences of 4096 to 97 tokens at head
 // dim 128: 108 to 112 us, 860 to 890 TFLOP/s (a library product of 8192^3 1217 on the same card).  W = 4: eight waves, which read K and V
 // half as often, took 124 us for those 112 and 660 for 620: twice as many waves wait at a barrier, and half as many workgroups share
 // the uneven rows.
@@ -190,8 +190,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
 //   columns   a workgroup holds 64 keys of one key head and walks the queries of all heads that share it:
 //             dv^T += dO^T P,  dk^T += Q^T dS
 // Sequences of 4096, 2976 and 1119 tokens, 16 heads over 4, head dim 128 (55 GFLOP a product): forward 145 us, rows 190, columns 328
-// (760, 870 and 670 TFLOP/s); 12 heads at head dim 64, six sequences of 1 to 1500 tokens 28, 37 and 36 us, most of it the longest
-// sequence's tiles one after the other.  Rows have the forward walk's bounds with three products to the exponentials' one.
+// (760, 870 and 670 TFLOP/s); 12 heads at head dim 64, six sequences of 1 to 1500 tokens 28, 37 and 36 us, one
+// generation of workgroups, as long as the 24 steps of the longest sequence.  Rows have the forward walk's bounds with three products to the exponentials' one.
 // ---------------------------------------------------------------------------
 template <int HD, bool BF, int W>
 __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p)
