@@ -61,6 +61,8 @@ class KeyValueCache:
         self.__dict__.update(state)
         self._held = tuple(t.view(self.dtype) for t in self._held[:2]) + self._held[2:]
         self.device = self.keys.device
+        if self.device.type != "cuda":              # loaded elsewhere: its calls would hand host addresses to kernels
+            raise ValueError("a cache lives on the GPU")
         self._native = _k.host_calls.new_cache(*self._held)
 
     def _tensors(self):

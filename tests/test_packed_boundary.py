@@ -145,6 +145,15 @@ def test_python_side_refuses_before_the_device_is_touched():
             KeyValueCache(**{**dict(pages=2, heads=2, head_dim=64), **kw})
 
 
+def test_a_cache_loaded_off_the_gpu_is_refused():
+    from sparse import KeyValueCache
+    rows = torch.zeros(2, 1, 32, 64, dtype=torch.uint8)
+    state = dict(pages=2, heads=1, head_dim=64, dtype=torch.int8, page=32, device=torch.device("cuda", 0),
+                 _held=(rows, rows.clone(), torch.zeros(2, 1, 32), torch.zeros(2, 1, 32)))
+    with pytest.raises(ValueError, match="lives on the GPU"):
+        KeyValueCache.__new__(KeyValueCache).__setstate__(state)
+
+
 @pytest.mark.parametrize("kind", ["slice", "heads first", "one token", "odd start", "odd stride", "broadcast"])
 def test_operands_are_copied_only_where_a_row_cannot_be_read_in_place(kind):
     from sparse.packed import rows_of, strides_of
