@@ -56,7 +56,7 @@ __host__ __device__ constexpr int panel_list_length(int kblocks) { return (kbloc
 // the panels (200 MB through the L2 -> LDS path: 18 us without the products).  us, panels through registers a step ahead and a
 // barrier per step, 96 rows a workgroup -> fetching waves and a barrier per step, 160 rows -> flags -> operands of a block read
 // together: 4224 rows x 2048 x 2048 at a quarter of its blocks, forward 31.3 -> 26.0 -> 24.6 -> 23.7, gradient of the dense operand
-// 32.3 -> 24.5 -> 24.3 -> 22.8; 8192 x 3072 x 3072 at 0.3 107 -> 91 and 111 -> 84; every block stored, 4224 rows 56 -> 46 and 56 -> 41.
+// 32.3 -> 24.5 -> 24.3 -> 22.8; every block stored, 4224 rows 56 -> 46 and 56 -> 41.
 // A group that has a block in every k-block makes its wave the chain; half of it goes to another wave (PANEL_CUT_FROM).  Launches of
 // two generations of workgroups in which that does not help are slower than two workgroups of eight waves a compute unit were: two such
 // columns among eight, 5632 rows 31.7 -> 38.6 (input gradient 32.5 -> 34.3); half and all of 48 x 80 blocks stored, 4800 rows 35.7 ->
