@@ -10,8 +10,8 @@
 //
 // What bounds it: 16 bytes a lane in, 8 out, 3 operations and a conversion a value between them: memory.  A row is 8 or 16
 // lanes, which share its maximum in 3 or 4 exchanges; key and value rows of a token and head go together.  65521 tokens of 8 heads at
-// head dim 64: written as int8 in 46 us, read back in 40 (4.2 and 5.0 TB/s); 8191 tokens in and out as e4m3 21 us, 4.6 TB/s, where a copy
-// of 1 GiB reaches 5.2.  48 rows 3.3 us: a launch.
+// head dim 64, written as int8 and read back: 69 us, 5.7 TB/s, where a copy of 1 GiB reaches 5.2 (part of it is still in the last
+// cache); 8191 tokens in and out as e4m3 21 us, 4.7 TB/s; 48 rows 3.3 us: a launch.
 #include "bsa_device.hpp"
 #include "bsa_internal.hpp"
 #include "cache_values.hpp"
@@ -90,19 +90,21 @@ __global__ __launch_bounds__(256) void cache_write_kernel(
     }
 }
 
+// What is read back leaves without a place in the caches: it would drive out the rows that the next calls read (65521 tokens in and out
+// 69 us of kernels, with ordinary stores 91; 8191 21.0 and 21.7).  Streaming the write's loads as well gives 76 and 19.9.
 // TO: 0 fp32, 1 fp16, 2 bf16 (the numbers of the ABI); FROM_BF: what a 16-bit cache holds
 template <int TO>
 __device__ __forceinline__ void store_values(void *out, long long at, const float (&y)[8])
 {
     if (TO == BSA_F32) {
         float *p = reinterpret_cast<float *>(out) + at;
-        *reinterpret_cast<float4 *>(p) = make_float4(y[0], y[1], y[2], y[3]);
-        *reinterpret_cast<float4 *>(p + 4) = make_float4(y[4], y[5], y[6], y[7]);
+        stg16_stream(p, __builtin_bit_cast(uint4, make_float4(y[0], y[1], y[2], y[3])));
+        stg16_stream(p + 4, __builtin_bit_cast(uint4, make_float4(y[4], y[5], y[6], y[7])));
     } else {
         h8 o;
 #pragma unroll
         for (int j = 0; j < 8; ++j) o[j] = narrow_16<TO == BSA_BF16>(y[j]);
-        stg16(reinterpret_cast<half_t *>(out) + at, __builtin_bit_cast(uint4, o));
+        stg16_stream(reinterpret_cast<half_t *>(out) + at, __builtin_bit_cast(uint4, o));
     }
 }
 
