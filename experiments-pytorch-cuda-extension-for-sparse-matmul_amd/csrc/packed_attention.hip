@@ -227,7 +227,12 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
         for (int j = 0; j < 8; ++j) delta += widen_16<BF>(dop[s][j]) * (widen_16<BF>(o[j]) + widen_16<BF>(rest[j]));
     }
     delta += at_lane_xor32(delta);               // the other half of the head dim sits in lane ^ 32
-    if (h == 0 && row < n) p.delta[(size_t)item.head * p.tokens + token] = delta;
+    // Rows whose keys all lie in the first tile make their delta again as sum P dP, of their own probabilities: with few keys the
+    // rounding of the forward pass's probabilities, which O has, weighs most (a bf16 batch of short sequences: dq and dk 1.65 times as far
+    // off as their own rounding, so 1.35; 37 tokens 1.48 and 1.446, which is dS's to three digits).  One more look at one tile, by the
+    // waves that have the fewest: 1 % of a training step.
+    const bool few = (p.causal ? min(row0 + 32, n) : n) <= 64;
+    if (!few && h == 0 && row < n) p.delta[(size_t)item.head * p.tokens + token] = delta;
     loaded(qop);
     loaded(dop);
 
@@ -241,6 +246,25 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
         if (row0 >= n || (p.causal && k0 > row0 + 31)) continue;
         const bool masked = k0 + 64 > n || (p.causal && k0 + 63 > row0);
         const int seen = (p.causal ? min(row, n - 1) : n - 1) - k0;
+        if (few) {
+            delta = 0.f;
+#pragma unroll 1
+            for (int u = 0; u < 2; ++u) {
+                f16v sacc = {0}, dpacc = {0};
+                h8 op[KS];
+                read_rows<HD>(tiles.rd, tiles.at(buffer, 0, u), op);
+                product<BF>(op, qop, sacc);
+                read_rows<HD>(tiles.rd, tiles.at(buffer, 1, u), op);
+                product<BF>(op, dop, dpacc);
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const float part = at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus_lse)) * dpacc[v];
+                    delta += 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? 0.f : part;
+                }
+            }
+            delta += at_lane_xor32(delta);
+            if (h == 0 && row < n) p.delta[(size_t)item.head * p.tokens + token] = delta;
+        }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
             f16v sacc = {0}, dpacc = {0};

@@ -199,21 +199,25 @@ def test_a_page_may_belong_to_several_sequences_and_come_twice():
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 128])
-def test_gradients_lose_no_more_than_the_rounding_of_ds(dim, dtype):
+@pytest.mark.parametrize("n,count", [(700, 1), (40, 20)])
+def test_gradients_lose_no_more_than_the_rounding_of_ds(n, count, dim, dtype):
     """Error of dq and dk against float64, as a multiple of what rounding the exact ones would leave.  Two roundings of the same relative
     size, of dS and of the result, give sqrt(2); delta from a rounded result would move all of a row of dS alike (measured: 1.6)."""
     import sparse
-    n, heads, key_heads, scale = 700, 4, 2, dim ** -0.5
-    q, k, v = (normal(i, n, h, dim, dtype=dtype).requires_grad_() for i, h in ((1, heads), (2, key_heads), (3, key_heads)))
-    dout = normal(4, n, heads, dim, dtype=dtype)
-    dq, dk = torch.autograd.grad(sparse.packed_attention(q, k, v, int32([0, n]), scale), (q, k), dout)
-    qd, kd, vd, dd = (t.detach().cpu().double().transpose(0, 1) for t in (q, k, v, dout))
-    kd, vd = (t.repeat_interleave(heads // key_heads, 0) for t in (kd, vd))
-    s = (scale * qd @ kd.transpose(1, 2).contiguous()).masked_fill(~torch.ones(n, n, dtype=torch.bool).tril(), -math.inf)
+    heads, key_heads, scale = 4, 2, dim ** -0.5
+    q, k, v = (normal(i, count * n, h, dim, dtype=dtype).requires_grad_() for i, h in ((1, heads), (2, key_heads), (3, key_heads)))
+    dout = normal(4, count * n, heads, dim, dtype=dtype)
+    offsets = torch.arange(0, count * n + 1, n, dtype=torch.int32, device="cuda")
+    dq, dk = torch.autograd.grad(sparse.packed_attention(q, k, v, offsets, scale), (q, k), dout)
+    # [count, heads, n, dim]
+    apart = lambda t: t.detach().cpu().double().view(count, n, -1, dim).transpose(1, 2)
+    qd, kd, vd, dd = (apart(t) for t in (q, k, v, dout))
+    kd, vd = (t.repeat_interleave(heads // key_heads, 1) for t in (kd, vd))
+    s = (scale * qd @ kd.transpose(2, 3).contiguous()).masked_fill(~torch.ones(n, n, dtype=torch.bool).tril(), -math.inf)
     p = s.softmax(-1)
-    ds = scale * p * (dd @ vd.transpose(1, 2).contiguous() - (dd * (p @ vd)).sum(-1, keepdim=True))
-    exact_q = (ds @ kd).transpose(0, 1)
-    exact_k = (ds.transpose(1, 2).contiguous() @ qd).view(key_heads, -1, n, dim).sum(1).transpose(0, 1)
+    ds = scale * p * (dd @ vd.transpose(2, 3).contiguous() - (dd * (p @ vd)).sum(-1, keepdim=True))
+    exact_q = ds @ kd
+    exact_k = (ds.transpose(2, 3).contiguous() @ qd).view(count, key_heads, -1, n, dim).sum(2)
     for got, exact in ((dq, exact_q), (dk, exact_k)):
         rounded = exact.to(dtype).double()
-        assert (got.cpu().double() - exact).norm() <= 1.1 * math.sqrt(2) * (rounded - exact).norm()
+        assert (apart(got) - exact).norm() <= 1.1 * math.sqrt(2) * (rounded - exact).norm()
