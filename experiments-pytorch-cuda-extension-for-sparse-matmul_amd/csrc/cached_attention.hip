@@ -3,8 +3,8 @@
 // there is none).  One new token a sequence is a decode step, a tree of drafted ones the check of a draft.
 //
 //   S_ij = scale (q_i . y_j) s_j     y: the 8-bit values as 16-bit ones (exact), s: the scale of the token's row
-//   O_i  = sum_j softmax(S)_ij t_j z_j      the scales of the values ride on the probabilities, relative to their
-//                                           largest so far, so that fp16 holds them
+//   O_i  = sum_j softmax(S)_ij t_j z_j      the scales of the values ride on the probabilities; what is rounded is
+//                                           exp2(S - m) t, m from the largest exp2(S) t that the row has met
 //
 // The query rows of a key head (N times the heads that share it) are the columns of 32 x 32 x 16 products; a tile is 32 tokens,
 // which lie in one page.  A workgroup has four waves: RG groups of 32 rows times 4 / RG groups of tiles.  RG = 1: every wave walks
@@ -38,7 +38,15 @@ constexpr int cached_row_groups(int rows) { return rows <= 64 ? 1 : 4; }
 constexpr int cached_subtiles(int hd, int rg) { return rg == 1 || hd == 128 ? 1 : 2; }
 // K, V and the scales of them
 constexpr int cached_set_bytes(int hd, int rg) { return cached_subtiles(hd, rg) * (128 * hd + 256) + 256; }
-constexpr float CACHED_LAZY_SUM = 256.f;
+// The reference point of a row moves once a step's exponentials sum up to more.  Over an 8-bit cache a weight is at most 2^15 then, and
+// the largest was 2^lift when the point was set: fp16 keeps all bits of those down to 2^-18 of it.  48 trees over int8 caches, fp16:
+// lift 6 248 us, 4 234, 0 226, a point that moved at 256 over a lift of 6 305.
+constexpr float CACHED_LAZY_SUM = 256.f, CACHED_LAZY_WEIGHTS = 32768.f;
+constexpr float cached_lift(bool bf) { return bf ? 0.f : 4.f; }
+// Scales count in the reference point from 2^-32 on, so that exponentials without them, whose sum the row is divided by, stay
+// within fp32, and up to 2^64 in bf16, so that those of other tokens do; what fp16 rows over larger ones give is infinite.
+constexpr float CACHED_LEAST_SCALE = -32.f;
+constexpr float cached_most_scale(bool bf) { return bf ? 64.f : 124.f; }
 
 struct CachedOperands {
     const half_t *q, *k, *v;
@@ -53,6 +61,7 @@ struct CachedOperands {
     int pages, page_shift, width;                // width: of the page table
     int rows, row_blocks, least, together, target;   // rows: drafts * group; a chunk has `least` tiles or more, a
                                                  // multiple of `together`; target: units wanted
+    int step_shift;                              // log2 of the tiles of a step: a sequence's cached ones are counted up to a multiple
     int tree_batch;                              // values between the masks of two sequences, 0: one mask for all
     float scale2;
     long long q_batch, q_token, q_head, k_batch, k_token, k_head, v_batch, v_token, v_head;
@@ -95,9 +104,10 @@ struct CachedUnit {
 };
 __device__ __forceinline__ CachedUnit cached_unit(const CachedOperands &p, int unit, int of)
 {
-    const int l = lane_id(), drafted = (p.drafts + 31) / 32;
+    const int l = lane_id(), drafted = (p.drafts + 31) / 32, shift = p.step_shift;
+    auto held = [&](int len) { return (len + (32 << shift) - 1) >> (5 + shift) << shift; };
     auto length = [&](int b0) { return b0 + l < p.batch ? cached_length(p, b0 + l) : 0; };
-    auto tiles = [&](int b0, int len) { return b0 + l < p.batch ? (len + 31) / 32 + drafted : 0; };
+    auto tiles = [&](int b0, int len) { return b0 + l < p.batch ? held(len) + drafted : 0; };
     int len = length(0);
     long long total = 0;
     for (int b0 = 0; b0 < p.batch; b0 += WAVE)
@@ -113,7 +123,7 @@ __device__ __forceinline__ CachedUnit cached_unit(const CachedOperands &p, int u
             const int at = __builtin_ctzll(found);
             const int parts = __builtin_amdgcn_readlane(mine, at), first = __builtin_amdgcn_readlane(upto, at) - parts;
             // as many units as such chunks make, but of even lengths: 48 trees over uneven sequences 239 us, 260 with a short last one
-            const int length = __builtin_amdgcn_readlane(len, at), even = ((length + 31) / 32 + drafted + parts - 1) / parts;
+            const int length = __builtin_amdgcn_readlane(len, at), even = (held(length) + drafted + parts - 1) / parts;
             return CachedUnit{b0 + at, length, unit - first, parts, first, (even + p.together - 1) / p.together * p.together};
         }
         before = __builtin_amdgcn_readlane(upto, WAVE - 1);
@@ -138,7 +148,9 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
     const CachedUnit u = cached_unit(p, unit, 0);
     if (u.b < 0) return;
     const int b = u.b, len = u.len, chunk = u.chunk;
-    const int held = (len + 31) / 32, tiles = held + (p.drafts + 31) / 32;
+    // tiles of the cache; the new tokens' begin a step of their own: their values come as they are, with scale 1, and beside weights of
+    // that size those of a cached tile with small values would lose bits
+    const int cached = (len + 31) / 32, held = (cached + SUBT - 1) / SUBT * SUBT, tiles = held + (p.drafts + 31) / 32;
     const int begin = u.part * chunk, end = min(tiles, begin + chunk);
 
     const int w = wave_id(), l = lane_id(), qq = l & 31, h = l >> 5, rg = w % RG, kg = w / RG;
@@ -162,7 +174,7 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
             const int t = t0 + s;
             step.there[s] = 0;
             step.first[s] = 0;
-            if (t >= held || t >= end) continue;
+            if (t >= cached || t >= end) continue;
             const int page_index = t >> (p.page_shift - 5);
             if (window < 0 || page_index - window >= WAVE) {
                 window = page_index;
@@ -243,7 +255,7 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
             const bool fresh = step.t0 + s >= held, is = (l & 31) < step.there[s];
             const float x = fresh ? (l < 32 ? p.scale2 : 1.f) : is ? (l < 32 ? raw[s] * p.scale2 : raw[s]) : l < 32 ? p.scale2 : 0.f;
             scales[64 * s + l] = x;
-            const float most = upper_half_most(x);
+            const float most = upper_half_most(__builtin_fabsf(x));
             if (l == 63) scales[64 * SUBT + s] = most;
         }
     };
@@ -262,10 +274,13 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
 #pragma unroll
     for (int s = 0; s < KS; ++s) qop[s] = as_h8(ldg16(q_row + 16 * s + 8 * h));
 
-    // Reference point of the exponentials: the row's own m, and `shift`, log2 of a power of two above every value scale so far.  A
-    // weight p t, t the scale of its value row, is then at most 256, whatever the scales are; sum and results are relative
-    // to both alike.
-    float m = NEG_INF, lsum = 0.f, shift = 0.f, most_scale = 0.f, minus_ref = 0.f, most_sum = CACHED_LAZY_SUM;
+    // Reference point of the row's exponentials, which its sum and results are relative to: the largest score, over an 8-bit cache the
+    // largest score + log2(scale of the value row).  A large value row of no weight is then no measure for the others: 4096 fp16
+    // tokens, one 1e4 times as large and of weight 1e-8, were off by 2.4e-3 when the largest scale was it, by 3.4e-4 as
+    // without that row with this.
+    float m = NEG_INF, lsum = 0.f, minus_ref = 0.f;
+    float most_sum = CACHED_LAZY_SUM;            // of a step's exponentials; declared in the step it costs 30 registers more
+    constexpr float LEAST_SCALE = CACHED_LEAST_SCALE, MOST_SCALE = cached_most_scale(BF);
     RowTile<HD> oacc;
     clear<HD>(oacc);
     auto scores = [&](unsigned k_tiles, f16v (&sacc)[SUBT]) {
@@ -283,17 +298,9 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
 #pragma unroll
         for (int s = 0; s < SUBT; ++s) partial = partial || step.t0 + s >= held || step.there[s] < 32;
         if (SCALED) {
-            float most = scales[64 * SUBT];
+            float most = scales[64 * SUBT];      // value scale of the step
             if (SUBT > 1) most = fmaxf(most, scales[64 * SUBT + 1]);
-            if (most > most_scale) {             // the same in all lanes
-                const float to = (float)__builtin_amdgcn_frexp_expf(most) + 1.f, keep = at_exp2(shift - to);       // twice: fewer of these
-                most_scale = at_exp2(to);
-                shift = to;
-                minus_ref = -(at_finite_or_zero(m) + shift);
-                most_sum = CACHED_LAZY_SUM / most_scale;
-                lsum *= keep;
-                each<HD>(oacc, [&](float x, int) { return x * keep; });
-            }
+            most_sum = CACHED_LAZY_WEIGHTS * __builtin_amdgcn_rcpf(__builtin_amdgcn_fmed3f(most, at_exp2(LEAST_SCALE), at_exp2(MOST_SCALE)));
         }
         unsigned sees[SUBT];                     // bit v: the key of accumulator value v is seen
         if (partial) {
@@ -355,14 +362,21 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     const f4v ks = scale_of(s, g);
+                    f4v vs = {1.f, 1.f, 1.f, 1.f};
+                    if (SCALED) vs = *reinterpret_cast<const f4v *>(scales + 64 * s + 32 + 8 * g + 4 * h);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) bm = fmaxf(bm, sacc[s][4 * g + j] * ks[j]);
+                    for (int j = 0; j < 4; ++j) {
+                        float point = sacc[s][4 * g + j] * ks[j];
+                        if (SCALED) point += __builtin_amdgcn_fmed3f(__builtin_amdgcn_logf(__builtin_fabsf(vs[j])), LEAST_SCALE, MOST_SCALE);
+                        bm = fmaxf(bm, point);
+                    }
                 }
+            if (SCALED) bm -= cached_lift(BF);
             bm = fmaxf(bm, at_lane_xor32(bm));
             const float m_new = move ? fmaxf(m, bm) : m;
             const float keep = m == NEG_INF ? 0.f : at_exp2(m - at_finite_or_zero(m_new));       // nothing accumulated so far: 0
             m = m_new;
-            minus_ref = -(at_finite_or_zero(m_new) + shift);
+            minus_ref = -at_finite_or_zero(m_new);
             lsum *= keep;
             each<HD>(oacc, [&](float x, int) { return x * keep; });
             exponentials();
@@ -412,7 +426,6 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
         if (RG == 1) wave_lds_fence();
     }
     lsum += at_lane_xor32(lsum);
-    m += shift;                                  // what sum and results are relative to
 
     // join the tile groups of the workgroup: all but the first park (max, sum) and O^T in LDS
     __syncthreads();
@@ -564,6 +577,8 @@ CachedOperands operands(const CachedArgs &a)
     p.row_blocks = (p.rows + 32 * rg - 1) / (32 * rg);
     p.least = CACHED_LEAST;
     p.together = CACHED_WAVES / rg * cached_subtiles(a.head_dim, rg);
+    p.step_shift = cached_subtiles(a.head_dim, rg) - 1;
+    static_assert(cached_subtiles(64, 4) <= 2, "the logarithm above");
     p.target = cached_units(rg);
     // A sequence may have one unit more than its share of the wanted ones.  With few of them the wanted ones make room, so that all
     // run at once: 33 sequences of 300 to 16000 tokens 64 us, without 78; 64 sequences 51 and 50.
@@ -614,7 +629,8 @@ hipError_t walk_kind(const CachedArgs &a, hipStream_t st)
 // most tiles a sequence can have
 static long long most_tiles(const CachedArgs &a)
 {
-    return (((long long)a.width << a.page_shift) + 31) / 32 + (a.drafts + 31) / 32;
+    const long long step = 32 * cached_subtiles(a.head_dim, cached_row_groups(a.drafts * (a.heads / a.key_heads)));
+    return (((long long)a.width << a.page_shift) + step - 1) / step * (step / 32) + (a.drafts + 31) / 32;
 }
 bool cached_attention_splits(const CachedArgs &a) { return most_tiles(a) > CACHED_LEAST; }
 // Most units (of all sequences) a launch can have: the chunk is at least total key_heads row_blocks / target, so that the whole

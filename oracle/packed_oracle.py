@@ -88,14 +88,16 @@ def quantise(x, kind):
     return np.where(fine[..., None], y, 0.0), np.where(fine, top / bound, np.nan)
 
 
-def cached(q, k, v, held_keys, held_values, value_scales, lengths, tree, scale, kind):
+def cached(q, k, v, held_keys, held_values, value_scales, lengths, tree, scale, kind, by_weight=False):
     """``q [B, n, Hq, D]``, new ``k``, ``v [B, n, Hk, D]``, ``held_* [b] -> [Hk, length, D]`` (dequantised), ``value_scales [b] ->
     [Hk, length]`` (None: a 16-bit cache), ``tree [B, n, n]``.
 
     Bound of a quantised cache.  The weight of value row j is p_j t_j / top before it is rounded, p_j relative to a reference point at
     which the sum of all p is at least 1, t_j the row's scale (1 of a new token) and top at most twice the largest of them.  Where that
     is below the smallest normal fp16 value the rounding is off by up to half the smallest step, ``TINY``, whatever the weight: by
-    TINY top / t_j of p_j, and of the normalised probability no more, the sum being at least 1."""
+    TINY top / t_j of p_j, and of the normalised probability no more, the sum being at least 1.  With ``by_weight`` top is what the
+    largest p_j t_j of the cached rows is, less a factor of 2^4 (for a new token, whose row comes as it is, of all that the token
+    sees): a row that weighs nothing is no measure for the others."""
     batch, n, heads, _ = q.shape
     group = heads // k.shape[2]
     value, bound = np.zeros(q.shape), np.zeros(q.shape)
@@ -109,5 +111,11 @@ def cached(q, k, v, held_keys, held_values, value_scales, lengths, tree, scale, 
             if value_scales is not None:
                 t = np.concatenate([value_scales[b][g], np.ones(n)])
                 tiny = np.where(t > 0, TINY[kind] * 2 * t.max() / np.where(t > 0, t, 1.0), 0.0)
+                if by_weight:
+                    w = _softmax(scale * (q[b, :, h] @ keys.T), visible) * t
+                    n_held = lengths[b]
+                    top = np.concatenate([np.broadcast_to(w[:, :n_held].max(-1, keepdims=True), (n, n_held)) if n_held else np.zeros((n, 0)),
+                                          np.broadcast_to(w.max(-1, keepdims=True), (n, n))], 1)
+                    tiny = np.where(t > 0, TINY[kind] * 2.0 ** -4 * top / np.where(t > 0, t, 1.0), 0.0)
             value[b, :, h], bound[b, :, h] = rows(q[b, :, h], keys, values, visible, scale, kind, weight_tiny=tiny)["out"]
     return value, bound

@@ -408,3 +408,83 @@ def test_a_request_from_prompt_to_accepted_drafts():
         assert close(out[b, 0], whole[b][n + 4])
     back = cache.read(int32(slots[2][:134]), torch.float16)
     assert torch.equal(back[0], text[2][1][:134]) and torch.equal(back[1], text[2][2][:134])
+
+
+# ---- sizes of values --------------------------------------------------------------------------------------
+def check_rows(k_rows, v_rows, drafts, group, held, low=None, small=1.0):
+    """One sequence of these rows ``[tokens, 1, dim]``, page after page; the bound does not grow with the ratio of the value rows' sizes.  Token
+    ``low`` has a score of -20 and less beside which the others' are a few: channel 0 of all queries is 8."""
+    import sparse
+    tokens, _, dim = k_rows.shape
+    dtype, page = k_rows.dtype, 64
+    cache = new_cache(-(-tokens // page), 1, dim, held, page)
+    g = torch.Generator().manual_seed(21)
+    q = torch.randn(1, drafts, group, dim, generator=g)
+    q[..., 0] = 8
+    k, v = torch.randn(1, drafts, 1, dim, generator=g), small * torch.randn(1, drafts, 1, dim, generator=g)
+    q, k, v = (t.to(dtype).cuda() for t in (q, k, v))
+    if low is not None:
+        k_rows[:, :, 0] = 0
+        k_rows[low] = 0
+        k_rows[low, :, 0] = -20
+    slots = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    cache.write(k_rows, v_rows, slots)
+    table = torch.arange(cache.pages, dtype=torch.int32, device="cuda")[None]
+    got = sparse.cached_attention(q, k, v, cache, table, torch.tensor([tokens], dtype=torch.int32, device="cuda"), scale=0.125)
+    rows = lambda which: values_of(getattr(cache, which)).transpose(1, 0, 2, 3).reshape(1, -1, dim)[:, :tokens]
+    scales = lambda which: values_of(getattr(cache, which)).transpose(1, 0, 2).reshape(1, -1)[:, :tokens]
+    mask = np.tril(np.ones((1, drafts, drafts), dtype=bool))
+    t = scales("value_scales")
+    value, bound = po.cached(*(values_of(x) for x in (q, k, v)), [rows("keys") * scales("key_scales")[..., None]], [rows("values") * t[..., None]],
+                             [t], [tokens], mask, 0.125, kind_of(dtype), by_weight=True)
+    bound = bound + (2.0 ** -134 if dtype == torch.bfloat16 else 0.0)       # half a step of its subnormal values
+    off = np.abs(values_of(got) - value)
+    assert torch.isfinite(got).all()
+    worst = (off - bound).argmax()
+    assert (off <= bound).all(), (off.max(), off.flat[worst], bound.flat[worst], np.unravel_index(worst, off.shape))
+
+
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("drafts,group", [(1, 2), (50, 3)])
+@pytest.mark.parametrize("low", [3, 1500])
+def test_a_large_value_row_of_no_weight_costs_the_others_no_bits(low, drafts, group, dim, held):
+    """One value row 2^15 times as large as the others, of a weight of 1e-9: in fp16 the others' weights relative to its size would
+    have a few bits left."""
+    g = torch.Generator().manual_seed(22)
+    k, v = (torch.randn(2000, 1, dim, generator=g).half() for _ in range(2))
+    v[low] *= 2.0 ** 13
+    v[torch.arange(2000) != low] *= 0.25
+    check_rows(k.cuda(), v.cuda(), drafts, group, held, low, 0.25)
+
+
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("drafts,group,tokens", [(50, 3, 40), (50, 3, 96), (1, 2, 40)])
+def test_small_cached_values_beside_new_tokens(drafts, group, tokens, held):
+    """New tokens' rows come as they are, cached ones with scales of 2^-17: in one step with them they would lose 17 bits."""
+    g = torch.Generator().manual_seed(23)
+    k, v = torch.randn(tokens, 1, 64, generator=g).half(), (2.0 ** -11 * torch.randn(tokens, 1, 64, generator=g)).half()
+    check_rows(k.cuda(), v.cuda(), drafts, group, held, small=2.0 ** -11)
+
+
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("drafts,group", [(1, 2), (50, 3)])
+@pytest.mark.parametrize("exponent", [-118, -60, 60, 110])
+@pytest.mark.parametrize("flat", [True, False])
+def test_values_of_any_size(flat, exponent, drafts, group, held):
+    """bf16 rows near the ends of the type's range: weights relative to their scales must neither overflow nor vanish."""
+    g = torch.Generator().manual_seed(24)
+    k, v = (torch.randn(1500, 1, 64, generator=g) for _ in range(2))
+    k, v = (k * (0 if flat else torch.linspace(0.1, 3, 1500)[:, None, None])).bfloat16(), (v * 2.0 ** exponent).bfloat16()
+    check_rows(k.cuda(), v.cuda(), drafts, group, held, small=2.0 ** exponent)
+
+
+@pytest.mark.parametrize("held", HELD)
+@pytest.mark.parametrize("drafts,group", [(1, 2), (50, 3)])
+@pytest.mark.parametrize("exponent", [-122, 100])
+def test_value_rows_of_sizes_far_apart(exponent, drafts, group, held):
+    """The first tiles are tiny or huge beside ordinary ones, which come later."""
+    g = torch.Generator().manual_seed(25)
+    k, v = (torch.randn(700, 1, 128, generator=g) for _ in range(2))
+    v[:128] *= 2.0 ** exponent
+    check_rows(k.bfloat16().cuda(), v.bfloat16().cuda(), drafts, group, held)
