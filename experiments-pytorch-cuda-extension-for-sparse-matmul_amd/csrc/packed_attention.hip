@@ -16,8 +16,6 @@
 // The lengths stay on the device: a launch has slots for the most tiles that T tokens in B sequences can make, and every workgroup
 // finds its sequence by a search over the offsets.  Slots that no sequence uses end at once.  Offsets are clamped to [0, T]
 // before anything is addressed with them.
-#include <type_traits>
-
 #include "attention_tiles.hpp"
 #include "bsa_device.hpp"
 #include "bsa_internal.hpp"
@@ -193,6 +191,13 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
 // (760, 870 and 670 TFLOP/s); 12 heads at head dim 64, six sequences of 1 to 1500 tokens 28, 37 and 36 us, one
 // generation of workgroups, as long as the 24 steps of the longest sequence.  Rows have the forward walk's bounds with three products to the exponentials' one.
 // ---------------------------------------------------------------------------
+// fp16 holds dS only times a power of two: with gradients of 1e-3 and a few thousand keys dS is 3e-6, a few steps of fp16's smallest, and
+// dq was 2.6 times as far off as its own rounding leaves it; above 65504 it was infinite where dq is not.  A row takes the
+// power from the largest dS of the first keys it sees, so that that is below 2^4, and a smaller one once a tile's squares sum up to more
+// than 2^30.  What it costs stands at the walks.
+constexpr float DS_LAZY_SQUARES = 0x1p30f;
+__device__ __forceinline__ float ds_lift(float most) { return fminf(4.f - (float)__builtin_amdgcn_frexp_expf(most), 40.f); }
+
 template <int HD, bool BF, int W>
 __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p)
 {
@@ -238,6 +243,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
 
     RowTile<HD> dq;
     clear<HD>(dq);
+    float lift = BF ? 0.f : __builtin_inff();    // dS of the row and dq are times 2^lift; not chosen yet
     for (int step = 0; step < steps; ++step) {
         const int k0 = 64 * step;
         const int buffer = step & 1;
@@ -279,22 +285,46 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
             }
             read_columns<HD>(tiles.rd, tiles.at(buffer, 0, u), ktr);
             issue_order();
-            auto gradients = [&](auto some_hidden) {     // a hidden score has no probability and no gradient, whatever it is
+            const float up = BF ? minus_lse : minus_lse + lift;
+            float squares = 0.f;
+            auto gradient = [&](int v, float minus, bool some_hidden) {  // a hidden score has no probability and no gradient, whatever it is
+                const float grad = at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus)) * (dpacc[v] - delta);
+                return some_hidden && 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? 0.f : grad;
+            };
+            auto gradients = [&](float minus, bool some_hidden) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) {
-                    float grad = at_exp2(__builtin_fmaf(sacc[v], p.scale2, minus_lse)) * (dpacc[v] - delta);
-                    if (some_hidden) grad = 32 * u + 8 * (v >> 2) + (v & 3) > seen - 4 * h ? 0.f : grad;
-                    ds[v >> 3][v & 7] = narrow_16<BF>(grad);
+                for (int v = 0; v < 16; v += 2) {
+                    const half_t a = narrow_16<BF>(gradient(v, minus, some_hidden)), b = narrow_16<BF>(gradient(v + 1, minus, some_hidden));
+                    ds[v >> 3][v & 7] = a;
+                    ds[v >> 3][(v & 7) + 1] = b;
+                    if (!BF) squares = __builtin_amdgcn_fdot2(h2{a, b}, h2{a, b}, squares, false);
                 }
             };
-            if (masked) gradients(std::true_type());
-            else gradients(std::false_type());
+            if (masked) gradients(up, true);
+            else gradients(up, false);
+            bool move = !BF && !(squares <= DS_LAZY_SQUARES);
+            if (__builtin_amdgcn_ballot_w64(move) != 0ull) {
+                const int other_moves = __builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)move);
+                move = move || other_moves != 0;
+                float most = 0.f;
+#pragma unroll
+                for (int v = 0; v < 16; ++v) most = fmaxf(most, __builtin_fabsf(gradient(v, minus_lse, masked)));
+                most = fmaxf(most, at_lane_xor32(most));
+                const float to = move ? fminf(lift, ds_lift(most)) : lift, keep = move ? at_exp2(to - lift) : 1.f;
+                lift = to;
+                each<HD>(dq, [&](float x, int) { return x * keep; });
+                // those of rows that stay are kept: made again, with another choice of fused instructions, they may differ by a bit
+                const h8 kept[2] = {ds[0], ds[1]};
+                gradients(minus_lse + lift, masked);
+#pragma unroll
+                for (int s = 0; s < 2; ++s) ds[s] = move ? ds[s] : kept[s];
+            }
             weigh<HD, BF>(ktr, ds, dq, masked);
             issue_order();
         }
     }
     __syncthreads();
-    store_token_rows<HD, BF>(dq, p.scale, lds_raw + 64 * HD * w, p.out + ((begin + row0) * p.heads + item.head) * HD,
+    store_token_rows<HD, BF>(dq, BF ? p.scale : p.scale * at_exp2(-lift), lds_raw + 64 * HD * w, p.out + ((begin + row0) * p.heads + item.head) * HD,
                              (long long)p.heads * HD, n - row0);
 }
 
