@@ -193,9 +193,9 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
 // ---------------------------------------------------------------------------
 // fp16 holds dS only times a power of two: with gradients of 1e-3 and a few thousand keys dS is 3e-6, a few steps of fp16's smallest, and
 // dq was 2.6 times as far off as its own rounding leaves it; above 65504 it was infinite where dq is not.  A row takes the
-// power from the largest dS of the first keys it sees, so that that is below 2^4, and a smaller one once a tile's squares sum up to more
-// than 2^30.  What it costs stands at the walks.
-constexpr float DS_LAZY_SQUARES = 0x1p30f;
+// power from the largest dS of the first keys it sees, so that that is below 2^4, and a smaller one once one would pass
+// 2^15.  The walk over the keys does the same for dk, where the error was 23 times that of dk's own rounding.
+constexpr float DS_MOST = 0x1p15f, DS_LAZY_SQUARES = DS_MOST * DS_MOST;
 __device__ __forceinline__ float ds_lift(float most) { return fminf(4.f - (float)__builtin_amdgcn_frexp_expf(most), 40.f); }
 
 template <int HD, bool BF, int W>
@@ -393,7 +393,8 @@ __global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOper
     };
     // fp16 probabilities of long sequences would be subnormal: they travel times 256
     constexpr float UP = BF ? 1.f : 256.f, DOWN = 1.f / UP, LOG_UP = BF ? 0.f : 8.f;
-    const float ds_scale = p.scale * DOWN;
+    // dS and dk of the key: times this, a power of two as in the row walk; not chosen yet
+    float ds_mul = BF ? 1.f : __builtin_inff();
 
     request(0);
     int q_tile = first;
@@ -447,6 +448,7 @@ __global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOper
             }
         }
         h8 pop[2], ds[2];
+        float most = 0.f;                        // largest dS of the lane
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
             const f4v dl = *reinterpret_cast<const f4v *>(stat_lds + TOKENS + 8 * g + 4 * h);
@@ -454,9 +456,26 @@ __global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOper
             for (int j = 0; j < 4; ++j) {
                 const int v = 4 * g + j;
                 pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
-                ds[v >> 3][v & 7] = narrow_16<BF>(prob[v] * ((dpacc[v] - dl[j]) * ds_scale));
+                dpacc[v] = prob[v] * (dpacc[v] - dl[j]);
+                if (!BF) most = fmaxf(most, __builtin_fabsf(dpacc[v]));
             }
         }
+        bool move = !BF && !(most * ds_mul <= DS_MOST);
+        if (__builtin_amdgcn_ballot_w64(move) != 0ull) {
+            const int other_moves = __builtin_amdgcn_ds_bpermute((l ^ 32) << 2, (int)move);
+            move = move || other_moves != 0;
+            most = fmaxf(most, at_lane_xor32(most));
+            const float to = move ? fminf(ds_mul, at_exp2(ds_lift(most))) : ds_mul, keep = move ? to * __builtin_amdgcn_rcpf(ds_mul) : 1.f;
+            ds_mul = to;
+            issue_order();                       // one accumulator after the other: all at once spill 14 registers, 12 of them K's
+#pragma unroll
+            for (int t = 0; t < HD / 32; ++t) {
+                dk[t] *= keep;
+                issue_order();
+            }
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v) ds[v >> 3][v & 7] = narrow_16<BF>(BF ? dpacc[v] : dpacc[v] * ds_mul);
 #pragma unroll
         for (int t = 0; t < HD / 32; ++t) {
             h8 qc[2], dc[2];
@@ -480,14 +499,15 @@ __global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOper
 #pragma unroll
     for (int set = 0; set < 2; ++set) {          // subtile `set` of each key tile sums and stores it
         RowTile<HD> &acc = set == 0 ? dv : dk;
+        const float out_scale = set == 0 ? DOWN : BF ? p.scale : p.scale * DOWN * __builtin_amdgcn_rcpf(ds_mul);     // of each wave's own key
         __syncthreads();                         // all are done with the tiles, or with the set before
-        each<HD>(acc, [&](float x, int i) { return park[i] = x; });
+        each<HD>(acc, [&](float x, int i) { return park[i] = x * out_scale; });
         __syncthreads();
         if (sub != set) continue;
         clear<HD>(acc);
 #pragma unroll 1
         for (int o = 0; o < SUB; ++o) each<HD>(acc, [&](float x, int i) { return x + parts[o * 32 * HD + i]; });
-        store_token_rows<HD, BF>(acc, set == 0 ? DOWN : 1.f, reinterpret_cast<unsigned char *>(park), (set == 0 ? p.dv : p.dk) + out, width,
+        store_token_rows<HD, BF>(acc, 1.f, reinterpret_cast<unsigned char *>(park), (set == 0 ? p.dv : p.dk) + out, width,
                                  n - key0);
     }
 }

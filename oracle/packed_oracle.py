@@ -21,8 +21,11 @@ def _softmax(s, visible):
     return np.where(total > 0, e / np.where(total > 0, total, 1.0), 0.0)
 
 
-def rows(q, k, v, visible, scale, kind, dout=None, weight_tiny=0.0):
-    """One head: ``q [n, d]``, ``k``, ``v [m, d]``, ``visible [n, m]``.  Returns ``{name: (value, bound)}``."""
+def rows(q, k, v, visible, scale, kind, dout=None, weight_tiny=0.0, lifted=False):
+    """One head: ``q [n, d]``, ``k``, ``v [m, d]``, ``visible [n, m]``.  Returns ``{name: (value, bound)}``.
+
+    ``lifted``: dS is rounded times a power of two that brings the largest of its query (for dq) or key (for dk) to 2^3 or more, so that
+    half the smallest step is 2^-3 ``TINY`` of that largest one; otherwise as it is."""
     unit, tiny = UNIT[kind], TINY[kind]
     d = q.shape[1]
     s = scale * (q @ k.T)
@@ -40,10 +43,12 @@ def rows(q, k, v, visible, scale, kind, dout=None, weight_tiny=0.0):
         ds = scale * p * (dp - delta)
         dp_off = (d + 4) * F32 * (np.abs(dout) @ np.abs(v).T)
         delta_off = (np.abs(dout) * (out_off + (d + 4) * F32 * np.abs(out))).sum(-1, keepdims=True)
-        ds_off = np.abs(ds) * (unit + 2 * e + 2 * m * F32 + 8 * F32) + abs(scale) * p * (dp_off + delta_off) + tiny * (p > 0) * max(1.0, abs(scale))
+        ds_off = np.abs(ds) * (unit + 2 * e + 2 * m * F32 + 8 * F32) + abs(scale) * p * (dp_off + delta_off)
+        largest = lambda axis: np.abs(ds).max(axis, keepdims=True) / 8 if lifted else max(1.0, abs(scale))
+        ds_off, ds_off_k = (ds_off + tiny * (p > 0) * largest(axis) for axis in (1, 0))
         dq, dk, dv = ds @ k, ds.T @ q, p.T @ dout
         found["dq"] = (dq, ds_off @ np.abs(k) + unit * np.abs(dq) + tiny)
-        found["dk"] = (dk, ds_off.T @ np.abs(q) + unit * np.abs(dk) + tiny)
+        found["dk"] = (dk, ds_off_k.T @ np.abs(q) + unit * np.abs(dk) + tiny)
         found["dv"] = (dv, off.T @ np.abs(dout) + unit * np.abs(dv) + tiny)
     return found
 
