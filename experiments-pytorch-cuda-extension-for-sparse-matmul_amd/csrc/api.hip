@@ -774,7 +774,7 @@ static int check_strides(const char *who, const int64_t *strides, int count)
 
 static int packed(const char *who, int dtype, const void *q, const void *k, const void *v, const int32_t *offsets, int tokens,
                   int sequences, int heads, int key_heads, int head_dim, const int64_t *strides, int operands, float scale,
-                  int causal, bsa::PackedArgs &p)
+                  int causal, bool key_gradients, bsa::PackedArgs &p)
 {
     int rc = check_16_bit(who, dtype);
     if (!rc) rc = check_heads(who, heads, key_heads, head_dim);
@@ -786,8 +786,6 @@ static int packed(const char *who, int dtype, const void *q, const void *k, cons
     for (int i = 0; i < operands; ++i)
         if (strides[2 * i] > (1LL << 24))
             return fail(BSA_ERR_UNSUPPORTED, "%s: %lld values between tokens are too many", who, (long long)strides[2 * i]);
-    if (heads * (tokens / 128 + sequences + 8LL) > (1LL << 24) - 64)     // workgroups of 256 threads: fewer than 2^32 threads
-        return fail(BSA_ERR_INVALID, "%s: %d tokens in %d sequences of %d heads are too many", who, tokens, sequences, heads);
     rc = check_alignment(who, {q, k, v});
     if (rc) return rc;
     p.q = q, p.k = k, p.v = v;
@@ -799,6 +797,8 @@ static int packed(const char *who, int dtype, const void *q, const void *k, cons
     p.scale = scale;
     p.causal = causal != 0;
     p.bf16 = dtype == BSA_BF16;
+    if (!bsa::packed_fits(p, key_gradients))
+        return fail(BSA_ERR_INVALID, "%s: %d tokens in %d sequences of %d heads are too many", who, tokens, sequences, heads);
     return BSA_OK;
 }
 
@@ -808,7 +808,7 @@ int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const 
 {
     const char *who = "bsa_packed_attention_forward";
     bsa::PackedArgs p;
-    int rc = packed(who, dtype, q, k, v, offsets, tokens, sequences, heads, key_heads, head_dim, strides, 3, scale, causal, p);
+    int rc = packed(who, dtype, q, k, v, offsets, tokens, sequences, heads, key_heads, head_dim, strides, 3, scale, causal, lse != nullptr, p);
     if (rc) return rc;
     if (!out) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
     rc = check_alignment(who, {out, rest});
@@ -827,7 +827,7 @@ int bsa_packed_attention_backward(int dtype, const void *q, const void *k, const
 {
     const char *who = "bsa_packed_attention_backward";
     bsa::PackedArgs p;
-    int rc = packed(who, dtype, q, k, v, offsets, tokens, sequences, heads, key_heads, head_dim, strides, 4, scale, causal, p);
+    int rc = packed(who, dtype, q, k, v, offsets, tokens, sequences, heads, key_heads, head_dim, strides, 4, scale, causal, dk_out != nullptr, p);
     if (rc) return rc;
     if (!dout || !out || !rest || !lse || !delta_ws || !dq_out || (dk_out == nullptr) != (dv_out == nullptr))
         return fail(BSA_ERR_INVALID, "%s: null pointer argument (dk_out and dv_out go together)", who);

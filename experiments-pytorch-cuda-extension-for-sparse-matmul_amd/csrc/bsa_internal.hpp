@@ -167,6 +167,9 @@ struct PackedArgs {
     float scale = 1.f;
     bool causal = true, bf16 = false;
 };
+// whether every launch has fewer than 2^32 threads; key_gradients: those of the backward call's walk over the keys too (a forward call whose
+// statistics are wanted asks for them, so that a training step is refused before it has begun)
+bool packed_fits(const PackedArgs &p, bool key_gradients);
 hipError_t launch_packed_forward(const PackedArgs &p, hipStream_t stream);
 hipError_t launch_packed_backward(const PackedArgs &p, hipStream_t stream);
 

@@ -514,6 +514,7 @@ __global__ __launch_bounds__(128 * SUB, 2) void packed_columns_kernel(PackedOper
 
 // ---- launchers ----------------------------------------------------------------------------------------
 constexpr int PACKED_WAVES = 4;
+constexpr int packed_subtiles(int hd) { return hd == 64 ? 2 : 4; }       // of queries in the walk over the keys
 
 PackedOperands operands(const PackedArgs &a)
 {
@@ -559,12 +560,21 @@ hipError_t backward(const PackedArgs &a, hipStream_t st)
     const PackedOperands p = operands(a);
     const hipError_t err = run_walk(packed_rows_kernel<HD, BF, W>, p, a.heads, 32 * W, W, PairTiles<HD, W, 2>::lds_bytes(), st);
     if (err != hipSuccess || a.dk == nullptr) return err;
-    constexpr int SUB = HD == 64 ? 2 : 4;
+    constexpr int SUB = packed_subtiles(HD);
     return run_walk(packed_columns_kernel<HD, BF, SUB>, p, a.key_heads, 64, 2 * SUB,
                     PairTiles<HD, 2 * SUB, SUB>::lds_bytes() + 16 * 32 * SUB + 2 * 64 * HD, st);
 }
 
 }  // namespace
+
+bool packed_fits(const PackedArgs &a, bool key_gradients)
+{
+    // packed_grid rounds the slots of a head up to at most 7 more; in 64 bits
+    auto fits = [&](int heads, int rows, int threads) {
+        return ((long long)heads * ((long long)a.tokens / rows + a.sequences + 7) + PACKED_CLEARING) * threads < (1ll << 32);
+    };
+    return fits(a.heads, 32 * PACKED_WAVES, 64 * PACKED_WAVES) && (!key_gradients || fits(a.key_heads, 64, 128 * packed_subtiles(a.head_dim)));
+}
 
 hipError_t launch_packed_forward(const PackedArgs &a, hipStream_t st)
 {

@@ -167,3 +167,21 @@ def test_operands_are_copied_only_where_a_row_cannot_be_read_in_place(kind):
     got = rows_of(t)
     assert torch.equal(got, t) and got.data_ptr() % 16 == 0 and all(s % 8 == 0 for s in strides_of(got))
     assert (got.data_ptr() == t.data_ptr()) == (kind not in ("odd start", "odd stride"))
+
+
+@pytest.mark.parametrize("dim,sequences", [(64, (1 << 24) // 16), (128, (1 << 23) // 16)])
+def test_a_training_step_whose_walk_over_the_keys_cannot_be_launched(k, dim, sequences):
+    """256 threads a workgroup at head dim 64, 512 at 128, and 2^32 in a launch: refused before the first launch of the backward call, and
+    by the forward call whose statistics are wanted."""
+    lse = P
+    given = (64, sequences, 16, 16, dim)
+    code = k.lib.bsa_packed_attention_backward(F16, P, P, P, P, P, P, lse, P, P, P, P, P, *given, strides(8), 1.0, 1, None)
+    refused(k, code, "bsa_packed_attention_backward", "too many")
+    code = k.lib.bsa_packed_attention_forward(F16, P, P, P, P, P, lse, P, *given, strides(6), 1.0, 1, None)
+    refused(k, code, "bsa_packed_attention_forward", "too many")
+
+
+def test_many_tokens_are_refused_by_the_slots_of_64_keys(k):
+    given = (600_000, 600_000, 16, 16, 128)
+    code = k.lib.bsa_packed_attention_backward(F16, P, P, P, P, P, P, P, P, P, P, P, P, *given, strides(8), 1.0, 1, None)
+    refused(k, code, "too many")
