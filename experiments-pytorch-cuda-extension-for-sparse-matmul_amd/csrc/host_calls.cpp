@@ -995,8 +995,9 @@ PyObject *cache_write(PyObject *, PyObject *const *args, Py_ssize_t nargs)  // c
     const Tensor &k = THPVariable_Unpack(args[1]), &v = THPVariable_Unpack(args[2]), &slots = THPVariable_Unpack(args[3]);
     for (const Tensor *t : {&k, &v})
         if (!plain_strided(*t) || !half_type(t->scalar_type()) || t->scalar_type() != k.scalar_type() || t->dim() != 3 || t->size(1) != c->heads ||
-            t->size(2) != c->head_dim || t->size(0) != k.size(0) || !readable_rows(*t))
+            t->size(2) != c->head_dim || t->size(0) != k.size(0) || !readable_rows(*t) || forward_mode(*t))
             Py_RETURN_NONE;
+    if (needs_grad({&k, &v})) Py_RETURN_NONE;           // refused there
     if (!on_current_device(c->keys) || !index_tensor(slots, 1) || slots.numel() != k.size(0) || k.size(0) > (1 << 30)) Py_RETURN_NONE;
     const int code = code_of(k.scalar_type());
     if (c->code != BSA_I8 && c->code != BSA_E4M3 && c->code != code) Py_RETURN_NONE;
@@ -1044,7 +1045,7 @@ PyObject *cached_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
     const Tensor tree = args[6] == Py_None ? Tensor() : THPVariable_Unpack(args[6]);
     const double scale = PyFloat_AsDouble(args[7]);
     if (scale == -1.0 && PyErr_Occurred()) return nullptr;
-    if (!heads_fit(q, k, v, 4) || !on_current_device(c->keys) || k.size(2) != c->heads || q.size(3) != c->head_dim) Py_RETURN_NONE;
+    if (!heads_fit(q, k, v, 4) || needs_grad({&q, &k, &v}) || !on_current_device(c->keys) || k.size(2) != c->heads || q.size(3) != c->head_dim) Py_RETURN_NONE;
     const int code = code_of(q.scalar_type());
     if (c->code != BSA_I8 && c->code != BSA_E4M3 && c->code != code) Py_RETURN_NONE;
     const int64_t batch = q.size(0), drafts = q.size(1);

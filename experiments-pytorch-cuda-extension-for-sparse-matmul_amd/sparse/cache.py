@@ -11,13 +11,19 @@ from typing import Optional, Tuple
 import torch
 
 from . import kernel as _k
-from .packed import HEAD_DIMS, MOST_ROWS, check_heads, check_index, rows_of, strides_of
+from .packed import HEAD_DIMS, MOST_ROWS, check_heads, check_index, forward_mode, rows_of, strides_of
 
 PAGES = (32, 64, 128, 256)
 MOST_DRAFTS = 1024
 _ROWS = {torch.float32: _k.BSA_F32, torch.float16: _k.BSA_F16, torch.bfloat16: _k.BSA_BF16}
 _QUANTISED = {torch.int8: _k.BSA_I8, torch.float8_e4m3fn: _k.BSA_E4M3}
 _HELD = {torch.float16: _k.BSA_F16, torch.bfloat16: _k.BSA_BF16, **_QUANTISED}
+
+
+def refuse_gradients(what: str, *operands: torch.Tensor) -> None:
+    """A result without history would cut a loss off from them without a word."""
+    if (torch.is_grad_enabled() and any(t.requires_grad for t in operands)) or any(forward_mode(t) for t in operands):
+        raise RuntimeError(f"{what} is not differentiable: call it under torch.no_grad() or detach its operands")
 
 
 class KeyValueCache:
@@ -76,7 +82,8 @@ class KeyValueCache:
         """Stores ``k``, ``v`` ``[tokens, heads, head_dim]`` at ``slots`` (int32 on the GPU, ``[tokens]``), quantised if the cache is:
         the scale is the row's largest magnitude over 127 or 448, values are rounded to the nearest, ties to even.  Rows
         with a negative slot (refused drafts, padding) or one behind the cache are left out; no two rows of a call may have the same
-        slot.  A row with an infinity or a NaN is kept as NaN.  Not differentiable."""
+        slot.  A row with an infinity or a NaN is kept as NaN.  Not differentiable: operands that
+        autograd follows are refused."""
         if _k.host_calls.cache_write(self._native, k, v, slots):
             return
         for t, name in ((k, "k"), (v, "v")):
@@ -88,6 +95,7 @@ class KeyValueCache:
                 raise ValueError(f"{name} must live on the cache's GPU")
         if self.dtype not in _QUANTISED and k.dtype != self.dtype:
             raise TypeError(f"a cache of {self.dtype} takes rows of that type, got {k.dtype}")
+        refuse_gradients("KeyValueCache.write", k, v)
         check_index(slots, "slots", self.device, 1)
         if slots.numel() != k.size(0) or k.size(0) > MOST_ROWS:
             raise ValueError(f"{k.size(0)} rows and {slots.numel()} slots")
@@ -123,13 +131,15 @@ def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: K
     kept go there by ``cache.write``).  ``pages [batch, width]`` lists the page numbers of every sequence, ``lengths [batch]`` says how
     many tokens it has in them, both int32 on the GPU.  ``tree``, bool ``[n, n]`` or ``[batch, n, n]``: whether new token ``i`` sees new
     token ``j`` (itself too, where it should); without it they are a chain, ``j <= i``.  ``n = 1`` is a decode step.  Every new token sees
-    the whole cached part of its sequence; one that sees nothing gets zeros.  At most 1024 new tokens a sequence.  Not differentiable."""
+    the whole cached part of its sequence; one that sees nothing gets zeros.  At most 1024 new tokens a sequence.  Not
+    differentiable: operands that autograd follows are refused."""
     if not isinstance(cache, KeyValueCache):
         raise TypeError(f"cache must be a KeyValueCache, got {type(cache).__name__}")
     out = _k.host_calls.cached_attention(q, k, v, cache._native, pages, lengths, tree, scale)
     if out is not None:
         return out
     check_heads(q, k, v, 4)
+    refuse_gradients("cached_attention", q, k, v)
     batch, drafts, heads, dim = q.shape
     if (cache.heads, cache.head_dim) != (k.size(2), dim) or cache.device != q.device:
         raise ValueError(f"k {tuple(k.shape)} on {k.device} does not fit a cache of {cache.heads} heads of {cache.head_dim} on {cache.device}")

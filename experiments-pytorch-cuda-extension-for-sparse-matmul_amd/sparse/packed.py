@@ -112,14 +112,14 @@ class PackedAttention(torch.autograd.Function):
         return grads + (None, None, None)
 
 
-def _forward_mode(t):
+def forward_mode(t):
     return torch.autograd.forward_ad.unpack_dual(t).tangent is not None
 
 
 def general(q, k, v, offsets, scale, causal):
     """The call without the native side, which hands over whatever it does not take."""
     tracked = torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (q, k, v))
-    if tracked or any(isinstance(t, torch.Tensor) and _forward_mode(t) for t in (q, k, v)):
+    if tracked or any(isinstance(t, torch.Tensor) and forward_mode(t) for t in (q, k, v)):
         return PackedAttention.apply(q, k, v, offsets, scale, causal)
     return _forward(q, k, v, offsets, scale, causal, False)[0]
 

@@ -221,3 +221,33 @@ def test_gradients_lose_no_more_than_the_rounding_of_ds(n, count, dim, dtype):
     for got, exact in ((dq, exact_q), (dk, exact_k)):
         rounded = exact.to(dtype).double()
         assert (apart(got) - exact).norm() <= 1.1 * math.sqrt(2) * (rounded - exact).norm()
+
+
+def test_calls_without_gradients_refuse_operands_that_autograd_follows():
+    """A result without history would cut a training loop off from them without a word."""
+    import torch.autograd.forward_ad as fwad
+    cache, rows, slots = new_cache(), normal(1, 4, 2, 64), int32([0, 1, 2, 3])
+    shapes = dict(q=(2, 3, 4, 64), k=(2, 3, 2, 64), v=(2, 3, 2, 64))
+    for name, shape in shapes.items():
+        leaf = normal(1, *shape).requires_grad_()
+        for operand in (leaf, leaf * 1, (leaf * 1).transpose(0, 1).contiguous().transpose(0, 1)):
+            with pytest.raises(RuntimeError, match="cached_attention is not differentiable"):
+                cached_call(cache, **{name: operand})
+        with torch.no_grad():
+            want = cached_call(cache, **{name: leaf})
+        assert torch.equal(cached_call(cache, **{name: leaf.detach()}), want) and not want.requires_grad
+        with fwad.dual_level():
+            with pytest.raises(RuntimeError, match="not differentiable"):
+                cached_call(cache, **{name: fwad.make_dual(leaf.detach(), leaf.detach().clone())})
+    before = cache.read(slots, torch.float32)
+    leaf = (2 * rows).requires_grad_()
+    for k, v in ((leaf, rows), (rows, leaf), (leaf * 1, rows)):
+        with pytest.raises(RuntimeError, match="write is not differentiable"):
+            cache.write(k, v, slots)
+    with fwad.dual_level():
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            cache.write(fwad.make_dual(rows, 2 * rows), rows, slots)
+    assert all(torch.equal(a, b) for a, b in zip(before, cache.read(slots, torch.float32)))
+    with torch.no_grad():
+        cache.write(leaf, rows, slots)
+    assert not torch.equal(before[0], cache.read(slots, torch.float32)[0])
