@@ -309,3 +309,12 @@ def test_the_same_bits_every_time():
         runs.append((out,) + torch.autograd.grad(out, (q, k, v), dout))
     for other in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+
+
+def test_a_sequence_that_ends_before_it_begins_alone_gives_zeros():
+    import sparse
+    q, k, v, dout = operands(17, 60, 2, 1, 64, torch.float16)
+    for values in ([60, 0], [2 ** 31 - 1, -2 ** 31], [40, 40], [60, 60, 0]):
+        out = sparse.packed_attention(q, k, v, torch.tensor(values, dtype=torch.int32, device="cuda"), 0.1)
+        for t in (out,) + torch.autograd.grad(out, (q, k, v), dout):
+            assert not t.any(), values
