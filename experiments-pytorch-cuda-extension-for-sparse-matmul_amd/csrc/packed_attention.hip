@@ -319,7 +319,8 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
 #pragma unroll
                 for (int s = 0; s < 2; ++s) ds[s] = move ? ds[s] : kept[s];
             }
-            weigh<HD, BF>(ktr, ds, dq, masked);
+            if (weigh<HD, BF>(ktr, ds, dq, masked))
+                add_not_finite<HD, BF>(tiles.rd, tiles.at(buffer, 0, u), dq, [&](int at) { return 32 * u + at <= seen; });
             issue_order();
         }
     }

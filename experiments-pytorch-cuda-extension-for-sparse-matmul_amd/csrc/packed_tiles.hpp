@@ -171,9 +171,8 @@ __device__ __forceinline__ void product(const h8 (&a)[N], const h8 (&b)[N], f16v
 }
 // Products with some weights zero because their place is hidden: an infinity or a NaN in a token must not reach the results of
 // those that do not see it, and zero times it would be NaN.  Where anything is hidden the operands are looked at and such values left
-// out of the products.  In the forward pass add_not_finite then adds them to the results of the lanes for which
-// sees(row of the tile) holds.  In the backward pass nothing has to be added: such a token's statistics are no numbers either, and
-// with them the weights of all that see it.
+// out of the products.  add_not_finite then adds them to the results of the lanes for which sees(row of the tile) holds.  In the walk over
+// the keys nothing has to be added: such a query's statistics are no numbers either, and with them the weights of all that it sees.
 template <bool BF, int T>
 __device__ __forceinline__ bool take_out_not_finite(h8 (&columns)[T][2])
 {
@@ -229,17 +228,18 @@ __device__ __forceinline__ void add_not_finite(const TileReader &rd, unsigned ti
     }
 }
 
-// acc[t] += columns 32 t .. of a 32-row tile, its rows weighted by op; the columns have been read
+// acc[t] += columns 32 t .. of a 32-row tile, its rows weighted by op; the columns have been read; whether values were left out
 template <int HD, bool BF>
-__device__ __forceinline__ void weigh(h8 (&columns)[HD / 32][2], const h8 (&op)[2], RowTile<HD> &acc, bool hidden)
+__device__ __forceinline__ bool weigh(h8 (&columns)[HD / 32][2], const h8 (&op)[2], RowTile<HD> &acc, bool hidden)
 {
-    if (hidden) take_out_not_finite<BF>(columns);
+    const bool out = hidden && take_out_not_finite<BF>(columns);
 #pragma unroll
     for (int s = 0; s < 2; ++s)
 #pragma unroll
         for (int t = 0; t < HD / 32; ++t) acc[t] = mfma_16<BF>(columns[t][s], op[s], acc[t]);
+    return out;
 }
-// the same, 64 columns read at a time; whether values were left out
+// the same, 64 columns read at a time
 template <int HD, bool BF>
 __device__ __forceinline__ bool weigh_tile(const TileReader &rd, unsigned tile, const h8 (&op)[2], RowTile<HD> &acc, bool hidden = false)
 {

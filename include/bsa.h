@@ -417,7 +417,7 @@ int bsa_weight_grad(int dtype, const void *a, const void *b, void *out, const in
  *   strides          host int64: values between tokens and between heads of q, k, v (and dout); multiples of 8, the head
  *                    dim itself is contiguous; at most 2^24 between tokens
  * Results are the same bits in every call: each is summed in one order, by one workgroup.  An infinity or a NaN in a token
- * reaches the results of the tokens that see it, not of others.
+ * reaches the results of the tokens that see it and the gradients of every token that one of these sees, not of others.
  * fp16 and bf16, head_dim 64 or 128; operands start at multiples of 16 bytes.  dk_out and dv_out both NULL: dq alone.
  */
 int bsa_packed_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, void *rest, float *lse,

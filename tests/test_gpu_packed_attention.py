@@ -318,3 +318,47 @@ def test_a_sequence_that_ends_before_it_begins_alone_gives_zeros():
         out = sparse.packed_attention(q, k, v, torch.tensor(values, dtype=torch.int32, device="cuda"), 0.1)
         for t in (out,) + torch.autograd.grad(out, (q, k, v), dout):
             assert not t.any(), values
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("at", [3, 70, 390])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf")])
+def test_an_infinite_key(bad, at, dim, dtype):
+    """A query whose score of it is +inf has no softmax: NaN in its result, its dq and every gradient that it has a part in.  One whose score
+    is -inf gives the key no weight: results and gradients as without it, but for dq's channel of the infinity, where 0 meets it.
+    The rest against float64, as a multiple of what rounding the exact results leaves."""
+    import math
+
+    import sparse
+    n, scale = 400, dim ** -0.5
+    q, k, v, dout = operands(18, n, 1, 1, dim, dtype)
+    with torch.no_grad():
+        q[:, 0, 5] = q[:, 0, 5].abs() + 0.25
+        q[300:, 0, 5] *= -1
+        if at == 3:
+            q[:60, 0, 5] *= -1
+        k[at, 0, 5] = bad
+    out = sparse.packed_attention(q, k, v, offsets_of([n]), scale)
+    got = (out,) + torch.autograd.grad(out, (q, k, v), dout)
+    qd, kd, vd, dd = (t[:, 0].detach().double() for t in (q, k, v, dout))
+    seen = torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+    none = (seen[:, at] & (qd[:, 5] * bad > 0))               # queries without a softmax
+    kd[at, 5] = 0
+    s = (scale * qd @ kd.t()).masked_fill(~seen, -math.inf)
+    s[:, at] = -math.inf                                      # of the others that see it
+    p = s.softmax(-1)
+    p[none] = 0
+    ds = scale * p * (dd @ vd.t() - (dd * (p @ vd)).sum(-1, keepdim=True))
+    below = torch.arange(n, device="cuda") <= (none.nonzero().max() if none.any() else -1)       # keys that a query of `none` sees
+    for name, x, exact, lost in zip(("out", "dq", "dk", "dv"), got, (p @ vd, ds @ kd, ds.t() @ qd, p.t() @ dd), (none, none, below, below)):
+        x = x[:, 0].detach()
+        assert torch.isnan(x[lost]).all(), name
+        keep = ~lost[:, None].expand_as(x)
+        if name == "dq":
+            keep = keep.clone()
+            assert not torch.isfinite(x[seen[:, at], 5]).any(), name
+            keep[seen[:, at], 5] = False
+        assert torch.isfinite(x[keep]).all(), name
+        off, rounded = (x.double() - exact)[keep].norm(), (exact.to(dtype).double() - exact)[keep].norm()
+        assert off <= 1.1 * math.sqrt(2) * rounded + (0 if keep.any() else 1), (name, off, rounded)
