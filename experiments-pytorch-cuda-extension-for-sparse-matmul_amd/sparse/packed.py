@@ -78,13 +78,28 @@ def _forward(q, k, v, offsets, scale, causal, for_backward):
     return out, rest, lse
 
 
+def _check_saved(q, k, v, dout, out, rest, lse, offsets):
+    """What autograd kept may come back as hooks on saved tensors made it."""
+    check_heads(q, k, v, 3)
+    for t, name, shape, dtype in ((dout, "gradient", q.shape, q.dtype), (out, "saved result", q.shape, q.dtype), (rest, "saved rest", q.shape, q.dtype),
+                                  (lse, "saved statistics", (q.size(1), q.size(0)), torch.float32)):
+        if t.shape != torch.Size(shape) or t.dtype != dtype or t.device != q.device:
+            raise ValueError(f"the {name} of {q.dtype} {tuple(q.shape)} on {q.device} came back as {t.dtype} {tuple(t.shape)} on {t.device}")
+    check_index(offsets, "offsets", q.device, 1)
+    if offsets.numel() < 1:
+        raise ValueError("offsets needs one entry more than there are sequences")
+
+
 def run_backward(q, k, v, dout, out, rest, lse, offsets, scale, causal, with_dkdv):
+    _check_saved(q, k, v, dout, out, rest, lse, offsets)
     tokens, heads, dim = q.shape
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2)) if with_dkdv else (None, None)
     if tokens == 0 or offsets.numel() == 1:
         return tuple(t if t is None else t.zero_() for t in (dq, dk, dv))
     q, k, v, dout = rows_of(q), rows_of(k), rows_of(v), rows_of(dout)
+    out, rest = (rows_of(t, copy=not t.is_contiguous()) for t in (out, rest))
+    lse = lse.contiguous()
     delta = torch.empty_like(lse)
     with _k.on_device(q.device):
         _k.check(_k.lib.bsa_packed_attention_backward(

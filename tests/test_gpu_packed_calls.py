@@ -251,3 +251,25 @@ def test_calls_without_gradients_refuse_operands_that_autograd_follows():
     with torch.no_grad():
         cache.write(leaf, rows, slots)
     assert not torch.equal(before[0], cache.read(slots, torch.float32)[0])
+
+
+def test_saved_tensors_that_hooks_give_back():
+    """As they were after a stay on the host, in another layout: the same gradients; as something else: refused before any launch."""
+    leaves = [normal(i, 9, h, 64).requires_grad_() for i, h in ((1, 4), (2, 2), (3, 2))]
+    dout = normal(4, 9, 4, 64)
+
+    def grads(pack, unpack, scale):
+        with torch.autograd.graph.saved_tensors_hooks(pack, unpack):
+            out = packed_call(q=leaves[0], k=leaves[1], v=leaves[2], scale=scale)
+        return torch.autograd.grad(out, leaves, dout)
+
+    spread = lambda t: torch.stack([t, t], -1)[..., 0] if t.dtype != torch.int32 else t        # every other value
+    for scale in (0.125, np.float64(0.125)):
+        want = grads(lambda t: t, lambda t: t, scale)
+        for pack, unpack in ((lambda t: t.cpu(), lambda t: t.cuda()), (lambda t: t, spread)):
+            assert all(torch.equal(a, b) for a, b in zip(grads(pack, unpack, scale), want))
+        for at in range(7):                                    # one of the saved tensors
+            for change in (lambda t: t.cpu(), lambda t: t[:-1] if t.dtype != torch.int32 else t[None], lambda t: t.to(torch.float64)):
+                count = iter(range(7))
+                with pytest.raises((ValueError, TypeError)):
+                    grads(lambda t: (next(count), t), lambda x: change(x[1]) if x[0] == at else x[1], scale)

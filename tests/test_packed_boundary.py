@@ -185,3 +185,13 @@ def test_many_tokens_are_refused_by_the_slots_of_64_keys(k):
     given = (600_000, 600_000, 16, 16, 128)
     code = k.lib.bsa_packed_attention_backward(F16, P, P, P, P, P, P, P, P, P, P, P, P, *given, strides(8), 1.0, 1, None)
     refused(k, code, "too many")
+
+
+def test_the_backward_pass_looks_at_what_autograd_hands_it():
+    """Hooks on saved tensors may give back anything: nothing off the GPU, of another type or shape gets to a kernel."""
+    from sparse.packed import run_backward
+    rows, keys, lse, offsets = torch.zeros(4, 2, 64).half(), torch.zeros(4, 1, 64).half(), torch.zeros(2, 4), torch.tensor([0, 4], dtype=torch.int32)
+    with pytest.raises(ValueError, match="same GPU"):
+        run_backward(rows, keys, keys, rows, rows, rows, lse, offsets, 1.0, True, True)
+    with pytest.raises(TypeError, match="float16 or all bfloat16"):
+        run_backward(rows.float(), keys, keys, rows, rows, rows, lse, offsets, 1.0, True, True)
