@@ -103,3 +103,42 @@ def test_cached_is_attention_over_everything():
             assert np.allclose(got[b, :, 2 * h:2 * h + 2], want, atol=1e-13)
     none = np.zeros((2, 3, 3), dtype=bool)
     assert not po.cached(q, k, v, keys, values, None, lengths, none, 0.25, "float16")[0][1].any()
+
+
+def fp16(x):
+    return np.asarray(x).astype(np.float16).astype(np.float64)
+
+
+def test_bounds_of_lifted_ds_hold_for_it_and_not_for_ds_as_it_is():
+    """Gradients of 1e-4: dS of a key is rounded times a power of two that brings its largest below 2^4, against dS as it is."""
+    n, d, scale = 400, 64, 0.125
+    rng = np.random.RandomState(6)
+    q, k, v, dout = (fp16(size * rng.randn(n, d)) for size in (1, 1, 1, 1e-4))
+    visible = np.tril(np.ones((n, n), dtype=bool))
+    want, bound = po.rows(q, k, v, visible, scale, "float16", dout, lifted=True)["dk"]
+    p = scipy_softmax(np.where(visible, scale * q @ k.T, -np.inf), axis=-1)
+    ds = p * (dout @ v.T - (dout * (p @ v)).sum(-1, keepdims=True))
+    lift = 2.0 ** (4 - np.frexp(np.abs(ds).max(0))[1])
+    assert (np.abs(fp16(scale / lift[:, None] * (fp16(ds * lift).T @ q)) - want) <= bound).all()
+    assert (np.abs(fp16(scale * (fp16(ds).T @ q)) - want) > bound).any()          # worst cases are summed: few elements pass them
+
+
+def test_bounds_by_weight_hold_for_the_largest_weight_and_not_for_the_largest_scale():
+    """One value row 2^15 times as large as the others and of no weight: the others' weights, rounded relative to the largest p t, and to
+    the largest t."""
+    n, d = 600, 16
+    rng = np.random.RandomState(7)
+    q, k, v = rng.randn(1, 1, 1, d), rng.randn(1, 1, 1, d), rng.randn(1, 1, 1, d)
+    keys, y, t = rng.randn(1, n, d), rng.randint(-127, 128, (1, n, d)).astype(float), np.full((1, n), 2.0 ** -9)
+    keys[0, 0], t[0, 0] = -30 * q[0, 0, 0] / np.linalg.norm(q), 2.0 ** 6
+    want, bound = po.cached(q, k, v, [keys], [y * t[..., None]], [t], [n], np.ones((1, 1, 1), dtype=bool), 1.0, "float16", by_weight=True)
+    s = np.append(keys[0], k[0, :, 0], 0) @ q[0, 0, 0]
+    e, scales, rows = np.exp(s - s.max()), np.append(t[0], 1.0), np.append(y[0], v[0, :, 0], 0)
+
+    def result(top):                                            # of the cached rows' weights; the new row's are relative to their own
+        held = fp16(e[:n] * scales[:n] / top) * top
+        new = fp16(e[n:])
+        return fp16((held @ rows[:n] + new @ rows[n:]) / e.sum())
+
+    assert (np.abs(result((e[:n] * scales[:n]).max() / 16) - want[0, 0, 0]) <= bound[0, 0, 0]).all()
+    assert (np.abs(result(2 * t.max()) - want[0, 0, 0]) > bound[0, 0, 0]).any()
