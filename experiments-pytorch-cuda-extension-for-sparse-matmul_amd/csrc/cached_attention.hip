@@ -11,9 +11,10 @@
 // tiles of its own through registers and its own LDS, with no barrier before the end.  RG = 4: 128 rows, whose waves share the
 // tile, double buffered.
 // What bounds it: with few rows the cache's bytes and the way of a chunk's first ones through page table, memory and LDS (one sequence of
-// 131071 int8 tokens, 2 key heads: 24 us, 2.9 TB/s; 16 of 0 to 8192 e4m3 tokens, 4 key heads: 11.5); with many the widening of a tile, its exponentials and the
-// barrier of a step (244 rows a sequence over 48 long ones: 235 us with the join, 283 TFLOP/s; the vector pipe is busy in 35 % of
-// the clocks, the matrix pipe in 11 %, and waves wait in 46 %).
+// 131071 int8 tokens, 2 key heads: 23 us, 3.0 TB/s; 16 of 0 to 8192 e4m3 tokens, 4 key heads: 12); with many the widening of a tile, its exponentials and the
+// barrier of a step (244 rows a sequence over 48 long ones: 235 us with the join, 281 TFLOP/s; the vector pipe is busy in 35 % of
+// the clocks, the matrix pipe in 11 %, and waves wait in 46 %).  At head dim 128 RG = 1 needs 5 or 6 registers more than there
+// are: they are spilled.
 // The work is cut where it lies: a unit is a chunk of the tiles of one sequence and key head, the chunk chosen on the device
 // from the lengths so that the units fill the machine, long sequences in many, short ones in one.  A sequence in several units
 // leaves (max, sum, O) of each in a workspace, which a second launch joins in the order of the chunks.
@@ -555,7 +556,10 @@ __global__ __launch_bounds__(JOIN_THREADS) void cached_join_kernel(CachedOperand
 // sequence a key head).  RG = 4 is better balanced with more (48 uneven sequences: 512 292 us, 768 258, 1536 250), but
 // 1536 took 171 us where 768 take 157 (64 sequences of 500 to 4000 tokens, 120 rows).
 constexpr int cached_units(int rg) { return rg == 1 ? 512 : 768; }
-constexpr int CACHED_LEAST = 8;                  // tiles of a chunk: two for each wave of RG = 1
+// Tiles of a chunk, 4 / 8 / 16 (us a pass).  RG = 1, two of 8 for each wave: 16 sequences of 0 to 8192 tokens, one row a head,
+// 15.1 / 15.4 / 19.2, one of 131071 30.7 in each.  RG = 4, 8 steps or 4 of two: 108 rows of 4 sequences 32.1 / 28.5 / 36.3, 244 rows of 48
+// long ones 235 in each.
+constexpr int CACHED_LEAST = 8;
 
 CachedOperands operands(const CachedArgs &a)
 {

@@ -8,7 +8,7 @@
 //   O^T += V^T P^T          the probabilities go from accumulators to operands without leaving the registers
 // What bounds it: a tile has 32 exponentials a lane (8 clocks each, as much again for scaling, rounding and sums) beside 16 products of 32
 // clocks at head dim 64 and 32 at 128, so the scores of the next tile are made beside the exponentials of this one, and two waves a
-// SIMD fill what is left.  Causal, 16384 tokens, 16 heads at head dim 64: 614 to 632 us, 870 to 895 TFLOP/s; sequences of 4096 to 97 tokens at head
+// SIMD fill what is left.  Causal, 16384 tokens, 16 heads at head dim 64: 611 to 632 us, 870 to 900 TFLOP/s; sequences of 4096 to 97 tokens at head
 // dim 128: 108 to 112 us, 860 to 890 TFLOP/s (a library product of 8192^3 1217 on the same card).  W = 4: eight waves, which read K and V
 // half as often, took 124 us for those 112 and 660 for 620: twice as many waves wait at a barrier, and half as many workgroups share
 // the uneven rows.
@@ -187,14 +187,15 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
 //             second operand would leave 1.05 but take 8 % (bf16, head dim 64)
 //   columns   a workgroup holds 64 keys of one key head and walks the queries of all heads that share it:
 //             dv^T += dO^T P,  dk^T += Q^T dS
-// Sequences of 4096, 2976 and 1119 tokens, 16 heads over 4, head dim 128 (55 GFLOP a product): forward 145 us, rows 190, columns 328
-// (760, 870 and 670 TFLOP/s); 12 heads at head dim 64, six sequences of 1 to 1500 tokens 28, 37 and 36 us, one
+// Sequences of 4096, 2976 and 1119 tokens, 16 heads over 4, head dim 128 (55 GFLOP a product): forward 135 to 140 us, rows 197 to 205, columns 311
+// to 319 (800, 820 and 700 TFLOP/s); 12 heads at head dim 64, six sequences of 1 to 1500 tokens 27, 39 and 36 us, one
 // generation of workgroups, as long as the 24 steps of the longest sequence.  Rows have the forward walk's bounds with three products to the exponentials' one.
 // ---------------------------------------------------------------------------
 // fp16 holds dS only times a power of two: with gradients of 1e-3 and a few thousand keys dS is 3e-6, a few steps of fp16's smallest, and
 // dq was 2.6 times as far off as its own rounding leaves it; above 65504 it was infinite where dq is not.  A row takes the
 // power from the largest dS of the first keys it sees, so that that is below 2^4, and a smaller one once one would pass
 // 2^15.  The walk over the keys does the same for dk, where the error was 23 times that of dk's own rounding.
+// A training step of the first case above 653 us, without both 639.
 constexpr float DS_MOST = 0x1p15f, DS_LAZY_SQUARES = DS_MOST * DS_MOST;
 __device__ __forceinline__ float ds_lift(float most) { return fminf(4.f - (float)__builtin_amdgcn_frexp_expf(most), 40.f); }
 
@@ -333,7 +334,7 @@ __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p
 // parts add up in LDS at the end.  128 queries a tile at head dim 128, 64 at 64.  K stays in registers, V in LDS: with the
 // accumulators they would leave too few for two waves a SIMD at head dim 128 (256 registers each, none spilled: what is spilled
 // is waited for behind the tiles on their way).  One wave a SIMD with 512 registers and both key tiles, which reads Q and dO half
-// as often, took 430 us where this takes 338 (sequences of 4096, 2976 and 1119 tokens, 16 heads over 4, 650 TFLOP/s of the four
+// as often, took 430 us where this took 338, now 311 to 319 (sequences of 4096, 2976 and 1119 tokens, 16 heads over 4, 700 TFLOP/s of the four
 // products): nothing runs beside what a wave waits for.  What bounds it: a step of the workgroup takes 6.3k clocks, of which the
 // products fill 2.0k, LDS 2.6k (Q and dO are read both ways) and the exponentials 1.0k, and the two waves of a SIMD, which the barrier
 // keeps in step, overlap little of it; and the first keys of the longest sequence have 128 steps where a compute unit has 106 on
