@@ -197,7 +197,10 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
 // 2^15.  The walk over the keys does the same for dk, where the error was 23 times that of dk's own rounding.
 // A training step of the first case above 653 us, without both 639.
 constexpr float DS_MOST = 0x1p15f, DS_LAZY_SQUARES = DS_MOST * DS_MOST;
-__device__ __forceinline__ float ds_lift(float most) { return fminf(4.f - (float)__builtin_amdgcn_frexp_expf(most), 40.f); }
+__device__ __forceinline__ float ds_lift(float most)              // where all are hidden or zero: the largest, there is room downwards only
+{
+    return most == 0.f ? 40.f : fminf(4.f - (float)__builtin_amdgcn_frexp_expf(most), 40.f);
+}
 
 template <int HD, bool BF, int W>
 __global__ __launch_bounds__(64 * W, 2) void packed_rows_kernel(PackedOperands p)

@@ -101,3 +101,16 @@ def test_a_key_with_gradients_unlike_its_neighbours(dim):
                           lifted=True)["dk"]
     off = np.abs(dk.cpu().numpy() - want)
     assert (off <= bound).all()                 # every rounding at its worst: a key near the end has few queries, which may round alike
+
+
+@pytest.mark.parametrize("n,count,heads,key_heads", SIZES[1:])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_dk_of_tiny_ds_and_large_queries(dim, n, count, heads, key_heads):
+    """dS of 1e-9 makes a dk of 1e-4.  Every other tile of keys begins with queries that do not see it: they say nothing of its dS."""
+    check(1, n, count, heads, key_heads, dim, torch.float16, 1e-6, queries=2.0 ** 13, keys=2.0 ** -13)
+
+
+@pytest.mark.parametrize("n,count,heads,key_heads", SIZES[1:])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_dq_of_tiny_ds_and_large_keys(dim, n, count, heads, key_heads):
+    check(0, n, count, heads, key_heads, dim, torch.float16, 1e-6, queries=2.0 ** -13, keys=2.0 ** 13)
