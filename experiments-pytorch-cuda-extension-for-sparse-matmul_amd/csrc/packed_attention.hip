@@ -191,11 +191,11 @@ __global__ __launch_bounds__(64 * W, 2) void packed_forward_kernel(PackedOperand
 // to 319 (800, 820 and 700 TFLOP/s); 12 heads at head dim 64, six sequences of 1 to 1500 tokens 27, 39 and 36 us, one
 // generation of workgroups, as long as the 24 steps of the longest sequence.  Rows have the forward walk's bounds with three products to the exponentials' one.
 // ---------------------------------------------------------------------------
-// fp16 holds dS only times a power of two: with gradients of 1e-3 and a few thousand keys dS is 3e-6, a few steps of fp16's smallest, and
-// dq was 2.6 times as far off as its own rounding leaves it; above 65504 it was infinite where dq is not.  A row takes the
+// fp16 holds dS only times a power of two: with gradients of 1e-3 and 4096 keys dS is 3e-6, a few steps of fp16's smallest, and
+// dq was 5.1 times as far off as its own rounding leaves it, now 1.2; above 65504 it was infinite where dq is not.  A row takes the
 // power from the largest dS of the first keys it sees, so that that is below 2^4, and a smaller one once one would pass
-// 2^15.  The walk over the keys does the same for dk, where the error was 23 times that of dk's own rounding.
-// A training step of the first case above 653 us, without both 639.
+// 2^15.  The walk over the keys does the same for dk, where the error was 47 times that of dk's own rounding,
+// now 1.3.  A training step of the first case above 648 us, without both 638.
 constexpr float DS_MOST = 0x1p15f, DS_LAZY_SQUARES = DS_MOST * DS_MOST;
 __device__ __forceinline__ float ds_lift(float most)              // where all are hidden or zero: the largest, there is room downwards only
 {
