@@ -41,7 +41,7 @@ constexpr int cached_subtiles(int hd, int rg) { return rg == 1 || hd == 128 ? 1 
 constexpr int cached_set_bytes(int hd, int rg) { return cached_subtiles(hd, rg) * (128 * hd + 256) + 256; }
 // The reference point of a row moves once a step's exponentials sum up to more.  Over an 8-bit cache a weight is at most 2^15 then, and
 // the largest was 2^lift when the point was set: fp16 keeps all bits of those down to 2^-18 of it.  48 trees over int8 caches, fp16:
-// lift 6 248 us, 4 234, 0 226, a point that moved at 256 over a lift of 6 305.
+// lift 6 248 us, 4 234, 0 226; lift 6 and a point that moves once the sum passes 256: 305.
 constexpr float CACHED_LAZY_SUM = 256.f, CACHED_LAZY_WEIGHTS = 32768.f;
 constexpr float cached_lift(bool bf) { return bf ? 0.f : 4.f; }
 // Scales count in the reference point from 2^-32 on, so that exponentials without them, whose sum the row is divided by, stay
@@ -299,7 +299,7 @@ __global__ __launch_bounds__(64 * CACHED_WAVES, 2) void cached_attention_kernel(
 #pragma unroll
         for (int s = 0; s < SUBT; ++s) partial = partial || step.t0 + s >= held || step.there[s] < 32;
         if (SCALED) {
-            float most = scales[64 * SUBT];      // value scale of the step
+            float most = scales[64 * SUBT];      // the largest value scale of the step
             if (SUBT > 1) most = fmaxf(most, scales[64 * SUBT + 1]);
             most_sum = CACHED_LAZY_WEIGHTS * __builtin_amdgcn_rcpf(__builtin_amdgcn_fmed3f(most, at_exp2(LEAST_SCALE), at_exp2(MOST_SCALE)));
         }
