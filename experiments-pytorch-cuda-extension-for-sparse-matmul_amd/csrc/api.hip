@@ -966,4 +966,214 @@ int bsa_cached_attention(int dtype, int cache_dtype, const void *q, const void *
     return check_launch(bsa::launch_cached_attention(p, (hipStream_t)stream), who);
 }
 
+// ---- linear attention ------------------------------------------------------------------------------------
+static int linear(const char *who, int dtype, const void *q, const void *k, const void *v, const float *log_decay, const int32_t *offsets,
+                  int segment, int tokens, int sequences, int heads, int key_heads, int head_dim, const int64_t *strides, int operands,
+                  float scale, bsa::LinearArgs &p)
+{
+    int rc = check_16_bit(who, dtype);
+    if (!rc) rc = check_heads(who, heads, key_heads, head_dim);
+    if (!rc) rc = check_strides(who, strides, 2 * operands);
+    if (rc) return rc;
+    if (tokens < 1 || sequences < 1 || tokens > (1 << 30) || sequences > 65535)
+        return fail(BSA_ERR_INVALID, "%s: %d tokens in %d sequences", who, tokens, sequences);
+    if (segment < 32 || segment > (1 << 20) || (segment & (segment - 1)) != 0)
+        return fail(BSA_ERR_INVALID, "%s: segments of %d tokens (a power of two from 32 on)", who, segment);
+    if (!q || !k || !v || !log_decay || !offsets) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    for (int i = 0; i < operands; ++i)
+        if (strides[2 * i] > (1LL << 24))
+            return fail(BSA_ERR_UNSUPPORTED, "%s: %lld values between tokens are too many", who, (long long)strides[2 * i]);
+    rc = check_alignment(who, {q, k, v});
+    if (rc) return rc;
+    p.q = q, p.k = k, p.v = v;
+    p.log_decay = log_decay, p.offsets = offsets;
+    p.segment = segment, p.tokens = tokens, p.sequences = sequences, p.heads = heads, p.key_heads = key_heads, p.head_dim = head_dim;
+    p.q_token = strides[0], p.q_head = strides[1], p.k_token = strides[2], p.k_head = strides[3];
+    p.v_token = strides[4], p.v_head = strides[5];
+    if (operands > 3) p.g_token = strides[6], p.g_head = strides[7];
+    p.scale = scale;
+    p.bf16 = dtype == BSA_BF16;
+    if (!bsa::linear_fits(p))
+        return fail(BSA_ERR_INVALID, "%s: %d tokens in %d sequences of %d heads are too many", who, tokens, sequences, heads);
+    return BSA_OK;
+}
+static int check_linear_states(const char *who, const bsa::LinearArgs &p, const void *states, size_t bytes)
+{
+    const size_t need = bsa::linear_workspace_bytes(p);
+    if (need > 0 && (!states || bytes < need)) return fail(BSA_ERR_INVALID, "%s: states of %zu bytes needed, %zu given", who, need, bytes);
+    return BSA_OK;
+}
+
+int bsa_linear_attention_segment(int tokens, int sequences, int heads, int head_dim)
+{
+    return tokens < 1 || sequences < 1 || heads < 1 ? 32 : bsa::linear_segment(tokens, sequences, heads, head_dim);
+}
+
+size_t bsa_linear_attention_states_bytes(int tokens, int key_heads, int head_dim, int segment)
+{
+    if (tokens < 1 || key_heads < 1 || head_dim < 1 || segment < 1) return 0;
+    bsa::LinearArgs p;
+    p.tokens = tokens, p.key_heads = key_heads, p.head_dim = head_dim, p.segment = segment;
+    return bsa::linear_workspace_bytes(p);
+}
+
+int bsa_linear_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, const float *log_decay,
+                                 const int32_t *offsets, const float *first, float *last, float *states, size_t states_bytes, int segment,
+                                 int tokens, int sequences, int heads, int key_heads, int head_dim, const int64_t *strides, float scale,
+                                 void *stream)
+{
+    const char *who = "bsa_linear_attention_forward";
+    bsa::LinearArgs p;
+    int rc = linear(who, dtype, q, k, v, log_decay, offsets, segment, tokens, sequences, heads, key_heads, head_dim, strides, 3, scale, p);
+    if (!rc) rc = check_linear_states(who, p, states, states_bytes);
+    if (rc) return rc;
+    if (!out) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    rc = check_alignment(who, {out, first, last, states});
+    if (rc) return rc;
+    p.out = out, p.first = first, p.last = last, p.states = states;
+    return check_launch(bsa::launch_linear_forward(p, (hipStream_t)stream), who);
+}
+
+int bsa_linear_attention_backward(int dtype, const void *q, const void *k, const void *v, const void *dout, const float *log_decay,
+                                  const int32_t *offsets, const float *first, const float *states, const float *dlast, void *dq_out,
+                                  void *dk_out, void *dv_out, float *dfirst, float *states_ws, size_t states_bytes, int segment, int tokens,
+                                  int sequences, int heads, int key_heads, int head_dim, const int64_t *strides, float scale, void *stream)
+{
+    const char *who = "bsa_linear_attention_backward";
+    bsa::LinearArgs p;
+    int rc = linear(who, dtype, q, k, v, log_decay, offsets, segment, tokens, sequences, heads, key_heads, head_dim, strides, 4, scale, p);
+    if (!rc) rc = check_linear_states(who, p, states, states_bytes);
+    if (!rc) rc = check_linear_states(who, p, states_ws, states_bytes);
+    if (rc) return rc;
+    if (!dout || !dq_out || !dk_out || !dv_out) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    rc = check_alignment(who, {dout, dq_out, dk_out, dv_out, first, states, dlast, dfirst, states_ws});
+    if (rc) return rc;
+    p.dout = dout, p.first = first, p.states = const_cast<float *>(states), p.dlast = dlast;
+    p.dq = dq_out, p.dk = dk_out, p.dv = dv_out, p.dfirst = dfirst, p.back_states = states_ws;
+    return check_launch(bsa::launch_linear_backward(p, (hipStream_t)stream), who);
+}
+
+int bsa_linear_attention_step(int dtype, const void *q, const void *k, const void *v, void *out, const float *log_decay, float *states,
+                              const int32_t *slots, int batch, int state_slots, int heads, int key_heads, int head_dim,
+                              const int64_t *strides, float scale, void *stream)
+{
+    const char *who = "bsa_linear_attention_step";
+    int rc = check_16_bit(who, dtype);
+    if (!rc) rc = check_heads(who, heads, key_heads, head_dim);
+    if (!rc) rc = check_strides(who, strides, 6);
+    if (rc) return rc;
+    if (batch < 1 || batch > 65535 || state_slots < 0)
+        return fail(BSA_ERR_INVALID, "%s: %d sequences and states for %d", who, batch, state_slots);
+    if (!q || !k || !v || !out || !log_decay || !slots || (!states && state_slots > 0)) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    rc = check_alignment(who, {q, k, v, out, states});
+    if (rc) return rc;
+    bsa::LinearStepArgs p;
+    p.q = q, p.k = k, p.v = v, p.out = out;
+    p.log_decay = log_decay, p.states = states, p.at = slots;
+    p.batch = batch, p.slots = state_slots, p.heads = heads, p.key_heads = key_heads, p.head_dim = head_dim;
+    p.q_token = strides[0], p.q_head = strides[1], p.k_token = strides[2], p.k_head = strides[3];
+    p.v_token = strides[4], p.v_head = strides[5];
+    p.scale = scale;
+    p.bf16 = dtype == BSA_BF16;
+    return check_launch(bsa::launch_linear_step(p, (hipStream_t)stream), who);
+}
+
+// ---- which pages each sequence has -------------------------------------------------------------------------
+static int pages_of_sequences(const char *who, int32_t *table, int32_t *lengths, int32_t *uses, int sequences, int width, int pages, int page,
+                              int entries, bsa::PagesArgs &p)
+{
+    const int shift = page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : page == 256 ? 8 : 0;
+    if (shift == 0) return fail(BSA_ERR_UNSUPPORTED, "%s: pages of 32, 64, 128 and 256 tokens are built, got %d", who, page);
+    if (pages < 1 || (long long)pages << shift > 2147483647LL) return fail(BSA_ERR_INVALID, "%s: %d pages of %d tokens", who, pages, page);
+    if (sequences < 1 || sequences > bsa::PAGES_MOST_SEQUENCES || width < 1 || (long long)width << shift > (1LL << 30))
+        return fail(BSA_ERR_INVALID, "%s: %d sequences of %d pages of %d", who, sequences, width, page);
+    if (entries < 0 || entries > bsa::PAGES_MOST_SEQUENCES)
+        return fail(BSA_ERR_INVALID, "%s: %d entries, at most %d", who, entries, bsa::PAGES_MOST_SEQUENCES);
+    if (!table || !lengths || !uses) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    p.table = table, p.lengths = lengths, p.uses = uses;
+    p.sequences = sequences, p.width = width, p.pages = pages, p.page_shift = shift, p.entries = entries;
+    return check_alignment(who, {table, uses});
+}
+
+int bsa_pages_append(int32_t *table, int32_t *lengths, int32_t *uses, int32_t *missing, const int32_t *offsets, int32_t *slots, int tokens,
+                     int sequences, int width, int pages, int page, int32_t *scratch, void *stream)
+{
+    const char *who = "bsa_pages_append";
+    bsa::PagesArgs p;
+    const int rc = pages_of_sequences(who, table, lengths, uses, sequences, width, pages, page, 0, p);
+    if (rc) return rc;
+    if (tokens < 0 || tokens > (1 << 30)) return fail(BSA_ERR_INVALID, "%s: %d tokens", who, tokens);
+    if (!missing || !offsets || (!slots && tokens > 0) || !scratch) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    p.missing = missing, p.offsets = offsets, p.slots = slots, p.tokens = tokens, p.scratch = scratch;
+    return check_launch(bsa::launch_pages_append(p, (hipStream_t)stream), who);
+}
+
+int bsa_pages_free(int32_t *table, int32_t *lengths, int32_t *uses, const int32_t *which, int entries, int sequences, int width, int pages,
+                   int page, void *stream)
+{
+    const char *who = "bsa_pages_free";
+    bsa::PagesArgs p;
+    const int rc = pages_of_sequences(who, table, lengths, uses, sequences, width, pages, page, entries, p);
+    if (rc || entries == 0) return rc;
+    if (!which) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    p.children = which;
+    return check_launch(bsa::launch_pages_free(p, (hipStream_t)stream), who);
+}
+
+size_t bsa_pages_fork_scratch_bytes(int entries, int width)
+{
+    return entries < 1 || width < 1 ? 0 : bsa::pages_fork_scratch(entries, width);
+}
+
+int bsa_pages_fork(int32_t *table, int32_t *lengths, int32_t *uses, int32_t *missing, const int32_t *parents, const int32_t *children,
+                   int32_t *sources, int32_t *targets, int entries, int sequences, int width, int pages, int page, void *scratch,
+                   size_t scratch_bytes, void *stream)
+{
+    const char *who = "bsa_pages_fork";
+    bsa::PagesArgs p;
+    int rc = pages_of_sequences(who, table, lengths, uses, sequences, width, pages, page, entries, p);
+    if (rc || entries == 0) return rc;
+    if (!missing || !parents || !children || !sources || !targets || !scratch) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    if (scratch_bytes < bsa::pages_fork_scratch(entries, width))
+        return fail(BSA_ERR_INVALID, "%s: scratch of %zu bytes needed, %zu given", who, bsa::pages_fork_scratch(entries, width), scratch_bytes);
+    rc = check_alignment(who, {scratch});
+    if (rc) return rc;
+    p.missing = missing, p.parents = parents, p.children = children, p.sources = sources, p.targets = targets;
+    p.scratch = (int32_t *)scratch;
+    return check_launch(bsa::launch_pages_fork(p, (hipStream_t)stream), who);
+}
+
+int bsa_pages_compact(int32_t *table, int32_t *lengths, int32_t *uses, int32_t *sources, int32_t *targets, int sequences, int width,
+                      int pages, int page, int32_t *scratch, void *stream)
+{
+    const char *who = "bsa_pages_compact";
+    bsa::PagesArgs p;
+    const int rc = pages_of_sequences(who, table, lengths, uses, sequences, width, pages, page, 0, p);
+    if (rc) return rc;
+    if (((!sources || !targets) && pages > 1) || !scratch) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    p.sources = sources, p.targets = targets, p.entries = pages / 2, p.scratch = scratch;
+    return check_launch(bsa::launch_pages_compact(p, (hipStream_t)stream), who);
+}
+
+int bsa_cache_copy(int cache_dtype, const void *from_keys, const void *from_values, const float *from_key_scales,
+                   const float *from_value_scales, int from_pages, void *keys, void *values, float *key_scales, float *value_scales, int pages,
+                   const int32_t *sources, const int32_t *targets, int count, int heads, int head_dim, int page, void *stream)
+{
+    const char *who = "bsa_cache_copy";
+    int kind, shift, rc = check_heads(who, heads, heads, head_dim);
+    if (!rc) rc = check_cache(who, cache_dtype, from_keys, from_values, from_key_scales, from_value_scales, from_pages, page, kind, shift);
+    if (!rc) rc = check_cache(who, cache_dtype, keys, values, key_scales, value_scales, pages, page, kind, shift);
+    if (rc) return rc;
+    if (count < 0 || count > (1 << 24)) return fail(BSA_ERR_INVALID, "%s: %d pages to copy", who, count);
+    if (count == 0) return BSA_OK;
+    if (!sources || !targets) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
+    bsa::PageCopyArgs p;
+    p.from_keys = from_keys, p.from_values = from_values, p.from_key_scales = from_key_scales, p.from_value_scales = from_value_scales;
+    p.keys = keys, p.values = values, p.key_scales = key_scales, p.value_scales = value_scales;
+    p.sources = sources, p.targets = targets, p.count = count, p.pages = pages, p.from_pages = from_pages;
+    p.page_bytes = (long long)heads * page * head_dim * (kind == 0 ? 2 : 1);
+    p.scale_bytes = kind == 0 ? 0 : 4LL * heads * page;
+    return check_launch(bsa::launch_pages_copy(p, (hipStream_t)stream), who);
+}
+
 }  // extern "C"

@@ -173,6 +173,42 @@ bool packed_fits(const PackedArgs &p, bool key_gradients);
 hipError_t launch_packed_forward(const PackedArgs &p, hipStream_t stream);
 hipError_t launch_packed_backward(const PackedArgs &p, hipStream_t stream);
 
+// linear attention over packed sequences (linear_attention.hip); strides in values
+struct LinearArgs {
+    const void *q = nullptr, *k = nullptr, *v = nullptr, *dout = nullptr;
+    void *out = nullptr, *dq = nullptr, *dk = nullptr, *dv = nullptr;
+    const float *log_decay = nullptr;            // [key_heads]
+    const int32_t *offsets = nullptr;
+    const float *first = nullptr;                // [sequences][key_heads][head_dim][head_dim], may be null; the same for the next three
+    float *last = nullptr;                       // forward
+    const float *dlast = nullptr;                // backward: gradients of the last states
+    float *dfirst = nullptr;                     // backward: of the first
+    float *states = nullptr, *back_states = nullptr;     // between segments: written by the forward pass; scratch of the backward pass
+    int tokens = 0, sequences = 0, heads = 0, key_heads = 0, head_dim = 64, segment = 0;     // segment: tokens, a power of two
+    long long q_token = 0, q_head = 0, k_token = 0, k_head = 0, v_token = 0, v_head = 0, g_token = 0, g_head = 0;
+    float scale = 1.f;
+    bool bf16 = false;
+};
+int linear_segment(int tokens, int sequences, int heads, int head_dim);
+size_t linear_workspace_bytes(const LinearArgs &p);
+bool linear_fits(const LinearArgs &p);
+hipError_t launch_linear_forward(const LinearArgs &p, hipStream_t stream);
+hipError_t launch_linear_backward(const LinearArgs &p, hipStream_t stream);
+
+// one token of every sequence against states in slots (linear_step.hip)
+struct LinearStepArgs {
+    const void *q = nullptr, *k = nullptr, *v = nullptr;
+    void *out = nullptr;
+    const float *log_decay = nullptr;
+    float *states = nullptr;                     // [slots][key_heads][head_dim][head_dim]
+    const int32_t *at = nullptr;                 // [batch]
+    int batch = 0, slots = 0, heads = 0, key_heads = 0, head_dim = 64;
+    long long q_token = 0, q_head = 0, k_token = 0, k_head = 0, v_token = 0, v_head = 0;
+    float scale = 1.f;
+    bool bf16 = false;
+};
+hipError_t launch_linear_step(const LinearStepArgs &p, hipStream_t stream);
+
 // rows into and out of a paged cache (cache_rows.hip); strides in values
 struct CacheRowsArgs {
     const void *k = nullptr, *v = nullptr;       // write: read; read: the results
@@ -205,5 +241,30 @@ long long cached_attention_units(const CachedArgs &p);
 long long cached_attention_parts(const CachedArgs &p);   // rows that chunks can leave in the workspace
 size_t cached_attention_workspace_bytes(const CachedArgs &p);
 hipError_t launch_cached_attention(const CachedArgs &p, hipStream_t stream);
+
+// which pages each sequence has (pages.hip)
+constexpr int PAGES_MOST_SEQUENCES = 4096;       // and entries of a call: the workgroup that deals pages has them in LDS
+struct PagesArgs {
+    int32_t *table = nullptr, *lengths = nullptr, *uses = nullptr, *missing = nullptr;
+    const int32_t *offsets = nullptr;            // append: of the new tokens, [sequences + 1]
+    int32_t *slots = nullptr;                    // append: [tokens]
+    const int32_t *parents = nullptr, *children = nullptr;       // fork; free: children
+    int32_t *sources = nullptr, *targets = nullptr;              // [entries]
+    int32_t *scratch = nullptr;
+    int tokens = 0, entries = 0, sequences = 0, width = 0, pages = 0, page_shift = 0;
+};
+size_t pages_fork_scratch(int entries, int width);
+hipError_t launch_pages_append(const PagesArgs &p, hipStream_t stream);
+hipError_t launch_pages_free(const PagesArgs &p, hipStream_t stream);
+hipError_t launch_pages_fork(const PagesArgs &p, hipStream_t stream);
+hipError_t launch_pages_compact(const PagesArgs &p, hipStream_t stream);
+struct PageCopyArgs {
+    const void *from_keys = nullptr, *from_values = nullptr, *from_key_scales = nullptr, *from_value_scales = nullptr;
+    void *keys = nullptr, *values = nullptr, *key_scales = nullptr, *value_scales = nullptr;
+    const int32_t *sources = nullptr, *targets = nullptr;
+    int count = 0, pages = 0, from_pages = 0;
+    long long page_bytes = 0, scale_bytes = 0;
+};
+hipError_t launch_pages_copy(const PageCopyArgs &p, hipStream_t stream);
 
 }  // namespace bsa

@@ -145,6 +145,18 @@ BSA_HD constexpr int get_panel_tr_addr(int lane, int step, int half, int x0)
     int x = x0 + 16 * (g & 1) + 4 * (s & 3);
     return 128 * k + 16 * ((x >> 3) ^ panel_swizzle(k)) + 2 * (x & 7);
 }
+// The same read with the columns in another order: lane i gets column perm16(i) (PANEL_PERM16: its 16 accumulator rows are consecutive
+// columns) or i with bits 2 and 3 exchanged (PANEL_SWAPPED: an accumulator of the product holds its rows in the order in which a
+// ds_read_b128 operand holds the contraction).  32 lanes together touch what the natural order touches.
+enum PanelOrder { PANEL_PERM16, PANEL_SWAPPED };
+BSA_HD constexpr int get_panel_tr_ordered_addr(PanelOrder order, int lane, int half)
+{
+    int g = lane >> 4, s = lane & 15;
+    int k = 4 * (g >> 1) + (s >> 2) + 8 * half;
+    int x = order == PANEL_PERM16 ? tr_chunk_base(true, g, s & 3) : 16 * (g & 1) + 8 * (s & 1) + 4 * ((s >> 1) & 1);
+    return 128 * k + 16 * ((x >> 3) ^ panel_swizzle(k)) + 2 * (x & 7);
+}
+BSA_HD constexpr int swapped16(int r) { return (r & 19) + 2 * (r & 4) + ((r >> 1) & 4); }
 // result rows of 64 or 128 halves (8 or 16 pieces) on their way to whole-line stores: half h of piece p of row `row`
 BSA_HD constexpr int out_row_addr(int head, int row, int p, int h) { return 2 * head * row + 16 * (p ^ (row & 7)) + 8 * h; }
 

@@ -1,0 +1,438 @@
+// Which pages of a cache each sequence has, kept on the device, and copies of pages.
+//
+//   table [sequences][width]   page numbers, -1 behind the last;  lengths [sequences]: tokens;  uses [pages]: sequences that have a page
+//
+// Whole pages may belong to several sequences, the last page of one that is not full belongs to it alone: a fork shares the whole pages
+// and copies that one.  New pages are the lowest free ones, in the order of the call's sequences, so that equal tables and equal
+// calls give equal tables.  Counting is by integer atomics, whose order changes nothing.
+//
+// What bounds it: latency.  Ranks of free pages are found by one workgroup that reads `uses` 16 bytes a lane and sums up in LDS, as far as it
+// has to; rows of the table are read and written by a workgroup each.
+#include "bsa_device.hpp"
+#include "bsa_internal.hpp"
+
+namespace bsa {
+
+namespace {
+
+constexpr int PG_THREADS = 1024, PG_WAVES = PG_THREADS / WAVE;
+constexpr int PG_MOST = PAGES_MOST_SEQUENCES, PG_PER = PG_MOST / PG_THREADS;
+
+__device__ __forceinline__ int wave_prefix(int x)        // inclusive, over the wave
+{
+#pragma unroll
+    for (int d = 1; d < WAVE; d *= 2) {
+        const int below = __builtin_amdgcn_ds_bpermute((lane_id() - d) << 2, x);
+        x += lane_id() >= d ? below : 0;
+    }
+    return x;
+}
+// exclusive prefix over the PG_THREADS threads of a workgroup, and the sum of all
+__device__ __forceinline__ int block_prefix(int x, int *parts, int &all)
+{
+    const int inclusive = wave_prefix(x);
+    __syncthreads();                                     // parts may still be read
+    if (lane_id() == WAVE - 1) parts[wave_id()] = inclusive;
+    __syncthreads();
+    int before = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < PG_WAVES; ++w) {
+        before += w < wave_id() ? parts[w] : 0;
+        all += parts[w];
+    }
+    return before + inclusive - x;
+}
+
+// taken(rank, page) for the `wanted` lowest pages for which free(uses), by rank; how many there are, at most `wanted`
+template <class Taken>
+__device__ __forceinline__ int lowest_free(const int32_t *uses, int pages, int wanted, int *parts, Taken taken)
+{
+    int found = 0;
+    for (int first = 0; first < pages && found < wanted; first += 4 * PG_THREADS) {
+        const int at = first + 4 * (int)threadIdx.x;
+        int use[4], mine = 0, all;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            use[j] = at + j < pages ? uses[at + j] : 1;
+            mine += use[j] == 0 ? 1 : 0;
+        }
+        int rank = found + block_prefix(mine, parts, all);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (use[j] == 0) {
+                if (rank < wanted) taken(rank, at + j);
+                ++rank;
+            }
+        found += all;
+    }
+    return found < wanted ? found : wanted;
+}
+
+__device__ __forceinline__ int pages_of(long long tokens, int page_shift) { return (int)((tokens + (1 << page_shift) - 1) >> page_shift); }
+__device__ __forceinline__ int length_of(const PagesArgs &p, int b)
+{
+    const long long n = p.lengths[b], most = (long long)p.width << p.page_shift;
+    return (int)(n < 0 ? 0 : n > most ? most : n);
+}
+__device__ __forceinline__ bool is_page(const PagesArgs &p, int x) { return x >= 0 && x < p.pages; }
+
+// ---- new tokens ---------------------------------------------------------------------------------------
+__device__ __forceinline__ int new_offset(const PagesArgs &p, int b)
+{
+    const int x = p.offsets[b];
+    return x < 0 ? 0 : x > p.tokens ? p.tokens : x;
+}
+// started[b]: the length before, -1 for a sequence whose tokens have no place
+__device__ __forceinline__ void write_slots(const PagesArgs &p, int first, int stride, const int32_t *started)
+{
+    for (int t = first; t < p.tokens; t += stride) {
+        int low = 0, count = p.sequences;                // the last sequence that begins at t or before
+        while (count > 1) {
+            const int half = count / 2;
+            if (new_offset(p, low + half) <= t) {
+                low += half;
+                count -= half;
+            } else {
+                count = half;
+            }
+        }
+        int slot = -1;
+        const int from = new_offset(p, low);
+        if (from <= t && t < new_offset(p, low + 1) && started[low] >= 0) {
+            const int place = started[low] + (t - from), at = place >> p.page_shift;
+            const int page = at < p.width ? p.table[(size_t)low * p.width + at] : -1;
+            if (is_page(p, page)) slot = (page << p.page_shift) + (place & ((1 << p.page_shift) - 1));
+        }
+        p.slots[t] = slot;
+    }
+}
+
+__global__ __launch_bounds__(PG_THREADS) void pages_append_kernel(PagesArgs p, bool with_slots)
+{
+    __shared__ int parts[PG_WAVES], ends[PG_MOST], had[PG_MOST];
+    int need[PG_PER], sum = 0, all;
+    bool wide[PG_PER];
+    // sequences PG_PER x thread .. of this thread; ends: pages that the sequences up to and with one need
+#pragma unroll
+    for (int j = 0; j < PG_PER; ++j) {
+        const int b = PG_PER * (int)threadIdx.x + j;
+        need[j] = 0, wide[j] = false;
+        if (b < p.sequences) {
+            const int from = new_offset(p, b), to = new_offset(p, b + 1), held = length_of(p, b);
+            const long long length = (long long)held + (to > from ? to - from : 0);
+            had[b] = pages_of(held, p.page_shift);
+            wide[j] = pages_of(length, p.page_shift) > p.width;
+            need[j] = wide[j] ? 0 : pages_of(length, p.page_shift) - had[b];
+        }
+        sum += need[j];
+    }
+    int end = block_prefix(sum, parts, all);
+#pragma unroll
+    for (int j = 0; j < PG_PER; ++j) {
+        end += need[j];
+        ends[PG_PER * threadIdx.x + j] = end;
+    }
+    __syncthreads();
+    // the sequence that the page of this rank goes to: the first whose end lies behind it
+    auto owner = [&](int rank) {
+        int low = 0, count = p.sequences;
+        while (count > 0) {
+            const int half = count / 2;
+            if (ends[low + half] <= rank) {
+                low += half + 1;
+                count -= half + 1;
+            } else {
+                count = half;
+            }
+        }
+        return low;
+    };
+    const int found = lowest_free(p.uses, p.pages, all, parts, [&](int rank, int page) {
+        const int b = owner(rank), begin = b > 0 ? ends[b - 1] : 0;
+        p.table[(size_t)b * p.width + had[b] + (rank - begin)] = page;
+        p.uses[page] = 1;
+    });
+    __syncthreads();
+    if (found < all) {                                   // the sequence that got a part of its pages only gives them back
+        const int b = owner(found), begin = b > 0 ? ends[b - 1] : 0;
+        for (int r = begin + (int)threadIdx.x; r < found; r += PG_THREADS) {
+            int32_t *at = p.table + (size_t)b * p.width + had[b] + (r - begin);
+            p.uses[*at] = 0;
+            *at = -1;
+        }
+    }
+    int refused = 0;
+#pragma unroll
+    for (int j = 0; j < PG_PER; ++j) {
+        const int b = PG_PER * (int)threadIdx.x + j;
+        if (b >= p.sequences) continue;
+        const int from = new_offset(p, b), to = new_offset(p, b + 1), held = length_of(p, b);
+        const bool fits = !wide[j] && (need[j] == 0 || ends[b] <= found);
+        p.scratch[b] = fits ? held : -1;
+        p.lengths[b] = held + (fits && to > from ? to - from : 0);
+        refused += fits ? 0 : 1;
+    }
+    if (refused > 0) atomicAdd(p.missing, refused);
+    __syncthreads();
+    if (with_slots) write_slots(p, (int)threadIdx.x, PG_THREADS, p.scratch);
+}
+__global__ __launch_bounds__(256) void pages_slots_kernel(PagesArgs p)
+{
+    write_slots(p, (int)(blockIdx.x * 256 + threadIdx.x), (int)(gridDim.x * 256), p.scratch);
+}
+
+// ---- sequences that end -------------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void pages_free_kernel(PagesArgs p)
+{
+    __shared__ int length;
+    const int b = p.children[blockIdx.x];
+    if (b < 0 || b >= p.sequences) return;
+    if (threadIdx.x == 0) length = atomicExch(p.lengths + b, 0);         // of several entries for a sequence one finds it
+    __syncthreads();
+    const long long most = (long long)p.width << p.page_shift;
+    const int count = pages_of(length < 0 ? 0 : length > most ? most : length, p.page_shift);
+    for (int j = (int)threadIdx.x; j < count; j += 256) {
+        int32_t *at = p.table + (size_t)b * p.width + j;
+        if (is_page(p, *at)) atomicAdd(p.uses + *at, -1);
+        *at = -1;
+    }
+}
+
+// ---- sequences that others continue -------------------------------------------------------------------
+// Scratch of an entry: its parent's row, then these
+struct ForkEntry {
+    int32_t tokens;                      // of the parent; -1: an entry that is left out
+    int32_t old_pages;                   // that the child had
+    int32_t copies;                      // the parent's last page is copied
+    int32_t unused;
+};
+__device__ __forceinline__ int32_t *fork_row(const PagesArgs &p, int i) { return p.scratch + (size_t)i * (p.width + 4); }
+__device__ __forceinline__ ForkEntry &fork_entry(const PagesArgs &p, int i) { return *reinterpret_cast<ForkEntry *>(fork_row(p, i) + p.width); }
+
+// Of the entries for a child the first counts; of the entries that continue a parent which is itself replaced, the first keeps its last
+// page.  by_child, by_parent: their places among the entries, or none.
+__device__ __forceinline__ void fork_claims(const PagesArgs &p, int *by_child, int *by_parent)
+{
+    const int none = 0x7FFFFFFF;
+    for (int b = (int)threadIdx.x; b < p.sequences; b += (int)blockDim.x) by_child[b] = by_parent[b] = none;
+    __syncthreads();
+    auto inside = [&](int x) { return x >= 0 && x < p.sequences; };
+    for (int i = (int)threadIdx.x; i < p.entries; i += (int)blockDim.x)
+        if (inside(p.parents[i]) && inside(p.children[i])) atomicMin(by_child + p.children[i], i);
+    __syncthreads();
+    for (int i = (int)threadIdx.x; i < p.entries; i += (int)blockDim.x)
+        if (inside(p.parents[i]) && inside(p.children[i]) && by_child[p.children[i]] == i) atomicMin(by_parent + p.parents[i], i);
+    __syncthreads();
+}
+
+// one entry: its parent's row into scratch, uses of what it shares and of what the child had
+__device__ __forceinline__ void fork_share(const PagesArgs &p, int i, const int *by_child, const int *by_parent)
+{
+    const int none = 0x7FFFFFFF, parent = p.parents[i], child = p.children[i];
+    const bool there = parent >= 0 && parent < p.sequences && child >= 0 && child < p.sequences && by_child[child] == i;
+    ForkEntry entry{-1, 0, 0, 0};
+    if (there) {
+        entry.tokens = length_of(p, parent);
+        entry.old_pages = pages_of(length_of(p, child), p.page_shift);
+        const bool partial = (entry.tokens & ((1 << p.page_shift) - 1)) != 0;
+        entry.copies = partial && (by_child[parent] == none || by_parent[parent] != i);
+        const int count = pages_of(entry.tokens, p.page_shift), shared = count - entry.copies;
+        int32_t *row = fork_row(p, i);
+        for (int j = (int)threadIdx.x; j < count; j += (int)blockDim.x) {
+            const int page = p.table[(size_t)parent * p.width + j];
+            row[j] = page;
+            if (j < shared && is_page(p, page)) atomicAdd(p.uses + page, 1);
+        }
+        for (int j = (int)threadIdx.x; j < entry.old_pages; j += (int)blockDim.x) {
+            const int page = p.table[(size_t)child * p.width + j];
+            if (is_page(p, page)) atomicAdd(p.uses + page, -1);
+        }
+    }
+    if (threadIdx.x == 0) fork_entry(p, i) = entry;
+}
+
+// pages for the copies, by one workgroup; an entry that gets none leaves its child empty
+__device__ __forceinline__ void fork_allocate(const PagesArgs &p, int *parts)
+{
+    int wanted = 0;
+    const int rounds = (p.entries + PG_THREADS - 1) / PG_THREADS;
+    // ranks: the copying entries in their order; p.targets holds the rank's entry until its page is known
+    for (int r = 0; r < rounds; ++r) {
+        const int i = r * PG_THREADS + (int)threadIdx.x;
+        const bool copies = i < p.entries && fork_entry(p, i).copies != 0;
+        int all;
+        const int rank = wanted + block_prefix(copies ? 1 : 0, parts, all);
+        if (copies) fork_entry(p, rank).unused = i;
+        wanted += all;
+        if (i < p.entries) p.sources[i] = p.targets[i] = -1;
+    }
+    __syncthreads();
+    const int found = lowest_free(p.uses, p.pages, wanted, parts, [&](int rank, int page) {
+        const int i = fork_entry(p, rank).unused, last = fork_entry(p, i).tokens >> p.page_shift;
+        p.sources[i] = fork_row(p, i)[last];
+        p.targets[i] = page;
+        fork_row(p, i)[last] = page;
+        p.uses[page] = 1;
+    });
+    __syncthreads();
+    for (int rank = found; rank < wanted; ++rank) {
+        const int i = fork_entry(p, rank).unused, shared = fork_entry(p, i).tokens >> p.page_shift;
+        for (int j = (int)threadIdx.x; j < shared; j += PG_THREADS)
+            if (is_page(p, fork_row(p, i)[j])) atomicAdd(p.uses + fork_row(p, i)[j], -1);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            fork_entry(p, i).tokens = 0;
+            atomicAdd(p.missing, 1);
+        }
+    }
+    __syncthreads();
+    for (int i = (int)threadIdx.x; i < p.entries; i += PG_THREADS)
+        if (fork_entry(p, i).tokens >= 0) p.lengths[p.children[i]] = fork_entry(p, i).tokens;
+}
+
+__device__ __forceinline__ void fork_place(const PagesArgs &p, int i)
+{
+    const ForkEntry entry = fork_entry(p, i);
+    if (entry.tokens < 0) return;
+    const int count = pages_of(entry.tokens, p.page_shift), old = entry.old_pages;
+    int32_t *to = p.table + (size_t)p.children[i] * p.width;
+    for (int j = (int)threadIdx.x; j < (count > old ? count : old); j += (int)blockDim.x) to[j] = j < count ? fork_row(p, i)[j] : -1;
+}
+
+__global__ __launch_bounds__(256) void pages_share_kernel(PagesArgs p)
+{
+    __shared__ int by_child[PG_MOST], by_parent[PG_MOST];
+    fork_claims(p, by_child, by_parent);
+    fork_share(p, (int)blockIdx.x, by_child, by_parent);
+}
+__global__ __launch_bounds__(PG_THREADS) void pages_allocate_kernel(PagesArgs p)
+{
+    __shared__ int parts[PG_WAVES];
+    fork_allocate(p, parts);
+}
+__global__ __launch_bounds__(256) void pages_place_kernel(PagesArgs p) { fork_place(p, (int)blockIdx.x); }
+
+// ---- what is left moves together ----------------------------------------------------------------------
+// The used pages number `used` and up move, in their order, into the free ones below.  scratch: [0] used, then the new number of every page.
+__global__ __launch_bounds__(PG_THREADS) void pages_moves_kernel(PagesArgs p)
+{
+    __shared__ int parts[PG_WAVES];
+    int mine = 0, used;
+    for (int i = (int)threadIdx.x; i < p.pages; i += PG_THREADS) mine += p.uses[i] > 0 ? 1 : 0;
+    block_prefix(mine, parts, used);
+    if (threadIdx.x == 0) p.scratch[0] = used;
+    const int holes = lowest_free(p.uses, used, used, parts, [&](int rank, int page) { p.targets[rank] = page; });
+    __syncthreads();
+    int moved = 0;
+    for (int first = used; first < p.pages && moved < holes; first += PG_THREADS) {
+        const int at = first + (int)threadIdx.x;
+        const int use = at < p.pages ? p.uses[at] : 0;
+        int all;
+        const int rank = moved + block_prefix(use > 0 ? 1 : 0, parts, all);
+        if (use > 0 && rank < holes) {
+            const int to = p.targets[rank];
+            p.sources[rank] = at;
+            p.scratch[1 + at] = to;
+            p.uses[to] = use;
+            p.uses[at] = 0;
+        }
+        moved += all;
+    }
+    for (int i = holes + (int)threadIdx.x; i < p.entries; i += PG_THREADS) p.sources[i] = p.targets[i] = -1;
+}
+__global__ __launch_bounds__(256) void pages_renumber_kernel(PagesArgs p)
+{
+    const int b = (int)blockIdx.x, used = p.scratch[0], count = pages_of(length_of(p, b), p.page_shift);
+    for (int j = (int)threadIdx.x; j < count; j += 256) {
+        int32_t *at = p.table + (size_t)b * p.width + j;
+        const int page = *at;
+        if (page >= used && page < p.pages) *at = p.scratch[1 + page];
+    }
+}
+
+// ---- copies of pages ----------------------------------------------------------------------------------
+// Pieces of 16 KB of a page's keys or values, dealt to the workgroups in order; the scales go with the first of each.
+constexpr int COPY_PIECE = 16384;
+__device__ __forceinline__ void copy_bytes(const unsigned char *from, unsigned char *to, int bytes)
+{
+    uint4 x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int at = 16 * (256 * j + (int)threadIdx.x);
+        if (at < bytes) x[j] = ldg16_stream(from + at);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int at = 16 * (256 * j + (int)threadIdx.x);
+        if (at < bytes) stg16_stream(to + at, x[j]);
+    }
+}
+__global__ __launch_bounds__(256) void pages_copy_kernel(PageCopyArgs p)
+{
+    const int per = (int)((p.page_bytes + COPY_PIECE - 1) / COPY_PIECE), whole = 2 * per;
+    const long long pieces = (long long)p.count * whole;
+    for (long long piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
+        const int pair = (int)(piece / whole), part = (int)(piece - (long long)pair * whole), at = part % per;
+        const int from = p.sources[pair], to = p.targets[pair];
+        if (from < 0 || from >= p.from_pages || to < 0 || to >= p.pages) continue;
+        const bool values = part >= per;
+        const size_t first = (size_t)at * COPY_PIECE;
+        const int bytes = (int)(p.page_bytes - (long long)first < COPY_PIECE ? p.page_bytes - (long long)first : COPY_PIECE);
+        copy_bytes((const unsigned char *)(values ? p.from_values : p.from_keys) + (size_t)from * p.page_bytes + first,
+                   (unsigned char *)(values ? p.values : p.keys) + (size_t)to * p.page_bytes + first, bytes);
+        if (at == 0)
+            for (long long s = 0; s < p.scale_bytes; s += COPY_PIECE)
+                copy_bytes((const unsigned char *)(values ? p.from_value_scales : p.from_key_scales) + (size_t)from * p.scale_bytes + s,
+                           (unsigned char *)(values ? p.value_scales : p.key_scales) + (size_t)to * p.scale_bytes + s,
+                           (int)(p.scale_bytes - s < COPY_PIECE ? p.scale_bytes - s : COPY_PIECE));
+    }
+}
+
+}  // namespace
+
+size_t pages_fork_scratch(int entries, int width) { return (size_t)entries * (width + 4) * sizeof(int32_t); }
+
+hipError_t launch_pages_append(const PagesArgs &p, hipStream_t st)
+{
+    constexpr int ALONE = 4096;                          // tokens whose slots the one workgroup writes itself
+    pages_append_kernel<<<1, PG_THREADS, 0, st>>>(p, p.tokens <= ALONE);
+    if (p.tokens > ALONE) {
+        const hipError_t err = hipGetLastError();
+        if (err != hipSuccess) return err;
+        pages_slots_kernel<<<(p.tokens + 255) / 256 < 2048 ? (p.tokens + 255) / 256 : 2048, 256, 0, st>>>(p);
+    }
+    return hipGetLastError();
+}
+hipError_t launch_pages_free(const PagesArgs &p, hipStream_t st)
+{
+    pages_free_kernel<<<p.entries, 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+hipError_t launch_pages_fork(const PagesArgs &p, hipStream_t st)
+{
+    pages_share_kernel<<<p.entries, 256, 0, st>>>(p);
+    hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    pages_allocate_kernel<<<1, PG_THREADS, 0, st>>>(p);
+    err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    pages_place_kernel<<<p.entries, 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+hipError_t launch_pages_compact(const PagesArgs &p, hipStream_t st)
+{
+    pages_moves_kernel<<<1, PG_THREADS, 0, st>>>(p);
+    const hipError_t err = hipGetLastError();
+    if (err != hipSuccess) return err;
+    pages_renumber_kernel<<<p.sequences, 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+hipError_t launch_pages_copy(const PageCopyArgs &p, hipStream_t st)
+{
+    const long long pieces = (long long)p.count * 2 * ((p.page_bytes + COPY_PIECE - 1) / COPY_PIECE);
+    pages_copy_kernel<<<(unsigned)(pieces < 4096 ? pieces : 4096), 256, 0, st>>>(p);
+    return hipGetLastError();
+}
+
+}  // namespace bsa

@@ -122,6 +122,27 @@ class KeyValueCache:
                                            v.data_ptr(), *self._sizes(slots.numel()), _k.current_stream()))
         return k, v
 
+    def copy(self, sources: torch.Tensor, targets: torch.Tensor, origin: Optional["KeyValueCache"] = None) -> None:
+        """Copies whole pages as they are, values and scales: page ``sources[i]`` of ``origin`` (this cache without one) to page
+        ``targets[i]`` of this one (int32 on the GPU).  ``origin`` has the same type, heads, head dim and page on the same GPU, and any number of
+        pages.  Pairs with a number outside either cache (-1) are left out.  No page may be the target of two pairs, nor, in one cache, the
+        target of one and the source of another."""
+        origin = self if origin is None else origin
+        if not isinstance(origin, KeyValueCache):
+            raise TypeError(f"origin must be a KeyValueCache, got {type(origin).__name__}")
+        for name in ("dtype", "heads", "head_dim", "page", "device"):
+            if getattr(origin, name) != getattr(self, name):
+                raise ValueError(f"pages of a cache with {name} {getattr(origin, name)} do not fit one with {getattr(self, name)}")
+        check_index(sources, "sources", self.device, 1)
+        check_index(targets, "targets", self.device, 1)
+        if sources.numel() != targets.numel() or sources.numel() > 1 << 24:
+            raise ValueError(f"{sources.numel()} sources and {targets.numel()} targets")
+        if sources.numel() == 0:
+            return
+        with _k.on_device(self.device):
+            _k.check(_k.lib.bsa_cache_copy(_HELD[self.dtype], *origin._tensors(), origin.pages, *self._tensors(), self.pages, sources.data_ptr(),
+                                           targets.data_ptr(), sources.numel(), self.heads, self.head_dim, self.page, _k.current_stream()))
+
 
 def cached_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: KeyValueCache, pages: torch.Tensor,
                      lengths: torch.Tensor, tree: Optional[torch.Tensor] = None, scale: float = 1.0) -> torch.Tensor:

@@ -67,6 +67,17 @@ SIGNATURES = {
     "bsa_cache_read": (_i, [_i, _i] + [_vp] * 7 + [_i] * 5 + [_vp]),
     "bsa_cached_attention_workspace_bytes": (ctypes.c_size_t, [_i] * 7),
     "bsa_cached_attention": (_i, [_i, _i] + [_vp] * 11 + [_i] * 9 + [_vp, _f, _vp, ctypes.c_size_t, _vp]),
+    "bsa_linear_attention_segment": (_i, [_i] * 4),
+    "bsa_linear_attention_states_bytes": (ctypes.c_size_t, [_i] * 4),
+    "bsa_linear_attention_forward": (_i, [_i] + [_vp] * 9 + [ctypes.c_size_t] + [_i] * 6 + [_vp, _f, _vp]),
+    "bsa_linear_attention_backward": (_i, [_i] + [_vp] * 14 + [ctypes.c_size_t] + [_i] * 6 + [_vp, _f, _vp]),
+    "bsa_linear_attention_step": (_i, [_i] + [_vp] * 7 + [_i] * 5 + [_vp, _f, _vp]),
+    "bsa_pages_append": (_i, [_vp] * 6 + [_i] * 5 + [_vp, _vp]),
+    "bsa_pages_free": (_i, [_vp] * 4 + [_i] * 5 + [_vp]),
+    "bsa_pages_fork_scratch_bytes": (ctypes.c_size_t, [_i] * 2),
+    "bsa_pages_fork": (_i, [_vp] * 8 + [_i] * 5 + [_vp, ctypes.c_size_t, _vp]),
+    "bsa_pages_compact": (_i, [_vp] * 5 + [_i] * 4 + [_vp, _vp]),
+    "bsa_cache_copy": (_i, [_i] + [_vp] * 4 + [_i] + [_vp] * 4 + [_i] + [_vp] * 2 + [_i] * 4 + [_vp]),
 }
 
 

@@ -468,6 +468,78 @@ int bsa_cached_attention(int dtype, int cache_dtype, const void *q, const void *
                          int key_heads, int head_dim, int pages, int page, int width, const int64_t *strides, float scale,
                          void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- linear attention with a decay for each key head ------------------------
+ * Inside every sequence of a packed batch, tokens t = 1 .. n, query head h over key head h / (heads / key_heads):
+ *   S_t = exp(log_decay) S_(t-1) + k_t v_t^T,   out_t = scale q_t S_t
+ *   q, k, v, out, offsets, strides   as bsa_packed_attention_forward has them (dout, dq, dk, dv too)
+ *   log_decay        device float [key_heads], 0 or less (-inf: a token sees itself only)
+ *   first, last      float [sequences, key_heads, head_dim, head_dim], S_0 (NULL: zero) and S_n (NULL: not wanted); an empty sequence's
+ *                    S_n is its S_0.  dlast, dfirst: their gradients, dlast NULL: zero
+ *   states           float, bsa_linear_attention_states_bytes: the states between the segments of long sequences, written by the
+ *                    forward call, read by the backward call, which has scratch of the same size of its own.  0 bytes up to `segment` tokens
+ *   segment          tokens, a power of two from 32 on; bsa_linear_attention_segment says which fills the machine.  Both calls have to have
+ *                    the same.  Results of different segments differ by rounding.
+ * Tokens outside every sequence get zeros.  States are fp32; results are the same bits in every call.  An infinity or a NaN
+ * in a token makes what it reaches, of its own token and later ones, something that is no finite number.
+ * fp16 and bf16, head_dim 64 or 128, at most 65535 sequences; log_decay has no gradient.
+ *
+ * bsa_linear_attention_step: one token of each of `batch` sequences against its state, in place:
+ *   q [batch, heads, head_dim], k, v [batch, key_heads, head_dim] with strides (sequence, head of each); out dense
+ *   states float [state_slots, key_heads, head_dim, head_dim];  slots: device int32 [batch], the sequence's state.  Sequences whose slot is
+ *   negative or not below state_slots get zeros and change nothing.  No two sequences of a call may have the same slot.
+ */
+int bsa_linear_attention_segment(int tokens, int sequences, int heads, int head_dim);
+size_t bsa_linear_attention_states_bytes(int tokens, int key_heads, int head_dim, int segment);
+int bsa_linear_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, const float *log_decay,
+                                 const int32_t *offsets, const float *first, float *last, float *states, size_t states_bytes, int segment,
+                                 int tokens, int sequences, int heads, int key_heads, int head_dim, const int64_t *strides, float scale,
+                                 void *stream);
+int bsa_linear_attention_backward(int dtype, const void *q, const void *k, const void *v, const void *dout, const float *log_decay,
+                                  const int32_t *offsets, const float *first, const float *states, const float *dlast, void *dq_out,
+                                  void *dk_out, void *dv_out, float *dfirst, float *states_ws, size_t states_bytes, int segment, int tokens,
+                                  int sequences, int heads, int key_heads, int head_dim, const int64_t *strides, float scale, void *stream);
+int bsa_linear_attention_step(int dtype, const void *q, const void *k, const void *v, void *out, const float *log_decay, float *states,
+                              const int32_t *slots, int batch, int state_slots, int heads, int key_heads, int head_dim,
+                              const int64_t *strides, float scale, void *stream);
+
+/* ---- which pages of a cache each sequence has --------------------------------
+ *   table   device int32 [sequences, width]: page numbers of a sequence, -1 behind its last one
+ *   lengths device int32 [sequences]: its tokens;   uses device int32 [pages]: how many sequences have a page
+ *   missing device int32 [1]: requests that found no pages are added to it
+ * All stay on the device.  Whole pages may be shared; a last page that is not full belongs to one sequence.  Pages are taken
+ * lowest first, in the order of the sequences or entries, so that results depend on nothing but the arguments.  At most 4096 sequences and
+ * entries, width * page at most 2^30; page is 32, 64, 128 or 256.  The calls for a table are to be ordered.
+ *
+ * bsa_pages_append: sequence b grows by offsets[b + 1] - offsets[b] tokens (device int32 [sequences + 1], ascending, taken as the nearer
+ *   end outside [0, tokens]); slots [tokens]: where each goes (bsa_cache_write).  A sequence whose tokens would need more pages than
+ *   are free, behind those in front of it, or than width, stays as it is, and its tokens get slot -1, as tokens outside
+ *   every sequence do.  scratch: device int32 [sequences], any contents.
+ * bsa_pages_free: the sequences which[0 .. entries - 1] end: length 0, their pages one use less.  Others' numbers are left out.
+ * bsa_pages_fork: sequence children[i] becomes what sequence parents[i] was before the call, for all entries at once; what the child had is
+ *   freed.  Whole pages are shared.  The last page, where it is not full, is a page of the child's own, to be copied by the
+ *   caller in every cache from sources[i] to targets[i] (bsa_cache_copy); -1: nothing to copy, also where the parent itself is replaced
+ *   and this entry, the first of its heirs, keeps the page.  A child whose page was not to be had is empty.  Of several entries for a
+ *   child the first counts; entries with a number outside [0, sequences) are left out.
+ * bsa_pages_compact: the used pages become the lowest ones: the k-th of those that lie too high moves to the k-th free one below.
+ *   sources, targets: int32 [pages / 2], filled up with -1; the caller copies them in every cache.  scratch: int32 [pages + 1].
+ * bsa_cache_copy copies whole pages, keys, values and scales, as they are: sources[i] of one cache to targets[i] of another (or the same)
+ *   with the same type, heads, head_dim and page.  Pairs with a number outside either cache are left out.  No target may be another
+ *   pair's source in the same cache, or another's target.
+ */
+int bsa_pages_append(int32_t *table, int32_t *lengths, int32_t *uses, int32_t *missing, const int32_t *offsets, int32_t *slots, int tokens,
+                     int sequences, int width, int pages, int page, int32_t *scratch, void *stream);
+int bsa_pages_free(int32_t *table, int32_t *lengths, int32_t *uses, const int32_t *which, int entries, int sequences, int width, int pages,
+                   int page, void *stream);
+size_t bsa_pages_fork_scratch_bytes(int entries, int width);
+int bsa_pages_fork(int32_t *table, int32_t *lengths, int32_t *uses, int32_t *missing, const int32_t *parents, const int32_t *children,
+                   int32_t *sources, int32_t *targets, int entries, int sequences, int width, int pages, int page, void *scratch,
+                   size_t scratch_bytes, void *stream);
+int bsa_pages_compact(int32_t *table, int32_t *lengths, int32_t *uses, int32_t *sources, int32_t *targets, int sequences, int width,
+                      int pages, int page, int32_t *scratch, void *stream);
+int bsa_cache_copy(int cache_dtype, const void *from_keys, const void *from_values, const float *from_key_scales,
+                   const float *from_value_scales, int from_pages, void *keys, void *values, float *key_scales, float *value_scales, int pages,
+                   const int32_t *sources, const int32_t *targets, int count, int heads, int head_dim, int page, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
