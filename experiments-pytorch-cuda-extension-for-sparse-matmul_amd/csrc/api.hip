@@ -977,8 +977,8 @@ static int linear(const char *who, int dtype, const void *q, const void *k, cons
     if (rc) return rc;
     if (tokens < 1 || sequences < 1 || tokens > (1 << 30) || sequences > 65535)
         return fail(BSA_ERR_INVALID, "%s: %d tokens in %d sequences", who, tokens, sequences);
-    if (segment < 32 || segment > (1 << 20) || (segment & (segment - 1)) != 0)
-        return fail(BSA_ERR_INVALID, "%s: segments of %d tokens (a power of two from 32 on)", who, segment);
+    if (segment < 32 || segment > (1 << 20) || segment % 32 != 0)
+        return fail(BSA_ERR_INVALID, "%s: segments of %d tokens (a multiple of 32)", who, segment);
     if (!q || !k || !v || !log_decay || !offsets) return fail(BSA_ERR_INVALID, "%s: null pointer argument", who);
     for (int i = 0; i < operands; ++i)
         if (strides[2 * i] > (1LL << 24))
@@ -1004,9 +1004,9 @@ static int check_linear_states(const char *who, const bsa::LinearArgs &p, const 
     return BSA_OK;
 }
 
-int bsa_linear_attention_segment(int tokens, int sequences, int heads, int head_dim)
+int bsa_linear_attention_segment(int tokens, int sequences, int key_heads, int head_dim)
 {
-    return tokens < 1 || sequences < 1 || heads < 1 ? 32 : bsa::linear_segment(tokens, sequences, heads, head_dim);
+    return tokens < 1 || sequences < 1 || key_heads < 1 ? 32 : bsa::linear_segment(tokens, sequences, key_heads, head_dim);
 }
 
 size_t bsa_linear_attention_states_bytes(int tokens, int key_heads, int head_dim, int segment)

@@ -184,12 +184,12 @@ struct LinearArgs {
     const float *dlast = nullptr;                // backward: gradients of the last states
     float *dfirst = nullptr;                     // backward: of the first
     float *states = nullptr, *back_states = nullptr;     // between segments: written by the forward pass; scratch of the backward pass
-    int tokens = 0, sequences = 0, heads = 0, key_heads = 0, head_dim = 64, segment = 0;     // segment: tokens, a power of two
+    int tokens = 0, sequences = 0, heads = 0, key_heads = 0, head_dim = 64, segment = 0;     // segment: tokens, a multiple of 32
     long long q_token = 0, q_head = 0, k_token = 0, k_head = 0, v_token = 0, v_head = 0, g_token = 0, g_head = 0;
     float scale = 1.f;
     bool bf16 = false;
 };
-int linear_segment(int tokens, int sequences, int heads, int head_dim);
+int linear_segment(int tokens, int sequences, int key_heads, int head_dim);
 size_t linear_workspace_bytes(const LinearArgs &p);
 bool linear_fits(const LinearArgs &p);
 hipError_t launch_linear_forward(const LinearArgs &p, hipStream_t stream);

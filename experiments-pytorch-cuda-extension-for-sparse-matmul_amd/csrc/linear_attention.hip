@@ -3,13 +3,14 @@
 //
 // Chunks of 32 tokens: with a, b, c for q, k, v and P_ts = scale l^(t-s) (a_t . b_s) for s <= t inside the chunk,
 //   o_t = sum_s P_ts c_s + scale l^(t+1) a_t S,      S <- l^32 S + sum_s l^(31-s) b_s c_s^T.
-// The gradients are the same sum over other operands and, for dk and dv, from the end of the sequence (R: what dk and dv take the place of S):
+// The gradients are the same sum over other operands and, for dk and dv, from the end of the sequence, R in the place of S:
 //   dq: a, b, c = dO, V, K (the state is S^T);   dv: K, Q, dO backwards;   dk: V, dO, Q backwards (R^T).
 //
-// A sequence is cut into segments of p.segment tokens.  One workgroup walks a segment of one head, its wave w has columns 32 w .. of c and of
-// the state, which stays in fp32 accumulators from chunk to chunk.  Where a sequence has several segments, two launches in front make
-// the state that each begins with: every segment's own sum, then the running sum over segments.  Chunks travel
-// straight to LDS two steps ahead of their use, in a ring of three.
+// A sequence is cut into segments of p.segment tokens.  One workgroup walks a segment of one key head with all query heads that share it; its
+// wave w has columns 32 w .. of c and of the state, which stays in fp32 accumulators from chunk to chunk.  dv and dk, which read the
+// same four operands, share a workgroup.  Where a sequence has several segments, two launches in front make the state that each begins
+// with: every segment's own sum, then the running sum over segments.  Chunks travel straight to LDS two steps ahead of their use, in
+// a ring of three.
 #include "attention_tiles.hpp"
 #include "bsa_device.hpp"
 #include "bsa_internal.hpp"
@@ -22,19 +23,21 @@ namespace {
 
 constexpr int LA_ROWS = 32;              // tokens of a chunk
 constexpr int LA_STAGES = 3;
+constexpr int LA_TABLE = 2 * 4 * 64 * 16;        // bytes behind the stages: decays of P and of what enters the state, four a lane and row of 1 KB
 
 struct LinearOperand {
     const half_t *x;
     long long token, head;               // strides in values
 };
 
-// one of the sums above, over all heads of its result
+// One of the sums above.  A key head has a_inner heads of a (and of the result), or c_inner heads of b and c, whose sums add up; one of the two
+// is 1.
 struct LinearSum {
     LinearOperand a, b, c;
-    half_t *out;                         // dense [T][heads][HD]
+    half_t *out;                         // dense [T][key heads * a_inner][HD]
     const float *first;                  // [sequences][key heads][HD][HD]: state at the walk's beginning, or null
     float *last;                         // the same at its end, or null
-    int heads, inner;                    // heads of the result; heads of b and c that each of them sums over
+    int a_inner, c_inner;
     bool transposed;                     // states are read as their transposes
     float a_mul, b_mul;                  // of a_t S, of what enters the state
 };
@@ -43,14 +46,14 @@ struct LinearWalk {
     const float *log_decay;              // [key heads]
     const int32_t *offsets;              // [sequences + 1]
     float *states;                       // [boundaries][key heads][HD][HD]: between segments, or null where there is none
-    int tokens, sequences, key_heads, group;
-    int shift;                           // a segment has 1 << shift tokens
-    int units, unit_sets, slots;         // of the launch: results' heads, as packed_grid takes them; slots of a head
+    int tokens, sequences, key_heads;
+    int segment;                         // tokens, a multiple of LA_ROWS
+    int head_sets, slots;                // of the launch, as packed_grid takes them; slots of a key head
     float scale;
 };
 
 struct LinearItem {
-    int unit, slot, sequence, begin, n;  // n: of the sequence
+    int head, sequence, begin, n;        // head: key head; n: of the sequence
     int segment, segments;
     bool there;
 };
@@ -64,17 +67,18 @@ __device__ __forceinline__ int linear_offset(const LinearWalk &p, int b)
 // Slot floor(offset / segment) + b is the first of sequence b, ascending in b, and an empty sequence has one: 64 lanes search together.
 __device__ __forceinline__ LinearItem linear_item(const LinearWalk &p, int block)
 {
-    LinearItem item{0, 0, 0, 0, 0, 0, 0, false};
+    LinearItem item{0, 0, 0, 0, 0, 0, false};
     const int x = block & 7, t = block >> 3;
-    const int share = 8 / p.unit_sets, in_set = p.units / p.unit_sets;
-    item.unit = x / share * in_set + t % in_set;
-    item.slot = t / in_set * share + x % share;
-    if (item.slot >= p.slots) return item;
+    const int share = 8 / p.head_sets, in_set = p.key_heads / p.head_sets;
+    item.head = x / share * in_set + t % in_set;
+    const int slot = t / in_set * share + x % share;
+    if (slot >= p.slots) return item;
+    const unsigned length = (unsigned)p.segment;
     const int l = lane_id();
     int first = 0, count = p.sequences;
     while (true) {
         const int stride = (count + 63) / 64, b = first + l * stride;
-        const bool before = b < first + count && (linear_offset(p, b) >> p.shift) + b <= item.slot;
+        const bool before = b < first + count && (int)((unsigned)linear_offset(p, b) / length) + b <= slot;
         const int seen = __popcll(__builtin_amdgcn_ballot_w64(before));
         const int skip = (seen > 0 ? seen - 1 : 0) * stride;
         first += skip;
@@ -85,21 +89,23 @@ __device__ __forceinline__ LinearItem linear_item(const LinearWalk &p, int block
     item.begin = __builtin_amdgcn_readfirstlane(linear_offset(p, item.sequence));
     const int end = __builtin_amdgcn_readfirstlane(linear_offset(p, item.sequence + 1));
     item.n = end > item.begin ? end - item.begin : 0;
-    item.segment = item.slot - ((item.begin >> p.shift) + item.sequence);
-    item.segments = item.n > 0 ? (item.n + (1 << p.shift) - 1) >> p.shift : 1;
+    item.segment = slot - ((int)((unsigned)item.begin / length) + item.sequence);
+    item.segments = item.n > 0 ? (int)(((unsigned)item.n + length - 1) / length) : 1;
     item.there = item.segment >= 0 && item.segment < item.segments;
     return item;
 }
 
-// Place of the state between segments j - 1 and j of a sequence, j >= 1.  A sequence's last boundary has floor((n - 1) / segment) =: j, and
+// Place of the state between segments j - 1 and j of a sequence, j >= 1.  A sequence's last boundary has j = floor((n - 1) / segment), and
 // floor(begin / segment) + j <= floor((begin + n - 1) / segment), so that the next sequence's first lies behind it and all are below
 // (tokens - 1) / segment.
 __device__ __forceinline__ size_t linear_boundary(const LinearWalk &p, int begin, int j, int key_head)
 {
-    return (size_t)((begin >> p.shift) + j - 1) * p.key_heads + key_head;
+    return ((size_t)((unsigned)begin / (unsigned)p.segment) + j - 1) * p.key_heads + key_head;
 }
 
-// exp(log_decay e): decays of e tokens
+// Decay of e tokens.  The exponent is made anew from e, not by products of decays: it is off by 2^-23 of itself, x, and what it
+// belongs to by x 2^-23 of 2^-x of what has not decayed.
+__device__ __forceinline__ float linear_log2(float log_decay) { return log_decay * 1.4426950408889634f; }
 __device__ __forceinline__ float linear_power(float log2_decay, int e) { return e == 0 ? 1.f : at_exp2(log2_decay * (float)e); }
 
 __device__ __forceinline__ float wave_most(float x)
@@ -108,18 +114,24 @@ __device__ __forceinline__ float wave_most(float x)
     for (int d = 1; d < WAVE; d *= 2) x = fmaxf(x, __int_as_float(__builtin_amdgcn_ds_bpermute((lane_id() ^ d) << 2, __float_as_int(x))));
     return x;
 }
-// 2^e that brings a finite x > 0 to 2^9 .. 2^10
-__device__ __forceinline__ float lift_of(float most)
+// 2^e that brings a finite x > 0 to 2^(to - 1) .. 2^to
+__device__ __forceinline__ float lift_of(float most, int to)
 {
-    const int e = 10 - __builtin_amdgcn_frexp_expf(most);
+    const int e = to - __builtin_amdgcn_frexp_expf(most);
     return __builtin_ldexpf(1.f, e > 120 ? 120 : e < -120 ? -120 : e);
 }
+__device__ __forceinline__ float larger(float most, float x)      // of magnitudes, NaN left out; one instruction
+{
+    return __builtin_amdgcn_fmed3f(most, __builtin_fabsf(x), __builtin_inff());
+}
+__device__ __forceinline__ bool is_finite(float x) { return __builtin_fabsf(x) < __builtin_inff(); }
 
-// Chunks of two or three operands on their way to LDS, fetched by all W waves
-template <int HD, bool WITH_A>
+// Chunks of OPERANDS operands on their way to LDS, fetched by all NW waves of a workgroup
+template <int HD, int OPERANDS, int NW>
 struct LinearTiles {
-    static constexpr int W = HD / 32, TILE = 64 * HD, OPERANDS = WITH_A ? 3 : 2, STAGE = OPERANDS * TILE;
-    static constexpr int PER_OPERAND = HD / 16 / W, REQUESTS = OPERANDS * PER_OPERAND;
+    static constexpr int TILE = 64 * HD, STAGE = OPERANDS * TILE, WAVES = NW;
+    static constexpr int EACH = HD / 16 / NW, REQUESTS = OPERANDS * EACH;        // of a wave
+    static_assert(NW == 2 || NW == 4 || NW == 8, "rows and panels below");
     unsigned lds;                        // of this wave's first request in stage 0
     int row, piece;
     const unsigned char *base[OPERANDS];
@@ -127,11 +139,11 @@ struct LinearTiles {
     __device__ __forceinline__ LinearTiles(unsigned char *lds_raw)
     {
         const int w = wave_id(), l = lane_id(), part = w & 3;
-        lds = __builtin_amdgcn_readfirstlane(lds_address(lds_raw)) + 1024 * part;
+        lds = __builtin_amdgcn_readfirstlane(lds_address(lds_raw)) + 1024 * part + (NW == 8 ? 4096 * (w >> 2) : 0);
         row = 8 * part + (l >> 3);
-        piece = 16 * panel_src_piece(l, part);
+        piece = 16 * panel_src_piece(l, part) + (NW == 8 ? 128 * (w >> 2) : 0);
     }
-    static constexpr size_t lds_bytes() { return (size_t)LA_STAGES * STAGE; }
+    static constexpr size_t lds_bytes() { return (size_t)LA_STAGES * STAGE + LA_TABLE; }
     __device__ __forceinline__ void set(int o, const LinearOperand &x, long long first_token, int head)
     {
         base[o] = (const unsigned char *)(x.x + first_token * x.token + head * x.head);
@@ -143,46 +155,46 @@ struct LinearTiles {
         const unsigned char *from = base[o] + (long long)token * stride[o];
         const unsigned to = lds + (unsigned)(stage * STAGE + o * TILE);
 #pragma unroll
-        for (int i = 0; i < PER_OPERAND; ++i) {
-            // HD 128: four waves, a panel a request; HD 64: two waves, 16 rows a request
-            const int r = W == 4 ? row : row + 16 * i, there = r < valid ? r : valid - 1;
-            dma16(from + (W == 4 ? 128 * i : 0), (unsigned)there * stride[o] + piece, to + (W == 4 ? 4096 * i : 2048 * i));
+        for (int i = 0; i < EACH; ++i) {
+            // a request is 8 rows of a panel of 64 columns: two waves fetch rows 16 apart, four a panel each time, eight both panels at once
+            const int r = NW == 2 ? row + 16 * i : row, there = r < valid ? r : valid - 1;
+            dma16(from + (NW == 4 ? 128 * i : 0), (unsigned)there * stride[o] + piece, to + (NW == 2 ? 2048 * i : 4096 * i));
         }
     }
 };
 
-// TERMS: how many 16-bit values stand for what enters the state (its operand of the product): see linear_terms
-template <int HD, bool BF, int TERMS, bool BACKWARDS, bool RESULT>
-__device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum &sum, const LinearItem &item, int head, unsigned char *lds_raw)
-{
-    using Tiles = LinearTiles<HD, RESULT>;
-    constexpr int KS = HD / 16, DT = HD / 32, B = RESULT ? 1 : 0, C = B + 1;
-    const int w = wave_id(), l = lane_id(), i = l & 31, h = l >> 5;
-    const int key_head = sum.inner > 1 || sum.heads == p.key_heads ? head : head / p.group;
-    const int b_head = sum.inner > 1 ? head * sum.inner : key_head;
-    const float log2_decay = p.log_decay[key_head] * 1.4426950408889634f;
+// What the waves of a workgroup read of a chunk: where their operands lie among the tiles
+struct LinearPlaces {
+    int a, b, c;
+};
 
-    // tokens of the segment, in chunks; step s is chunk s / inner (from the end: BACKWARDS) and head s % inner of b and c
-    const int from = item.segment << p.shift, here = min(item.n - from, 1 << p.shift);
-    const int chunks = (here + LA_ROWS - 1) / LA_ROWS, inner = sum.inner, steps = chunks * inner;
+// TERMS: how many 16-bit values stand for what enters the state (its operand of the product): see linear_terms.  A wave is wave w of
+// HD / 32 that share `sum`; the chunk's tiles are fetched by all waves of the workgroup.
+template <int HD, bool BF, int TERMS, bool BACKWARDS, bool RESULT, class Tiles>
+__device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum &sum, const LinearItem &item, int w, Tiles &tiles,
+                                            const LinearPlaces places, const long long (&inner_step)[Tiles::STAGE / Tiles::TILE], int inner,
+                                            unsigned char *lds_raw)
+{
+    constexpr int KS = HD / 16, DT = HD / 32, OPERANDS = Tiles::STAGE / Tiles::TILE;
+    // the state's decay is put off until it passes this power of two: operands are made of the state, in bf16 with the range of fp32
+    constexpr float PUT_OFF = BF ? 40.f : 5.f;
+    const int l = lane_id(), i = l & 31, h = l >> 5, key_head = item.head;
+    const float log2_decay = linear_log2(p.log_decay[key_head]);
+
+    // tokens of the segment, in chunks; step s is chunk s / inner (from the end: BACKWARDS) and head s % inner
+    const int from = item.segment * p.segment, here = min(item.n - from, p.segment);
+    const int chunks = (here + LA_ROWS - 1) / LA_ROWS, steps = chunks * inner;
     const long long begin = (long long)item.begin + from;
-    Tiles tiles(lds_raw);
-    if (RESULT) tiles.set(0, sum.a, begin, head);
-    tiles.set(B, sum.b, begin, b_head);
-    tiles.set(C, sum.c, begin, b_head);
-    int next = 0, next_inner = 0, next_stage = 0;          // the chunk requested next
+    int next = 0, next_inner = 0, next_stage = 0;          // the step requested next
     auto request = [&]() {
         const int at = LA_ROWS * (BACKWARDS ? chunks - 1 - next : next), valid = min(here - at, LA_ROWS);
 #pragma unroll
-        for (int o = 0; o < Tiles::OPERANDS; ++o) tiles.request(o, at, valid, next_stage);
+        for (int o = 0; o < OPERANDS; ++o) tiles.request(o, at, valid, next_stage);
         next_stage = next_stage == LA_STAGES - 1 ? 0 : next_stage + 1;
-        if (++next_inner == inner) {
-            next_inner = 0;
-            ++next;
-            tiles.base[B] -= 2 * (inner - 1) * sum.b.head, tiles.base[C] -= 2 * (inner - 1) * sum.c.head;
-        } else {
-            tiles.base[B] += 2 * sum.b.head, tiles.base[C] += 2 * sum.c.head;
-        }
+        const bool wrap = ++next_inner == inner;
+#pragma unroll
+        for (int o = 0; o < OPERANDS; ++o) tiles.base[o] += wrap ? (1 - inner) * inner_step[o] : inner_step[o];
+        if (wrap) next_inner = 0, ++next;
     };
     if (steps > 0) request();
     if (steps > 1) request();
@@ -202,6 +214,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             c_at[half] = base + (ct ^ (64u * (w & 1))) + 4096u * (w >> 1);
         }
     }
+    const unsigned a_tile = (unsigned)(places.a * Tiles::TILE), b_tile = (unsigned)(places.b * Tiles::TILE), c_tile = (unsigned)(places.c * Tiles::TILE);
     typedef const h8 __attribute__((address_space(3))) *lds_h8;
     typedef tr4 __attribute__((address_space(3))) *lds_tr4;
     auto rows = [&](unsigned tile, int s) { return *(lds_h8)(uintptr_t)(row_at[s % 4] + (tile + 4096u * (s / 4))); };
@@ -211,10 +224,13 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         return __builtin_shufflevector(__builtin_bit_cast(h4, lo), __builtin_bit_cast(h4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
     };
 
-    // the state: value v of state[t] is row 32 t + swapped16(r), column 32 w + perm16(i), r = 8 (v / 4) + 4 h + v % 4;
-    // times s_mul, a power of two (fp16: operands are made of it)
+    // The state: value v of state[t] is row 32 t + swapped16(r), column 32 w + perm16(i), r = 8 (v / 4) + 4 h + v % 4; times s_mul, a power
+    // of two (fp16), over the decay of the last `age` tokens, which it has not got yet.
     f16v state[DT];
-    float s_mul = 1.f;
+    float s_mul = 1.f, o_mul = 1.f;      // o_mul: of its operands besides, where what enters is much larger than it is
+    int age = 0;
+    float owed = 1.f, ahead = 1.f;       // that decay, and 1 over it
+    bool shrunk = false, dwarfed = false;        // it has got some of it, or was made small for what entered: too small for fp16 operands?
     bool zero = true;                    // nothing entered so far
     const int column = 32 * w + perm16(i);
     auto row_of = [&](int t, int v) { return 32 * t + (v & 3) + 4 * ((v >> 2) & 1) + 8 * h + 16 * (v >> 3); };
@@ -223,12 +239,22 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
-            for (int v = 0; v < 16; ++v) most = fmaxf(most, __builtin_fabsf(state[t][v]));
-        return most;
+            for (int v = 0; v < 16; ++v) most = larger(most, state[t][v]);
+        return wave_most(is_finite(most) ? most : 0.f);
     };
     auto scale_state = [&](float by) {
 #pragma unroll
         for (int t = 0; t < DT; ++t) state[t] *= by;
+    };
+    auto lift_state = [&]() {            // to a size that fp16 operands have room around
+        const float most = state_most();
+        if (most > 0.f) {
+            const float to_mul = fminf(fmaxf(s_mul * lift_of(most, 8), 0x1p-60f), 0x1p60f);
+            scale_state(to_mul / s_mul);
+            s_mul = to_mul;
+        }
+        o_mul = 1.f;
+        dwarfed = false;
     };
     {
         const bool given = BACKWARDS ? item.segment == item.segments - 1 : item.segment == 0;
@@ -258,45 +284,41 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             // arrived: the compiler would wait for them inside the loop, and with them for the chunks on their way
 #pragma unroll
             for (int t = 0; t < DT; ++t) asm volatile("" : "+v"(state[t]));
-            if (!BF) {
-                const float most = wave_most(state_most());
-                if (most > 0.f && most < __builtin_inff()) {
-                    s_mul = lift_of(most);
-                    scale_state(s_mul);
-                }
-            }
+            if (!BF) lift_state();
         }
     }
 
-    // decays inside a chunk of `valid` tokens: of P (and its mask), of what enters the state, of the state's way to this lane's token and
-    // to the chunk's other end
-    float within[16], entering[16], since = 0.f, over = 1.f;
+    // Decays inside a chunk of `valid` tokens, in LDS, where all waves read them: of P (zero where a token does not see the other), of
+    // what enters the state.  In a register: of the state's way to this lane's token.
+    float since = 0.f, p_mul = 1.f;      // p_mul: of P's operands (fp16), a power of two
     int decays_of = 0;
+    f4v *const table = reinterpret_cast<f4v *>(lds_raw + LA_STAGES * Tiles::STAGE) + l;      // [P, state][v / 4][lane]
+    auto sees = [&](int r, int valid) { return BACKWARDS ? r >= i && r < valid : r <= i; };
     auto set_decays = [&](int valid) {
         decays_of = valid;
+        for (int u = wave_id(); u < 8; u += Tiles::WAVES) {
+            f4v x;
 #pragma unroll
-        for (int v = 0; v < 16; ++v) {
-            const int r = 8 * (v >> 2) + 4 * h + (v & 3);
-            if (RESULT) {
-                const bool sees = BACKWARDS ? r >= i && r < valid : r <= i;
-                within[v] = sees ? p.scale * linear_power(log2_decay, BACKWARDS ? r - i : i - r) : 0.f;
+            for (int j = 0; j < 4; ++j) {
+                const int r = 8 * (u & 3) + 4 * h + j;
+                if (u < 4) x[j] = sees(r, valid) ? p.scale * linear_power(log2_decay, BACKWARDS ? r - i : i - r) : 0.f;
+                else x[j] = r < valid ? sum.b_mul * linear_power(log2_decay, BACKWARDS ? r + 1 : valid - 1 - r) : 0.f;
             }
-            entering[v] = r < valid ? sum.b_mul * linear_power(log2_decay, BACKWARDS ? r + 1 : valid - 1 - r) : 0.f;
+            table[64 * u] = x;
         }
         if (RESULT) since = BACKWARDS ? (i < valid ? sum.a_mul * linear_power(log2_decay, valid - 1 - i) : 0.f) : sum.a_mul * linear_power(log2_decay, i + 1);
-        over = linear_power(log2_decay, valid);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
 
     // whether the walk's end state is wanted
     const bool ends = RESULT ? sum.last != nullptr && (BACKWARDS ? item.segment == 0 : item.segment == item.segments - 1) : true;
 
-    h8 aop[KS];
     f16v oacc;
     uint4 result[2];
     int stored = 0;                      // tokens of `result` that are to be stored
     half_t *to = nullptr;
-    const long long width = (long long)sum.heads * HD;
-    half_t *const out = RESULT ? sum.out + begin * width + (long long)head * HD + 32 * w + 16 * h : nullptr;
+    const long long width = (long long)p.key_heads * sum.a_inner * HD;
+    half_t *const out = RESULT ? sum.out + begin * width + (long long)key_head * sum.a_inner * HD + 32 * w + 16 * h : nullptr;
     auto store = [&]() {
         if (i < stored) {
             stg16(to, result[0]);
@@ -314,53 +336,99 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         const int at = LA_ROWS * chunk, valid = min(here - at, LA_ROWS);
         const unsigned tile = (unsigned)(stage * Tiles::STAGE);
         if (valid != decays_of) set_decays(valid);
-        h8 cop[2];
+        const bool last_inner = g == inner - 1;
+        const bool fresh = !BACKWARDS || g == 0;             // of a token and head: the state's part comes first
+        // every head of b and c enters the state, heads of a share one; after the segment's last chunk it may not be needed
+        const bool enters = (BACKWARDS || last_inner) && (ends || step + inner - g < steps);
+        // Operands are read from LDS ahead of the work that hides them; the compiler left to itself waits for each.
+        h8 cop[2], bop[4];
+        f4v decays[4];
+        auto read_b_columns = [&](int t) {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) cop[s] = columns(c_at, tile + C * Tiles::TILE + 2048u * s);
-        if (RESULT && g == 0) {
+            for (int s = 0; s < 4; ++s) bop[s] = columns(b_at[s / 2], tile + b_tile + 4096u * (t / 2) + 2048u * (s % 2));
+        };
+        auto read_decays = [&](int which) {
 #pragma unroll
-            for (int s = 0; s < KS; ++s) aop[s] = rows(tile, s);
-            float up = since;
-            if (!BF && !zero) {          // operands of fp16 from the state
-                const float most = state_most();
-                const bool large = most >= 0x1p15f && most < __builtin_inff();
-                if (__builtin_amdgcn_ballot_w64(large) != 0ull || __builtin_amdgcn_ballot_w64(most >= 0.25f || most != most) == 0ull) {
-                    const float all = wave_most(most < __builtin_inff() ? most : 0.f);
-                    if (all > 0.f) {
-                        const float by = lift_of(all), to_mul = fminf(fmaxf(s_mul * by, 0x1p-120f), 0x1p120f);
-                        scale_state(to_mul / s_mul);
-                        s_mul = to_mul;
-                    }
-                }
-                up = since / s_mul;
-            }
-            oacc = f16v{0};
+            for (int u = 0; u < 4; ++u) decays[u] = table[64 * (4 * which + u)];
+        };
+        if (RESULT) {
+            h8 a[KS], b[KS];
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
-                h8 op;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) op[j] = narrow_16<BF>(state[s / 2][8 * (s % 2) + j]);
-                oacc = mfma_16<BF>(op, aop[s], oacc);
+                a[s] = rows(tile + a_tile, s);
+                b[s] = rows(tile + b_tile, s);
             }
 #pragma unroll
-            for (int v = 0; v < 16; ++v) oacc[v] *= up;
-        }
-        if (RESULT) {
+            for (int s = 0; s < 2; ++s) cop[s] = columns(c_at, tile + c_tile + 2048u * s);
+            read_decays(0);
+            issue_order();
             f16v prob = {0};
+            auto meet = [&](float by) {
+                oacc = f16v{0};
 #pragma unroll
-            for (int s = 0; s < KS; ++s) prob = mfma_16<BF>(rows(tile + B * Tiles::TILE, s), aop[s], prob);
-            float most = 0.f, down = 1.f;
+                for (int s = 0; s < KS; ++s) {
+                    h8 op;
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                prob[v] = within[v] == 0.f ? 0.f : prob[v] * within[v];      // whatever a hidden one is
-                if (!BF) most = fmaxf(most, __builtin_fabsf(prob[v]));
+                    for (int j = 0; j < 8; ++j) op[j] = narrow_16<BF>(state[s / 2][8 * (s % 2) + j] * by);
+                    oacc = mfma_16<BF>(op, a[s], oacc);
+                }
+            };
+            if (fresh) {
+                if (!BF && shrunk) {     // by a part of it: what entered since most often makes up for it
+                    float some = 0.f;
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) some = larger(some, state[0][v]);
+                    if (__builtin_amdgcn_ballot_w64(some >= 16.f) == 0ull) lift_state();
+                    shrunk = false;
+                }
+                if (!BF && dwarfed) {
+                    const float left = state_most();
+                    o_mul = left > 0.f && left < 16.f ? fminf(lift_of(left, 8), 0x1p60f) : 1.f;
+                    dwarfed = o_mul != 1.f;
+                }
+                oacc = f16v{0};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    prob = mfma_16<BF>(b[s], a[s], prob);
+                    h8 op;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) op[j] = narrow_16<BF>(state[s / 2][8 * (s % 2) + j]);
+                    oacc = mfma_16<BF>(op, a[s], oacc);
+                }
+                if (!BF) {               // a state that has outgrown fp16 or is too small for it, or infinities that it has
+                    float sure = 0.f;
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(oacc[v]);
+                    const bool broken = __builtin_amdgcn_ballot_w64(!is_finite(sure)) != 0ull;
+                    if (broken) lift_state();
+                    if (broken || o_mul != 1.f) meet(o_mul);
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) prob = mfma_16<BF>(b[s], a[s], prob);
             }
-            if (!BF) {
-                most = fmaxf(most, at_lane_xor32(most));
-                const float mul = most > 0.f && most < __builtin_inff() ? lift_of(most) : 1.f;
-                down = 1.f / mul;
+            issue_order();
+            if (enters) read_b_columns(0);
+            issue_order();
+            float most = 0.f;
 #pragma unroll
-                for (int v = 0; v < 16; ++v) prob[v] *= mul;
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    prob[4 * u + j] *= BF ? decays[u][j] : decays[u][j] * p_mul;
+                    if (!BF) most = larger(most, prob[4 * u + j]);
+                }
+            if (!BF) {
+                const bool large = most >= 0x1p15f, fair = most >= 1.f;
+                if (__builtin_amdgcn_ballot_w64(large) != 0ull || __builtin_amdgcn_ballot_w64(fair) == 0ull) {
+                    most = wave_most(is_finite(most) ? most : 0.f);
+                    if (most > 0.f) {
+                        const float to_mul = fminf(fmaxf(p_mul * lift_of(most, 8), 0x1p-60f), 0x1p60f), by = to_mul / p_mul;
+                        p_mul = to_mul;
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) prob[v] *= by;
+                    }
+                }
             }
             h8 pop[2];
 #pragma unroll
@@ -369,53 +437,89 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             float sure = 0.f;
 #pragma unroll
             for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
+            if (enters) read_decays(1);
+            issue_order();
 #pragma unroll
             for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(part[v]);
-            if (__builtin_amdgcn_ballot_w64(!(sure < __builtin_inff())) != 0ull) {
-                // An infinity or a NaN in c: zero times it is NaN, also for tokens that do not see it.  Left out of the product, it
-                // makes NaN of its column for those that do.
+            if (__builtin_amdgcn_ballot_w64(!is_finite(sure)) != 0ull) {
+                // An infinity or a NaN: zero times it is NaN, also for tokens that do not see it.  Weights of hidden ones are put to zero,
+                // and left out of c it makes NaN of its column for those that see it.
+#pragma unroll
+                for (int v = 0; v < 16; ++v) {
+                    const float weight = sees(8 * (v >> 2) + 4 * h + (v & 3), valid) ? prob[v] : 0.f;
+                    pop[v >> 3][v & 7] = narrow_16<BF>(weight);
+                }
                 h8 clean[1][2] = {{cop[0], cop[1]}};
                 take_out_not_finite<BF>(clean);
                 part = f16v{0};
 #pragma unroll
                 for (int s = 0; s < 2; ++s) part = mfma_16<BF>(clean[0][s], pop[s], part);
-                const unsigned first = __builtin_amdgcn_readfirstlane(lds_address(lds_raw)) + tile + C * Tiles::TILE + 4096u * (w >> 1);
+                const unsigned first = __builtin_amdgcn_readfirstlane(lds_address(lds_raw)) + tile + c_tile + 4096u * (w >> 1);
 #pragma unroll 1
                 for (int r = 0; r < valid; ++r) {
-                    const bool sees = BACKWARDS ? r >= i : r <= i;
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const h8 x = *(lds_h8)(uintptr_t)(first + 128u * r + 16u * (unsigned)((4 * (w & 1) + 2 * h + half) ^ panel_swizzle(r)));
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const float value = widen_16<BF>(x[j]);
-                            if (sees && !(__builtin_fabsf(value) < __builtin_inff())) part[8 * half + j] = __builtin_nanf("");
+                            const half_t one = x[j];
+                            if (sees(r, valid) && !is_finite(widen_16<BF>(one))) part[8 * half + j] = __builtin_nanf("");
                         }
                     }
                 }
             }
+            const float down = BF ? 1.f : 1.f / p_mul;
+            if (fresh) {
+                const float up = since * owed * (BF ? 1.f : 1.f / (s_mul * o_mul));
 #pragma unroll
-            for (int v = 0; v < 16; ++v) oacc[v] = BF ? oacc[v] + part[v] : __builtin_fmaf(part[v], down, oacc[v]);
+                for (int v = 0; v < 16; ++v) oacc[v] = BF ? __builtin_fmaf(oacc[v], up, part[v]) : __builtin_fmaf(part[v], down, oacc[v] * up);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) oacc[v] = BF ? oacc[v] + part[v] : __builtin_fmaf(part[v], down, oacc[v]);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) cop[s] = columns(c_at, tile + c_tile + 2048u * s);
+            read_decays(1);
+            read_b_columns(0);
+            issue_order();
         }
-        if (ends || step + inner - g < steps) {            // the state is needed once more
-            if (g == 0 && !zero) scale_state(over);
-            float x[2][8], most = 0.f;
+        if (enters) {
+            if (!BACKWARDS || g == 0) {
+                age = zero ? 0 : age + valid;
+                owed = linear_power(log2_decay, age);
+                if (age > 0 && !(__builtin_fabsf(log2_decay * (float)age) <= PUT_OFF)) {
+                    scale_state(owed);
+                    age = 0;
+                    owed = 1.f;
+                    shrunk = true;
+                }
+                ahead = age == 0 ? 1.f : at_exp2(-log2_decay * (float)age);
+            }
+            float with = ahead * s_mul, x[2][8], most = 0.f;
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int u = 0; u < 4; ++u)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const half_t one = cop[s][j];
-                    x[s][j] = widen_16<BF>(one) * entering[8 * s + j];
-                    if (!BF) most = fmaxf(most, __builtin_fabsf(x[s][j]));
+                for (int j = 0; j < 4; ++j) {
+                    const half_t one = cop[u >> 1][4 * (u & 1) + j];
+                    float &to_enter = x[u >> 1][4 * (u & 1) + j];
+                    to_enter = widen_16<BF>(one) * (decays[u][j] * with);
+                    if (!BF) most = larger(most, to_enter);
                 }
             if (!BF) {
-                const bool fits = most * s_mul < 0x1p15f || !(most < __builtin_inff());
-                if (zero || __builtin_amdgcn_ballot_w64(!fits) != 0ull) {
-                    const float all = wave_most(most < __builtin_inff() ? most : 0.f);
+                if (zero || __builtin_amdgcn_ballot_w64(most >= 0x1p15f) != 0ull) {
+                    const float all = wave_most(is_finite(most) ? most : 0.f);
                     if (all > 0.f) {
-                        const float to_mul = lift_of(all);
-                        if (!zero) scale_state(to_mul / s_mul);
+                        const float to_mul = fminf(fmaxf(s_mul * lift_of(all, 10), 0x1p-60f), 0x1p60f), by = to_mul / s_mul;
                         s_mul = to_mul;
+                        if (!zero) {
+                            scale_state(by);
+                            dwarfed = true;
+                        }
+#pragma unroll
+                        for (int s = 0; s < 2; ++s)
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) x[s][j] *= by;
                     }
                 }
             }
@@ -425,7 +529,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    float left = BF ? x[s][j] : x[s][j] * s_mul;
+                    float left = x[s][j];
 #pragma unroll
                     for (int e = 0; e < TERMS; ++e) {
                         cw[e][s][j] = narrow_16<BF>(left);
@@ -434,31 +538,32 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                     }
                 }
 #pragma unroll
-            for (int t = 0; t < DT; ++t)
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    const h8 bop = columns(b_at[t % 2], tile + B * Tiles::TILE + 4096u * (t / 2) + 2048u * s);
-#pragma unroll
-                    for (int e = 0; e < TERMS; ++e) state[t] = mfma_16<BF>(bop, cw[e][s], state[t]);
+            for (int t = 0; t < DT; t += 2) {
+                const h8 now[4] = {bop[0], bop[1], bop[2], bop[3]};
+                if (t + 2 < DT) {
+                    read_b_columns(t + 2);
+                    issue_order();
                 }
+#pragma unroll
+                for (int e = 0; e < TERMS; ++e)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) state[t + s / 2] = mfma_16<BF>(now[s], cw[e][s % 2], state[t + s / 2]);
+            }
         }
         stage = stage == LA_STAGES - 1 ? 0 : stage + 1;
-        if (++g == inner) {
-            if (RESULT) {
-                pack16<BF>(oacc, result[0], result[1]);
-                to = out + (long long)(at + i) * width;
-                stored = valid;
-            }
-            g = 0;
-            chunk += BACKWARDS ? -1 : 1;
+        if (RESULT && (!BACKWARDS || last_inner)) {
+            pack16<BF>(oacc, result[0], result[1]);
+            to = out + (long long)(at + i) * width + (BACKWARDS ? 0 : g * HD);
+            stored = valid;
         }
+        g = last_inner ? 0 : g + 1;
+        if (last_inner) chunk += BACKWARDS ? -1 : 1;
     }
     if (RESULT) store();
     if (ends) {
         float *dst = RESULT ? sum.last + ((size_t)item.sequence * p.key_heads + key_head) * HD * HD
                             : p.states + linear_boundary(p, item.begin, BACKWARDS ? item.segment : item.segment + 1, key_head) * HD * HD;
-        if (RESULT && !BACKWARDS && sum.heads != p.key_heads && head % p.group != 0) return;
-        const float down = BF ? 1.f : 1.f / s_mul;
+        const float down = owed * (BF ? 1.f : 1.f / s_mul);
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -478,42 +583,52 @@ __device__ __forceinline__ void linear_clear(const LinearWalk &p, int part, half
     clear(tail, p.tokens);
 }
 
+template <int HD> using ResultTiles = LinearTiles<HD, 3, HD / 32>;
+template <int HD> using StateTiles = LinearTiles<HD, 2, HD / 32>;
+template <int HD> using PairSumTiles = LinearTiles<HD, 4, HD / 16>;
+
+// the forward pass, or dq
 template <int HD, bool BF, int TERMS>
-__global__ __launch_bounds__(2 * HD, 2) void linear_forward_kernel(LinearWalk p, LinearSum sum)
+__global__ __launch_bounds__(2 * HD, 2) void linear_result_kernel(LinearWalk p, LinearSum sum)
 {
     extern __shared__ __align__(16) unsigned char lds_raw[];
-    const int cells = packed_grid(p.units, p.unit_sets, p.slots);
-    if ((int)blockIdx.x >= cells) return linear_clear(p, (int)blockIdx.x - cells, sum.out, (long long)sum.heads * HD);
+    const int cells = packed_grid(p.key_heads, p.head_sets, p.slots);
+    if ((int)blockIdx.x >= cells) return linear_clear(p, (int)blockIdx.x - cells, sum.out, (long long)p.key_heads * sum.a_inner * HD);
     const LinearItem item = linear_item(p, (int)blockIdx.x);
     if (!item.there) return;
-    linear_walk<HD, BF, TERMS, false, true>(p, sum, item, item.unit, lds_raw);
+    const long long begin = (long long)item.begin + item.segment * p.segment;
+    ResultTiles<HD> tiles(lds_raw);
+    tiles.set(0, sum.a, begin, item.head * sum.a_inner);
+    tiles.set(1, sum.b, begin, item.head);
+    tiles.set(2, sum.c, begin, item.head);
+    const long long inner_step[3] = {2 * sum.a.head, 0, 0};
+    linear_walk<HD, BF, TERMS, false, true>(p, sum, item, wave_id(), tiles, LinearPlaces{0, 1, 2}, inner_step, sum.a_inner, lds_raw);
 }
 
-// the three gradients: units are the query heads (dq), then for each key head dv and dk
-struct LinearGradients {
-    LinearSum dq, dv, dk;
-    const float *states;                 // those of the forward pass
-};
+// dv by the first half of the waves, dk by the others: a, b, c of dv are K, Q, dO, of dk V, dO, Q
 template <int HD, bool BF, int TERMS>
-__global__ __launch_bounds__(2 * HD, 2) void linear_backward_kernel(LinearWalk p, LinearGradients g)
+__global__ __launch_bounds__(4 * HD, 2) void linear_keys_kernel(LinearWalk p, LinearSum dv, LinearSum dk)
 {
     extern __shared__ __align__(16) unsigned char lds_raw[];
-    const int cells = packed_grid(p.units, p.unit_sets, p.slots);
+    const int cells = packed_grid(p.key_heads, p.head_sets, p.slots);
     if ((int)blockIdx.x >= cells) {
-        const int part = (int)blockIdx.x - cells;
-        linear_clear(p, part, g.dq.out, (long long)g.dq.heads * HD);
-        linear_clear(p, part, g.dv.out, (long long)g.dv.heads * HD);
-        return linear_clear(p, part, g.dk.out, (long long)g.dk.heads * HD);
+        linear_clear(p, (int)blockIdx.x - cells, dv.out, (long long)p.key_heads * HD);
+        return linear_clear(p, (int)blockIdx.x - cells, dk.out, (long long)p.key_heads * HD);
     }
     const LinearItem item = linear_item(p, (int)blockIdx.x);
     if (!item.there) return;
-    if (item.unit < g.dq.heads) {
-        p.states = const_cast<float *>(g.states);
-        return linear_walk<HD, BF, 2, false, true>(p, g.dq, item, item.unit, lds_raw);
-    }
-    const int at = item.unit - g.dq.heads;
-    const bool values = (at & 1) == 0;
-    linear_walk<HD, BF, TERMS, true, true>(p, values ? g.dv : g.dk, item, at >> 1, lds_raw);
+    const long long begin = (long long)item.begin + item.segment * p.segment;
+    PairSumTiles<HD> tiles(lds_raw);
+    tiles.set(0, dv.a, begin, item.head);
+    tiles.set(1, dk.a, begin, item.head);
+    tiles.set(2, dv.b, begin, item.head * dv.c_inner);
+    tiles.set(3, dv.c, begin, item.head * dv.c_inner);
+    const long long inner_step[4] = {0, 0, 2 * dv.b.head, 2 * dv.c.head};
+    const int w = wave_id(), half = w / (HD / 32);
+    const LinearPlaces places = half == 0 ? LinearPlaces{0, 2, 3} : LinearPlaces{1, 3, 2};
+    LinearSum sum = dv;
+    if (half != 0) sum = dk;
+    linear_walk<HD, BF, TERMS, true, true>(p, sum, item, w % (HD / 32), tiles, places, inner_step, dv.c_inner, lds_raw);
 }
 
 // every segment's own sum, of those that have a neighbour behind (BACKWARDS: in front)
@@ -523,63 +638,72 @@ __global__ __launch_bounds__(2 * HD, 2) void linear_segments_kernel(LinearWalk p
     extern __shared__ __align__(16) unsigned char lds_raw[];
     const LinearItem item = linear_item(p, (int)blockIdx.x);
     if (!item.there || (BACKWARDS ? item.segment == 0 : item.segment == item.segments - 1)) return;
-    linear_walk<HD, BF, TERMS, BACKWARDS, false>(p, sum, item, item.unit, lds_raw);
+    const long long begin = (long long)item.begin + item.segment * p.segment;
+    StateTiles<HD> tiles(lds_raw);
+    tiles.set(0, sum.b, begin, item.head * sum.c_inner);
+    tiles.set(1, sum.c, begin, item.head * sum.c_inner);
+    const long long inner_step[2] = {2 * sum.b.head, 2 * sum.c.head};
+    linear_walk<HD, BF, TERMS, BACKWARDS, false>(p, sum, item, wave_id(), tiles, LinearPlaces{0, 0, 1}, inner_step, sum.c_inner, lds_raw);
 }
 
-// the running sum over the segments of a sequence, in place: what each segment begins with
+// The running sum over the segments of a sequence, in place: what each segment begins with.  A lane has four values of a state; the
+// segments' sums are requested RUN_AHEAD at a time.
+constexpr int RUN_AHEAD = 8;
 template <bool BACKWARDS>
 __global__ __launch_bounds__(256) void linear_running_kernel(LinearWalk p, const float *__restrict__ first, int square)
 {
     const int b = (int)blockIdx.z, key_head = (int)blockIdx.y;
-    const int begin = linear_offset(p, b), n = linear_offset(p, b + 1) - begin, segments = (n + (1 << p.shift) - 1) >> p.shift;
-    if (n <= 0 || segments < 2) return;
-    const float log2_decay = p.log_decay[key_head] * 1.4426950408889634f;
+    const int begin = linear_offset(p, b), n = linear_offset(p, b + 1) - begin;
+    if (n <= p.segment) return;
+    const int bounds = (n - 1) / p.segment;
+    const float log2_decay = linear_log2(p.log_decay[key_head]);
     const size_t at = 4 * ((size_t)blockIdx.x * 256 + threadIdx.x), stride = (size_t)p.key_heads * square;
-    float *sums = p.states + linear_boundary(p, begin, 1, key_head) * square + at;       // of boundary 1
+    float *sums = p.states + linear_boundary(p, begin, 1, key_head) * square + at;
     f4v run = {0, 0, 0, 0};
     if (first != nullptr) run = *reinterpret_cast<const f4v *>(first + ((size_t)b * p.key_heads + key_head) * square + at);
-    const float whole = linear_power(log2_decay, 1 << p.shift), rest = linear_power(log2_decay, n - ((segments - 1) << p.shift));
-    auto place = [&](int j) { return reinterpret_cast<f4v *>(sums + (size_t)(BACKWARDS ? segments - 2 - j : j) * stride); };
-    f4v own = *place(0);
-    for (int j = 0; j + 1 < segments; ++j) {
-        const f4v after = *place(j + 2 < segments ? j + 1 : j);
-        run = run * (BACKWARDS && j == 0 ? rest : whole) + own;
-        *place(j) = run;
-        own = after;
+    const float whole = linear_power(log2_decay, p.segment), rest = linear_power(log2_decay, n - bounds * p.segment);
+    auto place = [&](int j) { return reinterpret_cast<f4v *>(sums + (size_t)(BACKWARDS ? bounds - 1 - j : j) * stride); };
+    for (int j0 = 0; j0 < bounds; j0 += RUN_AHEAD) {
+        f4v own[RUN_AHEAD];
+#pragma unroll
+        for (int e = 0; e < RUN_AHEAD; ++e) own[e] = *place(j0 + e < bounds ? j0 + e : bounds - 1);
+#pragma unroll
+        for (int e = 0; e < RUN_AHEAD; ++e) {
+            if (j0 + e >= bounds) break;
+            run = run * (BACKWARDS && j0 + e == 0 ? rest : whole) + own[e];
+            *place(j0 + e) = run;
+        }
     }
 }
 
-LinearWalk walk_of(const LinearArgs &a)
+LinearWalk walk_of(const LinearArgs &a, float *states)
 {
     LinearWalk p;
-    p.log_decay = a.log_decay, p.offsets = a.offsets;
-    p.states = nullptr;
-    p.tokens = a.tokens, p.sequences = a.sequences, p.key_heads = a.key_heads, p.group = a.heads / a.key_heads;
-    p.shift = __builtin_ctz((unsigned)a.segment);
+    p.log_decay = a.log_decay, p.offsets = a.offsets, p.states = states;
+    p.tokens = a.tokens, p.sequences = a.sequences, p.key_heads = a.key_heads;
+    p.segment = a.segment;
     p.slots = packed_slots(a.tokens, a.sequences, a.segment);
-    p.units = p.unit_sets = 0;
+    p.head_sets = packed_head_sets(a.key_heads);
     p.scale = a.scale;
     return p;
 }
 LinearOperand operand(const void *x, long long token, long long head) { return LinearOperand{(const half_t *)x, token, head}; }
 
-template <class Kernel, class... Args>
-hipError_t run_linear(Kernel kernel, LinearWalk p, int units, int clearing, int hd, size_t lds, hipStream_t st, const Args &...args)
+template <class Kernel, class... Sums>
+hipError_t run_linear(Kernel kernel, const LinearWalk &p, int clearing, int threads, size_t lds, hipStream_t st, const Sums &...sums)
 {
     if (lds > 65536) {
         const hipError_t err = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (err != hipSuccess) return err;
     }
-    p.units = units;
-    p.unit_sets = packed_head_sets(units);
-    kernel<<<packed_grid(units, p.unit_sets, p.slots) + clearing, 2 * hd, lds, st>>>(p, args...);
+    kernel<<<packed_grid(p.key_heads, p.head_sets, p.slots) + clearing, threads, lds, st>>>(p, sums...);
     return hipGetLastError();
 }
 
 template <int HD, bool BF, int TERMS, bool BACKWARDS>
-hipError_t segment_states(LinearWalk p, const LinearSum &sum, const float *first, hipStream_t st)
+hipError_t segment_states(const LinearWalk &p, const LinearSum &sum, const float *first, hipStream_t st)
 {
-    const hipError_t err = run_linear(linear_segments_kernel<HD, BF, TERMS, BACKWARDS>, p, p.key_heads, 0, HD, LinearTiles<HD, false>::lds_bytes(), st, sum);
+    const hipError_t err = run_linear(linear_segments_kernel<HD, BF, TERMS, BACKWARDS>, p, 0, 2 * HD, StateTiles<HD>::lds_bytes(), st, sum);
     if (err != hipSuccess) return err;
     linear_running_kernel<BACKWARDS><<<dim3(HD * HD / 1024, p.key_heads, p.sequences), 256, 0, st>>>(p, first, HD * HD);
     return hipGetLastError();
@@ -588,36 +712,32 @@ hipError_t segment_states(LinearWalk p, const LinearSum &sum, const float *first
 template <int HD, bool BF, int TERMS>
 hipError_t forward(const LinearArgs &a, hipStream_t st)
 {
-    LinearWalk p = walk_of(a);
-    p.states = a.states;
-    LinearSum sum{operand(a.q, a.q_token, a.q_head), operand(a.k, a.k_token, a.k_head), operand(a.v, a.v_token, a.v_head), (half_t *)a.out,
-                  a.first, a.last, a.heads, 1, false, a.scale, 1.f};
+    const LinearWalk p = walk_of(a, a.states);
+    const LinearSum sum{operand(a.q, a.q_token, a.q_head), operand(a.k, a.k_token, a.k_head), operand(a.v, a.v_token, a.v_head), (half_t *)a.out,
+                        a.first, a.last, a.heads / a.key_heads, 1, false, a.scale, 1.f};
     if (a.tokens > a.segment) {
-        LinearSum own = sum;
-        own.heads = a.key_heads;
-        const hipError_t err = segment_states<HD, BF, TERMS, false>(p, own, a.first, st);
+        const hipError_t err = segment_states<HD, BF, TERMS, false>(p, sum, a.first, st);
         if (err != hipSuccess) return err;
     }
-    return run_linear(linear_forward_kernel<HD, BF, TERMS>, p, a.heads, PACKED_CLEARING, HD, LinearTiles<HD, true>::lds_bytes(), st, sum);
+    return run_linear(linear_result_kernel<HD, BF, TERMS>, p, PACKED_CLEARING, 2 * HD, ResultTiles<HD>::lds_bytes(), st, sum);
 }
 
 template <int HD, bool BF, int TERMS>
 hipError_t backward(const LinearArgs &a, hipStream_t st)
 {
-    LinearWalk p = walk_of(a);
-    p.states = a.back_states;
     const int group = a.heads / a.key_heads;
     const LinearOperand q = operand(a.q, a.q_token, a.q_head), k = operand(a.k, a.k_token, a.k_head), v = operand(a.v, a.v_token, a.v_head),
                         g = operand(a.dout, a.g_token, a.g_head);
-    LinearGradients grads{LinearSum{g, v, k, (half_t *)a.dq, a.first, nullptr, a.heads, 1, true, a.scale, 1.f},
-                          LinearSum{k, q, g, (half_t *)a.dv, a.dlast, a.dfirst, a.key_heads, group, false, 1.f, a.scale},
-                          LinearSum{v, g, q, (half_t *)a.dk, a.dlast, nullptr, a.key_heads, group, true, 1.f, a.scale}, a.states};
+    const LinearSum dq{g, v, k, (half_t *)a.dq, a.first, nullptr, group, 1, true, a.scale, 1.f},
+        dv{k, q, g, (half_t *)a.dv, a.dlast, a.dfirst, 1, group, false, 1.f, a.scale}, dk{v, g, q, (half_t *)a.dk, a.dlast, nullptr, 1, group, true, 1.f, a.scale};
+    hipError_t err = run_linear(linear_result_kernel<HD, BF, 2>, walk_of(a, a.states), PACKED_CLEARING, 2 * HD, ResultTiles<HD>::lds_bytes(), st, dq);
+    if (err != hipSuccess) return err;
+    const LinearWalk p = walk_of(a, a.back_states);
     if (a.tokens > a.segment) {
-        const hipError_t err = segment_states<HD, BF, TERMS, true>(p, grads.dv, a.dlast, st);
+        err = segment_states<HD, BF, TERMS, true>(p, dv, a.dlast, st);
         if (err != hipSuccess) return err;
     }
-    return run_linear(linear_backward_kernel<HD, BF, TERMS>, p, a.heads + 2 * a.key_heads, PACKED_CLEARING, HD, LinearTiles<HD, true>::lds_bytes(), st,
-                      grads);
+    return run_linear(linear_keys_kernel<HD, BF, TERMS>, p, PACKED_CLEARING, 4 * HD, PairSumTiles<HD>::lds_bytes(), st, dv, dk);
 }
 
 }  // namespace
@@ -629,19 +749,21 @@ static int linear_terms(const LinearArgs &a, const void *states_out) { return a.
 bool linear_fits(const LinearArgs &a)
 {
     const long long slots = (long long)a.tokens / a.segment + a.sequences + 7;
-    return ((long long)(a.heads + 2 * a.key_heads) * slots + PACKED_CLEARING) * 2 * a.head_dim < (1ll << 32) && a.sequences <= 65535;
+    return ((long long)a.key_heads * slots + PACKED_CLEARING) * 4 * a.head_dim < (1ll << 32) && a.sequences <= 65535;
 }
 size_t linear_workspace_bytes(const LinearArgs &a)
 {
     if (a.tokens <= a.segment) return 0;
     return sizeof(float) * (size_t)((a.tokens - 1) / a.segment) * a.key_heads * a.head_dim * a.head_dim;
 }
-int linear_segment(int tokens, int sequences, int heads, int head_dim)
+// Segments of which every compute unit has its workgroups at once (two at head dim 128, four at 64), no more: a second generation would leave
+// most of the machine idle at its end, and every boundary is a state to write and read.
+int linear_segment(int tokens, int sequences, int key_heads, int head_dim)
 {
-    (void)sequences, (void)head_dim;
-    int segment = 256;
-    while (segment < 4096 && (long long)tokens * heads / segment > 1024) segment *= 2;
-    return segment;
+    const int room = 512 * (head_dim == 64 ? 2 : 1) / key_heads;
+    const int parts = room - (sequences < room / 2 ? sequences : room / 2);
+    const int segment = ((tokens + (parts > 0 ? parts : 1) - 1) / (parts > 0 ? parts : 1) + LA_ROWS - 1) / LA_ROWS * LA_ROWS;
+    return segment < 256 ? 256 : segment > 8192 ? 8192 : segment;
 }
 
 hipError_t launch_linear_forward(const LinearArgs &a, hipStream_t st)

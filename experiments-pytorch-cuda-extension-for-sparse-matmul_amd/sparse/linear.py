@@ -80,7 +80,7 @@ def run_forward(q, k, v, log_decay, offsets, scale, states, return_states):
             last.zero_() if states is None else last.copy_(states)
         return out.zero_(), last, torch.empty(0, dtype=torch.float32, device=q.device)
     q, k, v, states = rows_of(q), rows_of(k), rows_of(v), _dense(states)
-    segment = _k.lib.bsa_linear_attention_segment(tokens, offsets.numel() - 1, heads, dim)
+    segment = _k.lib.bsa_linear_attention_segment(tokens, offsets.numel() - 1, k.size(1), dim)
     between, need = _between(k, tokens, segment)
     with _k.on_device(q.device):
         _k.check(_k.lib.bsa_linear_attention_forward(
@@ -100,7 +100,7 @@ def run_backward(q, k, v, states, log_decay, offsets, between, dout, dlast, scal
         raise ValueError(f"the gradient of {q.dtype} {tuple(q.shape)} on {q.device} came back as {dout.dtype} {tuple(dout.shape)} on {dout.device}")
     if dlast is not None:
         check_states(dlast, state_shape(k, offsets), q.device, "the gradient of the states")
-    segment = _k.lib.bsa_linear_attention_segment(max(tokens, 1), max(offsets.numel() - 1, 1), heads, dim)
+    segment = _k.lib.bsa_linear_attention_segment(max(tokens, 1), max(offsets.numel() - 1, 1), k.size(1), dim)
     behind, need = _between(k, tokens, segment)
     if between.dtype != torch.float32 or between.numel() != behind.numel() or between.device != q.device or not between.is_contiguous():
         raise ValueError("the saved states came back as others")

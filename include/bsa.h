@@ -477,7 +477,7 @@ int bsa_cached_attention(int dtype, int cache_dtype, const void *q, const void *
  *                    S_n is its S_0.  dlast, dfirst: their gradients, dlast NULL: zero
  *   states           float, bsa_linear_attention_states_bytes: the states between the segments of long sequences, written by the
  *                    forward call, read by the backward call, which has scratch of the same size of its own.  0 bytes up to `segment` tokens
- *   segment          tokens, a power of two from 32 on; bsa_linear_attention_segment says which fills the machine.  Both calls have to have
+ *   segment          tokens, a multiple of 32; bsa_linear_attention_segment says which fills the machine.  Both calls have to have
  *                    the same.  Results of different segments differ by rounding.
  * Tokens outside every sequence get zeros.  States are fp32; results are the same bits in every call.  An infinity or a NaN
  * in a token makes what it reaches, of its own token and later ones, something that is no finite number.
@@ -488,7 +488,7 @@ int bsa_cached_attention(int dtype, int cache_dtype, const void *q, const void *
  *   states float [state_slots, key_heads, head_dim, head_dim];  slots: device int32 [batch], the sequence's state.  Sequences whose slot is
  *   negative or not below state_slots get zeros and change nothing.  No two sequences of a call may have the same slot.
  */
-int bsa_linear_attention_segment(int tokens, int sequences, int heads, int head_dim);
+int bsa_linear_attention_segment(int tokens, int sequences, int key_heads, int head_dim);
 size_t bsa_linear_attention_states_bytes(int tokens, int key_heads, int head_dim, int segment);
 int bsa_linear_attention_forward(int dtype, const void *q, const void *k, const void *v, void *out, const float *log_decay,
                                  const int32_t *offsets, const float *first, float *last, float *states, size_t states_bytes, int segment,
