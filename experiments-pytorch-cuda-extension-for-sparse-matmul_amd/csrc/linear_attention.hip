@@ -23,7 +23,9 @@ namespace {
 
 constexpr int LA_ROWS = 32;              // tokens of a chunk
 constexpr int LA_STAGES = 3;
-constexpr int LA_TABLE = 2 * 4 * 64 * 16;        // bytes behind the stages: decays of P and of what enters the state, four a lane and row of 1 KB
+// Behind the stages, floats: decays of P by how many tokens lie between, in four copies a float apart, so that four neighbours begin at a
+// multiple of 16 bytes; then those of what enters the state, by token.
+constexpr int LA_BETWEEN = 72, LA_TABLE = 4 * (4 * LA_BETWEEN + LA_ROWS);
 
 struct LinearOperand {
     const half_t *x;
@@ -229,7 +231,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     f16v state[DT];
     float s_mul = 1.f, o_mul = 1.f;      // o_mul: of its operands besides, where what enters is much larger than it is
     int age = 0;
-    float owed = 1.f, ahead = 1.f;       // that decay, and 1 over it
+    float owed = 1.f;                    // that decay
     bool shrunk = false, dwarfed = false;        // it has got some of it, or was made small for what entered: too small for fp16 operands?
     bool zero = true;                    // nothing entered so far
     const int column = 32 * w + perm16(i);
@@ -292,23 +294,24 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     // what enters the state.  In a register: of the state's way to this lane's token.
     float since = 0.f, p_mul = 1.f;      // p_mul: of P's operands (fp16), a power of two
     int decays_of = 0;
-    f4v *const table = reinterpret_cast<f4v *>(lds_raw + LA_STAGES * Tiles::STAGE) + l;      // [P, state][v / 4][lane]
+    float *const table = reinterpret_cast<float *>(lds_raw + LA_STAGES * Tiles::STAGE);
     auto sees = [&](int r, int valid) { return BACKWARDS ? r >= i && r < valid : r <= i; };
     auto set_decays = [&](int valid) {
         decays_of = valid;
-        for (int u = wave_id(); u < 8; u += Tiles::WAVES) {
-            f4v x;
+        const int thread = (int)threadIdx.x;
+        if (RESULT && thread < 2 * LA_ROWS) {
+            // entry 32 + r - i: zero where token r is hidden from token i
+            const int e = thread - LA_ROWS, gap = BACKWARDS ? e : -e;
+            const float x = gap >= 0 ? p.scale * linear_power(log2_decay, gap) : 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int r = 8 * (u & 3) + 4 * h + j;
-                if (u < 4) x[j] = sees(r, valid) ? p.scale * linear_power(log2_decay, BACKWARDS ? r - i : i - r) : 0.f;
-                else x[j] = r < valid ? sum.b_mul * linear_power(log2_decay, BACKWARDS ? r + 1 : valid - 1 - r) : 0.f;
-            }
-            table[64 * u] = x;
+            for (int copy = 0; copy < 4; ++copy) table[LA_BETWEEN * copy + thread + copy] = x;
         }
+        if (thread < LA_ROWS) table[4 * LA_BETWEEN + thread] = thread < valid ? sum.b_mul * linear_power(log2_decay, BACKWARDS ? thread + 1 : valid - 1 - thread) : 0.f;
         if (RESULT) since = BACKWARDS ? (i < valid ? sum.a_mul * linear_power(log2_decay, valid - 1 - i) : 0.f) : sum.a_mul * linear_power(log2_decay, i + 1);
         asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
+    // of this lane: entries 32 + r - i for r = 4 h .. + 3 and on in steps of 8, from the copy that has them at a multiple of four floats
+    const float *const between = table + LA_BETWEEN * (i & 3) + (LA_ROWS + 4 * h - i + (i & 3)), *const entering = table + 4 * LA_BETWEEN + 4 * h;
 
     // whether the walk's end state is wanted
     const bool ends = RESULT ? sum.last != nullptr && (BACKWARDS ? item.segment == 0 : item.segment == item.segments - 1) : true;
@@ -336,33 +339,102 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         const int at = LA_ROWS * chunk, valid = min(here - at, LA_ROWS);
         const unsigned tile = (unsigned)(stage * Tiles::STAGE);
         if (valid != decays_of) set_decays(valid);
+        if (BACKWARDS && RESULT && valid < LA_ROWS) {        // tokens behind the sequence see nothing
+            for (int e = (int)threadIdx.x; e < (Tiles::STAGE / 4096) * (LA_ROWS - valid) * 8; e += WAVE * Tiles::WAVES) {
+                const int in = e % ((LA_ROWS - valid) * 8), panel = e / ((LA_ROWS - valid) * 8);
+                *reinterpret_cast<uint4 *>(lds_raw + tile + 4096 * panel + 128 * valid + 16 * in) = make_uint4(0, 0, 0, 0);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
         const bool last_inner = g == inner - 1;
         const bool fresh = !BACKWARDS || g == 0;             // of a token and head: the state's part comes first
         // every head of b and c enters the state, heads of a share one; after the segment's last chunk it may not be needed
         const bool enters = (BACKWARDS || last_inner) && (ends || step + inner - g < steps);
         // Operands are read from LDS ahead of the work that hides them; the compiler left to itself waits for each.
-        h8 cop[2], bop[4];
-        f4v decays[4];
+        h8 a[KS], b[KS], cop[2], bop[4];
+        f4v decays[4], enter[4];
         auto read_b_columns = [&](int t) {
 #pragma unroll
             for (int s = 0; s < 4; ++s) bop[s] = columns(b_at[s / 2], tile + b_tile + 4096u * (t / 2) + 2048u * (s % 2));
         };
-        auto read_decays = [&](int which) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) decays[u] = table[64 * (4 * which + u)];
-        };
-        if (RESULT) {
-            h8 a[KS], b[KS];
+        for (int s = 0; s < 2; ++s) cop[s] = columns(c_at, tile + c_tile + 2048u * s);
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
+        for (int u = 0; u < 4; ++u) enter[u] = *reinterpret_cast<const f4v *>(entering + 8 * u);
+        auto read_rows_of = [&](int first) {
+#pragma unroll
+            for (int s = first; s < first + 4; ++s) {
                 a[s] = rows(tile + a_tile, s);
                 b[s] = rows(tile + b_tile, s);
             }
+        };
+        if (RESULT) {
+            read_rows_of(0);
 #pragma unroll
-            for (int s = 0; s < 2; ++s) cop[s] = columns(c_at, tile + c_tile + 2048u * s);
-            read_decays(0);
-            issue_order();
-            f16v prob = {0};
+            for (int u = 0; u < 4; ++u) decays[u] = *reinterpret_cast<const f4v *>(between + 8 * u);
+        } else {
+            read_b_columns(0);
+        }
+        issue_order();
+        // What enters the state: c with its decay, times s_mul over the decay that the state has not got.
+        const int aged = zero ? 0 : BACKWARDS && g > 0 ? age : age + valid;
+        const bool gets = !(__builtin_fabsf(log2_decay * (float)aged) <= PUT_OFF);           // the state gets its decay with this chunk
+        const float with = gets || aged == 0 ? 1.f : at_exp2(-log2_decay * (float)aged);
+        float x[2][8], x_most = 0.f;
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const half_t one = cop[u >> 1][4 * (u & 1) + j];
+                float &to_enter = x[u >> 1][4 * (u & 1) + j];
+                to_enter = widen_16<BF>(one) * (enter[u][j] * (BF ? with : with * s_mul));
+                if (!BF) x_most = larger(x_most, to_enter);
+            }
+        if (!BF) {                       // it has to fit, and the state with it
+            if ((zero || __builtin_amdgcn_ballot_w64(x_most >= 0x1p15f) != 0ull) && enters) {
+                const float all = wave_most(is_finite(x_most) ? x_most : 0.f);
+                if (all > 0.f) {
+                    const float to_mul = fminf(fmaxf(s_mul * lift_of(all, 10), 0x1p-60f), 0x1p60f), by = to_mul / s_mul;
+                    s_mul = to_mul;
+                    if (!zero) {
+                        scale_state(by);
+                        dwarfed = true;
+                    }
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) x[s][j] *= by;
+                }
+            }
+            if (RESULT && fresh && (shrunk || dwarfed)) {
+                if (dwarfed) {           // operands of another size than the state, as long as it is so
+                    const float left = state_most();
+                    o_mul = left > 0.f && left < 16.f ? fminf(lift_of(left, 8), 0x1p60f) : 1.f;
+                    dwarfed = o_mul != 1.f;
+                } else {                 // by a part of it: what has entered since most often makes up for it
+                    float some = 0.f;
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) some = larger(some, state[0][v]);
+                    if (__builtin_amdgcn_ballot_w64(some >= 16.f) == 0ull) {
+                        const float left = state_most(), by = left > 0.f ? fminf(lift_of(left, 8), 0x1p60f / s_mul) : 1.f;
+                        if (__builtin_amdgcn_ballot_w64(x_most * by >= 0x1p15f) == 0ull) {
+                            scale_state(by);
+                            s_mul *= by;
+#pragma unroll
+                            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) x[s][j] *= by;
+                        } else {
+                            o_mul = by;
+                            dwarfed = true;
+                        }
+                    }
+                }
+                shrunk = false;
+            }
+        }
+        f16v prob = {0};
+        if (RESULT) {
             auto meet = [&](float by) {
                 oacc = f16v{0};
 #pragma unroll
@@ -374,21 +446,13 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                 }
             };
             if (fresh) {
-                if (!BF && shrunk) {     // by a part of it: what entered since most often makes up for it
-                    float some = 0.f;
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) some = larger(some, state[0][v]);
-                    if (__builtin_amdgcn_ballot_w64(some >= 16.f) == 0ull) lift_state();
-                    shrunk = false;
-                }
-                if (!BF && dwarfed) {
-                    const float left = state_most();
-                    o_mul = left > 0.f && left < 16.f ? fminf(lift_of(left, 8), 0x1p60f) : 1.f;
-                    dwarfed = o_mul != 1.f;
-                }
                 oacc = f16v{0};
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
+                    if (s == 2 && KS > 4) {
+                        read_rows_of(4);
+                        issue_order();
+                    }
                     prob = mfma_16<BF>(b[s], a[s], prob);
                     h8 op;
 #pragma unroll
@@ -400,47 +464,97 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
                     for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(oacc[v]);
                     const bool broken = __builtin_amdgcn_ballot_w64(!is_finite(sure)) != 0ull;
-                    if (broken) lift_state();
-                    if (broken || o_mul != 1.f) meet(o_mul);
+                    if (broken || o_mul != 1.f) {
+                        if (broken) {
+                            const float was = s_mul;
+                            lift_state();
+#pragma unroll
+                            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) x[s][j] *= s_mul / was;
+                        }
+                        meet(o_mul);
+                    }
                 }
+                const float up = since * owed * (BF ? 1.f : 1.f / (s_mul * o_mul));
+#pragma unroll
+                for (int v = 0; v < 16; ++v) oacc[v] *= up;
             } else {
+                if (KS > 4) read_rows_of(4);
 #pragma unroll
                 for (int s = 0; s < KS; ++s) prob = mfma_16<BF>(b[s], a[s], prob);
             }
             issue_order();
-            if (enters) read_b_columns(0);
+            read_b_columns(0);
             issue_order();
-            float most = 0.f;
+        }
+        h8 cw[TERMS][2];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+        for (int s = 0; s < 2; ++s)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    prob[4 * u + j] *= BF ? decays[u][j] : decays[u][j] * p_mul;
-                    if (!BF) most = larger(most, prob[4 * u + j]);
+            for (int j = 0; j < 8; ++j) {
+                float left = x[s][j];
+#pragma unroll
+                for (int e = 0; e < TERMS; ++e) {
+                    cw[e][s][j] = narrow_16<BF>(left);
+                    const half_t one = cw[e][s][j];
+                    if (e + 1 < TERMS) left -= widen_16<BF>(one);
                 }
-            if (!BF) {
-                const bool large = most >= 0x1p15f, fair = most >= 1.f;
+            }
+        h8 pop[2];
+        f16v part = {0};
+        float p_most = 0.f;
+        if (RESULT) {
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+                prob[v] *= BF ? decays[v >> 2][v & 3] : decays[v >> 2][v & 3] * p_mul;
+                if (!BF) p_most = larger(p_most, prob[v]);
+                pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
+            }
+#pragma unroll
+            for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
+        }
+        if (enters) {
+            if (gets) scale_state(linear_power(log2_decay, aged));
+            if (!BF) shrunk = shrunk || gets;
+            age = gets ? 0 : aged;
+            owed = gets ? 1.f : linear_power(log2_decay, age);
+            zero = false;
+#pragma unroll
+            for (int t = 0; t < DT; t += 2) {
+                const h8 now[4] = {bop[0], bop[1], bop[2], bop[3]};
+                if (t + 2 < DT) read_b_columns(t + 2);
+#pragma unroll
+                for (int e = 0; e < TERMS; ++e)
+#pragma unroll
+                    for (int s = 0; s < 4; ++s) state[t + s / 2] = mfma_16<BF>(now[s], cw[e][s % 2], state[t + s / 2]);
+            }
+        }
+        if (RESULT) {
+            float sure = 0.f;
+#pragma unroll
+            for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(part[v]);
+            if (!BF) {                   // P too large for fp16, or all of it too small
+                const bool large = p_most >= 0x1p15f, fair = p_most >= 1.f;
                 if (__builtin_amdgcn_ballot_w64(large) != 0ull || __builtin_amdgcn_ballot_w64(fair) == 0ull) {
-                    most = wave_most(is_finite(most) ? most : 0.f);
-                    if (most > 0.f) {
-                        const float to_mul = fminf(fmaxf(p_mul * lift_of(most, 8), 0x1p-60f), 0x1p60f), by = to_mul / p_mul;
+                    const float all = wave_most(is_finite(p_most) ? p_most : 0.f);
+                    if (all > 0.f) {
+                        const float to_mul = fminf(fmaxf(p_mul * lift_of(all, 8), 0x1p-60f), 0x1p60f), by = to_mul / p_mul;
                         p_mul = to_mul;
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) prob[v] *= by;
+                        for (int v = 0; v < 16; ++v) {
+                            prob[v] *= by;
+                            pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
+                        }
+                        part = f16v{0};
+#pragma unroll
+                        for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
+                        sure = 0.f;
+#pragma unroll
+                        for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(part[v]);
                     }
                 }
             }
-            h8 pop[2];
-#pragma unroll
-            for (int v = 0; v < 16; ++v) pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
-            f16v part = {0};
-            float sure = 0.f;
-#pragma unroll
-            for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
-            if (enters) read_decays(1);
-            issue_order();
-#pragma unroll
-            for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(part[v]);
             if (__builtin_amdgcn_ballot_w64(!is_finite(sure)) != 0ull) {
                 // An infinity or a NaN: zero times it is NaN, also for tokens that do not see it.  Weights of hidden ones are put to zero,
                 // and left out of c it makes NaN of its column for those that see it.
@@ -459,96 +573,18 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                 for (int r = 0; r < valid; ++r) {
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const h8 x = *(lds_h8)(uintptr_t)(first + 128u * r + 16u * (unsigned)((4 * (w & 1) + 2 * h + half) ^ panel_swizzle(r)));
+                        const h8 one_row = *(lds_h8)(uintptr_t)(first + 128u * r + 16u * (unsigned)((4 * (w & 1) + 2 * h + half) ^ panel_swizzle(r)));
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const half_t one = x[j];
+                            const half_t one = one_row[j];
                             if (sees(r, valid) && !is_finite(widen_16<BF>(one))) part[8 * half + j] = __builtin_nanf("");
                         }
                     }
                 }
             }
             const float down = BF ? 1.f : 1.f / p_mul;
-            if (fresh) {
-                const float up = since * owed * (BF ? 1.f : 1.f / (s_mul * o_mul));
 #pragma unroll
-                for (int v = 0; v < 16; ++v) oacc[v] = BF ? __builtin_fmaf(oacc[v], up, part[v]) : __builtin_fmaf(part[v], down, oacc[v] * up);
-            } else {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) oacc[v] = BF ? oacc[v] + part[v] : __builtin_fmaf(part[v], down, oacc[v]);
-            }
-        } else {
-#pragma unroll
-            for (int s = 0; s < 2; ++s) cop[s] = columns(c_at, tile + c_tile + 2048u * s);
-            read_decays(1);
-            read_b_columns(0);
-            issue_order();
-        }
-        if (enters) {
-            if (!BACKWARDS || g == 0) {
-                age = zero ? 0 : age + valid;
-                owed = linear_power(log2_decay, age);
-                if (age > 0 && !(__builtin_fabsf(log2_decay * (float)age) <= PUT_OFF)) {
-                    scale_state(owed);
-                    age = 0;
-                    owed = 1.f;
-                    shrunk = true;
-                }
-                ahead = age == 0 ? 1.f : at_exp2(-log2_decay * (float)age);
-            }
-            float with = ahead * s_mul, x[2][8], most = 0.f;
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const half_t one = cop[u >> 1][4 * (u & 1) + j];
-                    float &to_enter = x[u >> 1][4 * (u & 1) + j];
-                    to_enter = widen_16<BF>(one) * (decays[u][j] * with);
-                    if (!BF) most = larger(most, to_enter);
-                }
-            if (!BF) {
-                if (zero || __builtin_amdgcn_ballot_w64(most >= 0x1p15f) != 0ull) {
-                    const float all = wave_most(is_finite(most) ? most : 0.f);
-                    if (all > 0.f) {
-                        const float to_mul = fminf(fmaxf(s_mul * lift_of(all, 10), 0x1p-60f), 0x1p60f), by = to_mul / s_mul;
-                        s_mul = to_mul;
-                        if (!zero) {
-                            scale_state(by);
-                            dwarfed = true;
-                        }
-#pragma unroll
-                        for (int s = 0; s < 2; ++s)
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) x[s][j] *= by;
-                    }
-                }
-            }
-            zero = false;
-            h8 cw[TERMS][2];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    float left = x[s][j];
-#pragma unroll
-                    for (int e = 0; e < TERMS; ++e) {
-                        cw[e][s][j] = narrow_16<BF>(left);
-                        const half_t one = cw[e][s][j];
-                        if (e + 1 < TERMS) left -= widen_16<BF>(one);
-                    }
-                }
-#pragma unroll
-            for (int t = 0; t < DT; t += 2) {
-                const h8 now[4] = {bop[0], bop[1], bop[2], bop[3]};
-                if (t + 2 < DT) {
-                    read_b_columns(t + 2);
-                    issue_order();
-                }
-#pragma unroll
-                for (int e = 0; e < TERMS; ++e)
-#pragma unroll
-                    for (int s = 0; s < 4; ++s) state[t + s / 2] = mfma_16<BF>(now[s], cw[e][s % 2], state[t + s / 2]);
-            }
+            for (int v = 0; v < 16; ++v) oacc[v] = BF ? oacc[v] + part[v] : __builtin_fmaf(part[v], down, oacc[v]);
         }
         stage = stage == LA_STAGES - 1 ? 0 : stage + 1;
         if (RESULT && (!BACKWARDS || last_inner)) {
