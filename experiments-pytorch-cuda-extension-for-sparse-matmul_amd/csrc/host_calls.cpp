@@ -59,12 +59,23 @@ struct Entry {
     decltype(&bsa_cache_read) cache_read;
     decltype(&bsa_cached_attention_workspace_bytes) cached_workspace;
     decltype(&bsa_cached_attention) cached_attention;
+    decltype(&bsa_linear_attention_segment) linear_segment;
+    decltype(&bsa_linear_attention_states_bytes) linear_states_bytes;
+    decltype(&bsa_linear_attention_forward) linear_forward;
+    decltype(&bsa_linear_attention_backward) linear_backward;
+    decltype(&bsa_linear_attention_step) linear_step;
+    decltype(&bsa_pages_append) pages_append;
+    decltype(&bsa_pages_free) pages_free;
+    decltype(&bsa_pages_fork_scratch_bytes) fork_scratch;
+    decltype(&bsa_pages_fork) pages_fork;
+    decltype(&bsa_pages_compact) pages_compact;
+    decltype(&bsa_cache_copy) cache_copy;
 } lib;
 struct PythonSide {
     PyObject *matmul, *softmax, *attention;                                     // autograd Functions' apply
     PyObject *plan_matmul, *plan_weight, *plan_softmax, *plan_softmax_backward, *plan_attention, *plan_attention_backward;
     PyObject *run_matmul, *run_weight, *run_softmax_backward, *run_attention_backward;      // without a plan
-    PyObject *packed, *run_packed_backward;
+    PyObject *packed, *run_packed_backward, *run_linear_backward;
     PyObject *failed;
     PyDictObject *settings[2];               // of the modules whose globals decide routes
     PyObject *name_plans, *name_row, *name_col, *modes[3];
@@ -1078,6 +1089,305 @@ PyObject *cached_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs) 
     END_HANDLE_TH_ERRORS
 }
 
+PyObject *pair_of(Tensor a, Tensor b)
+{
+    return PyTuple_Pack(2, py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(a))).ptr(),
+                        py::reinterpret_steal<py::object>(THPVariable_Wrap(std::move(b))).ptr());
+}
+
+PyObject *cache_copy(PyObject *, PyObject *const *args, Py_ssize_t nargs)   // capsule, capsule of the origin, sources, targets
+{
+    HANDLE_TH_ERRORS
+    HeldCache *c = nargs == 4 ? cache_of(args[0]) : nullptr, *from = nargs == 4 ? cache_of(args[1]) : nullptr;
+    if (c == nullptr || from == nullptr || !tensors(args + 2, 2) || !plain_thread()) Py_RETURN_NONE;
+    const Tensor &sources = THPVariable_Unpack(args[2]), &targets = THPVariable_Unpack(args[3]);
+    if (c->code != from->code || c->heads != from->heads || c->head_dim != from->head_dim || c->page != from->page ||
+        c->keys.device() != from->keys.device() || !on_current_device(c->keys))
+        Py_RETURN_NONE;
+    if (!index_tensor(sources, 1) || !index_tensor(targets, 1) || sources.numel() != targets.numel() || sources.numel() > (1 << 24)) Py_RETURN_NONE;
+    {
+        py::gil_scoped_release unlocked;
+        launched(lib.cache_copy(c->code, from->keys.data_ptr(), from->values.data_ptr(), from->scales(from->key_scales), from->scales(from->value_scales),
+                                from->pages, c->keys.data_ptr(), c->values.data_ptr(), const_cast<float *>(c->scales(c->key_scales)),
+                                const_cast<float *>(c->scales(c->value_scales)), c->pages, sources.data_ptr<int32_t>(), targets.data_ptr<int32_t>(),
+                                (int)sources.numel(), c->heads, c->head_dim, c->page, current_stream()));
+    }
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- linear attention --------------------------------------------------------------------------------------
+// linear.check_decay, linear.check_states
+bool decay_fits(const Tensor &t, int64_t key_heads)
+{
+    return plain(t) && on_current_device(t) && t.scalar_type() == at::kFloat && t.dim() == 1 && t.size(0) == key_heads && !forward_mode(t) &&
+           !(at::GradMode::is_enabled() && t.requires_grad());
+}
+bool states_fit(const Tensor &t, int64_t count, const Tensor &k)
+{
+    return plain(t) && on_current_device(t) && t.scalar_type() == at::kFloat && t.dim() == 4 && t.size(0) == count && t.size(1) == k.size(1) &&
+           t.size(2) == k.size(2) && t.size(3) == k.size(2) && at_16_bytes(t) && !forward_mode(t);
+}
+float *floats(const Tensor &t) { return t.defined() && t.numel() > 0 ? t.data_ptr<float>() : nullptr; }
+
+// sparse/linear.py, PackedLinearAttention.backward
+struct LinearNode : public Node {
+    SavedVariable q_, k_, v_, states_, decay_, offsets_, between_;
+    double scale;
+    bool with_states;                        // q, k, v's gradients are followed by the states'
+    std::string name() const override { return "PackedLinearAttentionBackward"; }
+    void release_variables() override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        for (SavedVariable *s : {&q_, &k_, &v_, &states_, &decay_, &offsets_, &between_}) s->reset_data();
+    }
+    variable_list apply(variable_list &&grads) override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        const Tensor q = q_.unpack(), k = k_.unpack(), v = v_.unpack(), states = states_.unpack(), decay = decay_.unpack(), offsets = offsets_.unpack(),
+                     between = between_.unpack();
+        Tensor dout = grads[0].defined() ? grads[0] : input_metadata(0).zeros_like(), dlast = grads.size() > 1 ? grads[1] : Tensor();
+        const bool dstates = with_states && task_should_compute_output(3);
+        variable_list result;
+        {
+            at::AutoGradMode off(false);
+            if (plain_strided(dout) && !readable_rows(dout)) dout = dout.clone(at::MemoryFormat::Contiguous);
+            const int64_t count = offsets.numel() - 1;
+            bool direct = heads_fit(q, k, v, 3) && plain_strided(dout) && readable_rows(dout) && dout.sizes() == q.sizes() &&
+                          dout.scalar_type() == q.scalar_type() && index_tensor(offsets, 1) && count >= 1 && count <= 65535 && q.size(0) > 0 &&
+                          decay_fits(decay, k.size(1)) && plain(between) && on_current_device(between) && between.scalar_type() == at::kFloat;
+            if (direct && states.defined()) direct = states_fit(states, count, k);
+            if (direct && dlast.defined()) direct = states_fit(dlast, count, k);
+            const int tokens = direct ? (int)q.size(0) : 0, key_heads = direct ? (int)k.size(1) : 0, dim = direct ? (int)q.size(2) : 0;
+            const int segment = direct ? lib.linear_segment(tokens, (int)count, key_heads, dim) : 0;
+            const size_t need = direct ? lib.linear_states_bytes(tokens, key_heads, dim, segment) : 0;
+            if (!direct || between.numel() != (int64_t)(need / 4)) {
+                py::gil_scoped_acquire gil;
+                auto wrapped = [](const Tensor &t) { return t.defined() ? py::reinterpret_steal<py::object>(THPVariable_Wrap(t)) : py::object(py::none()); };
+                const py::object given[9] = {wrapped(q), wrapped(k), wrapped(v), wrapped(states), wrapped(decay), wrapped(offsets), wrapped(between),
+                                             wrapped(dout), wrapped(dlast)};
+                const py::object s = py::float_(scale);
+                PyObject *got = PyObject_CallFunctionObjArgs(python.run_linear_backward, given[0].ptr(), given[1].ptr(), given[2].ptr(), given[3].ptr(),
+                                                             given[4].ptr(), given[5].ptr(), given[6].ptr(), given[7].ptr(), given[8].ptr(), s.ptr(),
+                                                             py_bool(dstates), nullptr);
+                if (got == nullptr) raise_pending();
+                py::tuple t = py::reinterpret_steal<py::tuple>(got);
+                for (auto x : t) result.push_back(x.is_none() ? Tensor() : THPVariable_Unpack(x.ptr()));
+            } else {
+                const auto floating = q.options().dtype(at::kFloat);
+                Tensor dq = at::empty(q.sizes(), q.options()), dk = at::empty(k.sizes(), k.options()), dv = at::empty(k.sizes(), k.options());
+                const Tensor behind = at::empty({(int64_t)(need / 4)}, floating);
+                Tensor dfirst;
+                if (dstates) dfirst = at::empty({count, k.size(1), k.size(2), k.size(2)}, floating);
+                const int64_t strides[8] = {stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0), stride_of(v, 1),
+                                            stride_of(dout, 0), stride_of(dout, 1)};
+                launched(lib.linear_backward(code_of(q.scalar_type()), q.data_ptr(), k.data_ptr(), v.data_ptr(), dout.data_ptr(), decay.data_ptr<float>(),
+                                             offsets.data_ptr<int32_t>(), floats(states), floats(between), floats(dlast), dq.data_ptr(), dk.data_ptr(),
+                                             dv.data_ptr(), floats(dfirst), floats(behind), need, segment, tokens, (int)count, (int)q.size(1), key_heads,
+                                             dim, strides, (float)scale, current_stream()));
+                result = {dq, dk, dv, dfirst};
+            }
+        }
+        if (!with_states) result.resize(3);
+        if (at::GradMode::is_enabled()) {    // asked for a graph of the gradients: there is none, and who differentiates them is told
+            for (Tensor &t : result)
+                if (t.defined()) t.set_requires_grad(true);
+            result = torch::autograd::DelayedError("trying to differentiate twice a function that was marked with @once_differentiable",
+                                                   (int64_t)result.size()).apply(std::move(result));
+        }
+        return result;
+    }
+};
+
+// None where the Python side has to look at the call, as with the others below
+PyObject *linear_attention(PyObject *, PyObject *const *args, Py_ssize_t nargs)     // q, k, v, log_decay, offsets, scale, states, return_states
+{
+    HANDLE_TH_ERRORS
+    const int ends = nargs == 8 ? truth(args[7]) : -1;
+    if (ends < 0 || !number(args[5]) || !tensors(args, 5) || !plain_thread()) Py_RETURN_NONE;
+    if (args[6] != Py_None && !THPVariable_CheckExact(args[6])) Py_RETURN_NONE;
+    const Tensor &q = THPVariable_Unpack(args[0]), &k = THPVariable_Unpack(args[1]), &v = THPVariable_Unpack(args[2]),
+                 &decay = THPVariable_Unpack(args[3]), &offsets = THPVariable_Unpack(args[4]);
+    const Tensor states = args[6] == Py_None ? Tensor() : THPVariable_Unpack(args[6]);
+    if (!heads_fit(q, k, v, 3) || !index_tensor(offsets, 1) || offsets.numel() < 2 || offsets.numel() > 65536 || q.size(0) < 1 ||
+        q.size(0) > (1 << 30) || !decay_fits(decay, k.size(1)))
+        Py_RETURN_NONE;
+    const int64_t count = offsets.numel() - 1;
+    if (states.defined() && !states_fit(states, count, k)) Py_RETURN_NONE;
+    const double scale = PyFloat_AsDouble(args[5]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    std::shared_ptr<LinearNode> node;
+    const bool states_grad = states.defined() && needs_grad({&states});
+    if (needs_grad({&q, &k, &v}) || states_grad) {
+        node = std::shared_ptr<LinearNode>(new LinearNode(), torch::autograd::deleteNode);
+        node->with_states = states.defined();
+        if (states.defined()) node->set_next_edges(torch::autograd::collect_next_edges(q, k, v, states));
+        else node->set_next_edges(torch::autograd::collect_next_edges(q, k, v));
+        node->q_ = SavedVariable(q, false);
+        node->k_ = SavedVariable(k, false);
+        node->v_ = SavedVariable(v, false);
+        node->states_ = SavedVariable(states, false);
+        node->decay_ = SavedVariable(decay, false);
+        node->offsets_ = SavedVariable(offsets, false);
+        node->scale = scale;
+    }
+    Tensor out, last, between;
+    {
+        py::gil_scoped_release unlocked;
+        const auto floating = q.options().dtype(at::kFloat);
+        const int tokens = (int)q.size(0), key_heads = (int)k.size(1), dim = (int)q.size(2);
+        out = at::empty(q.sizes(), q.options());
+        if (ends) last = at::empty({count, k.size(1), k.size(2), k.size(2)}, floating);
+        const int segment = lib.linear_segment(tokens, (int)count, key_heads, dim);
+        const size_t need = lib.linear_states_bytes(tokens, key_heads, dim, segment);
+        between = at::empty({(int64_t)(need / 4)}, floating);
+        const int64_t strides[6] = {stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0), stride_of(v, 1)};
+        launched(lib.linear_forward(code_of(q.scalar_type()), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr<float>(),
+                                    offsets.data_ptr<int32_t>(), floats(states), floats(last), floats(between), need, segment, tokens, (int)count,
+                                    (int)q.size(1), key_heads, dim, strides, (float)scale, current_stream()));
+    }
+    if (node) {
+        torch::autograd::set_history(out, node);
+        if (ends) torch::autograd::set_history(last, node);
+        node->between_ = SavedVariable(between, false);
+    }
+    if (ends) return pair_of(std::move(out), std::move(last));
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *linear_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)          // q, k, v, log_decay, states, slots, scale
+{
+    HANDLE_TH_ERRORS
+    if (nargs != 7 || !tensors(args, 6) || !number(args[6]) || !plain_thread()) Py_RETURN_NONE;
+    const Tensor &q = THPVariable_Unpack(args[0]), &k = THPVariable_Unpack(args[1]), &v = THPVariable_Unpack(args[2]),
+                 &decay = THPVariable_Unpack(args[3]), &states = THPVariable_Unpack(args[4]), &slots = THPVariable_Unpack(args[5]);
+    if (!heads_fit(q, k, v, 3) || !decay_fits(decay, k.size(1)) || !index_tensor(slots, 1)) Py_RETURN_NONE;
+    if (!states.defined() || states.dim() != 4 || !states_fit(states, states.size(0), k) || needs_grad({&q, &k, &v, &states})) Py_RETURN_NONE;
+    const int64_t batch = q.size(0);
+    if (batch < 1 || batch > 65535 || slots.numel() != batch || states.size(0) < 1 || states.size(0) > INT32_MAX) Py_RETURN_NONE;
+    const double scale = PyFloat_AsDouble(args[6]);
+    if (scale == -1.0 && PyErr_Occurred()) return nullptr;
+    Tensor out;
+    {
+        py::gil_scoped_release unlocked;
+        out = at::empty(q.sizes(), q.options());
+        const int64_t strides[6] = {stride_of(q, 0), stride_of(q, 1), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0), stride_of(v, 1)};
+        launched(lib.linear_step(code_of(q.scalar_type()), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr<float>(),
+                                 states.data_ptr<float>(), slots.data_ptr<int32_t>(), (int)batch, (int)states.size(0), (int)q.size(1), (int)k.size(1),
+                                 (int)q.size(2), strides, (float)scale, current_stream()));
+    }
+    return THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// ---- page tables -------------------------------------------------------------------------------------------
+// What a PageTable holds, as its calls need it
+struct HeldTable {
+    Tensor table, lengths, uses, missing;
+    int sequences, width, pages, page;
+    Tensor ints(int64_t n) const { return at::empty({n}, table.options()); }
+};
+constexpr const char *TABLE_CAPSULE = "bsa_page_table";
+HeldTable *table_of(PyObject *capsule)
+{
+    HeldTable *t = PyCapsule_IsValid(capsule, TABLE_CAPSULE) ? static_cast<HeldTable *>(PyCapsule_GetPointer(capsule, TABLE_CAPSULE)) : nullptr;
+    return t != nullptr && on_current_device(t->table) && plain_thread() ? t : nullptr;
+}
+PyObject *new_page_table(PyObject *, PyObject *args)         // table, lengths, uses, missing, page
+{
+    HANDLE_TH_ERRORS
+    PyObject *t[4];
+    int page;
+    if (!PyArg_ParseTuple(args, "OOOOi", &t[0], &t[1], &t[2], &t[3], &page)) return nullptr;
+    auto held = std::make_unique<HeldTable>();
+    held->table = THPVariable_Unpack(t[0]), held->lengths = THPVariable_Unpack(t[1]);
+    held->uses = THPVariable_Unpack(t[2]), held->missing = THPVariable_Unpack(t[3]);
+    held->sequences = (int)held->table.size(0), held->width = (int)held->table.size(1), held->pages = (int)held->uses.size(0), held->page = page;
+    return PyCapsule_New(held.release(), TABLE_CAPSULE, [](PyObject *capsule) {
+        delete static_cast<HeldTable *>(PyCapsule_GetPointer(capsule, TABLE_CAPSULE));
+    });
+    END_HANDLE_TH_ERRORS
+}
+constexpr int64_t MOST_ENTRIES = 4096;
+
+PyObject *pages_append(PyObject *, PyObject *const *args, Py_ssize_t nargs)         // capsule, offsets, tokens
+{
+    HANDLE_TH_ERRORS
+    HeldTable *t = nargs == 3 ? table_of(args[0]) : nullptr;
+    if (t == nullptr || !tensors(args + 1, 1) || !PyLong_CheckExact(args[2])) Py_RETURN_NONE;
+    const Tensor &offsets = THPVariable_Unpack(args[1]);
+    const long long tokens = PyLong_AsLongLong(args[2]);
+    if (tokens == -1 && PyErr_Occurred()) PyErr_Clear();
+    if (tokens < 1 || tokens > (1 << 30) || !index_tensor(offsets, 1) || offsets.numel() != t->sequences + 1) Py_RETURN_NONE;
+    Tensor slots;
+    {
+        py::gil_scoped_release unlocked;
+        slots = t->ints(tokens);
+        const Tensor scratch = t->ints(t->sequences);
+        launched(lib.pages_append(t->table.data_ptr<int32_t>(), t->lengths.data_ptr<int32_t>(), t->uses.data_ptr<int32_t>(), t->missing.data_ptr<int32_t>(),
+                                  offsets.data_ptr<int32_t>(), slots.data_ptr<int32_t>(), (int)tokens, t->sequences, t->width, t->pages, t->page,
+                                  scratch.data_ptr<int32_t>(), current_stream()));
+    }
+    return THPVariable_Wrap(std::move(slots));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *pages_free(PyObject *, PyObject *const *args, Py_ssize_t nargs)           // capsule, which
+{
+    HANDLE_TH_ERRORS
+    HeldTable *t = nargs == 2 ? table_of(args[0]) : nullptr;
+    if (t == nullptr || !tensors(args + 1, 1)) Py_RETURN_NONE;
+    const Tensor &which = THPVariable_Unpack(args[1]);
+    if (!index_tensor(which, 1) || which.numel() > MOST_ENTRIES) Py_RETURN_NONE;
+    {
+        py::gil_scoped_release unlocked;
+        launched(lib.pages_free(t->table.data_ptr<int32_t>(), t->lengths.data_ptr<int32_t>(), t->uses.data_ptr<int32_t>(), which.data_ptr<int32_t>(),
+                                (int)which.numel(), t->sequences, t->width, t->pages, t->page, current_stream()));
+    }
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *pages_fork(PyObject *, PyObject *const *args, Py_ssize_t nargs)           // capsule, parents, children
+{
+    HANDLE_TH_ERRORS
+    HeldTable *t = nargs == 3 ? table_of(args[0]) : nullptr;
+    if (t == nullptr || !tensors(args + 1, 2)) Py_RETURN_NONE;
+    const Tensor &parents = THPVariable_Unpack(args[1]), &children = THPVariable_Unpack(args[2]);
+    const int64_t count = parents.numel();
+    if (!index_tensor(parents, 1) || !index_tensor(children, 1) || children.numel() != count || count < 1 || count > MOST_ENTRIES) Py_RETURN_NONE;
+    Tensor sources, targets;
+    {
+        py::gil_scoped_release unlocked;
+        sources = t->ints(count), targets = t->ints(count);
+        const size_t need = lib.fork_scratch((int)count, t->width);
+        const Tensor scratch = t->ints((int64_t)(need / 4));
+        launched(lib.pages_fork(t->table.data_ptr<int32_t>(), t->lengths.data_ptr<int32_t>(), t->uses.data_ptr<int32_t>(), t->missing.data_ptr<int32_t>(),
+                                parents.data_ptr<int32_t>(), children.data_ptr<int32_t>(), sources.data_ptr<int32_t>(), targets.data_ptr<int32_t>(),
+                                (int)count, t->sequences, t->width, t->pages, t->page, scratch.data_ptr(), need, current_stream()));
+    }
+    return pair_of(std::move(sources), std::move(targets));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject *pages_compact(PyObject *, PyObject *const *args, Py_ssize_t nargs)        // capsule
+{
+    HANDLE_TH_ERRORS
+    HeldTable *t = nargs == 1 ? table_of(args[0]) : nullptr;
+    if (t == nullptr || t->pages < 2) Py_RETURN_NONE;
+    Tensor sources, targets;
+    {
+        py::gil_scoped_release unlocked;
+        sources = t->ints(t->pages / 2), targets = t->ints(t->pages / 2);
+        const Tensor scratch = t->ints(t->pages + 1);
+        launched(lib.pages_compact(t->table.data_ptr<int32_t>(), t->lengths.data_ptr<int32_t>(), t->uses.data_ptr<int32_t>(), sources.data_ptr<int32_t>(),
+                                   targets.data_ptr<int32_t>(), t->sequences, t->width, t->pages, t->page, scratch.data_ptr<int32_t>(), current_stream()));
+    }
+    return pair_of(std::move(sources), std::move(targets));
+    END_HANDLE_TH_ERRORS
+}
+
 // entry points (addresses by name), Python functions (by name), the two modules' dicts
 PyObject *setup(PyObject *, PyObject *args)
 {
@@ -1108,6 +1418,17 @@ PyObject *setup(PyObject *, PyObject *args)
     address("bsa_cache_read", lib.cache_read);
     address("bsa_cached_attention_workspace_bytes", lib.cached_workspace);
     address("bsa_cached_attention", lib.cached_attention);
+    address("bsa_linear_attention_segment", lib.linear_segment);
+    address("bsa_linear_attention_states_bytes", lib.linear_states_bytes);
+    address("bsa_linear_attention_forward", lib.linear_forward);
+    address("bsa_linear_attention_backward", lib.linear_backward);
+    address("bsa_linear_attention_step", lib.linear_step);
+    address("bsa_pages_append", lib.pages_append);
+    address("bsa_pages_free", lib.pages_free);
+    address("bsa_pages_fork_scratch_bytes", lib.fork_scratch);
+    address("bsa_pages_fork", lib.pages_fork);
+    address("bsa_pages_compact", lib.pages_compact);
+    address("bsa_cache_copy", lib.cache_copy);
     auto function = [&](const char *name, PyObject *&f) {
         PyObject *x = PyDict_GetItemString(functions, name);
         if (x == nullptr) PyErr_Format(PyExc_KeyError, "%s", name);
@@ -1129,6 +1450,7 @@ PyObject *setup(PyObject *, PyObject *args)
     function("run_attention_backward", python.run_attention_backward);
     function("packed", python.packed);
     function("run_packed_backward", python.run_packed_backward);
+    function("run_linear_backward", python.run_linear_backward);
     function("failed", python.failed);
     Py_INCREF(first);
     Py_INCREF(second);
@@ -1159,6 +1481,15 @@ PyMethodDef methods[] = {
     {"cache_read", (PyCFunction)(void (*)(void))cache_read, METH_FASTCALL, "cache_read(cache, slots, dtype)"},
     {"cached_attention", (PyCFunction)(void (*)(void))cached_attention, METH_FASTCALL,
      "cached_attention(q, k, v, cache, pages, lengths, tree, scale)"},
+    {"cache_copy", (PyCFunction)(void (*)(void))cache_copy, METH_FASTCALL, "cache_copy(cache, origin, sources, targets)"},
+    {"linear_attention", (PyCFunction)(void (*)(void))linear_attention, METH_FASTCALL,
+     "linear_attention(q, k, v, log_decay, offsets, scale, states, return_states)"},
+    {"linear_step", (PyCFunction)(void (*)(void))linear_step, METH_FASTCALL, "linear_step(q, k, v, log_decay, states, slots, scale)"},
+    {"new_page_table", new_page_table, METH_VARARGS, nullptr},
+    {"pages_append", (PyCFunction)(void (*)(void))pages_append, METH_FASTCALL, "pages_append(table, offsets, tokens)"},
+    {"pages_free", (PyCFunction)(void (*)(void))pages_free, METH_FASTCALL, "pages_free(table, which)"},
+    {"pages_fork", (PyCFunction)(void (*)(void))pages_fork, METH_FASTCALL, "pages_fork(table, parents, children)"},
+    {"pages_compact", (PyCFunction)(void (*)(void))pages_compact, METH_FASTCALL, "pages_compact(table)"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "bsa_host_calls", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

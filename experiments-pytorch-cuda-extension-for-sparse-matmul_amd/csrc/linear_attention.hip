@@ -252,7 +252,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         const float most = state_most();
         if (most > 0.f) {
             const float to_mul = fminf(fmaxf(s_mul * lift_of(most, 8), 0x1p-60f), 0x1p60f);
-            scale_state(to_mul / s_mul);
+            scale_state(to_mul * __builtin_amdgcn_rcpf(s_mul));
             s_mul = to_mul;
         }
         o_mul = 1.f;
@@ -394,7 +394,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             if ((zero || __builtin_amdgcn_ballot_w64(x_most >= 0x1p15f) != 0ull) && enters) {
                 const float all = wave_most(is_finite(x_most) ? x_most : 0.f);
                 if (all > 0.f) {
-                    const float to_mul = fminf(fmaxf(s_mul * lift_of(all, 10), 0x1p-60f), 0x1p60f), by = to_mul / s_mul;
+                    const float to_mul = fminf(fmaxf(s_mul * lift_of(all, 10), 0x1p-60f), 0x1p60f), by = to_mul * __builtin_amdgcn_rcpf(s_mul);
                     s_mul = to_mul;
                     if (!zero) {
                         scale_state(by);
@@ -416,7 +416,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
                     for (int v = 0; v < 16; ++v) some = larger(some, state[0][v]);
                     if (__builtin_amdgcn_ballot_w64(some >= 16.f) == 0ull) {
-                        const float left = state_most(), by = left > 0.f ? fminf(lift_of(left, 8), 0x1p60f / s_mul) : 1.f;
+                        const float left = state_most(), by = left > 0.f ? fminf(lift_of(left, 8), 0x1p60f * __builtin_amdgcn_rcpf(s_mul)) : 1.f;
                         if (__builtin_amdgcn_ballot_w64(x_most * by >= 0x1p15f) == 0ull) {
                             scale_state(by);
                             s_mul *= by;
@@ -434,6 +434,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             }
         }
         f16v prob = {0};
+        float up = 0.f;
         if (RESULT) {
             auto meet = [&](float by) {
                 oacc = f16v{0};
@@ -471,14 +472,12 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
                             for (int s = 0; s < 2; ++s)
 #pragma unroll
-                                for (int j = 0; j < 8; ++j) x[s][j] *= s_mul / was;
+                                for (int j = 0; j < 8; ++j) x[s][j] *= s_mul * __builtin_amdgcn_rcpf(was);
                         }
                         meet(o_mul);
                     }
                 }
-                const float up = since * owed * (BF ? 1.f : 1.f / (s_mul * o_mul));
-#pragma unroll
-                for (int v = 0; v < 16; ++v) oacc[v] *= up;
+                up = since * owed * (BF ? 1.f : __builtin_amdgcn_rcpf(s_mul * o_mul));      // of a power of two: exact
             } else {
                 if (KS > 4) read_rows_of(4);
 #pragma unroll
@@ -539,7 +538,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                 if (__builtin_amdgcn_ballot_w64(large) != 0ull || __builtin_amdgcn_ballot_w64(fair) == 0ull) {
                     const float all = wave_most(is_finite(p_most) ? p_most : 0.f);
                     if (all > 0.f) {
-                        const float to_mul = fminf(fmaxf(p_mul * lift_of(all, 8), 0x1p-60f), 0x1p60f), by = to_mul / p_mul;
+                        const float to_mul = fminf(fmaxf(p_mul * lift_of(all, 8), 0x1p-60f), 0x1p60f), by = to_mul * __builtin_amdgcn_rcpf(p_mul);
                         p_mul = to_mul;
 #pragma unroll
                         for (int v = 0; v < 16; ++v) {
@@ -582,9 +581,14 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                     }
                 }
             }
-            const float down = BF ? 1.f : 1.f / p_mul;
+            const float down = BF ? 1.f : __builtin_amdgcn_rcpf(p_mul);
+            if (fresh) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) oacc[v] = BF ? oacc[v] + part[v] : __builtin_fmaf(part[v], down, oacc[v]);
+                for (int v = 0; v < 16; ++v) oacc[v] = __builtin_fmaf(oacc[v], up, BF ? part[v] : part[v] * down);
+            } else {
+#pragma unroll
+                for (int v = 0; v < 16; ++v) oacc[v] = BF ? oacc[v] + part[v] : __builtin_fmaf(part[v], down, oacc[v]);
+            }
         }
         stage = stage == LA_STAGES - 1 ? 0 : stage + 1;
         if (RESULT && (!BACKWARDS || last_inner)) {
@@ -599,7 +603,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     if (ends) {
         float *dst = RESULT ? sum.last + ((size_t)item.sequence * p.key_heads + key_head) * HD * HD
                             : p.states + linear_boundary(p, item.begin, BACKWARDS ? item.segment : item.segment + 1, key_head) * HD * HD;
-        const float down = owed * (BF ? 1.f : 1.f / s_mul);
+        const float down = owed * (BF ? 1.f : __builtin_amdgcn_rcpf(s_mul));
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
@@ -684,7 +688,7 @@ __global__ __launch_bounds__(2 * HD, 2) void linear_segments_kernel(LinearWalk p
 
 // The running sum over the segments of a sequence, in place: what each segment begins with.  A lane has four values of a state; the
 // segments' sums are requested RUN_AHEAD at a time.
-constexpr int RUN_AHEAD = 8;
+constexpr int RUN_AHEAD = 16;
 template <bool BACKWARDS>
 __global__ __launch_bounds__(256) void linear_running_kernel(LinearWalk p, const float *__restrict__ first, int square)
 {

@@ -130,6 +130,8 @@ class KeyValueCache:
         origin = self if origin is None else origin
         if not isinstance(origin, KeyValueCache):
             raise TypeError(f"origin must be a KeyValueCache, got {type(origin).__name__}")
+        if _k.host_calls.cache_copy(self._native, origin._native, sources, targets):
+            return
         for name in ("dtype", "heads", "head_dim", "page", "device"):
             if getattr(origin, name) != getattr(self, name):
                 raise ValueError(f"pages of a cache with {name} {getattr(origin, name)} do not fit one with {getattr(self, name)}")

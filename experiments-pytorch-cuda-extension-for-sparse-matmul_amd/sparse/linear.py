@@ -153,6 +153,14 @@ def packed_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
     outside every sequence (the padding of a batch) are not read; their results and gradients are zero.  Operands may be slices of a
     larger tensor; they are copied only where a row does not start at a multiple of 16 bytes.  Differentiable once in ``q``, ``k``, ``v``
     and ``states``, with the same bits in every call; ``log_decay`` has no gradient and is refused if autograd follows it."""
+    found = _k.host_calls.linear_attention(q, k, v, log_decay, offsets, scale, states, return_states)
+    if found is not None:
+        return found
+    return general(q, k, v, log_decay, offsets, scale, states, return_states)
+
+
+def general(q, k, v, log_decay, offsets, scale, states, return_states):
+    """The call without the native side, which leaves to it whatever it does not take."""
     leaves = [t for t in (q, k, v, states) if isinstance(t, torch.Tensor)]
     if (torch.is_grad_enabled() and any(t.requires_grad for t in leaves)) or any(forward_mode(t) for t in leaves):
         return PackedLinearAttention.apply(q, k, v, states, log_decay, offsets, scale, bool(return_states))
@@ -168,6 +176,9 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
     states go on here.  ``states``, float32 ``[places, key heads, D, D]``, contiguous; ``slots``, int32 on the GPU, ``[batch]``: the place of
     each sequence.  A sequence whose slot is negative or behind the states (an idle row of the batch) gets zeros and changes nothing;
     no two rows of a call may have the same slot.  Not differentiable: operands that autograd follows are refused."""
+    out = _k.host_calls.linear_step(q, k, v, log_decay, states, slots, scale)
+    if out is not None:
+        return out
     check_heads(q, k, v, 3)
     refuse_gradients("linear_attention_step", q, k, v, *([states] if isinstance(states, torch.Tensor) else []))
     check_decay(log_decay, k.size(1), q.device)

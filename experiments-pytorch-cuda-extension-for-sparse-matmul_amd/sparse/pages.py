@@ -38,17 +38,22 @@ class PageTable:
         self.pages, self.page, self.sequences, self.width, self.device = pages, page, sequences, width, device
         self._tensors = (torch.full((sequences, width), -1, dtype=torch.int32, device=device),
                          *(torch.zeros(n, dtype=torch.int32, device=device) for n in (sequences, pages, 1)))
+        self._native = _k.host_calls.new_page_table(*self._tensors, page)
 
     table = property(lambda self: self._tensors[0])
     lengths = property(lambda self: self._tensors[1])
     uses = property(lambda self: self._tensors[2])
     missing = property(lambda self: self._tensors[3])
 
+    def __getstate__(self):
+        return {name: value for name, value in self.__dict__.items() if name != "_native"}
+
     def __setstate__(self, state):
         self.__dict__.update(state)
         self.device = self.table.device
         if self.device.type != "cuda":              # loaded elsewhere: its calls would hand host addresses to kernels
             raise ValueError("a table lives on the GPU")
+        self._native = _k.host_calls.new_page_table(*self._tensors, self.page)
 
     def _pointers(self, count):
         return [t.data_ptr() for t in self._tensors[:count]]
@@ -69,6 +74,9 @@ class PageTable:
         sequence ``b`` has (int32 on the GPU, ``[sequences + 1]``, ascending).  Returns their slots, int32 ``[tokens]``, for
         ``KeyValueCache.write``.  A sequence whose tokens would need more pages than are free, after those in front of it, or than its row
         has stays as it is, is counted in ``missing``, and its tokens have slot -1, as those outside every sequence have."""
+        slots = _k.host_calls.pages_append(self._native, offsets, tokens)
+        if slots is not None:
+            return slots
         check_index(offsets, "offsets", self.device, 1)
         if offsets.numel() != self.sequences + 1:
             raise ValueError(f"offsets of {self.sequences} sequences have {self.sequences + 1} entries, got {offsets.numel()}")
@@ -83,6 +91,8 @@ class PageTable:
     def free(self, which: torch.Tensor) -> None:
         """The sequences numbered in ``which`` (int32 on the GPU) end: their length is 0, their pages have one user less.  Numbers that are
         no sequence's (-1, say) are left out."""
+        if _k.host_calls.pages_free(self._native, which):
+            return
         self._entries(which, "which")
         if which.numel() == 0:
             return
@@ -96,6 +106,9 @@ class PageTable:
         full, -1 where none is to be copied (the first heir of a parent that is itself replaced keeps its page).  A child whose page was
         not to be had is left empty and counted in ``missing``.  Of several entries for a child the first counts; an entry with a number that
         is no sequence's is left out."""
+        moves = _k.host_calls.pages_fork(self._native, parents, children)
+        if moves is not None:
+            return moves
         self._entries(parents, "parents")
         self._entries(children, "children")
         count = parents.numel()
@@ -114,6 +127,9 @@ class PageTable:
     def compact(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """The used pages become the lowest ones: those that lie too high move, in their order, to the free ones below.  Returns ``(sources,
         targets)`` for ``KeyValueCache.copy``, int32 ``[pages // 2]``, filled up with -1, to be called for the cache of every layer."""
+        moves = _k.host_calls.pages_compact(self._native)
+        if moves is not None:
+            return moves
         sources, targets = self._int32(self.pages // 2), self._int32(self.pages // 2)
         with _k.on_device(self.device):
             _k.check(_k.lib.bsa_pages_compact(*self._pointers(3), sources.data_ptr() or None, targets.data_ptr() or None, *self._sizes(),
