@@ -128,6 +128,25 @@ __device__ __forceinline__ float larger(float most, float x)      // of magnitud
 }
 __device__ __forceinline__ bool is_finite(float x) { return __builtin_fabsf(x) < __builtin_inff(); }
 
+// x y of a 16-bit x: fp16 is widened by the product itself
+template <bool BF>
+__device__ __forceinline__ float times(half_t x, float y) { return BF ? widen_16<BF>(x) * y : __builtin_fmaf((float)x, y, 0.f); }
+// Two values as sums of TERMS 16-bit ones.  All but the last are cut, not rounded, in fp16 (one instruction for two); what is left is exact.
+template <bool BF, int TERMS>
+__device__ __forceinline__ void in_parts(float x0, float x1, h2 (&parts)[TERMS])
+{
+#pragma unroll
+    for (int e = 0; e < TERMS; ++e) {
+        if (!BF && e + 1 < TERMS) parts[e] = __builtin_bit_cast(h2, __builtin_amdgcn_cvt_pkrtz(x0, x1));
+        else parts[e] = h2{narrow_16<BF>(x0), narrow_16<BF>(x1)};
+        if (e + 1 < TERMS) {
+            const half_t a = parts[e][0], b = parts[e][1];
+            x0 = BF ? x0 - widen_16<BF>(a) : __builtin_fmaf((float)a, -1.f, x0);
+            x1 = BF ? x1 - widen_16<BF>(b) : __builtin_fmaf((float)b, -1.f, x1);
+        }
+    }
+}
+
 // Chunks of OPERANDS operands on their way to LDS, fetched by all NW waves of a workgroup
 template <int HD, int OPERANDS, int NW>
 struct LinearTiles {
@@ -151,16 +170,15 @@ struct LinearTiles {
         base[o] = (const unsigned char *)(x.x + first_token * x.token + head * x.head);
         stride[o] = (unsigned)(2 * x.token);
     }
-    // `valid` tokens from `token` on, those behind as the last
-    __device__ __forceinline__ void request(int o, int token, int valid, int stage) const
+    // `valid` tokens from base on, those behind as the last
+    __device__ __forceinline__ void request(int o, int valid, int stage) const
     {
-        const unsigned char *from = base[o] + (long long)token * stride[o];
         const unsigned to = lds + (unsigned)(stage * STAGE + o * TILE);
 #pragma unroll
         for (int i = 0; i < EACH; ++i) {
             // a request is 8 rows of a panel of 64 columns: two waves fetch rows 16 apart, four a panel each time, eight both panels at once
             const int r = NW == 2 ? row + 16 * i : row, there = r < valid ? r : valid - 1;
-            dma16(from + (NW == 4 ? 128 * i : 0), (unsigned)there * stride[o] + piece, to + (NW == 2 ? 2048 * i : 4096 * i));
+            dma16(base[o] + (NW == 4 ? 128 * i : 0), (unsigned)there * stride[o] + piece, to + (NW == 2 ? 2048 * i : 4096 * i));
         }
     }
 };
@@ -187,15 +205,21 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     const int from = item.segment * p.segment, here = min(item.n - from, p.segment);
     const int chunks = (here + LA_ROWS - 1) / LA_ROWS, steps = chunks * inner;
     const long long begin = (long long)item.begin + from;
-    int next = 0, next_inner = 0, next_stage = 0;          // the step requested next
-    auto request = [&]() {
-        const int at = LA_ROWS * (BACKWARDS ? chunks - 1 - next : next), valid = min(here - at, LA_ROWS);
+    int next = 0, next_inner = 0, next_stage = 0;          // the step requested next, whose chunk and heads tiles.base has
+    long long chunk_step[OPERANDS];
 #pragma unroll
-        for (int o = 0; o < OPERANDS; ++o) tiles.request(o, at, valid, next_stage);
+    for (int o = 0; o < OPERANDS; ++o) {
+        chunk_step[o] = (BACKWARDS ? -LA_ROWS : LA_ROWS) * (long long)tiles.stride[o] + (1 - inner) * inner_step[o];
+        if (BACKWARDS && chunks > 1) tiles.base[o] += (long long)LA_ROWS * (chunks - 1) * tiles.stride[o];
+    }
+    auto request = [&]() {
+        const int valid = min(here - LA_ROWS * (BACKWARDS ? chunks - 1 - next : next), LA_ROWS);
+#pragma unroll
+        for (int o = 0; o < OPERANDS; ++o) tiles.request(o, valid, next_stage);
         next_stage = next_stage == LA_STAGES - 1 ? 0 : next_stage + 1;
         const bool wrap = ++next_inner == inner;
 #pragma unroll
-        for (int o = 0; o < OPERANDS; ++o) tiles.base[o] += wrap ? (1 - inner) * inner_step[o] : inner_step[o];
+        for (int o = 0; o < OPERANDS; ++o) tiles.base[o] += wrap ? chunk_step[o] : inner_step[o];
         if (wrap) next_inner = 0, ++next;
     };
     if (steps > 0) request();
@@ -334,8 +358,6 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         if (step + 1 < steps) tile_wait<Tiles::REQUESTS>();
         else tile_wait<0>();
         asm volatile("s_barrier" ::: "memory");
-        if (RESULT) store();
-        if (step + 2 < steps) request();
         const int at = LA_ROWS * chunk, valid = min(here - at, LA_ROWS);
         const unsigned tile = (unsigned)(stage * Tiles::STAGE);
         if (valid != decays_of) set_decays(valid);
@@ -387,7 +409,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             for (int j = 0; j < 4; ++j) {
                 const half_t one = cop[u >> 1][4 * (u & 1) + j];
                 float &to_enter = x[u >> 1][4 * (u & 1) + j];
-                to_enter = widen_16<BF>(one) * (enter[u][j] * (BF ? with : with * s_mul));
+                to_enter = times<BF>(one, enter[u][j] * (BF ? with : with * s_mul));
                 if (!BF) x_most = larger(x_most, to_enter);
             }
         if (!BF) {                       // it has to fit, and the state with it
@@ -486,19 +508,19 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             issue_order();
             read_b_columns(0);
             issue_order();
+            store();
         }
+        // while the products run: memory takes its time to accept the next chunk's requests
+        if (step + 2 < steps) request();
         h8 cw[TERMS][2];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float left = x[s][j];
+            for (int j = 0; j < 8; j += 2) {
+                h2 parts[TERMS];
+                in_parts<BF, TERMS>(x[s][j], x[s][j + 1], parts);
 #pragma unroll
-                for (int e = 0; e < TERMS; ++e) {
-                    cw[e][s][j] = narrow_16<BF>(left);
-                    const half_t one = cw[e][s][j];
-                    if (e + 1 < TERMS) left -= widen_16<BF>(one);
-                }
+                for (int e = 0; e < TERMS; ++e) cw[e][s][j] = parts[e][0], cw[e][s][j + 1] = parts[e][1];
             }
         h8 pop[2];
         f16v part = {0};
@@ -506,9 +528,9 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         if (RESULT) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
-                prob[v] *= BF ? decays[v >> 2][v & 3] : decays[v >> 2][v & 3] * p_mul;
+                prob[v] *= decays[v >> 2][v & 3];
                 if (!BF) p_most = larger(p_most, prob[v]);
-                pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
+                pop[v >> 3][v & 7] = narrow_16<BF>(BF ? prob[v] : __builtin_fmaf(prob[v], p_mul, 0.f));
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
@@ -534,17 +556,13 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
             for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(part[v]);
             if (!BF) {                   // P too large for fp16, or all of it too small
-                const bool large = p_most >= 0x1p15f, fair = p_most >= 1.f;
+                const bool large = p_most * p_mul >= 0x1p15f, fair = p_most * p_mul >= 1.f;
                 if (__builtin_amdgcn_ballot_w64(large) != 0ull || __builtin_amdgcn_ballot_w64(fair) == 0ull) {
                     const float all = wave_most(is_finite(p_most) ? p_most : 0.f);
                     if (all > 0.f) {
-                        const float to_mul = fminf(fmaxf(p_mul * lift_of(all, 8), 0x1p-60f), 0x1p60f), by = to_mul * __builtin_amdgcn_rcpf(p_mul);
-                        p_mul = to_mul;
+                        p_mul = fminf(fmaxf(lift_of(all, 8), 0x1p-60f), 0x1p60f);
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) {
-                            prob[v] *= by;
-                            pop[v >> 3][v & 7] = narrow_16<BF>(prob[v]);
-                        }
+                        for (int v = 0; v < 16; ++v) pop[v >> 3][v & 7] = narrow_16<BF>(prob[v] * p_mul);
                         part = f16v{0};
 #pragma unroll
                         for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
@@ -559,7 +577,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                 // and left out of c it makes NaN of its column for those that see it.
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    const float weight = sees(8 * (v >> 2) + 4 * h + (v & 3), valid) ? prob[v] : 0.f;
+                    const float weight = sees(8 * (v >> 2) + 4 * h + (v & 3), valid) ? (BF ? prob[v] : prob[v] * p_mul) : 0.f;
                     pop[v >> 3][v & 7] = narrow_16<BF>(weight);
                 }
                 h8 clean[1][2] = {{cop[0], cop[1]}};
