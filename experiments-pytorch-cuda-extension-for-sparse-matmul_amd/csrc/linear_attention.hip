@@ -66,7 +66,8 @@ __device__ __forceinline__ int linear_offset(const LinearWalk &p, int b)
     return x < 0 ? 0 : x > p.tokens ? p.tokens : x;
 }
 
-// Slot floor(offset / segment) + b is the first of sequence b, ascending in b, and an empty sequence has one: 64 lanes search together.
+// Slot floor(offset / segment) + b is the first of sequence b, ascending in b, and an empty sequence has one: 64 lanes search together,
+// up to 64 sequences by one look at the offsets.
 __device__ __forceinline__ LinearItem linear_item(const LinearWalk &p, int block)
 {
     LinearItem item{0, 0, 0, 0, 0, 0, false};
@@ -77,19 +78,20 @@ __device__ __forceinline__ LinearItem linear_item(const LinearWalk &p, int block
     if (slot >= p.slots) return item;
     const unsigned length = (unsigned)p.segment;
     const int l = lane_id();
-    int first = 0, count = p.sequences;
-    while (true) {
-        const int stride = (count + 63) / 64, b = first + l * stride;
-        const bool before = b < first + count && (int)((unsigned)linear_offset(p, b) / length) + b <= slot;
-        const int seen = __popcll(__builtin_amdgcn_ballot_w64(before));
-        const int skip = (seen > 0 ? seen - 1 : 0) * stride;
-        first += skip;
-        count = count - skip < stride ? count - skip : stride;
-        if (stride == 1) break;
-    }
+    int first = 0, count = p.sequences, stride, lane, from, to;
+    do {
+        stride = (count + WAVE - 1) / WAVE;
+        const int b = first + l * stride;
+        const bool there = b < first + count;
+        from = linear_offset(p, there ? b : p.sequences), to = linear_offset(p, there ? b + 1 : p.sequences);
+        const int seen = __popcll(__builtin_amdgcn_ballot_w64(there && (int)((unsigned)from / length) + b <= slot));
+        lane = seen > 0 ? seen - 1 : 0;
+        first += lane * stride;
+        count = count - lane * stride < stride ? count - lane * stride : stride;
+    } while (stride > 1);
     item.sequence = __builtin_amdgcn_readfirstlane(first);
-    item.begin = __builtin_amdgcn_readfirstlane(linear_offset(p, item.sequence));
-    const int end = __builtin_amdgcn_readfirstlane(linear_offset(p, item.sequence + 1));
+    item.begin = __builtin_amdgcn_readlane(from, lane);
+    const int end = __builtin_amdgcn_readlane(to, lane);
     item.n = end > item.begin ? end - item.begin : 0;
     item.segment = slot - ((int)((unsigned)item.begin / length) + item.sequence);
     item.segments = item.n > 0 ? (int)(((unsigned)item.n + length - 1) / length) : 1;
@@ -257,7 +259,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     int age = 0;
     float owed = 1.f;                    // that decay
     bool shrunk = false, dwarfed = false;        // it has got some of it, or was made small for what entered: too small for fp16 operands?
-    bool zero = true;                    // nothing entered so far
+    bool zero = true;                    // nothing entered so far, or (fp16) only zeros
     const int column = 32 * w + perm16(i);
     auto row_of = [&](int t, int v) { return 32 * t + (v & 3) + 4 * ((v >> 2) & 1) + 8 * h + 16 * (v >> 3); };
     auto state_most = [&]() {
@@ -310,7 +312,10 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             // arrived: the compiler would wait for them inside the loop, and with them for the chunks on their way
 #pragma unroll
             for (int t = 0; t < DT; ++t) asm volatile("" : "+v"(state[t]));
-            if (!BF) lift_state();
+            if (!BF) {
+                lift_state();
+                zero = s_mul == 1.f && state_most() == 0.f;
+            }
         }
     }
 
@@ -412,6 +417,27 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                 to_enter = times<BF>(one, enter[u][j] * (BF ? with : with * s_mul));
                 if (!BF) x_most = larger(x_most, to_enter);
             }
+        bool some_enters = true, small = false;
+        auto look_at_entering = [&](float most) {
+            some_enters = __builtin_amdgcn_ballot_w64(most > 0.f) != 0ull;
+            small = __builtin_amdgcn_ballot_w64(most >= 1.f) == 0ull;
+        };
+        auto entering_most = [&]() {
+            float most = 0.f;
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) most = larger(most, x[s][j]);
+            return most;
+        };
+        auto scale_entering = [&](float by) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[s][j] *= by;
+            look_at_entering(entering_most());
+        };
+        if (!BF) look_at_entering(x_most);
         if (!BF) {                       // it has to fit, and the state with it
             if ((zero || __builtin_amdgcn_ballot_w64(x_most >= 0x1p15f) != 0ull) && enters) {
                 const float all = wave_most(is_finite(x_most) ? x_most : 0.f);
@@ -422,10 +448,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                         scale_state(by);
                         dwarfed = true;
                     }
-#pragma unroll
-                    for (int s = 0; s < 2; ++s)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) x[s][j] *= by;
+                    scale_entering(by);
                 }
             }
             if (RESULT && fresh && (shrunk || dwarfed)) {
@@ -442,10 +465,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                         if (__builtin_amdgcn_ballot_w64(x_most * by >= 0x1p15f) == 0ull) {
                             scale_state(by);
                             s_mul *= by;
-#pragma unroll
-                            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) x[s][j] *= by;
+                            scale_entering(by);
                         } else {
                             o_mul = by;
                             dwarfed = true;
@@ -491,10 +511,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                         if (broken) {
                             const float was = s_mul;
                             lift_state();
-#pragma unroll
-                            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) x[s][j] *= s_mul * __builtin_amdgcn_rcpf(was);
+                            scale_entering(s_mul * __builtin_amdgcn_rcpf(was));
                         }
                         meet(o_mul);
                     }
@@ -512,6 +529,14 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         }
         // while the products run: memory takes its time to accept the next chunk's requests
         if (step + 2 < steps) request();
+        float with_decay = 1.f;
+        if (!BF && gets && enters && small && some_enters) {
+            // small beside the state, but not beside what its decay leaves of it: in the backward direction it comes with that decay itself
+            const float to_mul = fminf(s_mul * lift_of(wave_most(entering_most()), 10), 0x1p60f);
+            with_decay = to_mul * __builtin_amdgcn_rcpf(s_mul);
+            s_mul = to_mul;
+            scale_entering(with_decay);
+        }
         h8 cw[TERMS][2];
 #pragma unroll
         for (int s = 0; s < 2; ++s)
@@ -536,11 +561,11 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
         }
         if (enters) {
-            if (gets) scale_state(linear_power(log2_decay, aged));
+            if (gets) scale_state(linear_power(log2_decay, aged) * with_decay);
             if (!BF) shrunk = shrunk || gets;
             age = gets ? 0 : aged;
             owed = gets ? 1.f : linear_power(log2_decay, age);
-            zero = false;
+            zero = !BF && zero && !some_enters;
 #pragma unroll
             for (int t = 0; t < DT; t += 2) {
                 const h8 now[4] = {bop[0], bop[1], bop[2], bop[3]};
@@ -814,14 +839,26 @@ size_t linear_workspace_bytes(const LinearArgs &a)
     if (a.tokens <= a.segment) return 0;
     return sizeof(float) * (size_t)((a.tokens - 1) / a.segment) * a.key_heads * a.head_dim * a.head_dim;
 }
-// Segments of which every compute unit has its workgroups at once (two at head dim 128, four at 64), no more: a second generation would leave
-// most of the machine idle at its end, and every boundary is a state to write and read.
+// Large batches: segments of which every compute unit has its workgroups at once (two at head dim 128, four at 64) and no more: a second
+// generation would leave most of the machine idle at its end, and every boundary is a state to write and read.  65519 tokens, 4 key
+// heads, head dim 128: 153 us with the 500 workgroups of segments of 544 tokens, 190 with 512 tokens, 184 with 800.
+// Others: two walks a segment long (0.06 us a token together) and the running sum over the boundaries (0.1 us each) are shortest
+// together at sqrt(1.5 length).  One sequence of 65536, a head, head dim 64: 50 us with 384 tokens, 69 with 128, 74 with 1024; six texts of 1 to
+// 1500, 12 heads: 30 us with 96 or 128, 41 with 32, 37 with 384.  The lengths are on the device, so this goes by their mean; up to 192 the two
+// launches in front of the walk take longer than they save.
 int linear_segment(int tokens, int sequences, int key_heads, int head_dim)
 {
     const int room = 512 * (head_dim == 64 ? 2 : 1) / key_heads;
     const int parts = room - (sequences < room / 2 ? sequences : room / 2);
-    const int segment = ((tokens + (parts > 0 ? parts : 1) - 1) / (parts > 0 ? parts : 1) + LA_ROWS - 1) / LA_ROWS * LA_ROWS;
-    return segment < 256 ? 256 : segment > 8192 ? 8192 : segment;
+    const long long fill = ((long long)tokens + (parts > 0 ? parts : 1) - 1) / (parts > 0 ? parts : 1);
+    const int mean = tokens / sequences;
+    int least = 512;
+    if (mean > 192) {
+        least = 96;
+        while (least < 512 && (long long)least * least * 2 < 3ll * mean) least += LA_ROWS;
+    }
+    const long long segment = (fill + LA_ROWS - 1) / LA_ROWS * LA_ROWS;
+    return segment < least ? least : segment > 8192 ? 8192 : (int)segment;
 }
 
 hipError_t launch_linear_forward(const LinearArgs &a, hipStream_t st)

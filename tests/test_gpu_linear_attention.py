@@ -139,6 +139,30 @@ def test_decays(log_decay, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("log_decay", [-8.0, -15.0, -25.0, -41.0])
+@pytest.mark.parametrize("lengths", [[90, 33], [600]])
+def test_what_enters_is_small_beside_a_state_that_goes(lengths, log_decay, dtype):
+    """Towards the front every token's part comes with its own decay, to a state that still has dlast's size and is nothing after.
+    Of 2^-59 the exponent alone is rounded by 2^-19, more than the 1e-6 of the norms."""
+    x = inputs(lengths, 2, 1, 64, dtype)
+    x["log_decay"].fill_(log_decay)
+    check(x, run(x), norms=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("states", [False, True])
+def test_small_values_behind_zeros(states, dtype):
+    """Chunks of zeros say nothing about the size of what comes; 2^-13 of it has few bits in fp16 beside a state of nothing."""
+    x = inputs([150, 70], 2, 1, 64, dtype, mul=2.0 ** -13)
+    x["v"][:64] = 0
+    x["dout"][-64:] = 0
+    if states:
+        x["states"].zero_()
+        x["dlast"].zero_()
+    check(x, run(x), norms=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.0])
 def test_scales(scale, dtype):
     x = inputs([70], 2, 1, 128, dtype)
