@@ -48,15 +48,25 @@ __device__ __forceinline__ int block_prefix(int x, int *parts, int &all)
 template <class Taken>
 __device__ __forceinline__ int lowest_free(const int32_t *uses, int pages, int wanted, int *parts, Taken taken)
 {
-    int found = 0;
+    int found = 0, next[4];
+    auto fetch = [&](int at) {
+        if (at + 4 <= pages) {
+            const int4 x = *reinterpret_cast<const int4 *>(uses + at);
+            next[0] = x.x, next[1] = x.y, next[2] = x.z, next[3] = x.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) next[j] = at + j < pages ? uses[at + j] : 1;
+        }
+    };
+    if (wanted > 0) fetch(4 * (int)threadIdx.x);
     for (int first = 0; first < pages && found < wanted; first += 4 * PG_THREADS) {
         const int at = first + 4 * (int)threadIdx.x;
         int use[4], mine = 0, all;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            use[j] = at + j < pages ? uses[at + j] : 1;
-            mine += use[j] == 0 ? 1 : 0;
-        }
+        for (int j = 0; j < 4; ++j) use[j] = next[j];
+        fetch(at + 4 * PG_THREADS);                      // on their way while these are counted
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mine += use[j] == 0 ? 1 : 0;
         int rank = found + block_prefix(mine, parts, all);
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -211,45 +221,56 @@ __device__ __forceinline__ int32_t *fork_row(const PagesArgs &p, int i) { return
 __device__ __forceinline__ ForkEntry &fork_entry(const PagesArgs &p, int i) { return *reinterpret_cast<ForkEntry *>(fork_row(p, i) + p.width); }
 
 // Of the entries for a child the first counts; of the entries that continue a parent which is itself replaced, the first keeps its last
-// page.  by_child, by_parent: their places among the entries, or none.
-__device__ __forceinline__ void fork_claims(const PagesArgs &p, int *by_child, int *by_parent)
+// page.  by_child, by_parent: their places among the entries, or none; heirs: how many entries continue a sequence.
+struct ForkClaims {
+    int by_child[PG_MOST], by_parent[PG_MOST], heirs[PG_MOST];
+};
+constexpr int PG_NONE = 0x7FFFFFFF;
+__device__ __forceinline__ void fork_claims(const PagesArgs &p, ForkClaims &claims)
 {
-    const int none = 0x7FFFFFFF;
-    for (int b = (int)threadIdx.x; b < p.sequences; b += (int)blockDim.x) by_child[b] = by_parent[b] = none;
+    for (int b = (int)threadIdx.x; b < p.sequences; b += (int)blockDim.x) {
+        claims.by_child[b] = claims.by_parent[b] = PG_NONE;
+        claims.heirs[b] = 0;
+    }
     __syncthreads();
     auto inside = [&](int x) { return x >= 0 && x < p.sequences; };
     for (int i = (int)threadIdx.x; i < p.entries; i += (int)blockDim.x)
-        if (inside(p.parents[i]) && inside(p.children[i])) atomicMin(by_child + p.children[i], i);
+        if (inside(p.parents[i]) && inside(p.children[i])) atomicMin(claims.by_child + p.children[i], i);
     __syncthreads();
     for (int i = (int)threadIdx.x; i < p.entries; i += (int)blockDim.x)
-        if (inside(p.parents[i]) && inside(p.children[i]) && by_child[p.children[i]] == i) atomicMin(by_parent + p.parents[i], i);
+        if (inside(p.parents[i]) && inside(p.children[i]) && claims.by_child[p.children[i]] == i) {
+            atomicMin(claims.by_parent + p.parents[i], i);
+            atomicAdd(claims.heirs + p.parents[i], 1);
+        }
     __syncthreads();
 }
 
-// one entry: its parent's row into scratch, uses of what it shares and of what the child had
-__device__ __forceinline__ void fork_share(const PagesArgs &p, int i, const int *by_child, const int *by_parent)
+// One entry, by the threads `thread` of `threads`: its parent's row into scratch, uses of what the child had and, by a parent's first heir
+// for all of them, of what they share.  The parent's last page, where it is not full, is the first heir's if the parent itself is
+// replaced, and nobody's share.
+__device__ __forceinline__ void fork_share(const PagesArgs &p, int i, const ForkClaims &claims, int thread, int threads)
 {
-    const int none = 0x7FFFFFFF, parent = p.parents[i], child = p.children[i];
-    const bool there = parent >= 0 && parent < p.sequences && child >= 0 && child < p.sequences && by_child[child] == i;
+    const int parent = p.parents[i], child = p.children[i];
+    const bool there = parent >= 0 && parent < p.sequences && child >= 0 && child < p.sequences && claims.by_child[child] == i;
     ForkEntry entry{-1, 0, 0, 0};
     if (there) {
         entry.tokens = length_of(p, parent);
         entry.old_pages = pages_of(length_of(p, child), p.page_shift);
-        const bool partial = (entry.tokens & ((1 << p.page_shift) - 1)) != 0;
-        entry.copies = partial && (by_child[parent] == none || by_parent[parent] != i);
-        const int count = pages_of(entry.tokens, p.page_shift), shared = count - entry.copies;
+        const bool first = claims.by_parent[parent] == i;
+        const int whole = entry.tokens >> p.page_shift, count = pages_of(entry.tokens, p.page_shift);
+        entry.copies = count > whole && (claims.by_child[parent] == PG_NONE || !first);
         int32_t *row = fork_row(p, i);
-        for (int j = (int)threadIdx.x; j < count; j += (int)blockDim.x) {
+        for (int j = thread; j < count; j += threads) {
             const int page = p.table[(size_t)parent * p.width + j];
             row[j] = page;
-            if (j < shared && is_page(p, page)) atomicAdd(p.uses + page, 1);
+            if (first && is_page(p, page) && (j < whole || entry.copies == 0)) atomicAdd(p.uses + page, j < whole ? claims.heirs[parent] : 1);
         }
-        for (int j = (int)threadIdx.x; j < entry.old_pages; j += (int)blockDim.x) {
+        for (int j = thread; j < entry.old_pages; j += threads) {
             const int page = p.table[(size_t)child * p.width + j];
             if (is_page(p, page)) atomicAdd(p.uses + page, -1);
         }
     }
-    if (threadIdx.x == 0) fork_entry(p, i) = entry;
+    if (thread == 0) fork_entry(p, i) = entry;
 }
 
 // pages for the copies, by one workgroup; an entry that gets none leaves its child empty
@@ -291,27 +312,40 @@ __device__ __forceinline__ void fork_allocate(const PagesArgs &p, int *parts)
         if (fork_entry(p, i).tokens >= 0) p.lengths[p.children[i]] = fork_entry(p, i).tokens;
 }
 
-__device__ __forceinline__ void fork_place(const PagesArgs &p, int i)
+__device__ __forceinline__ void fork_place(const PagesArgs &p, int i, int thread, int threads)
 {
     const ForkEntry entry = fork_entry(p, i);
     if (entry.tokens < 0) return;
     const int count = pages_of(entry.tokens, p.page_shift), old = entry.old_pages;
     int32_t *to = p.table + (size_t)p.children[i] * p.width;
-    for (int j = (int)threadIdx.x; j < (count > old ? count : old); j += (int)blockDim.x) to[j] = j < count ? fork_row(p, i)[j] : -1;
+    for (int j = thread; j < (count > old ? count : old); j += threads) to[j] = j < count ? fork_row(p, i)[j] : -1;
 }
 
 __global__ __launch_bounds__(256) void pages_share_kernel(PagesArgs p)
 {
-    __shared__ int by_child[PG_MOST], by_parent[PG_MOST];
-    fork_claims(p, by_child, by_parent);
-    fork_share(p, (int)blockIdx.x, by_child, by_parent);
+    __shared__ ForkClaims claims;
+    fork_claims(p, claims);
+    fork_share(p, (int)blockIdx.x, claims, (int)threadIdx.x, 256);
 }
 __global__ __launch_bounds__(PG_THREADS) void pages_allocate_kernel(PagesArgs p)
 {
     __shared__ int parts[PG_WAVES];
     fork_allocate(p, parts);
 }
-__global__ __launch_bounds__(256) void pages_place_kernel(PagesArgs p) { fork_place(p, (int)blockIdx.x); }
+__global__ __launch_bounds__(256) void pages_place_kernel(PagesArgs p) { fork_place(p, (int)blockIdx.x, (int)threadIdx.x, 256); }
+// the three in one, a wave an entry
+__global__ __launch_bounds__(PG_THREADS) void pages_fork_kernel(PagesArgs p)
+{
+    __shared__ ForkClaims claims;
+    __shared__ int parts[PG_WAVES];
+    fork_claims(p, claims);
+    for (int i = wave_id(); i < p.entries; i += PG_WAVES) fork_share(p, i, claims, lane_id(), WAVE);
+    __threadfence();                                     // counts of uses are made in memory, by atomics
+    __syncthreads();
+    fork_allocate(p, parts);
+    __syncthreads();
+    for (int i = wave_id(); i < p.entries; i += PG_WAVES) fork_place(p, i, lane_id(), WAVE);
+}
 
 // ---- what is left moves together ----------------------------------------------------------------------
 // The used pages number `used` and up move, in their order, into the free ones below.  scratch: [0] used, then the new number of every page.
@@ -319,24 +353,32 @@ __global__ __launch_bounds__(PG_THREADS) void pages_moves_kernel(PagesArgs p)
 {
     __shared__ int parts[PG_WAVES];
     int mine = 0, used;
+#pragma unroll 8
     for (int i = (int)threadIdx.x; i < p.pages; i += PG_THREADS) mine += p.uses[i] > 0 ? 1 : 0;
     block_prefix(mine, parts, used);
     if (threadIdx.x == 0) p.scratch[0] = used;
     const int holes = lowest_free(p.uses, used, used, parts, [&](int rank, int page) { p.targets[rank] = page; });
     __syncthreads();
     int moved = 0;
-    for (int first = used; first < p.pages && moved < holes; first += PG_THREADS) {
-        const int at = first + (int)threadIdx.x;
-        const int use = at < p.pages ? p.uses[at] : 0;
-        int all;
-        const int rank = moved + block_prefix(use > 0 ? 1 : 0, parts, all);
-        if (use > 0 && rank < holes) {
-            const int to = p.targets[rank];
-            p.sources[rank] = at;
-            p.scratch[1 + at] = to;
-            p.uses[to] = use;
-            p.uses[at] = 0;
+    for (int first = used; first < p.pages && moved < holes; first += 4 * PG_THREADS) {
+        const int at = first + 4 * (int)threadIdx.x;
+        int use[4], some = 0, all;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            use[j] = at + j < p.pages ? p.uses[at + j] : 0;
+            some += use[j] > 0 ? 1 : 0;
         }
+        int rank = moved + block_prefix(some, parts, all);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (use[j] > 0 && rank < holes) {
+                const int to = p.targets[rank];
+                p.sources[rank] = at + j;
+                p.scratch[1 + at + j] = to;
+                p.uses[to] = use[j];
+                p.uses[at + j] = 0;
+                ++rank;
+            }
         moved += all;
     }
     for (int i = holes + (int)threadIdx.x; i < p.entries; i += PG_THREADS) p.sources[i] = p.targets[i] = -1;
@@ -391,6 +433,8 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(PageCopyArgs p)
 
 }  // namespace
 
+constexpr int FORK_ALONE = 16384;
+
 size_t pages_fork_scratch(int entries, int width) { return (size_t)entries * (width + 4) * sizeof(int32_t); }
 
 hipError_t launch_pages_append(const PagesArgs &p, hipStream_t st)
@@ -411,6 +455,11 @@ hipError_t launch_pages_free(const PagesArgs &p, hipStream_t st)
 }
 hipError_t launch_pages_fork(const PagesArgs &p, hipStream_t st)
 {
+    // rows that one workgroup is through with sooner than two more launches
+    if ((long long)p.entries * p.width <= FORK_ALONE) {
+        pages_fork_kernel<<<1, PG_THREADS, 0, st>>>(p);
+        return hipGetLastError();
+    }
     pages_share_kernel<<<p.entries, 256, 0, st>>>(p);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
