@@ -262,12 +262,16 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     bool zero = true;                    // nothing entered so far, or (fp16) only zeros
     const int column = 32 * w + perm16(i);
     auto row_of = [&](int t, int v) { return 32 * t + (v & 3) + 4 * ((v >> 2) & 1) + 8 * h + 16 * (v >> 3); };
-    auto state_most = [&]() {
+    auto lane_most = [&]() {
         float most = 0.f;
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll
             for (int v = 0; v < 16; ++v) most = larger(most, state[t][v]);
+        return most;
+    };
+    auto state_most = [&]() {
+        const float most = lane_most();
         return wave_most(is_finite(most) ? most : 0.f);
     };
     auto scale_state = [&](float by) {
@@ -312,9 +316,9 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             // arrived: the compiler would wait for them inside the loop, and with them for the chunks on their way
 #pragma unroll
             for (int t = 0; t < DT; ++t) asm volatile("" : "+v"(state[t]));
-            if (!BF) {
+            if (!BF && steps > 0) {      // an empty sequence's comes out as it went in
+                zero = __builtin_amdgcn_ballot_w64(lane_most() > 0.f) == 0ull;
                 lift_state();
-                zero = s_mul == 1.f && state_most() == 0.f;
             }
         }
     }

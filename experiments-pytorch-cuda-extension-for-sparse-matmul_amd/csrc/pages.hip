@@ -321,18 +321,28 @@ __device__ __forceinline__ void fork_place(const PagesArgs &p, int i, int thread
     for (int j = thread; j < (count > old ? count : old); j += threads) to[j] = j < count ? fork_row(p, i)[j] : -1;
 }
 
+// an entry a workgroup, or, where there are more of them, a wave
+template <class Work>
+__device__ __forceinline__ void each_entry(const PagesArgs &p, Work work)
+{
+    if ((int)gridDim.x == p.entries) return work((int)blockIdx.x, (int)threadIdx.x, 256);
+    for (int i = 4 * (int)blockIdx.x + wave_id(); i < p.entries; i += 4 * (int)gridDim.x) work(i, lane_id(), WAVE);
+}
 __global__ __launch_bounds__(256) void pages_share_kernel(PagesArgs p)
 {
     __shared__ ForkClaims claims;
     fork_claims(p, claims);
-    fork_share(p, (int)blockIdx.x, claims, (int)threadIdx.x, 256);
+    each_entry(p, [&](int i, int thread, int threads) { fork_share(p, i, claims, thread, threads); });
 }
 __global__ __launch_bounds__(PG_THREADS) void pages_allocate_kernel(PagesArgs p)
 {
     __shared__ int parts[PG_WAVES];
     fork_allocate(p, parts);
 }
-__global__ __launch_bounds__(256) void pages_place_kernel(PagesArgs p) { fork_place(p, (int)blockIdx.x, (int)threadIdx.x, 256); }
+__global__ __launch_bounds__(256) void pages_place_kernel(PagesArgs p)
+{
+    each_entry(p, [&](int i, int thread, int threads) { fork_place(p, i, thread, threads); });
+}
 // the three in one, a wave an entry
 __global__ __launch_bounds__(PG_THREADS) void pages_fork_kernel(PagesArgs p)
 {
@@ -433,7 +443,7 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(PageCopyArgs p)
 
 }  // namespace
 
-constexpr int FORK_ALONE = 16384;
+constexpr int FORK_GROUPS = 512;
 
 size_t pages_fork_scratch(int entries, int width) { return (size_t)entries * (width + 4) * sizeof(int32_t); }
 
@@ -455,18 +465,21 @@ hipError_t launch_pages_free(const PagesArgs &p, hipStream_t st)
 }
 hipError_t launch_pages_fork(const PagesArgs &p, hipStream_t st)
 {
-    // rows that one workgroup is through with sooner than two more launches
-    if ((long long)p.entries * p.width <= FORK_ALONE) {
+    // An entry a wave and a row one load: 11 us in one launch, 10.5 in three, which take the host 4 us longer.  16 entries of 256 pages: 14.3
+    // and 11.1 us, 64 of 32: 17.2 and 11.1.
+    if (p.entries <= PG_WAVES && p.width <= WAVE) {
         pages_fork_kernel<<<1, PG_THREADS, 0, st>>>(p);
         return hipGetLastError();
     }
-    pages_share_kernel<<<p.entries, 256, 0, st>>>(p);
+    // every workgroup goes through all entries for the claims: 4000 entries 99 us with a workgroup each, 55 with 512 of them
+    const int groups = p.entries < FORK_GROUPS ? p.entries : FORK_GROUPS;
+    pages_share_kernel<<<groups, 256, 0, st>>>(p);
     hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
     pages_allocate_kernel<<<1, PG_THREADS, 0, st>>>(p);
     err = hipGetLastError();
     if (err != hipSuccess) return err;
-    pages_place_kernel<<<p.entries, 256, 0, st>>>(p);
+    pages_place_kernel<<<groups, 256, 0, st>>>(p);
     return hipGetLastError();
 }
 hipError_t launch_pages_compact(const PagesArgs &p, hipStream_t st)

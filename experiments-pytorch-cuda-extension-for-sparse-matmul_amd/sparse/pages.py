@@ -5,6 +5,7 @@ The reference keeps nothing between calls.  The table, the lengths and the count
 knowing their lengths, so that these calls can be captured into a graph with the attention they serve.  One table serves all layers of a
 model: every layer has a ``KeyValueCache`` of its own with the same pages.
 """
+import operator
 from typing import Tuple
 
 import torch
@@ -80,12 +81,13 @@ class PageTable:
         check_index(offsets, "offsets", self.device, 1)
         if offsets.numel() != self.sequences + 1:
             raise ValueError(f"offsets of {self.sequences} sequences have {self.sequences + 1} entries, got {offsets.numel()}")
+        tokens = operator.index(tokens)
         if not 0 <= tokens <= MOST_ROWS:
             raise ValueError(f"{tokens} tokens")
-        slots = self._int32(tokens)
+        slots, scratch = self._int32(tokens), self._int32(self.sequences)
         with _k.on_device(self.device):
             _k.check(_k.lib.bsa_pages_append(*self._pointers(4), offsets.data_ptr(), slots.data_ptr() or None, tokens, *self._sizes(),
-                                             self._int32(self.sequences).data_ptr(), _k.current_stream()))
+                                             scratch.data_ptr(), _k.current_stream()))
         return slots
 
     def free(self, which: torch.Tensor) -> None:
@@ -130,8 +132,8 @@ class PageTable:
         moves = _k.host_calls.pages_compact(self._native)
         if moves is not None:
             return moves
-        sources, targets = self._int32(self.pages // 2), self._int32(self.pages // 2)
+        sources, targets, scratch = self._int32(self.pages // 2), self._int32(self.pages // 2), self._int32(self.pages + 1)
         with _k.on_device(self.device):
             _k.check(_k.lib.bsa_pages_compact(*self._pointers(3), sources.data_ptr() or None, targets.data_ptr() or None, *self._sizes(),
-                                              self._int32(self.pages + 1).data_ptr(), _k.current_stream()))
+                                              scratch.data_ptr(), _k.current_stream()))
         return sources, targets
