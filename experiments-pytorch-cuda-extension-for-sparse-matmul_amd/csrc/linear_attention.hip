@@ -130,6 +130,7 @@ __device__ __forceinline__ float larger(float most, float x)      // of magnitud
 }
 __device__ __forceinline__ bool is_finite(float x) { return __builtin_fabsf(x) < __builtin_inff(); }
 
+typedef __fp16 fp16x2 __attribute__((ext_vector_type(2)));          // as builtins take them
 // x y of a 16-bit x: fp16 is widened by the product itself
 template <bool BF>
 __device__ __forceinline__ float times(half_t x, float y) { return BF ? widen_16<BF>(x) * y : __builtin_fmaf((float)x, y, 0.f); }
@@ -143,8 +144,10 @@ __device__ __forceinline__ void in_parts(float x0, float x1, h2 (&parts)[TERMS])
         else parts[e] = h2{narrow_16<BF>(x0), narrow_16<BF>(x1)};
         if (e + 1 < TERMS) {
             const half_t a = parts[e][0], b = parts[e][1];
-            x0 = BF ? x0 - widen_16<BF>(a) : __builtin_fmaf((float)a, -1.f, x0);
-            x1 = BF ? x1 - widen_16<BF>(b) : __builtin_fmaf((float)b, -1.f, x1);
+            float minus = -1.f;          // not known to the compiler, which would widen and subtract and round: three instructions in the place of one
+            if (!BF) asm("" : "+s"(minus));
+            x0 = BF ? x0 - widen_16<BF>(a) : __builtin_fmaf((float)a, minus, x0);
+            x1 = BF ? x1 - widen_16<BF>(b) : __builtin_fmaf((float)b, minus, x1);
         }
     }
 }
@@ -208,21 +211,28 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     const int chunks = (here + LA_ROWS - 1) / LA_ROWS, steps = chunks * inner;
     const long long begin = (long long)item.begin + from;
     int next = 0, next_inner = 0, next_stage = 0;          // the step requested next, whose chunk and heads tiles.base has
-    long long chunk_step[OPERANDS];
 #pragma unroll
-    for (int o = 0; o < OPERANDS; ++o) {
-        chunk_step[o] = (BACKWARDS ? -LA_ROWS : LA_ROWS) * (long long)tiles.stride[o] + (1 - inner) * inner_step[o];
+    for (int o = 0; o < OPERANDS; ++o)
         if (BACKWARDS && chunks > 1) tiles.base[o] += (long long)LA_ROWS * (chunks - 1) * tiles.stride[o];
-    }
     auto request = [&]() {
         const int valid = min(here - LA_ROWS * (BACKWARDS ? chunks - 1 - next : next), LA_ROWS);
 #pragma unroll
         for (int o = 0; o < OPERANDS; ++o) tiles.request(o, valid, next_stage);
         next_stage = next_stage == LA_STAGES - 1 ? 0 : next_stage + 1;
-        const bool wrap = ++next_inner == inner;
+        // steps are made anew: kept, they are more scalars than there is room for
+        if (++next_inner == inner) {
+            next_inner = 0, ++next;
+            int back = inner - 1;
+            asm("" : "+s"(back));
 #pragma unroll
-        for (int o = 0; o < OPERANDS; ++o) tiles.base[o] += wrap ? chunk_step[o] : inner_step[o];
-        if (wrap) next_inner = 0, ++next;
+            for (int o = 0; o < OPERANDS; ++o) {
+                const long long chunk_step = (long long)LA_ROWS * tiles.stride[o];
+                tiles.base[o] += (BACKWARDS ? -chunk_step : chunk_step) - back * inner_step[o];
+            }
+        } else {
+#pragma unroll
+            for (int o = 0; o < OPERANDS; ++o) tiles.base[o] += inner_step[o];
+        }
     };
     if (steps > 0) request();
     if (steps > 1) request();
@@ -553,13 +563,21 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             }
         h8 pop[2];
         f16v part = {0};
-        float p_most = 0.f;
+        float p_size = 0.f;
         if (RESULT) {
+            if (!BF && p_mul != 1.f) {
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-                prob[v] *= decays[v >> 2][v & 3];
-                if (!BF) p_most = larger(p_most, prob[v]);
-                pop[v >> 3][v & 7] = narrow_16<BF>(BF ? prob[v] : __builtin_fmaf(prob[v], p_mul, 0.f));
+                for (int u = 0; u < 4; ++u) decays[u] *= p_mul;
+            }
+#pragma unroll
+            for (int v = 0; v < 16; ++v)
+                pop[v >> 3][v & 7] = narrow_16<BF>(BF ? prob[v] * decays[v >> 2][v & 3] : __builtin_fmaf(prob[v], decays[v >> 2][v & 3], 0.f));
+            if (!BF) {                   // the sum of their squares tells their size in half the instructions
+#pragma unroll
+                for (int v = 0; v < 16; v += 2) {
+                    const fp16x2 two = __builtin_bit_cast(fp16x2, h2{pop[v >> 3][v & 7], pop[v >> 3][(v & 7) + 1]});
+                    p_size = __builtin_amdgcn_fdot2(two, two, p_size, false);
+                }
             }
 #pragma unroll
             for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
@@ -585,13 +603,15 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
             for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(part[v]);
             if (!BF) {                   // P too large for fp16, or all of it too small
-                const bool large = p_most * p_mul >= 0x1p15f, fair = p_most * p_mul >= 1.f;
-                if (__builtin_amdgcn_ballot_w64(large) != 0ull || __builtin_amdgcn_ballot_w64(fair) == 0ull) {
+                if (__builtin_amdgcn_ballot_w64(p_size >= 0x1p28f) != 0ull || __builtin_amdgcn_ballot_w64(p_size >= 1.f) == 0ull) {
+                    float p_most = 0.f;
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) p_most = larger(p_most, prob[v] * between[8 * (v >> 2) + (v & 3)]);
                     const float all = wave_most(is_finite(p_most) ? p_most : 0.f);
                     if (all > 0.f) {
                         p_mul = fminf(fmaxf(lift_of(all, 8), 0x1p-60f), 0x1p60f);
 #pragma unroll
-                        for (int v = 0; v < 16; ++v) pop[v >> 3][v & 7] = narrow_16<BF>(prob[v] * p_mul);
+                        for (int v = 0; v < 16; ++v) pop[v >> 3][v & 7] = narrow_16<BF>(prob[v] * between[8 * (v >> 2) + (v & 3)] * p_mul);
                         part = f16v{0};
 #pragma unroll
                         for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
@@ -606,8 +626,8 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                 // and left out of c it makes NaN of its column for those that see it.
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
-                    const float weight = sees(8 * (v >> 2) + 4 * h + (v & 3), valid) ? (BF ? prob[v] : prob[v] * p_mul) : 0.f;
-                    pop[v >> 3][v & 7] = narrow_16<BF>(weight);
+                    const float weight = prob[v] * between[8 * (v >> 2) + (v & 3)] * (BF ? 1.f : p_mul);
+                    pop[v >> 3][v & 7] = narrow_16<BF>(sees(8 * (v >> 2) + 4 * h + (v & 3), valid) ? weight : 0.f);
                 }
                 h8 clean[1][2] = {{cop[0], cop[1]}};
                 take_out_not_finite<BF>(clean);
@@ -628,13 +648,12 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                     }
                 }
             }
-            const float down = BF ? 1.f : __builtin_amdgcn_rcpf(p_mul);
+            if (!BF && p_mul != 1.f) part *= __builtin_amdgcn_rcpf(p_mul);
             if (fresh) {
 #pragma unroll
-                for (int v = 0; v < 16; ++v) oacc[v] = __builtin_fmaf(oacc[v], up, BF ? part[v] : part[v] * down);
+                for (int v = 0; v < 16; ++v) oacc[v] = __builtin_fmaf(oacc[v], up, part[v]);
             } else {
-#pragma unroll
-                for (int v = 0; v < 16; ++v) oacc[v] = BF ? oacc[v] + part[v] : __builtin_fmaf(part[v], down, oacc[v]);
+                oacc += part;
             }
         }
         stage = stage == LA_STAGES - 1 ? 0 : stage + 1;
