@@ -398,10 +398,6 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
             for (int s = 0; s < 4; ++s) bop[s] = columns(b_at[s / 2], tile + b_tile + 4096u * (t / 2) + 2048u * (s % 2));
         };
-#pragma unroll
-        for (int s = 0; s < 2; ++s) cop[s] = columns(c_at, tile + c_tile + 2048u * s);
-#pragma unroll
-        for (int u = 0; u < 4; ++u) enter[u] = *reinterpret_cast<const f4v *>(entering + 8 * u);
         auto read_rows_of = [&](int first) {
 #pragma unroll
             for (int s = first; s < first + 4; ++s) {
@@ -409,14 +405,25 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                 b[s] = rows(tile + b_tile, s);
             }
         };
+        if (RESULT) read_rows_of(0);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) cop[s] = columns(c_at, tile + c_tile + 2048u * s);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) enter[u] = *reinterpret_cast<const f4v *>(entering + 8 * u);
+        if (!RESULT) read_b_columns(0);
+        issue_order();
+        // P's products run while what enters the state is made
+        f16v prob = {0};
         if (RESULT) {
-            read_rows_of(0);
+#pragma unroll
+            for (int s = 0; s < 4; ++s) prob = mfma_16<BF>(b[s], a[s], prob);
+            if (KS > 4) read_rows_of(4);
 #pragma unroll
             for (int u = 0; u < 4; ++u) decays[u] = *reinterpret_cast<const f4v *>(between + 8 * u);
-        } else {
-            read_b_columns(0);
+            issue_order();
+#pragma unroll
+            for (int s = 4; s < KS; ++s) prob = mfma_16<BF>(b[s], a[s], prob);
         }
-        issue_order();
         // What enters the state: c with its decay, times s_mul over the decay that the state has not got.
         const int aged = zero ? 0 : BACKWARDS && g > 0 ? age : age + valid;
         const bool gets = !(__builtin_fabsf(log2_decay * (float)aged) <= PUT_OFF);           // the state gets its decay with this chunk
@@ -489,7 +496,6 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                 shrunk = false;
             }
         }
-        f16v prob = {0};
         float up = 0.f;
         if (RESULT) {
             auto meet = [&](float by) {
@@ -506,11 +512,6 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                 oacc = f16v{0};
 #pragma unroll
                 for (int s = 0; s < KS; ++s) {
-                    if (s == 2 && KS > 4) {
-                        read_rows_of(4);
-                        issue_order();
-                    }
-                    prob = mfma_16<BF>(b[s], a[s], prob);
                     h8 op;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) op[j] = narrow_16<BF>(state[s / 2][8 * (s % 2) + j]);
@@ -531,10 +532,6 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                     }
                 }
                 up = since * owed * (BF ? 1.f : __builtin_amdgcn_rcpf(s_mul * o_mul));      // of a power of two: exact
-            } else {
-                if (KS > 4) read_rows_of(4);
-#pragma unroll
-                for (int s = 0; s < KS; ++s) prob = mfma_16<BF>(b[s], a[s], prob);
             }
             issue_order();
             read_b_columns(0);
