@@ -11,6 +11,15 @@
 // same four operands, share a workgroup.  Where a sequence has several segments, two launches in front make the state that each begins
 // with: every segment's own sum, then the running sum over segments.  Chunks travel straight to LDS two steps ahead of their use, in
 // a ring of three.
+//
+// What bounds it (times of launches, the least of 60):
+//   results: memory.  65519 tokens, 8 heads over 4, head dim 128, bf16: 100 us for 430 MB, operands, result and states (4.3 TB/s); one workgroup
+//   of the two on a compute unit gets what the other leaves and ends a fifth later.  24575 tokens, 16 heads, fp16: 93 us (4.7 TB/s).
+//   segments' sums: memory, 134 MB in 34 us (3.9 TB/s), 201 MB in 45; the running sum over them 11 to 14 us for 62 MB.
+//   dv and dk: the clocks of a step, 24575 tokens, 16 heads, head dim 128: 200 us for 400 MB; of 6.7k clocks a step the vector pipe works 45 %
+//   and the matrix pipe 27 %, two waves on each side of a barrier.  512 threads and 97 KB of LDS: one workgroup a compute unit.
+//   short texts: what a segment costs before its first product (5 us: its place, the state, the first chunks' way through memory) and
+//   1 us a chunk.  368 tokens, 12 heads, head dim 64: 12 us.
 #include "attention_tiles.hpp"
 #include "bsa_device.hpp"
 #include "bsa_internal.hpp"
@@ -734,7 +743,8 @@ __global__ __launch_bounds__(4 * HD, 2) void linear_keys_kernel(LinearWalk p, Li
     linear_walk<HD, BF, TERMS, true, true>(p, sum, item, w % (HD / 32), tiles, places, inner_step, dv.c_inner, lds_raw);
 }
 
-// every segment's own sum, of those that have a neighbour behind (BACKWARDS: in front)
+// every segment's own sum, of those that have a neighbour behind (BACKWARDS: in front): b and c are read once more than the results need them,
+// which costs less than a chain over the segments would
 template <int HD, bool BF, int TERMS, bool BACKWARDS>
 __global__ __launch_bounds__(2 * HD, 2) void linear_segments_kernel(LinearWalk p, LinearSum sum)
 {
@@ -750,7 +760,7 @@ __global__ __launch_bounds__(2 * HD, 2) void linear_segments_kernel(LinearWalk p
 }
 
 // The running sum over the segments of a sequence, in place: what each segment begins with.  A lane has four values of a state; the
-// segments' sums are requested RUN_AHEAD at a time.
+// segments' sums are requested RUN_AHEAD at a time: 30 states of each of 32 heads, 64 KB a state, 11.4 us (15.6 with one value a lane).
 constexpr int RUN_AHEAD = 16;
 template <bool BACKWARDS>
 __global__ __launch_bounds__(256) void linear_running_kernel(LinearWalk p, const float *__restrict__ first, int square)

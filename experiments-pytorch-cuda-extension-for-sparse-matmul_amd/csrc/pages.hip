@@ -7,7 +7,9 @@
 // calls give equal tables.  Counting is by integer atomics, whose order changes nothing.
 //
 // What bounds it: latency.  Ranks of free pages are found by one workgroup that reads `uses` 16 bytes a lane and sums up in LDS, as far as it
-// has to; rows of the table are read and written by a workgroup each.
+// has to; rows of the table are read and written by a workgroup each.  A step of 64 sequences 4.6 us, 24 prompts of 64 to 4096 tokens 6.3 and, their
+// slots, 3; a fork of 8 sequences to 504 children of up to 235 pages 8.4, 8.1 and 4.2 (three launches); a compaction of 6650 pages 8.3 and 1.5.
+// Copies of pages: memory, 5.7 TB/s (217 MB each way in 76 us).
 #include "bsa_device.hpp"
 #include "bsa_internal.hpp"
 
