@@ -1085,7 +1085,8 @@ static int pages_of_sequences(const char *who, int32_t *table, int32_t *lengths,
     const int shift = page == 32 ? 5 : page == 64 ? 6 : page == 128 ? 7 : page == 256 ? 8 : 0;
     if (shift == 0) return fail(BSA_ERR_UNSUPPORTED, "%s: pages of 32, 64, 128 and 256 tokens are built, got %d", who, page);
     if (pages < 1 || (long long)pages << shift > 2147483647LL) return fail(BSA_ERR_INVALID, "%s: %d pages of %d tokens", who, pages, page);
-    if (sequences < 1 || sequences > bsa::PAGES_MOST_SEQUENCES || width < 1 || (long long)width << shift > (1LL << 30))
+    if (sequences < 1 || sequences > bsa::PAGES_MOST_SEQUENCES || width < 1 || (long long)width << shift > (1LL << 30) ||
+        (long long)sequences * width > 2147483647LL)
         return fail(BSA_ERR_INVALID, "%s: %d sequences of %d pages of %d", who, sequences, width, page);
     if (entries < 0 || entries > bsa::PAGES_MOST_SEQUENCES)
         return fail(BSA_ERR_INVALID, "%s: %d entries, at most %d", who, entries, bsa::PAGES_MOST_SEQUENCES);

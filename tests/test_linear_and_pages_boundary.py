@@ -90,6 +90,7 @@ SIZES = dict(sequences=4, width=3, pages=10, page=32)
 @pytest.mark.parametrize("kw,needle", [
     (dict(page=48), "pages of 32"), (dict(pages=0), "0 pages"), (dict(pages=1 << 26), "pages of"), (dict(sequences=0), "0 sequences"),
     (dict(sequences=4097), "4097 sequences"), (dict(width=0), "sequences of 0"), (dict(width=1 << 26), "sequences of"),
+    (dict(sequences=4096, width=1 << 19), "4096 sequences of"),
 ])
 def test_tables(k, kw, needle):
     z = list({**SIZES, **kw}.values())
