@@ -1276,6 +1276,7 @@ PyObject *linear_step(PyObject *, PyObject *const *args, Py_ssize_t nargs)      
         launched(lib.linear_step(code_of(q.scalar_type()), q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr<float>(),
                                  states.data_ptr<float>(), slots.data_ptr<int32_t>(), (int)batch, (int)states.size(0), (int)q.size(1), (int)k.size(1),
                                  (int)q.size(2), strides, (float)scale, current_stream()));
+        if (!states.is_inference()) states.unsafeGetTensorImpl()->bump_version();      // a graph that kept them is told that they changed
     }
     return THPVariable_Wrap(std::move(out));
     END_HANDLE_TH_ERRORS

@@ -197,4 +197,6 @@ def linear_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, log
         _k.check(_k.lib.bsa_linear_attention_step(
             _DTYPES[q.dtype], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), log_decay.data_ptr(), states.data_ptr() or None,
             slots.data_ptr(), batch, states.size(0), heads, k.size(1), dim, strides_of(q, k, v), float(scale), _k.current_stream()))
+    if not states.is_inference():
+        torch.autograd.graph.increment_version(states)       # a graph that kept them is told that they changed
     return out

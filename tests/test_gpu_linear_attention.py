@@ -382,6 +382,50 @@ def test_gradients_of_parts_of_the_results():
         g.sum().backward()
 
 
+def test_saved_tensors_that_come_back_from_elsewhere_and_the_call_without_native_code():
+    import sparse
+    from sparse import linear
+    x = inputs([40, 300], 2, 2, 64, torch.float16)
+    base = run(x)
+
+    def gradients(call):
+        leaves = [x[n].clone().requires_grad_() for n in ("q", "k", "v", "states")]
+        outs = call(*leaves[:3], x["log_decay"], x["offsets"], x["scale"], leaves[3], True)
+        return [t.detach() for t in outs] + list(torch.autograd.grad(outs, leaves, [x["dout"], x["dlast"]]))
+
+    def spaced(t):                                           # the same values, in rows that are no multiple of 16 bytes apart
+        return torch.cat([t, t[..., :3]], -1)[..., :t.size(-1)] if t.dim() == 3 else t.clone()
+    found = [gradients(linear.general)]
+    with torch.autograd.graph.save_on_cpu():
+        found.append(gradients(sparse.packed_linear_attention))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spaced):
+        found.append(gradients(sparse.packed_linear_attention))
+    for made in found:
+        for n, t in zip(("out", "last", "dq", "dk", "dv", "dfirst"), made):
+            assert torch.equal(t, base[n]), n
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:1] if t.dtype == torch.float32 and t.dim() == 1 else t):
+        with pytest.raises((ValueError, RuntimeError)):
+            gradients(sparse.packed_linear_attention)
+
+
+@pytest.mark.parametrize("odd", [False, True])
+def test_a_step_between_a_pass_and_its_gradients_is_noticed(odd):
+    import sparse
+    x = inputs([40, 20], 2, 1, 64, torch.float16)
+    leaves = [x[n].clone().requires_grad_() for n in "qkv"]
+    pool = x["states"].clone()
+    out = sparse.packed_linear_attention(*leaves, x["log_decay"], x["offsets"], scale=x["scale"], states=pool)
+    rows = [x[n][:2] for n in "qkv"]
+    if odd:                                                  # rows that the native call leaves to Python
+        rows = [torch.cat([t, t[..., :3]], -1)[..., :64] for t in rows]
+    sparse.linear_attention_step(*rows, x["log_decay"], pool, int32([1, 0]))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.backward(x["dout"])
+    with torch.inference_mode():
+        pool = x["states"].clone()
+        sparse.linear_attention_step(*rows, x["log_decay"], pool, int32([1, 0]))
+
+
 def call(**changed):
     import sparse
     given = dict(q=normal(1, 9, 4, 64), k=normal(2, 9, 2, 64), v=normal(3, 9, 2, 64), log_decay=decays(2), offsets=int32([0, 4, 9]), scale=0.125)
