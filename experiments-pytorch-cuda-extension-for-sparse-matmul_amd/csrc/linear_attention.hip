@@ -699,14 +699,13 @@ template <int HD> using ResultTiles = LinearTiles<HD, 3, HD / 32>;
 template <int HD> using StateTiles = LinearTiles<HD, 2, HD / 32>;
 template <int HD> using PairSumTiles = LinearTiles<HD, 4, HD / 16>;
 
-// the forward pass, or dq
+// the forward pass, or dq, by packed_grid workgroups and PACKED_CLEARING
 template <int HD, bool BF, int TERMS>
-__global__ __launch_bounds__(2 * HD, 2) void linear_result_kernel(LinearWalk p, LinearSum sum)
+__device__ __forceinline__ void linear_result(const LinearWalk &p, const LinearSum &sum, int block, unsigned char *lds_raw)
 {
-    extern __shared__ __align__(16) unsigned char lds_raw[];
     const int cells = packed_grid(p.key_heads, p.head_sets, p.slots);
-    if ((int)blockIdx.x >= cells) return linear_clear(p, (int)blockIdx.x - cells, sum.out, (long long)p.key_heads * sum.a_inner * HD);
-    const LinearItem item = linear_item(p, (int)blockIdx.x);
+    if (block >= cells) return linear_clear(p, block - cells, sum.out, (long long)p.key_heads * sum.a_inner * HD);
+    const LinearItem item = linear_item(p, block);
     if (!item.there) return;
     const long long begin = (long long)item.begin + item.segment * p.segment;
     ResultTiles<HD> tiles(lds_raw);
@@ -715,6 +714,12 @@ __global__ __launch_bounds__(2 * HD, 2) void linear_result_kernel(LinearWalk p, 
     tiles.set(2, sum.c, begin, item.head);
     const long long inner_step[3] = {2 * sum.a.head, 0, 0};
     linear_walk<HD, BF, TERMS, false, true>(p, sum, item, wave_id(), tiles, LinearPlaces{0, 1, 2}, inner_step, sum.a_inner, lds_raw);
+}
+template <int HD, bool BF, int TERMS>
+__global__ __launch_bounds__(2 * HD, 2) void linear_result_kernel(LinearWalk p, LinearSum sum)
+{
+    extern __shared__ __align__(16) unsigned char lds_raw[];
+    linear_result<HD, BF, TERMS>(p, sum, (int)blockIdx.x, lds_raw);
 }
 
 // dv by the first half of the waves, dk by the others: a, b, c of dv are K, Q, dO, of dk V, dO, Q
@@ -746,10 +751,9 @@ __global__ __launch_bounds__(4 * HD, 2) void linear_keys_kernel(LinearWalk p, Li
 // every segment's own sum, of those that have a neighbour behind (BACKWARDS: in front): b and c are read once more than the results need them,
 // which costs less than a chain over the segments would
 template <int HD, bool BF, int TERMS, bool BACKWARDS>
-__global__ __launch_bounds__(2 * HD, 2) void linear_segments_kernel(LinearWalk p, LinearSum sum)
+__device__ __forceinline__ void linear_segment_sum(const LinearWalk &p, const LinearSum &sum, int block, unsigned char *lds_raw)
 {
-    extern __shared__ __align__(16) unsigned char lds_raw[];
-    const LinearItem item = linear_item(p, (int)blockIdx.x);
+    const LinearItem item = linear_item(p, block);
     if (!item.there || (BACKWARDS ? item.segment == 0 : item.segment == item.segments - 1)) return;
     const long long begin = (long long)item.begin + item.segment * p.segment;
     StateTiles<HD> tiles(lds_raw);
@@ -757,6 +761,22 @@ __global__ __launch_bounds__(2 * HD, 2) void linear_segments_kernel(LinearWalk p
     tiles.set(1, sum.c, begin, item.head * sum.c_inner);
     const long long inner_step[2] = {2 * sum.b.head, 2 * sum.c.head};
     linear_walk<HD, BF, TERMS, BACKWARDS, false>(p, sum, item, wave_id(), tiles, LinearPlaces{0, 0, 1}, inner_step, sum.c_inner, lds_raw);
+}
+template <int HD, bool BF, int TERMS>
+__global__ __launch_bounds__(2 * HD, 2) void linear_segments_kernel(LinearWalk p, LinearSum sum)
+{
+    extern __shared__ __align__(16) unsigned char lds_raw[];
+    linear_segment_sum<HD, BF, TERMS, false>(p, sum, (int)blockIdx.x, lds_raw);
+}
+// the backward pass begins with two things that do not need one another: dq, and the sums from the end; walks differ in `states` alone
+template <int HD, bool BF, int TERMS>
+__global__ __launch_bounds__(2 * HD, 2) void linear_queries_kernel(LinearWalk p, LinearSum dq, LinearSum dv, float *back_states)
+{
+    extern __shared__ __align__(16) unsigned char lds_raw[];
+    const int results = packed_grid(p.key_heads, p.head_sets, p.slots) + PACKED_CLEARING;
+    if ((int)blockIdx.x < results) return linear_result<HD, BF, 2>(p, dq, (int)blockIdx.x, lds_raw);
+    p.states = back_states;
+    linear_segment_sum<HD, BF, TERMS, true>(p, dv, (int)blockIdx.x - results, lds_raw);
 }
 
 // The running sum over the segments of a sequence, in place: what each segment begins with.  A lane has four values of a state; the
@@ -813,12 +833,10 @@ hipError_t run_linear(Kernel kernel, const LinearWalk &p, int clearing, int thre
     return hipGetLastError();
 }
 
-template <int HD, bool BF, int TERMS, bool BACKWARDS>
-hipError_t segment_states(const LinearWalk &p, const LinearSum &sum, const float *first, hipStream_t st)
+template <bool BACKWARDS>
+hipError_t running_sums(const LinearWalk &p, const float *first, int head_dim, hipStream_t st)
 {
-    const hipError_t err = run_linear(linear_segments_kernel<HD, BF, TERMS, BACKWARDS>, p, 0, 2 * HD, StateTiles<HD>::lds_bytes(), st, sum);
-    if (err != hipSuccess) return err;
-    linear_running_kernel<BACKWARDS><<<dim3(HD * HD / 1024, p.key_heads, p.sequences), 256, 0, st>>>(p, first, HD * HD);
+    linear_running_kernel<BACKWARDS><<<dim3(head_dim * head_dim / 1024, p.key_heads, p.sequences), 256, 0, st>>>(p, first, head_dim * head_dim);
     return hipGetLastError();
 }
 
@@ -829,7 +847,8 @@ hipError_t forward(const LinearArgs &a, hipStream_t st)
     const LinearSum sum{operand(a.q, a.q_token, a.q_head), operand(a.k, a.k_token, a.k_head), operand(a.v, a.v_token, a.v_head), (half_t *)a.out,
                         a.first, a.last, a.heads / a.key_heads, 1, false, a.scale, 1.f};
     if (a.tokens > a.segment) {
-        const hipError_t err = segment_states<HD, BF, TERMS, false>(p, sum, a.first, st);
+        hipError_t err = run_linear(linear_segments_kernel<HD, BF, TERMS>, p, 0, 2 * HD, StateTiles<HD>::lds_bytes(), st, sum);
+        if (err == hipSuccess) err = running_sums<false>(p, a.first, HD, st);
         if (err != hipSuccess) return err;
     }
     return run_linear(linear_result_kernel<HD, BF, TERMS>, p, PACKED_CLEARING, 2 * HD, ResultTiles<HD>::lds_bytes(), st, sum);
@@ -843,13 +862,16 @@ hipError_t backward(const LinearArgs &a, hipStream_t st)
                         g = operand(a.dout, a.g_token, a.g_head);
     const LinearSum dq{g, v, k, (half_t *)a.dq, a.first, nullptr, group, 1, true, a.scale, 1.f},
         dv{k, q, g, (half_t *)a.dv, a.dlast, a.dfirst, 1, group, false, 1.f, a.scale}, dk{v, g, q, (half_t *)a.dk, a.dlast, nullptr, 1, group, true, 1.f, a.scale};
-    hipError_t err = run_linear(linear_result_kernel<HD, BF, 2>, walk_of(a, a.states), PACKED_CLEARING, 2 * HD, ResultTiles<HD>::lds_bytes(), st, dq);
-    if (err != hipSuccess) return err;
-    const LinearWalk p = walk_of(a, a.back_states);
+    const LinearWalk towards = walk_of(a, a.states), p = walk_of(a, a.back_states);
+    hipError_t err;
     if (a.tokens > a.segment) {
-        err = segment_states<HD, BF, TERMS, true>(p, dv, a.dlast, st);
-        if (err != hipSuccess) return err;
+        const int sums = packed_grid(p.key_heads, p.head_sets, p.slots);
+        err = run_linear(linear_queries_kernel<HD, BF, TERMS>, towards, PACKED_CLEARING + sums, 2 * HD, ResultTiles<HD>::lds_bytes(), st, dq, dv, a.back_states);
+        if (err == hipSuccess) err = running_sums<true>(p, a.dlast, HD, st);
+    } else {
+        err = run_linear(linear_result_kernel<HD, BF, 2>, towards, PACKED_CLEARING, 2 * HD, ResultTiles<HD>::lds_bytes(), st, dq);
     }
+    if (err != hipSuccess) return err;
     return run_linear(linear_keys_kernel<HD, BF, TERMS>, p, PACKED_CLEARING, 4 * HD, PairSumTiles<HD>::lds_bytes(), st, dv, dk);
 }
 
@@ -862,7 +884,7 @@ static int linear_terms(const LinearArgs &a, const void *states_out) { return a.
 bool linear_fits(const LinearArgs &a)
 {
     const long long slots = (long long)a.tokens / a.segment + a.sequences + 7;
-    return ((long long)a.key_heads * slots + PACKED_CLEARING) * 4 * a.head_dim < (1ll << 32) && a.sequences <= 65535;
+    return (2 * (long long)a.key_heads * slots + PACKED_CLEARING) * 4 * a.head_dim < (1ll << 32) && a.sequences <= 65535;
 }
 size_t linear_workspace_bytes(const LinearArgs &a)
 {
