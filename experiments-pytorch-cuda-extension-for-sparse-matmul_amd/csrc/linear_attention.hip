@@ -14,9 +14,9 @@
 //
 // What bounds it (times of launches, the least of 60):
 //   results: memory.  65519 tokens, 8 heads over 4, head dim 128, bf16: 100 us for 430 MB, operands, result and states (4.3 TB/s); one workgroup
-//   of the two on a compute unit gets what the other leaves and ends a fifth later.  24575 tokens, 16 heads, fp16: 93 us (4.7 TB/s).
-//   segments' sums: memory, 134 MB in 34 us (3.9 TB/s), 201 MB in 45; the running sum over them 11 to 14 us for 62 MB.
-//   dv and dk: the clocks of a step, 24575 tokens, 16 heads, head dim 128: 200 us for 400 MB; of 6.7k clocks a step the vector pipe works 45 %
+//   of the two on a compute unit gets what the other leaves and ends a fifth later.  24575 tokens, 16 heads, fp16: 96 us (4.5 TB/s).
+//   segments' sums: memory, 134 MB in 34 us (3.9 TB/s), 201 MB in 46; with dq 137 us together; the running sum over them 11 to 14 us for 62 MB.
+//   dv and dk: the clocks of a step, 24575 tokens, 16 heads, head dim 128: 204 us for 600 MB; of 6.7k clocks a step the vector pipe works 45 %
 //   and the matrix pipe 27 %, two waves on each side of a barrier.  512 threads and 97 KB of LDS: one workgroup a compute unit.
 //   short texts: what a segment costs before its first product (5 us: its place, the state, the first chunks' way through memory) and
 //   1 us a chunk.  368 tokens, 12 heads, head dim 64: 12 us.

@@ -347,3 +347,19 @@ def test_nothing_to_do():
     assert table.fork(none, none)[0].numel() == 0
     filled(2, 1, 64, torch.int8, 32, 1).copy(none, none)
     same(table, plain)
+
+
+def test_the_largest_table():
+    """4096 sequences and as many entries: every one a child of one of a few, then what is left moves together."""
+    table, plain = pair(9000, 32, 4096, 4)
+    new = np.zeros(4096, int)
+    new[::512] = np.arange(8) * 15 + 1
+    offsets = [0] + np.cumsum(new).tolist()
+    same(table, plain, (table.append(int32(offsets), offsets[-1]), plain.append(offsets, offsets[-1])))
+    parents, children = (512 * (np.arange(4096) * 7 % 8)).tolist(), np.arange(4096)[::-1].tolist()
+    same(table, plain, *zip(table.fork(int32(parents), int32(children)), plain.fork(parents, children)))
+    gone = np.arange(0, 4096, 3).tolist()
+    plain.free(gone)
+    table.free(int32(gone))
+    same(table, plain, *zip(table.compact(), plain.compact()))
+    plain.check()
