@@ -212,6 +212,8 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     constexpr int KS = HD / 16, DT = HD / 32, OPERANDS = Tiles::STAGE / Tiles::TILE;
     // the state's decay is put off until it passes this power of two: operands are made of the state, in bf16 with the range of fp32
     constexpr float PUT_OFF = BF ? 40.f : 5.f;
+    // P as an operand is this much larger (fp16 has least below 1), and the result until it is rounded
+    constexpr float P_LIFT = BF ? 1.f : 64.f;
     const int l = lane_id(), i = l & 31, h = l >> 5, key_head = item.head;
     const float log2_decay = linear_log2(p.log_decay[key_head]);
 
@@ -354,7 +356,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         if (RESULT && thread < 2 * LA_ROWS) {
             // entry 32 + r - i: zero where token r is hidden from token i
             const int e = thread - LA_ROWS, gap = BACKWARDS ? e : -e;
-            const float x = gap >= 0 ? p.scale * linear_power(log2_decay, gap) : 0.f;
+            const float x = gap >= 0 ? P_LIFT * p.scale * linear_power(log2_decay, gap) : 0.f;
 #pragma unroll
             for (int copy = 0; copy < 4; ++copy) table[LA_BETWEEN * copy + thread + copy] = x;
         }
@@ -540,7 +542,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                         meet(o_mul);
                     }
                 }
-                up = since * owed * (BF ? 1.f : __builtin_amdgcn_rcpf(s_mul * o_mul));      // of a power of two: exact
+                up = since * owed * (BF ? 1.f : P_LIFT * __builtin_amdgcn_rcpf(s_mul * o_mul));     // of a power of two: exact
             }
             issue_order();
             read_b_columns(0);
@@ -549,13 +551,15 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         }
         // while the products run: memory takes its time to accept the next chunk's requests
         if (step + 2 < steps) request();
-        float with_decay = 1.f;
-        if (!BF && gets && enters && small && some_enters) {
-            // small beside the state, but not beside what its decay leaves of it: in the backward direction it comes with that decay itself
-            const float to_mul = fminf(s_mul * lift_of(wave_most(entering_most()), 10), 0x1p60f);
-            with_decay = to_mul * __builtin_amdgcn_rcpf(s_mul);
+        float by = 1.f;
+        const bool closes = RESULT && ends && step + inner - g >= steps && g == (BACKWARDS ? 0 : inner - 1);
+        if (!BF && enters && some_enters && (closes || (gets && small))) {
+            // Small beside the state, but not beside what its decay leaves of it: in the backward direction it comes with that decay itself.  What
+            // closes the walk is no operand any more, and may be as large as its own parts can: a state of few tokens has all its bits.
+            const float to_mul = fminf(fmaxf(s_mul * lift_of(wave_most(entering_most()), closes ? 14 : 10), 0x1p-60f), 0x1p60f);
+            by = to_mul * __builtin_amdgcn_rcpf(s_mul);
             s_mul = to_mul;
-            scale_entering(with_decay);
+            scale_entering(by);
         }
         h8 cw[TERMS][2];
 #pragma unroll
@@ -589,7 +593,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
         }
         if (enters) {
-            if (gets) scale_state(linear_power(log2_decay, aged) * with_decay);
+            if (gets || by != 1.f) scale_state((gets ? linear_power(log2_decay, aged) : 1.f) * by);
             if (!BF) shrunk = shrunk || gets;
             age = gets ? 0 : aged;
             owed = gets ? 1.f : linear_power(log2_decay, age);
@@ -609,7 +613,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
             for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(part[v]);
             if (!BF) {                   // P too large for fp16, or all of it too small
-                if (__builtin_amdgcn_ballot_w64(p_size >= 0x1p28f) != 0ull || __builtin_amdgcn_ballot_w64(p_size >= 1.f) == 0ull) {
+                if (__builtin_amdgcn_ballot_w64(p_size >= 0x1p30f) != 0ull || __builtin_amdgcn_ballot_w64(p_size >= 0x1p8f) == 0ull) {
                     float p_most = 0.f;
 #pragma unroll
                     for (int v = 0; v < 16; ++v) p_most = larger(p_most, prob[v] * between[8 * (v >> 2) + (v & 3)]);
@@ -664,7 +668,14 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         }
         stage = stage == LA_STAGES - 1 ? 0 : stage + 1;
         if (RESULT && (!BACKWARDS || last_inner)) {
-            pack16<BF>(oacc, result[0], result[1]);
+            if (BF) {
+                pack16<BF>(oacc, result[0], result[1]);
+            } else {
+                h8 half[2];
+#pragma unroll
+                for (int v = 0; v < 16; ++v) half[v >> 3][v & 7] = narrow_16<BF>(__builtin_fmaf(oacc[v], 1.f / P_LIFT, 0.f));
+                result[0] = __builtin_bit_cast(uint4, half[0]), result[1] = __builtin_bit_cast(uint4, half[1]);
+            }
             to = out + (long long)(at + i) * width + (BACKWARDS ? 0 : g * HD);
             stored = valid;
         }

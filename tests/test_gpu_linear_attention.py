@@ -69,11 +69,13 @@ def want(x, grads=True):
     return lo.bounds(*given, x["offsets"].cpu().numpy(), x["scale"], kind_of(x["q"].dtype), first, *more)
 
 
-def check(x, found, grads=True, norms=True):
+def check(x, found, grads=True, norms=True, more=None):
     unit = lo.UNIT[kind_of(x["q"].dtype)]
     for name, (value, bound) in want(x, grads).items():
         if name not in found:
             continue
+        if more is not None:
+            bound = bound + more[name]
         got = to_np(found[name])
         # fp16 has nothing between 65504 and infinity: from the middle on (65520) a result is rounded to infinity
         border = 65520.0 if found[name].dtype == torch.float16 else np.inf
@@ -147,6 +149,57 @@ def test_what_enters_is_small_beside_a_state_that_goes(lengths, log_decay, dtype
     x = inputs(lengths, 2, 1, 64, dtype)
     x["log_decay"].fill_(log_decay)
     check(x, run(x), norms=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("log_decay", [-0.1, -14.0])
+@pytest.mark.parametrize("lengths", [[1, 2, 1], [33, 65]])
+def test_states_of_few_tokens_have_their_small_columns_too(lengths, log_decay, dtype):
+    """Each value of such a state is its own product: columns of 2^-12 of the others' size have bits of their own.
+
+    In fp16 what enters a state in its last chunk travels times a power of two that brings the largest of it, X, to 2^13 .. 2^14, as a high part, cut,
+    and a low part, rounded: it is off by 2^-22 of itself where the low part is a normal number and by half of fp16's smallest step,
+    2^-25, where it is not, which is 2^-25 / 2^13 = 2^-38 of X.  Where the last token's k is zero or nearly so, what older tokens left is all there
+    is, e^-14 a token of X: a value of row r may be off by the sum of |k_t[r]| times 2^-38 X besides (2^-37 below: both parts)."""
+    x = inputs(lengths, 2, 1, 64, dtype)
+    x["log_decay"].fill_(log_decay)
+    for name in ("v", "dout"):
+        x[name][..., ::2] *= 2.0 ** -12
+    for name in ("states", "dlast"):
+        x[name] *= 2.0 ** -12
+    more = {name: 0.0 for name in ("out", "dq", "dk", "dv")}
+    more.update({name: np.zeros((len(lengths), 2, 64, 1)) for name in ("last", "dfirst")})
+    if dtype == torch.float16:
+        offsets = np.cumsum([0] + lengths)
+        for b, n in enumerate(lengths):
+            ends, begins = slice(offsets[b] + (n - 1) // 32 * 32, offsets[b + 1]), slice(offsets[b], offsets[b] + min(n, 32))
+            for h in range(2):
+                q, k, v, dout = (to_np(x[name])[:, h] for name in ("q", "k", "v", "dout"))
+                more["last"][b, h, :, 0] = 2.0 ** -37 * np.abs(v[ends]).max() * np.abs(k[ends]).sum(0)
+                more["dfirst"][b, h, :, 0] = 2.0 ** -37 * np.abs(dout[begins]).max() * x["scale"] * np.exp(log_decay) * np.abs(q[begins]).sum(0)
+    check(x, run(x), norms=False, more=more)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tokens_of_different_sizes_in_one_chunk(dtype):
+    """In fp16 P is an operand times 64 and a power of two that leaves the largest of a chunk at 4 or more: P_ts is off by 2^-11 of itself where it
+    is a normal number and by half of fp16's smallest step, 2^-25, where it is not, 2^-27 of the chunk's largest.  A result is off by the sum
+    of that times |c_s| besides, c being v, k, dout and q for out, dq, dv and dk."""
+    x = inputs([90, 20], 2, 2, 64, dtype, states=False)
+    x["log_decay"].fill_(-4.0)                               # a token's result is its own and its neighbours'
+    size = torch.exp2(-(torch.arange(110, device="cuda") % 4).float() * 3.5).view(-1, 1, 1)
+    for name in ("q", "v", "dout"):
+        x[name] = (x[name].float() * size).to(dtype)
+    more = {}
+    q, k, v, dout = (to_np(x[name]) for name in ("q", "k", "v", "dout"))
+    for name, (a, b, c) in {"out": (q, k, v), "dq": (dout, v, k), "dv": (k, q, dout), "dk": (v, dout, q)}.items():
+        by_head = lambda y, h: y.reshape(110, 2, -1, 64)[:, h].transpose(1, 0, 2)          # [heads that share, tokens, 64]
+        term = np.zeros(a.shape[:1] + (2, 1, 64))
+        for h in range(2):
+            most = abs(x["scale"]) * max(np.abs(one @ other.T).max() for one in by_head(a, h) for other in by_head(b, h))
+            term[:, h, 0] = 2.0 ** -27 * most * np.abs(by_head(c, h)).sum((0, 1)) if dtype == torch.float16 else 0.0
+        more[name] = np.broadcast_to(term, (110, 2, a.shape[1] // 2, 64)).reshape(a.shape)
+    check(x, run(x), norms=False, more=more)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
