@@ -299,8 +299,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
         for (int t = 0; t < DT; ++t) state[t] *= by;
     };
-    auto lift_state = [&]() {            // to a size that fp16 operands have room around
-        const float most = state_most();
+    auto lift_state = [&](float most) {  // to a size that fp16 operands have room around
         if (most > 0.f) {
             const float to_mul = fminf(fmaxf(s_mul * lift_of(most, 8), 0x1p-60f), 0x1p60f);
             scale_state(to_mul * __builtin_amdgcn_rcpf(s_mul));
@@ -339,7 +338,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             for (int t = 0; t < DT; ++t) asm volatile("" : "+v"(state[t]));
             if (!BF && steps > 0) {      // an empty sequence's comes out as it went in
                 zero = __builtin_amdgcn_ballot_w64(lane_most() > 0.f) == 0ull;
-                lift_state();
+                lift_state(state_most());
             }
         }
     }
@@ -528,19 +527,20 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                     for (int j = 0; j < 8; ++j) op[j] = narrow_16<BF>(state[s / 2][8 * (s % 2) + j]);
                     oacc = mfma_16<BF>(op, a[s], oacc);
                 }
-                if (!BF) {               // a state that has outgrown fp16 or is too small for it, or infinities that it has
+                if (!BF) {               // a state that has outgrown fp16, or is too small for it
                     float sure = 0.f;
 #pragma unroll
                     for (int v = 0; v < 16; ++v) sure += __builtin_fabsf(oacc[v]);
-                    const bool broken = __builtin_amdgcn_ballot_w64(!is_finite(sure)) != 0ull;
-                    if (broken || o_mul != 1.f) {
-                        if (broken) {
-                            const float was = s_mul;
-                            lift_state();
-                            scale_entering(s_mul * __builtin_amdgcn_rcpf(was));
-                        }
-                        meet(o_mul);
+                    // No number: brought back, and what enters with it, only if the state has outgrown fp16.  Otherwise a token of a, or what the
+                    // state got before, is no number, which says nothing about its size: what enters has been fitted to s_mul already.
+                    const float most = __builtin_amdgcn_ballot_w64(!is_finite(sure)) != 0ull ? state_most() : 0.f;
+                    const bool outgrown = most >= 0x1p15f;
+                    if (outgrown) {
+                        const float was = s_mul;
+                        lift_state(most);
+                        scale_entering(s_mul * __builtin_amdgcn_rcpf(was));
                     }
+                    if (outgrown || o_mul != 1.f) meet(o_mul);
                 }
                 up = since * owed * (BF ? 1.f : P_LIFT * __builtin_amdgcn_rcpf(s_mul * o_mul));     // of a power of two: exact
             }

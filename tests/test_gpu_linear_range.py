@@ -1,0 +1,64 @@
+"""GPU: linear attention where a value is no number, or far from one, and what must not suffer from it.
+
+The oracle and its bounds are those of ``test_gpu_linear_attention``; what each test adds is derived beside it."""
+import numpy as np
+import pytest
+import torch
+
+from helpers import to_np
+from test_gpu_linear_attention import DTYPES, inputs, run, want
+
+pytestmark = pytest.mark.gpu
+
+
+REACH = {"q": ("dk", "dv", "out", "dfirst"), "k": ("out", "dq", "dv", "last"), "v": ("out", "dq", "dk", "last"), "dout": ("dq", "dk", "dv", "dfirst")}
+
+
+def reached(name, result, at, dim, tokens, end):
+    """Where a value of token ``at``, head 0, place 3 of operand ``name`` goes: tokens (results), rows or columns (states)."""
+    if result in ("last", "dfirst"):
+        place = torch.zeros(dim, dim, dtype=torch.bool, device="cuda")
+        if name in ("k", "q"):
+            place[3] = True
+        else:
+            place[:, 3] = True
+        return place
+    token = torch.arange(tokens, device="cuda")
+    if (name, result) in (("q", "out"), ("k", "dv"), ("v", "dk"), ("dout", "dq")):
+        return token == at
+    return (token >= at) & (token < end) if result in ("out", "dq") else token <= at
+
+
+def check_reach(x, name, at, value, end):
+    """A value that is no number in the first sequence, whose tokens end at ``end``: all that it does not reach is what the oracle makes
+    of a zero in its place, and some of what it reaches is no number either."""
+    dim, tokens = x["k"].size(2), x["k"].size(0)
+    x[name] = x[name].clone()
+    x[name][at, 0, 3] = value
+    found = run(x)
+    x[name][at, 0, 3] = 0
+    for result, (exact, bound) in want(x).items():
+        got, far = to_np(found[result]), np.zeros(exact.shape, bool)
+        if result in REACH[name]:
+            places = reached(name, result, at, dim, tokens, end).cpu().numpy()
+            if result in ("last", "dfirst"):
+                far[0, 0] = places
+            else:
+                far[places, 0 if result in ("dk", "dv") else slice(0, x["q"].size(1) // x["k"].size(1))] = True
+            assert not np.isfinite(got[places] if far.ndim == 3 else got[0, 0][places]).all(), result
+        off = np.abs(got - exact)[~far]
+        assert (off <= bound[~far]).all(), (result, float(np.nanmax(off / np.maximum(bound[~far], 1e-300))), np.isnan(off).sum())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("name", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("small", ["states", "k", "q"])
+@pytest.mark.parametrize("at", [5, 40, 97])
+@pytest.mark.parametrize("group,dim", [(1, 64), (2, 128)])
+def test_a_nan_beside_small_states(group, dim, at, small, name, dtype):
+    """A token that meets the state and is no number says nothing about the state's size, which here is 1e-4 of what enters it: given so and met
+    by the first chunk from either end, or kept so by small k (towards the front, by small q)."""
+    x = inputs([100, 11], 1, group, dim, dtype)
+    for n in {"states", "dlast", small}:
+        x[n] = (x[n].float() * 1e-4).to(x[n].dtype)
+    check_reach(x, name, at, float("nan"), 100)
