@@ -472,7 +472,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         if (!BF) {                       // it has to fit, and the state with it
             if ((zero || __builtin_amdgcn_ballot_w64(x_most >= 0x1p15f) != 0ull) && enters) {
                 const float all = wave_most(is_finite(x_most) ? x_most : 0.f);
-                if (all > 0.f) {
+                if (zero ? all > 0.f : all >= 0x1p15f) {     // infinities fit nowhere and ask for nothing
                     const float to_mul = fminf(fmaxf(s_mul * lift_of(all, 10), 0x1p-60f), 0x1p60f), by = to_mul * __builtin_amdgcn_rcpf(s_mul);
                     s_mul = to_mul;
                     if (!zero) {
@@ -556,10 +556,14 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         if (!BF && enters && some_enters && (closes || (gets && small))) {
             // Small beside the state, but not beside what its decay leaves of it: in the backward direction it comes with that decay itself.  What
             // closes the walk is no operand any more, and may be as large as its own parts can: a state of few tokens has all its bits.
-            const float to_mul = fminf(fmaxf(s_mul * lift_of(wave_most(entering_most()), closes ? 14 : 10), 0x1p-60f), 0x1p60f);
-            by = to_mul * __builtin_amdgcn_rcpf(s_mul);
-            s_mul = to_mul;
-            scale_entering(by);
+            // An infinity has its column to itself, and the others their bits: lanes that have one are left out.
+            const float most = entering_most(), all = wave_most(is_finite(most) ? most : 0.f);
+            if (all > 0.f) {
+                const float to_mul = fminf(fmaxf(s_mul * lift_of(all, closes ? 14 : 10), 0x1p-60f), 0x1p60f);
+                by = to_mul * __builtin_amdgcn_rcpf(s_mul);
+                s_mul = to_mul;
+                scale_entering(by);
+            }
         }
         h8 cw[TERMS][2];
 #pragma unroll

@@ -62,3 +62,18 @@ def test_a_nan_beside_small_states(group, dim, at, small, name, dtype):
     for n in {"states", "dlast", small}:
         x[n] = (x[n].float() * 1e-4).to(x[n].dtype)
     check_reach(x, name, at, float("nan"), 100)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("value", [float("inf"), -float("inf")])
+@pytest.mark.parametrize("name,at", [("v", 5), ("v", 97), ("k", 97), ("dout", 5), ("dout", 97), ("q", 5)])
+@pytest.mark.parametrize("small", [None, "states", "k", "q"])
+@pytest.mark.parametrize("group,dim,lengths", [(1, 64, [700, 3]), (2, 128, [100, 11])])
+def test_an_infinity_has_its_column_to_itself(group, dim, lengths, small, name, at, value, dtype):
+    """What closes a walk is as large as its parts can be; an infinity among it is not what they are fitted to.  It ruins a column (k, q: a row)
+    of the states and the tokens that see it.  At 97 of 100, or at 697 of 700, tokens from the end, in the chunk that closes the
+    states; at 5 in the one that closes their gradients."""
+    x = inputs(lengths, 1, group, dim, dtype)
+    for n in {"states", "dlast", small} if small else ():
+        x[n] = (x[n].float() * 1e-4).to(x[n].dtype)
+    check_reach(x, name, at if at < 50 else lengths[0] - 3, value, lengths[0])
