@@ -299,14 +299,20 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
 #pragma unroll
         for (int t = 0; t < DT; ++t) state[t] *= by;
     };
-    auto lift_state = [&](float most) {  // to a size that fp16 operands have room around
-        if (most > 0.f) {
-            const float to_mul = fminf(fmaxf(s_mul * lift_of(most, 8), 0x1p-60f), 0x1p60f);
-            scale_state(to_mul * __builtin_amdgcn_rcpf(s_mul));
-            s_mul = to_mul;
-        }
+    // `by` as far as s_mul may go, which is at `mul`: from where the largest state of fp32 fits fp16, to where what enters next has room in fp32
+    // (2^16, 2^5 of decay, a scale of 2^16); s_mul o_mul to 2^120
+    constexpr float MUL_LEAST = 0x1p-113f, MUL_MOST = 0x1p90f, MUL_LAST = 0x1p120f;
+    auto reach = [&](float mul, float by, float most) {
+        const float under = __builtin_amdgcn_rcpf(mul);
+        return fminf(fmaxf(by, MUL_LEAST * under), most * under);
+    };
+    auto lift_state = [&](float most) {  // to a size that fp16 operands have room around; by how much
+        const float by = most > 0.f ? reach(s_mul, lift_of(most, 8), MUL_MOST) : 1.f;
+        scale_state(by);
+        s_mul *= by;
         o_mul = 1.f;
         dwarfed = false;
+        return by;
     };
     {
         const bool given = BACKWARDS ? item.segment == item.segments - 1 : item.segment == 0;
@@ -438,6 +444,13 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         const int aged = zero ? 0 : BACKWARDS && g > 0 ? age : age + valid;
         const bool gets = !(__builtin_fabsf(log2_decay * (float)aged) <= PUT_OFF);           // the state gets its decay with this chunk
         const float with = gets || aged == 0 ? 1.f : at_exp2(-log2_decay * (float)aged);
+        // by, more: of the state and s_mul once the state has been an operand; what enters is made for them.  A state so large that nothing beside it
+        // is a number above zero may be about to decay to what enters, or to nothing.
+        float by = 1.f, more = 1.f;
+        if (!BF && enters && gets && s_mul < 0x1p-20f) {
+            const float left = state_most() * linear_power(log2_decay, aged), most = __builtin_amdgcn_rcpf(s_mul);
+            by = left > 0.f ? fminf(most, fmaxf(1.f, lift_of(left, 8))) : most;
+        }
         float x[2][8], x_most = 0.f;
 #pragma unroll
         for (int u = 0; u < 4; ++u)
@@ -445,7 +458,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             for (int j = 0; j < 4; ++j) {
                 const half_t one = cop[u >> 1][4 * (u & 1) + j];
                 float &to_enter = x[u >> 1][4 * (u & 1) + j];
-                to_enter = times<BF>(one, enter[u][j] * (BF ? with : with * s_mul));
+                to_enter = times<BF>(one, enter[u][j] * (BF ? with : with * (s_mul * by)));
                 if (!BF) x_most = larger(x_most, to_enter);
             }
         bool some_enters = true, small = false;
@@ -473,32 +486,36 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             if ((zero || __builtin_amdgcn_ballot_w64(x_most >= 0x1p15f) != 0ull) && enters) {
                 const float all = wave_most(is_finite(x_most) ? x_most : 0.f);
                 if (zero ? all > 0.f : all >= 0x1p15f) {     // infinities fit nowhere and ask for nothing
-                    const float to_mul = fminf(fmaxf(s_mul * lift_of(all, 10), 0x1p-60f), 0x1p60f), by = to_mul * __builtin_amdgcn_rcpf(s_mul);
-                    s_mul = to_mul;
-                    if (!zero) {
-                        scale_state(by);
-                        dwarfed = true;
+                    const float to_fit = reach(s_mul * by, lift_of(all, 10), MUL_MOST);
+                    if (by != 1.f) {
+                        by *= to_fit;
+                    } else {
+                        s_mul *= to_fit;
+                        if (!zero) {
+                            scale_state(to_fit);
+                            dwarfed = true;
+                        }
                     }
-                    scale_entering(by);
+                    scale_entering(to_fit);
                 }
             }
             if (RESULT && fresh && (shrunk || dwarfed)) {
                 if (dwarfed) {           // operands of another size than the state, as long as it is so
                     const float left = state_most();
-                    o_mul = left > 0.f && left < 16.f ? fminf(lift_of(left, 8), 0x1p60f) : 1.f;
+                    o_mul = left > 0.f && left < 16.f ? fminf(lift_of(left, 8), MUL_LAST * __builtin_amdgcn_rcpf(s_mul)) : 1.f;
                     dwarfed = o_mul != 1.f;
                 } else {                 // by a part of it: what has entered since most often makes up for it
                     float some = 0.f;
 #pragma unroll
                     for (int v = 0; v < 16; ++v) some = larger(some, state[0][v]);
                     if (__builtin_amdgcn_ballot_w64(some >= 16.f) == 0ull) {
-                        const float left = state_most(), by = left > 0.f ? fminf(lift_of(left, 8), 0x1p60f * __builtin_amdgcn_rcpf(s_mul)) : 1.f;
-                        if (__builtin_amdgcn_ballot_w64(x_most * by >= 0x1p15f) == 0ull) {
-                            scale_state(by);
-                            s_mul *= by;
-                            scale_entering(by);
+                        const float left = state_most(), up = left > 0.f ? reach(s_mul * by, lift_of(left, 8), MUL_MOST) : 1.f;
+                        if (__builtin_amdgcn_ballot_w64(x_most * up >= 0x1p15f) == 0ull) {
+                            scale_state(up);
+                            s_mul *= up;
+                            scale_entering(up);
                         } else {
-                            o_mul = by;
+                            o_mul = up;
                             dwarfed = true;
                         }
                     }
@@ -535,14 +552,10 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                     // state got before, is no number, which says nothing about its size: what enters has been fitted to s_mul already.
                     const float most = __builtin_amdgcn_ballot_w64(!is_finite(sure)) != 0ull ? state_most() : 0.f;
                     const bool outgrown = most >= 0x1p15f;
-                    if (outgrown) {
-                        const float was = s_mul;
-                        lift_state(most);
-                        scale_entering(s_mul * __builtin_amdgcn_rcpf(was));
-                    }
+                    if (outgrown) scale_entering(lift_state(most));
                     if (outgrown || o_mul != 1.f) meet(o_mul);
                 }
-                up = since * owed * (BF ? 1.f : P_LIFT * __builtin_amdgcn_rcpf(s_mul * o_mul));     // of a power of two: exact
+                up = since * (owed * (BF ? 1.f : P_LIFT * __builtin_amdgcn_rcpf(s_mul * o_mul)));    // of a power of two: exact
             }
             issue_order();
             read_b_columns(0);
@@ -551,7 +564,6 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         }
         // while the products run: memory takes its time to accept the next chunk's requests
         if (step + 2 < steps) request();
-        float by = 1.f;
         const bool closes = RESULT && ends && step + inner - g >= steps && g == (BACKWARDS ? 0 : inner - 1);
         if (!BF && enters && some_enters && (closes || (gets && small))) {
             // Small beside the state, but not beside what its decay leaves of it: in the backward direction it comes with that decay itself.  What
@@ -559,10 +571,13 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             // An infinity has its column to itself, and the others their bits: lanes that have one are left out.
             const float most = entering_most(), all = wave_most(is_finite(most) ? most : 0.f);
             if (all > 0.f) {
-                const float to_mul = fminf(fmaxf(s_mul * lift_of(all, closes ? 14 : 10), 0x1p-60f), 0x1p60f);
-                by = to_mul * __builtin_amdgcn_rcpf(s_mul);
-                s_mul = to_mul;
-                scale_entering(by);
+                more = reach(s_mul * by, lift_of(all, closes ? 14 : 10), closes ? MUL_LAST : MUL_MOST);
+                // the state comes along: it stays an operand or, at the end, in fp32 (it is below 2^44)
+                if (!closes || more > 0x1p60f) {
+                    const float held = state_most() * ((gets ? linear_power(log2_decay, aged) : 1.f) * by);
+                    more = fminf(more, fmaxf(1.f, (closes ? 0x1p100f : 0x1p14f) * __builtin_amdgcn_rcpf(held)));
+                }
+                scale_entering(more);
             }
         }
         h8 cw[TERMS][2];
@@ -597,7 +612,8 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             for (int s = 0; s < 2; ++s) part = mfma_16<BF>(cop[s], pop[s], part);
         }
         if (enters) {
-            if (gets || by != 1.f) scale_state((gets ? linear_power(log2_decay, aged) : 1.f) * by);
+            if (!BF) s_mul = s_mul * by * more;
+            if (gets || more != 1.f) scale_state((gets ? linear_power(log2_decay, aged) : 1.f) * by * more);      // by: of what the decay leaves
             if (!BF) shrunk = shrunk || gets;
             age = gets ? 0 : aged;
             owed = gets ? 1.f : linear_power(log2_decay, age);

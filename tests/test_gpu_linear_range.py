@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from helpers import to_np
-from test_gpu_linear_attention import DTYPES, inputs, run, want
+from test_gpu_linear_attention import DTYPES, check, inputs, run, want
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,18 @@ def test_an_infinity_has_its_column_to_itself(group, dim, lengths, small, name, 
     for n in {"states", "dlast", small} if small else ():
         x[n] = (x[n].float() * 1e-4).to(x[n].dtype)
     check_reach(x, name, at if at < 50 else lengths[0] - 3, value, lengths[0])
+
+
+@pytest.mark.parametrize("log_decay", [-0.01, -2.5, -40.0])
+@pytest.mark.parametrize("mul", [1.0, 2.0 ** -12])
+@pytest.mark.parametrize("lengths", [[70, 33, 1], [700]])
+def test_large_given_states_in_fp16(lengths, mul, log_decay):
+    """States of 1e35 come back as what fp32 makes of them, not as infinities of their powers of two, and what enters is there when their decay
+    has made them small."""
+    x = inputs(lengths, 2, 1, 64, torch.float16)
+    x["log_decay"].fill_(log_decay)
+    for n in ("states", "dlast"):
+        x[n] *= 1e35
+    for n in ("v", "dout"):
+        x[n] = (x[n].float() * mul).half()
+    check(x, run(x), norms=False)
