@@ -210,12 +210,17 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                                             unsigned char *lds_raw)
 {
     constexpr int KS = HD / 16, DT = HD / 32, OPERANDS = Tiles::STAGE / Tiles::TILE;
-    // the state's decay is put off until it passes this power of two: operands are made of the state, in bf16 with the range of fp32
-    constexpr float PUT_OFF = BF ? 40.f : 5.f;
+    // The state's decay is put off until it passes this power of two: operands are made of the state, in bf16 with the range of fp32.  There the
+    // state is held smaller by as much, so that putting off makes nothing larger than it is: it goes as far up as fp32 does, and what
+    // is lost at the other end is lost below 2^-126, of what the parts of bf16 carry below 2^-111 (65519 tokens, 4 key heads: 40 takes as long, 5 1 % longer).
+    constexpr float PUT_OFF = BF ? 23.f : 5.f;
+    constexpr float HELD = 0x1p-23f, FREED = 0x1p23f;
     // P as an operand is this much larger (fp16 has least below 1), and the result until it is rounded
     constexpr float P_LIFT = BF ? 1.f : 64.f;
     const int l = lane_id(), i = l & 31, h = l >> 5, key_head = item.head;
     const float log2_decay = linear_log2(p.log_decay[key_head]);
+    // where a chunk's own decay is near the end of fp32, nothing is put off to its product
+    const float put_off = __builtin_fabsf(log2_decay * LA_ROWS) > 64.f ? 0.f : PUT_OFF;
 
     // tokens of the segment, in chunks; step s is chunk s / inner (from the end: BACKWARDS) and head s % inner
     const int from = item.segment * p.segment, here = min(item.n - from, p.segment);
@@ -274,9 +279,9 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     };
 
     // The state: value v of state[t] is row 32 t + swapped16(r), column 32 w + perm16(i), r = 8 (v / 4) + 4 h + v % 4; times s_mul, a power
-    // of two (fp16), over the decay of the last `age` tokens, which it has not got yet.
+    // of two (bf16: HELD), over the decay of the last `age` tokens, which it has not got yet.
     f16v state[DT];
-    float s_mul = 1.f, o_mul = 1.f;      // o_mul: of its operands besides, where what enters is much larger than it is
+    float s_mul = BF && steps > 0 ? HELD : 1.f, o_mul = 1.f;      // o_mul: of its operands besides, where what enters is much larger than it is
     int age = 0;
     float owed = 1.f;                    // that decay
     bool shrunk = false, dwarfed = false;        // it has got some of it, or was made small for what entered: too small for fp16 operands?
@@ -342,6 +347,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             // arrived: the compiler would wait for them inside the loop, and with them for the chunks on their way
 #pragma unroll
             for (int t = 0; t < DT; ++t) asm volatile("" : "+v"(state[t]));
+            if (BF) scale_state(s_mul);
             if (!BF && steps > 0) {      // an empty sequence's comes out as it went in
                 zero = __builtin_amdgcn_ballot_w64(lane_most() > 0.f) == 0ull;
                 lift_state(state_most());
@@ -442,7 +448,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         }
         // What enters the state: c with its decay, times s_mul over the decay that the state has not got.
         const int aged = zero ? 0 : BACKWARDS && g > 0 ? age : age + valid;
-        const bool gets = !(__builtin_fabsf(log2_decay * (float)aged) <= PUT_OFF);           // the state gets its decay with this chunk
+        const bool gets = !(__builtin_fabsf(log2_decay * (float)aged) <= put_off);           // the state gets its decay with this chunk
         const float with = gets || aged == 0 ? 1.f : at_exp2(-log2_decay * (float)aged);
         // by, more: of the state and s_mul once the state has been an operand; what enters is made for them.  A state so large that nothing beside it
         // is a number above zero may be about to decay to what enters, or to nothing.
@@ -458,7 +464,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             for (int j = 0; j < 4; ++j) {
                 const half_t one = cop[u >> 1][4 * (u & 1) + j];
                 float &to_enter = x[u >> 1][4 * (u & 1) + j];
-                to_enter = times<BF>(one, enter[u][j] * (BF ? with : with * (s_mul * by)));
+                to_enter = times<BF>(one, enter[u][j] * with * (BF ? HELD : s_mul * by));
                 if (!BF) x_most = larger(x_most, to_enter);
             }
         bool some_enters = true, small = false;
@@ -555,7 +561,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                     if (outgrown) scale_entering(lift_state(most));
                     if (outgrown || o_mul != 1.f) meet(o_mul);
                 }
-                up = since * (owed * (BF ? 1.f : P_LIFT * __builtin_amdgcn_rcpf(s_mul * o_mul)));    // of a power of two: exact
+                up = since * (owed * (BF ? FREED : P_LIFT * __builtin_amdgcn_rcpf(s_mul * o_mul)));      // of a power of two: exact
             }
             issue_order();
             read_b_columns(0);
@@ -706,7 +712,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     if (ends) {
         float *dst = RESULT ? sum.last + ((size_t)item.sequence * p.key_heads + key_head) * HD * HD
                             : p.states + linear_boundary(p, item.begin, BACKWARDS ? item.segment : item.segment + 1, key_head) * HD * HD;
-        const float down = owed * (BF ? 1.f : __builtin_amdgcn_rcpf(s_mul));
+        const float down = owed * __builtin_amdgcn_rcpf(s_mul);
 #pragma unroll
         for (int t = 0; t < DT; ++t)
 #pragma unroll

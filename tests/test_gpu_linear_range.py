@@ -92,3 +92,44 @@ def test_large_given_states_in_fp16(lengths, mul, log_decay):
     for n in ("v", "dout"):
         x[n] = (x[n].float() * mul).half()
     check(x, run(x), norms=False)
+
+
+@pytest.mark.parametrize("large", ["v", "dout"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("lengths", [[70, 33, 1], [700]])
+def test_bf16_goes_as_far_as_fp32(lengths, dim, large):
+    """Values of 2^112, and states and sums of them up to 2^124: a decay that is put off, 2^-16 a chunk, makes nothing larger."""
+    x = inputs(lengths, 3, 2, dim, torch.bfloat16)
+    x["log_decay"].fill_(-0.35)
+    x[large] *= 2.0 ** 112
+    x["states" if large == "v" else "dlast"] *= 2.0 ** 112
+    check(x, run(x))
+
+
+@pytest.mark.parametrize("lengths", [[70, 33, 1], [700]])
+def test_large_given_states_in_bf16(lengths):
+    """1e35, and e^-2.5 a token: of 38 tokens that is 2^-137, which fp32 has few bits of; of 6 and of 32 it has all."""
+    x = inputs(lengths, 2, 1, 64, torch.bfloat16)
+    x["log_decay"].fill_(-2.5)
+    for n in ("states", "dlast"):
+        x[n] *= 1e35
+    for n in ("v", "dout"):
+        x[n] *= 2.0 ** -12
+    check(x, run(x), norms=False)
+
+
+@pytest.mark.parametrize("small", ["v", "dout"])
+@pytest.mark.parametrize("lengths", [[70, 33, 1], [700]])
+@pytest.mark.parametrize("mul", [-75, -100])
+def test_small_values_in_bf16(mul, lengths, small):
+    """What enters a state (of the gradients' walk: with the scale) is held at least 2^-23 as large as it is, as three parts of bf16, whose smallest
+    step is 2^-133: a value of row r of the states is off by the sum of |k_t[r]| (of their gradients: |q_t[r]|) times 2^23 2^-134
+    besides, and by 2^23 2^-150 for each of the 700 roundings of the state.  Of a result that is 2^-111 of its terms' factors, which are 2^-100 or more: within its unit."""
+    x = inputs(lengths, 2, 1, 64, torch.bfloat16)
+    state, key = {"v": ("last", "k"), "dout": ("dfirst", "q")}[small]
+    for n in (small, {"v": "states", "dout": "dlast"}[small]):
+        x[n] *= 2.0 ** mul
+    more, offsets = dict.fromkeys(("out", "last", "dq", "dk", "dv", "dfirst"), 0.0), np.cumsum([0] + lengths)
+    sums = np.stack([np.abs(to_np(x[key])[offsets[b]:offsets[b + 1]]).sum(0) for b in range(len(lengths))])
+    more[state] = 2.0 ** -111 * sums[..., None] + 700 * 2.0 ** -127
+    check(x, run(x), norms=False, more=more)
