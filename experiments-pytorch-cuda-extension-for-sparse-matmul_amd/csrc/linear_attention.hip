@@ -660,6 +660,16 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
             if (__builtin_amdgcn_ballot_w64(!is_finite(sure)) != 0ull) {
                 // An infinity or a NaN: zero times it is NaN, also for tokens that do not see it.  Weights of hidden ones are put to zero,
                 // and left out of c it makes NaN of its column for those that see it.
+                if (!BF) {               // beside a NaN the sum of squares is silent about weights too large for fp16
+                    float p_most = 0.f;
+#pragma unroll
+                    for (int v = 0; v < 16; ++v) {
+                        const float weight = prob[v] * between[8 * (v >> 2) + (v & 3)];
+                        p_most = larger(p_most, is_finite(weight) ? weight : 0.f);
+                    }
+                    const float all = wave_most(p_most);
+                    if (all * p_mul >= 0x1p15f) p_mul = fmaxf(lift_of(all, 8), 0x1p-60f);
+                }
 #pragma unroll
                 for (int v = 0; v < 16; ++v) {
                     const float weight = prob[v] * between[8 * (v >> 2) + (v & 3)] * (BF ? 1.f : p_mul);

@@ -133,3 +133,26 @@ def test_small_values_in_bf16(mul, lengths, small):
     sums = np.stack([np.abs(to_np(x[key])[offsets[b]:offsets[b + 1]]).sum(0) for b in range(len(lengths))])
     more[state] = 2.0 ** -111 * sums[..., None] + 700 * 2.0 ** -127
     check(x, run(x), norms=False, more=more)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("walk", ["out", "dq", "dv", "dk"])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_large_weights_beside_no_numbers(value, walk, dtype):
+    """Weights P of 2^12 are more than fp16 holds at P's usual size.  Tokens 0 to 3 (or 28 to 31, seen from the end) have them; a value that is no
+    number in the same chunk, in a place that shares their lanes and that tokens next to them do not see, hides them from the sum that tells
+    P's size, but those tokens' results are numbers."""
+    x = inputs([32], 1, 1, 64, dtype, states=False)
+    x["scale"] = 1.0
+    x["log_decay"].zero_()
+    b, c = {"out": ("k", "v"), "dq": ("v", "k"), "dv": ("q", "dout"), "dk": ("dout", "q")}[walk]
+    large, at = (slice(0, 4), 8) if walk in ("out", "dq") else (slice(24, 28), 16)
+    x[b][large] *= 512
+    x[c] = (x[c].float() / 64).to(dtype)
+    value_at = x[b][at, 0, 3].clone()
+    x[b][at, 0, 3] = value
+    found = run(x)[walk]
+    x[b][at, 0, 3] = value_at
+    exact, bound = want(x)[walk]
+    clear = slice(0, at) if walk in ("out", "dq") else slice(at + 1, 32)
+    assert (np.abs(to_np(found) - exact) <= bound)[clear].all()
