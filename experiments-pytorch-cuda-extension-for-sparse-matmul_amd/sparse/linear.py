@@ -100,10 +100,6 @@ def run_backward(q, k, v, states, log_decay, offsets, between, dout, dlast, scal
         raise ValueError(f"the gradient of {q.dtype} {tuple(q.shape)} on {q.device} came back as {dout.dtype} {tuple(dout.shape)} on {dout.device}")
     if dlast is not None:
         check_states(dlast, state_shape(k, offsets), q.device, "the gradient of the states")
-    segment = _k.lib.bsa_linear_attention_segment(max(tokens, 1), max(offsets.numel() - 1, 1), k.size(1), dim)
-    behind, need = _between(k, tokens, segment)
-    if between.dtype != torch.float32 or between.numel() != behind.numel() or between.device != q.device or not between.is_contiguous():
-        raise ValueError("the saved states came back as others")
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk, dv = (torch.empty(k.shape, dtype=k.dtype, device=k.device) for _ in range(2))
     dfirst = torch.empty(state_shape(k, offsets), dtype=torch.float32, device=q.device) if with_states else None
@@ -111,6 +107,10 @@ def run_backward(q, k, v, states, log_decay, offsets, between, dout, dlast, scal
         if dfirst is not None:
             dfirst.zero_() if dlast is None else dfirst.copy_(dlast)
         return dq.zero_(), dk.zero_(), dv.zero_(), dfirst
+    segment = _k.lib.bsa_linear_attention_segment(tokens, offsets.numel() - 1, k.size(1), dim)
+    behind, need = _between(k, tokens, segment)
+    if between.dtype != torch.float32 or between.numel() != behind.numel() or between.device != q.device or not between.is_contiguous():
+        raise ValueError("the saved states came back as others")
     q, k, v, dout = rows_of(q), rows_of(k), rows_of(v), rows_of(dout)
     states, dlast = _dense(states), _dense(dlast)
     with _k.on_device(q.device):

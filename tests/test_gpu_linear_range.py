@@ -156,3 +156,14 @@ def test_large_weights_beside_no_numbers(value, walk, dtype):
     exact, bound = want(x)[walk]
     clear = slice(0, at) if walk in ("out", "dq") else slice(at + 1, 32)
     assert (np.abs(to_np(found) - exact) <= bound)[clear].all()
+
+
+@pytest.mark.parametrize("tokens", [5, 513, 2000])
+def test_gradients_without_sequences(tokens):
+    """Offsets of one entry: all tokens are padding, also where they would be several segments of a sequence."""
+    import sparse
+    x = inputs([tokens], 2, 1, 64, torch.float16, states=False)
+    leaves = [x[n].requires_grad_() for n in "qkv"]
+    out = sparse.packed_linear_attention(*leaves, x["log_decay"], x["offsets"][:1])
+    for t in (out, *torch.autograd.grad(out, leaves, x["dout"])):
+        assert not t.any()
