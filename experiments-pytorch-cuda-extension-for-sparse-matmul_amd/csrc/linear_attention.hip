@@ -210,17 +210,15 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
                                             unsigned char *lds_raw)
 {
     constexpr int KS = HD / 16, DT = HD / 32, OPERANDS = Tiles::STAGE / Tiles::TILE;
-    // The state's decay is put off until it passes this power of two: operands are made of the state, in bf16 with the range of fp32.  There the
-    // state is held smaller by as much, so that putting off makes nothing larger than it is: it goes as far up as fp32 does, and what
-    // is lost at the other end is lost below 2^-126, of what the parts of bf16 carry below 2^-111 (65519 tokens, 4 key heads: 40 takes as long, 5 1 % longer).
-    constexpr float PUT_OFF = BF ? 23.f : 5.f;
-    constexpr float HELD = 0x1p-23f, FREED = 0x1p23f;
+    // The state's decay is put off until it passes this power of two: operands are made of the state, fp16 has no room for more.  In bf16 the state
+    // is held smaller by as much, so that putting off makes nothing larger than it is: it goes as far up as fp32 does, and what is lost at
+    // the other end is 2^-129 of what the parts of bf16 carry (until 2^23, at 2^-111: 1 % faster, 65519 tokens, 4 key heads).
+    constexpr float PUT_OFF = 5.f;
+    constexpr float HELD = 0x1p-5f, FREED = 0x1p5f;
     // P as an operand is this much larger (fp16 has least below 1), and the result until it is rounded
     constexpr float P_LIFT = BF ? 1.f : 64.f;
     const int l = lane_id(), i = l & 31, h = l >> 5, key_head = item.head;
     const float log2_decay = linear_log2(p.log_decay[key_head]);
-    // where a chunk's own decay is near the end of fp32, nothing is put off to its product
-    const float put_off = __builtin_fabsf(log2_decay * LA_ROWS) > 64.f ? 0.f : PUT_OFF;
 
     // tokens of the segment, in chunks; step s is chunk s / inner (from the end: BACKWARDS) and head s % inner
     const int from = item.segment * p.segment, here = min(item.n - from, p.segment);
@@ -448,7 +446,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         }
         // What enters the state: c with its decay, times s_mul over the decay that the state has not got.
         const int aged = zero ? 0 : BACKWARDS && g > 0 ? age : age + valid;
-        const bool gets = !(__builtin_fabsf(log2_decay * (float)aged) <= put_off);           // the state gets its decay with this chunk
+        const bool gets = !(__builtin_fabsf(log2_decay * (float)aged) <= PUT_OFF);           // the state gets its decay with this chunk
         const float with = gets || aged == 0 ? 1.f : at_exp2(-log2_decay * (float)aged);
         // by, more: of the state and s_mul once the state has been an operand; what enters is made for them.  A state so large that nothing beside it
         // is a number above zero may be about to decay to what enters, or to nothing.

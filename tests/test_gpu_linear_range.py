@@ -120,18 +120,18 @@ def test_large_given_states_in_bf16(lengths):
 
 @pytest.mark.parametrize("small", ["v", "dout"])
 @pytest.mark.parametrize("lengths", [[70, 33, 1], [700]])
-@pytest.mark.parametrize("mul", [-75, -100])
+@pytest.mark.parametrize("mul", [-75, -100, -115])
 def test_small_values_in_bf16(mul, lengths, small):
-    """What enters a state (of the gradients' walk: with the scale) is held at least 2^-23 as large as it is, as three parts of bf16, whose smallest
-    step is 2^-133: a value of row r of the states is off by the sum of |k_t[r]| (of their gradients: |q_t[r]|) times 2^23 2^-134
-    besides, and by 2^23 2^-150 for each of the 700 roundings of the state.  Of a result that is 2^-111 of its terms' factors, which are 2^-100 or more: within its unit."""
+    """What enters a state (of the gradients' walk: with the scale) is held at least 2^-5 as large as it is, as three parts of bf16, whose smallest
+    step is 2^-133: a value of row r of the states is off by the sum of |k_t[r]| (of their gradients: |q_t[r]|) times 2^5 2^-134
+    besides, and by 2^5 2^-150 for each of the 700 roundings of the state.  Of a result that is 2^-129 of its terms' factors, which are 2^-115 or more: within its unit."""
     x = inputs(lengths, 2, 1, 64, torch.bfloat16)
     state, key = {"v": ("last", "k"), "dout": ("dfirst", "q")}[small]
     for n in (small, {"v": "states", "dout": "dlast"}[small]):
         x[n] *= 2.0 ** mul
     more, offsets = dict.fromkeys(("out", "last", "dq", "dk", "dv", "dfirst"), 0.0), np.cumsum([0] + lengths)
     sums = np.stack([np.abs(to_np(x[key])[offsets[b]:offsets[b + 1]]).sum(0) for b in range(len(lengths))])
-    more[state] = 2.0 ** -111 * sums[..., None] + 700 * 2.0 ** -127
+    more[state] = 2.0 ** -129 * sums[..., None] + 700 * 2.0 ** -145
     check(x, run(x), norms=False, more=more)
 
 
