@@ -23,6 +23,7 @@ extern "C" int bsa_lds_access(const char *name, int permuted, int arg0, int arg1
         else if (!strcmp(name, "get_linear")) a = get_linear_addr(lane, arg0);
         else if (!strcmp(name, "get_panel")) a = get_panel_addr(lane, arg0);
         else if (!strcmp(name, "get_panel_tr")) a = get_panel_tr_addr(lane, arg0, arg1, arg2);
+        else if (!strcmp(name, "get_panel_tr_ordered")) a = get_panel_tr_ordered_addr(permuted ? PANEL_PERM16 : PANEL_SWAPPED, lane, arg0);
         else if (!strcmp(name, "put_f32")) a = put_f32_addr(lane, arg0);
         else if (!strcmp(name, "get_f32_kc")) a = get_f32_kc_addr(permuted, lane, arg0);
         else if (!strcmp(name, "get_f32_ks")) a = get_f32_ks_addr(permuted, lane, arg0);
@@ -36,6 +37,7 @@ extern "C" int bsa_panel_src_piece(int lane, int chunk) { return bsa::panel_src_
 extern "C" int bsa_col16(int t, int i) { return bsa::col16(t, i); }
 extern "C" int bsa_strip16_half_swapped(int k) { return bsa::strip16_half_swapped(k); }
 extern "C" int bsa_perm16(int i) { return bsa::perm16(i); }
+extern "C" int bsa_swapped16(int i) { return bsa::swapped16(i); }
 extern "C" int bsa_invperm16(int i) { return bsa::invperm16(i); }
 
 extern "C" int bsa_panel_stages(int row_tiles) { return bsa::panel_stages(row_tiles); }

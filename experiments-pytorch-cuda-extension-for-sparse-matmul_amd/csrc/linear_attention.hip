@@ -276,7 +276,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         return __builtin_shufflevector(__builtin_bit_cast(h4, lo), __builtin_bit_cast(h4, hi), 0, 1, 2, 3, 4, 5, 6, 7);
     };
 
-    // The state: value v of state[t] is row 32 t + swapped16(r), column 32 w + perm16(i), r = 8 (v / 4) + 4 h + v % 4; times s_mul, a power
+    // The state: value v of state[t] is row 32 t + swapped16(8 (v / 4) + 4 h + v % 4), column 32 w + perm16(i); times s_mul, a power
     // of two (bf16: HELD), over the decay of the last `age` tokens, which it has not got yet.
     f16v state[DT];
     float s_mul = BF && steps > 0 ? HELD : 1.f, o_mul = 1.f;      // o_mul: of its operands besides, where what enters is much larger than it is
@@ -285,7 +285,7 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
     bool shrunk = false, dwarfed = false;        // it has got some of it, or was made small for what entered: too small for fp16 operands?
     bool zero = true;                    // nothing entered so far, or (fp16) only zeros
     const int column = 32 * w + perm16(i);
-    auto row_of = [&](int t, int v) { return 32 * t + (v & 3) + 4 * ((v >> 2) & 1) + 8 * h + 16 * (v >> 3); };
+    auto row_of = [&](int t, int v) { return 32 * t + swapped16(8 * (v >> 2) + (v & 3)) + 8 * h; };
     auto lane_most = [&]() {
         float most = 0.f;
 #pragma unroll

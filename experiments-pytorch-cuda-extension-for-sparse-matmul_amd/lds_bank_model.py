@@ -102,6 +102,7 @@ KERNEL_ACCESSES = [
     ("get_linear", 16, [dict(arg0=q) for q in (0, 1)]),
     ("get_panel", 16, [dict(arg0=s) for s in range(4)]),
     ("get_panel_tr", 8, [dict(arg0=s, arg1=h, arg2=x0) for s in (0, 1) for h in (0, 1) for x0 in (0, 32)]),
+    ("get_panel_tr_ordered", 8, [dict(permuted=p, arg0=h) for p in (False, True) for h in (0, 1)]),
     # fp32 tiles: written and read back linearly (put_f32: both directions), read as MFMA operands along k
     # (get_f32_kc: also the write of the SDD result) and across k (get_f32_ks)
     ("put_f32", 16, [dict(arg0=j) for j in range(4)]),
@@ -117,7 +118,7 @@ KNOWN_COST_FACTOR = {"put_f32": 2}
 
 # how the probe binary (csrc/lds_bank_probe.hip) issues each access
 PROBE_OPS = {"put_kc": "w128", "put_ks": "w128", "put_strip": "w128", "put_result": "w128", "put_strip16": "w128", "get_strip16": "tr64",
-             "get_kc": "b128", "get_panel": "b128", "get_panel_tr": "tr64", "get_linear": "b128", "put_f32": "w128", "get_f32_kc": "b128", "get_f32_ks": "b32", "get_ks": "tr64", "get_strip": "tr64"}
+             "get_kc": "b128", "get_panel": "b128", "get_panel_tr": "tr64", "get_panel_tr_ordered": "tr64", "get_linear": "b128", "put_f32": "w128", "get_f32_kc": "b128", "get_f32_ks": "b32", "get_ks": "tr64", "get_strip": "tr64"}
 
 
 def _probe(binary: str, op: str, addresses: Sequence[int]) -> float:
