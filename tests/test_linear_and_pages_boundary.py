@@ -141,3 +141,10 @@ def test_copies(k, kw, needle):
 
 def test_copies_of_nothing(k):
     assert copying(k, count=0, lists=(None, None)) == 0 and copying(k, dtype=F16, tensors=[P, P, None, None] * 2, count=0) == 0
+
+
+def test_lengths_of_segments(k):
+    """What fills the machine where tokens are many, by the mean length where they are few, one launch where sequences are short."""
+    segment = k.lib.bsa_linear_attention_segment
+    assert segment(65519, 5, 4, 128) == 544 and segment(24575, 2, 16, 128) == 832 and segment(10 ** 7, 1, 64, 128) == 8192
+    assert segment(65536, 1, 1, 64) == 320 and segment(2000, 1, 1, 64) == 96 and segment(368, 5, 12, 64) == 512
