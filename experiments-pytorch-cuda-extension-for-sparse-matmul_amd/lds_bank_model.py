@@ -133,7 +133,7 @@ if __name__ == "__main__":
     probe = sys.argv[sys.argv.index("--probe") + 1] if "--probe" in sys.argv else None
     linear = {}
     if probe:
-        for op, step in (("b128", 16), ("w128", 16), ("tr64", 8)):
+        for op, step in (("b128", 16), ("w128", 16), ("tr64", 8), ("b32", 4)):
             linear[op] = _probe(probe, op, [step * lane for lane in range(WAVE)])
             print(f"linear      {op:5s} measured {linear[op]:.2f} ticks per wave-instruction (conflict-free yardstick)")
     for name, width, variants in KERNEL_ACCESSES:
