@@ -167,3 +167,25 @@ def test_gradients_without_sequences(tokens):
     out = sparse.packed_linear_attention(*leaves, x["log_decay"], x["offsets"][:1])
     for t in (out, *torch.autograd.grad(out, leaves, x["dout"])):
         assert not t.any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("name", ["states", "dlast"])
+@pytest.mark.parametrize("lengths,dim", [([70, 20], 64), ([300, 0], 128)])
+def test_given_states_with_a_value_that_is_no_number(lengths, dim, name, value, dtype):
+    """Row 3, column 5 of the first state: column 5 of the results, column 3 of dq, and its own place in the last state; likewise of the last
+    state's gradient: column 5 of dv, column 3 of dk, its place in the first state's gradient."""
+    x = inputs(lengths, 2, 2, dim, dtype)
+    x[name][0, 0, 3, 5] = value
+    found = run(x)
+    x[name][0, 0, 3, 5] = 0
+    columns, place = ({"out": 5, "dq": 3}, "last") if name == "states" else ({"dv": 5, "dk": 3}, "dfirst")
+    for result, (exact, bound) in want(x).items():
+        got, reached = to_np(found[result]), np.zeros(exact.shape, bool)
+        if result in columns:
+            reached[:lengths[0], slice(0, 2) if result in ("out", "dq") else 0, columns[result]] = True
+        if result == place:
+            reached[0, 0, 3, 5] = True
+        assert not np.isfinite(got[reached]).any(), result
+        assert (np.abs(got - exact) <= bound)[~reached].all(), result
