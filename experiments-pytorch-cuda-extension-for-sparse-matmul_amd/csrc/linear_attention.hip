@@ -12,14 +12,15 @@
 // with: every segment's own sum, then the running sum over segments.  Chunks travel straight to LDS two steps ahead of their use, in
 // a ring of three.
 //
-// What bounds it (times of launches, the least of 60):
-//   results: memory.  65519 tokens, 8 heads over 4, head dim 128, bf16: 100 us for 430 MB, operands, result and states (4.3 TB/s); one workgroup
-//   of the two on a compute unit gets what the other leaves and ends a fifth later.  24575 tokens, 16 heads, fp16: 96 us (4.5 TB/s).
-//   segments' sums: memory, 134 MB in 34 us (3.9 TB/s), 201 MB in 46; with dq 137 us together; the running sum over them 11 to 14 us for 62 MB.
-//   dv and dk: the clocks of a step, 24575 tokens, 16 heads, head dim 128: 204 us for 600 MB; of 6.7k clocks a step the vector pipe works 45 %
+// What bounds it (times of launches, the least of 60 and their median):
+//   results: memory.  65519 tokens, 8 heads over 4, head dim 128, bf16: 104 us (121) for 430 MB, operands, result and states, 4.1 TB/s (3.6); one
+//   workgroup of the two on a compute unit gets what the other leaves and ends a fifth later.  24575 tokens, 16 heads, fp16: 98 us (101), 4.4 TB/s.
+//   segments' sums: memory, 134 MB in 37 us (45), 3.6 TB/s (3.0), 201 MB in 46 (47); with dq 139 us (141) together; the running sum over them 11 to
+//   13 us (12 to 15) for 62 MB.
+//   dv and dk: the clocks of a step, 24575 tokens, 16 heads, head dim 128: 205 us (209) for 600 MB; of 6.7k clocks a step the vector pipe works 45 %
 //   and the matrix pipe 27 %, two waves on each side of a barrier.  512 threads and 97 KB of LDS: one workgroup a compute unit.
 //   short texts: what a segment costs before its first product (5 us: its place, the state, the first chunks' way through memory) and
-//   1 us a chunk.  368 tokens, 12 heads, head dim 64: 12 us.
+//   1 us a chunk.  368 tokens, 12 heads, head dim 64: 13.6 us (15).
 #include "attention_tiles.hpp"
 #include "bsa_device.hpp"
 #include "bsa_internal.hpp"
@@ -116,8 +117,9 @@ __device__ __forceinline__ size_t linear_boundary(const LinearWalk &p, int begin
     return ((size_t)((unsigned)begin / (unsigned)p.segment) + j - 1) * p.key_heads + key_head;
 }
 
-// Decay of e tokens.  The exponent is made anew from e, not by products of decays: it is off by 2^-23 of itself, x, and what it
-// belongs to by x 2^-23 of 2^-x of what has not decayed.
+// Decay of e tokens of one stretch: a chunk and what was put off before it, or a segment.  The exponent, x, is made from e and is off by about
+// 2^-23 of itself.  Stretches multiply, each factor rounded: over m of them with exponents x1 .. xm what is left of a state is off by
+// (x1 + .. + xm + m) 2^-23 of itself; m is at most a chunk's worth of tokens each, and one a segment.
 __device__ __forceinline__ float linear_log2(float log_decay) { return log_decay * 1.4426950408889634f; }
 __device__ __forceinline__ float linear_power(float log2_decay, int e) { return e == 0 ? 1.f : at_exp2(log2_decay * (float)e); }
 
@@ -938,10 +940,10 @@ size_t linear_workspace_bytes(const LinearArgs &a)
 }
 // Large batches: segments of which every compute unit has its workgroups at once (two at head dim 128, four at 64) and no more: a second
 // generation would leave most of the machine idle at its end, and every boundary is a state to write and read.  65519 tokens, 4 key
-// heads, head dim 128: 153 us with the 500 workgroups of segments of 544 tokens, 190 with 512 tokens, 184 with 800.
+// heads, head dim 128: 168 us with the 500 workgroups of segments of 544 tokens, 200 with 512 tokens, 195 with 800.
 // Others: two walks a segment long (0.06 us a token together) and the running sum over the boundaries (0.1 us each) are shortest
-// together at sqrt(1.5 length).  One sequence of 65536, a head, head dim 64: 50 us with 384 tokens, 69 with 128, 74 with 1024; six texts of 1 to
-// 1500, 12 heads: 30 us with 96 or 128, 41 with 32, 37 with 384.  The lengths are on the device, so this goes by their mean; up to 192 the two
+// together at sqrt(1.5 length).  One sequence of 65536, a head, head dim 64: 50 us with 320 or 384 tokens, 70 with 128, 77 with 1024; six texts of 1 to
+// 1500, 12 heads: 31 us with 96, 30 with 128, 41 with 32, 38 with 384.  The lengths are on the device, so this goes by their mean; up to 192 the two
 // launches in front of the walk take longer than they save.
 int linear_segment(int tokens, int sequences, int key_heads, int head_dim)
 {

@@ -1,7 +1,7 @@
 // One token of every sequence against its recurrent state, in place:  S <- l S + k v^T,  o = scale q S.
 //
 // What bounds it: the state, 4 D^2 bytes a sequence and key head, read and written once; 3 to 4 operations a value.  250 sequences, 16 key heads,
-// head dim 128: 524 MB in 84 to 88 us, 6.0 TB/s; 3 sequences, 4 heads, head dim 64: 3.1 us.  A workgroup has COLUMNS
+// head dim 128: 524 MB in 84 to 88 us, 6.0 TB/s; 3 sequences, 4 heads, head dim 64: 3.2 us.  A workgroup has COLUMNS
 // columns of one state, 16 bytes a lane, every lane all its loads in flight at once; the query heads of a key head share the pass.
 // Results of the rows that different lanes have add up in LDS.
 #include "bsa_device.hpp"

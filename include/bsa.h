@@ -479,8 +479,11 @@ int bsa_cached_attention(int dtype, int cache_dtype, const void *q, const void *
  *                    forward call, read by the backward call, which has scratch of the same size of its own.  0 bytes up to `segment` tokens
  *   segment          tokens, a multiple of 32; bsa_linear_attention_segment says which fills the machine.  Both calls have to have
  *                    the same.  Results of different segments differ by rounding.
- * Tokens outside every sequence get zeros.  States are fp32; results are the same bits in every call.  An infinity or a NaN
- * in a token makes what it reaches, of its own token and later ones, something that is no finite number.
+ * Tokens outside every sequence get zeros.  States are fp32; results are the same bits in every call (with and without last, or dfirst, they differ
+ * in bf16 by rounding: what enters a state that is itself a result has more bits).  An infinity or a NaN in a token makes what it reaches, of
+ * its own token and later ones (gradients of k and v: earlier ones), something that is no finite number, and nothing else.  States and values may be as
+ * large as fp32 holds; below about 2^-120 they and their decays have fewer bits, and in fp16 what enters a state is off by up to
+ * 2^-29 of the largest value that its 32 columns hold or get.
  * fp16 and bf16, head_dim 64 or 128, at most 65535 sequences; log_decay has no gradient.
  *
  * bsa_linear_attention_step: one token of each of `batch` sequences against its state, in place:
