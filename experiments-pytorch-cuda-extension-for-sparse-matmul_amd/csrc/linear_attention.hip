@@ -119,7 +119,7 @@ __device__ __forceinline__ size_t linear_boundary(const LinearWalk &p, int begin
 
 // Decay of e tokens of one stretch: a chunk and what was put off before it, or a segment.  The exponent, x, is made from e and is off by about
 // 2^-23 of itself.  Stretches multiply, each factor rounded: over m of them with exponents x1 .. xm what is left of a state is off by
-// (x1 + .. + xm + m) 2^-23 of itself; m is at most a chunk's worth of tokens each, and one a segment.
+// (x1 + .. + xm + m) 2^-23 of itself; a chunk ends one stretch at the most, a segment another.  Decays below 2^-126 are nothing.
 __device__ __forceinline__ float linear_log2(float log_decay) { return log_decay * 1.4426950408889634f; }
 __device__ __forceinline__ float linear_power(float log2_decay, int e) { return e == 0 ? 1.f : at_exp2(log2_decay * (float)e); }
 
@@ -450,8 +450,8 @@ __device__ __forceinline__ void linear_walk(const LinearWalk &p, const LinearSum
         const int aged = zero ? 0 : BACKWARDS && g > 0 ? age : age + valid;
         const bool gets = !(__builtin_fabsf(log2_decay * (float)aged) <= PUT_OFF);           // the state gets its decay with this chunk
         const float with = gets || aged == 0 ? 1.f : at_exp2(-log2_decay * (float)aged);
-        // by, more: of the state and s_mul once the state has been an operand; what enters is made for them.  A state so large that nothing beside it
-        // is a number above zero may be about to decay to what enters, or to nothing.
+        // by, more: of the state and s_mul once the state has been an operand; what enters is made for them.  Beside a state so large (2^-20: beyond
+        // what fp16's own values add up to) what enters may be less than fp32's least, and the state about to decay to that, or to nothing.
         float by = 1.f, more = 1.f;
         if (!BF && enters && gets && s_mul < 0x1p-20f) {
             const float left = state_most() * linear_power(log2_decay, aged), most = __builtin_amdgcn_rcpf(s_mul);

@@ -152,7 +152,8 @@ def packed_linear_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, l
     without; with ``return_states`` the call gives ``(o, final states)``, an empty sequence's being those it began with.  Tokens
     outside every sequence (the padding of a batch) are not read; their results and gradients are zero.  Operands may be slices of a
     larger tensor; they are copied only where a row does not start at a multiple of 16 bytes.  Differentiable once in ``q``, ``k``, ``v``
-    and ``states``, with the same bits in every call (in bfloat16 ``return_states`` changes ``o`` within its rounding); ``log_decay`` has no gradient and is refused if autograd follows it."""
+    and ``states``, with the same bits in every call (in bfloat16 ``return_states`` changes ``o`` within its rounding); ``log_decay`` has no
+    gradient and is refused if autograd follows it."""
     found = _k.host_calls.linear_attention(q, k, v, log_decay, offsets, scale, states, return_states)
     if found is not None:
         return found

@@ -21,8 +21,9 @@ class PageTable:
     """Pages of ``page`` tokens, ``pages`` of them, for up to ``sequences`` sequences of at most ``width`` pages: ``table [sequences, width]``
     (-1 behind the last page of each), ``lengths [sequences]`` in tokens, ``uses [pages]``: how many sequences have a page, and
     ``missing [1]``: how many requests for pages could not be met so far.  A whole page may belong to several sequences, a last page
-    that is not full belongs to one.  The lowest free pages are taken first.  The tensors may be written to, not replaced (whoever lowers a length by whole pages
-    frees them too: ``uses`` and -1 behind the last page are what the calls go by); the calls for a table are to be ordered, on one stream or by events."""
+    that is not full belongs to one.  The lowest free pages are taken first.  The tensors may be written to, not replaced (whoever lowers a
+    length by whole pages frees them too, in ``uses`` and in the row); the calls for a table are to be ordered, on one stream or by
+    events."""
 
     def __init__(self, pages: int, page: int, sequences: int, width: int, device=None):
         if page not in PAGES:
