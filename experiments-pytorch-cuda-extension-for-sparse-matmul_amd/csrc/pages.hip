@@ -9,7 +9,8 @@
 // What bounds it: latency.  Ranks of free pages are found by one workgroup that reads `uses` 16 bytes a lane and sums up in LDS, as far as it
 // has to; rows of the table are read and written by a workgroup each.  Least of 60 launches and their median: a step of 64
 // sequences 4.5 us (4.7), 24 prompts of 64 to 4096 tokens 6.3 (6.6) and, their slots, 2.6 (3.8); a fork of 8 sequences to 504 children of up to 235
-// pages 8.9 (11.4), 8.2 (8.4) and 4.2 (4.8), three launches; a compaction of 6650 pages 8.2 (8.4) and 2.8 (4.6).
+// pages 8.9 (11.4), 8.2 (8.4) and 4.2 (4.8), three launches; a compaction of 6650 pages 8.2 (8.4) and 2.8 (4.6).  The end
+// of 8 sequences of 22 pages 3.0 us (3.9), of 504 of 235 pages 3.6 (4.3): a launch, each page's use an atomic.
 // Copies of pages: memory, 5.7 TB/s (217 MB each way in 76 us, 78).
 #include "bsa_device.hpp"
 #include "bsa_internal.hpp"
